@@ -20,7 +20,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "gs_voxelizer", "libgsvox.so")
 AUTOGRAD = os.path.join(HERE, "gs_voxelizer", "_autograd.so")
-SOURCES = ["scan.hip", "project.hip", "binning.hip", "voxelize.hip"]
+SOURCES = ["scan.hip", "project.hip", "binning.hip", "voxelize.hip", "rotary.hip",
+           "gated_norm.hip", "attention_fwd.hip", "attention_bwd.hip", "attention_cached.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

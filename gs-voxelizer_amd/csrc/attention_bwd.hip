@@ -1,0 +1,436 @@
+// attention_bwd.hip — attention inside packed scenes, backward.
+//
+// With p_ij the weights, recomputed from the saved log sums, and D_i = do_i.o_i:
+//   dv_j = sum_i p_ij do_i            dt_ij = p_ij (do_i.v_j - D_i)
+//   dslope = - sum_ij dt_ij |p_i - p_j|
+//   ds_ij = dt_ij (1 - tanh^2)        dq_i = scale sum_j ds_ij k_j
+//                                     dk_j = scale sum_i ds_ij q_i
+// Two kernels form the scores twice, one with the rows' sums (dq, D, dslope) and one with
+// the keys' (dk, dv): each sum stays in the registers of one wave, in a fixed order, with
+// no atomics and no partial gradients in memory.
+#include "gsv_attention.h"
+
+namespace gsv {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kRows = 128;  // rows (dq) or keys (dk, dv) of a workgroup, 32 a wave
+
+template <typename T> struct BwdTile { static constexpr int kOther = sizeof(T) == 2 ? 64 : 32; };
+
+struct BwdArgs {
+    const void *out, *dout;
+    int64_t dout_row, dout_head;
+    const float *lse;
+    float *delta;   // (heads, q_tokens)
+    float *dslope;  // (slots * scenes, heads) partial sums
+    void *dq, *dk, *dv;
+};
+
+// dt (before the cap's factor) and ds of a block from its scores w, as the matrix product
+// leaves them, and dp - D.
+template <typename T>
+__device__ __forceinline__ void weigh(f32x16 &w, f32x16 &u, const f32x16 &d, bool capped, bool far,
+                                      float in_cap, float cap, float far_unit) {
+    if (!capped) return;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        u[r] = tanh_of<T>(w[r] * in_cap);
+        w[r] = cap * u[r];
+        if (far) w[r] = fmaf(-far_unit, d[r], w[r]);
+    }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_attention_dq(const AttnArgs a, const BwdArgs g) {
+    constexpr int KB = BwdTile<T>::kOther, LD = DP + Elem<T>::kPad;
+    typedef typename Elem<T>::frag frag;
+    __shared__ __align__(16) T sk[2][KB * LD];
+    __shared__ __align__(16) T sv[2][KB * LD];
+    __shared__ __align__(16) float spos[2][3 * KB];
+    __shared__ double sums[4];
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int h = blockIdx.x % a.heads, rest = blockIdx.x / a.heads;
+    const int s = rest % a.scenes, slot = rest / a.scenes;
+    const Scene c = scene_rows(a, s);
+    const int nq = c.q1 - c.q0, nk = c.k1 - c.k0;
+    const int tiles = (nq + kRows - 1) / kRows;
+    const int hk = h / (a.heads / a.kv_heads);
+    const T *kbase = static_cast<const T *>(a.k) + (int64_t)c.k0 * a.k_row + hk * a.k_head;
+    const T *vbase = static_cast<const T *>(a.v) + (int64_t)c.k0 * a.v_row + hk * a.v_head;
+    const bool far = a.slopes != nullptr, capped = a.cap > 0.f;
+    const float slope = slope_of(a, h);
+    const float unit = capped ? kLog2e : a.scale * kLog2e;
+    const float far_unit = capped ? slope : slope / a.scale;
+    const float in_cap = capped ? a.scale / a.cap : 0.f;
+    double dslope = 0.0;
+
+    for (int tile = slot; tile < tiles; tile += a.slots) {
+        const int first = (tiles - 1 - tile) * kRows;
+        const int i = first + wave * 32 + (lane & 31);
+        const bool row = i < nq;
+        const int64_t qi = c.q0 + i;
+        frag q[DP / 16], dO[DP / 16];
+        load_column<T, DP>(q, static_cast<const T *>(a.q) + qi * a.q_row + h * a.q_head, a.dim, row,
+                           lane);
+        load_column<T, DP>(dO, static_cast<const T *>(g.dout) + qi * g.dout_row + h * g.dout_head,
+                           a.dim, row, lane);
+        float delta = 0.f, lse = INFINITY, x = 0.f, y = 0.f, z = 0.f;
+        {
+            const T *o = static_cast<const T *>(g.out) + (qi * a.heads + h) * a.dim;
+#pragma unroll
+            for (int st = 0; st < DP / 16; ++st) {
+                const int d = st * 16 + 8 * (lane >> 5);
+                if (row && d < a.dim) {
+                    const frag f = row_frag(o + d);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) delta = fmaf((float)f[e], (float)dO[st][e], delta);
+                }
+            }
+        }
+        delta += other_half(delta);
+        if (row) {
+            if (lane < 32) g.delta[(int64_t)h * a.q_tokens + qi] = delta;
+            lse = g.lse[(int64_t)h * a.q_tokens + qi];
+            if (far) {
+                const float *p = a.q_pos + qi * a.q_pos_row;
+                x = p[0], y = p[1], z = p[2];
+            }
+        }
+        const int limit = row ? key_limit(a, c, i) : 0;
+        const int all = first + wave * 32 + 31 < nq ? key_limit(a, c, first + wave * 32) : 0;
+        const int most = key_limit(a, c, min(first + kRows, nq) - 1);
+        const int mine = first + wave * 32 < nq
+                             ? key_limit(a, c, min(first + wave * 32 + 32, nq) - 1) : 0;
+        f32x16 dq[DP / 32] = {};
+
+        Staged<T, DP, KB> gk, gv;
+        float gp = 0.f;
+        auto fetch = [&](int j0) {
+            auto live = [&](int r) { return j0 + r < most && kept(a, c.k0 + j0 + r); };
+            gk.load(kbase + j0 * a.k_row, a.k_row, a.dim, live);
+            gv.load(vbase + j0 * a.v_row, a.v_row, a.dim, live);
+            if (far && threadIdx.x < 3 * KB) {
+                const int r = threadIdx.x % KB, ax = threadIdx.x / KB;
+                gp = j0 + r < most ? a.k_pos[(int64_t)(c.k0 + j0 + r) * a.k_pos_row + ax] : 0.f;
+            }
+        };
+        auto put = [&](int b) {
+            gk.store(sk[b]);
+            gv.store(sv[b]);
+            if (far && threadIdx.x < 3 * KB) spos[b][threadIdx.x] = gp;
+        };
+        __syncthreads();
+        if (most > 0) {
+            fetch(0);
+            put(0);
+        }
+        __syncthreads();
+        int b = 0;
+        for (int j0 = 0; j0 < most; j0 += KB, b ^= 1) {
+            const bool more = j0 + KB < most;
+            if (more) fetch(j0 + KB);
+            if (j0 < mine) {
+                uint64_t live = ~0ull;
+                if (a.keep || j0 + KB > all)
+                    live = __ballot(j0 + lane < nk && lane < KB && kept(a, c.k0 + min(j0 + lane, nk - 1)));
+                const bool masked = j0 + KB > all || (KB == 64 ? ~live : (~live & 0xffffffffull)) != 0;
+                float here = 0.f;
+#pragma unroll
+                for (int kb = 0; kb < KB / 32; ++kb) {
+                    f32x16 d = {}, w = {}, u = {}, dp;
+                    if (far) d = distances(spos[b], KB, kb * 32, lane, x, y, z);
+                    if (far && !capped)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) w[r] = -far_unit * d[r];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dp[r] = -delta;
+                    const int at0 = (kb * 32 + (lane & 31)) * LD + 8 * (lane >> 5);
+#pragma unroll
+                    for (int st = 0; st < DP / 16; ++st) {
+                        w = mma(row_frag(sk[b] + at0 + st * 16), q[st], w);
+                        dp = mma(row_frag(sv[b] + at0 + st * 16), dO[st], dp);
+                    }
+                    weigh<T>(w, u, d, capped, far, in_cap, a.cap, far_unit);
+                    if (masked) {
+                        const uint32_t bits = (uint32_t)(live >> (kb * 32)) >> (4 * (lane >> 5));
+                        const int lim = limit - j0 - kb * 32 - 4 * (lane >> 5);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int at = 8 * (r >> 2) + (r & 3);
+                            if (at >= lim || !((bits >> at) & 1)) {
+                                w[r] = -INFINITY;
+                                if (far) d[r] = 0.f;  // a masked key's position may be anything
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        dp[r] *= fast_exp2(fmaf(w[r], unit, -lse));
+                        if (far) here = fmaf(dp[r], d[r], here);
+                        if (capped) dp[r] *= fmaf(-u[r], u[r], 1.f);
+                    }
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const frag ds = to_frag<T>(dp, half);
+#pragma unroll
+                        for (int n = 0; n < DP / 32; ++n)
+                            dq[n] = mma(tr_frag<LD>(sk[b] + (kb * 32 + half * 16) * LD + n * 32, lane),
+                                        ds, dq[n]);
+                    }
+                }
+                dslope -= here;
+            }
+            if (more) put(b ^ 1);
+            __syncthreads();
+        }
+        if (row)
+            store_column<T, DP>(static_cast<T *>(g.dq) + (qi * a.heads + h) * a.dim, dq, a.scale,
+                                a.dim, lane);
+    }
+    if (far) {
+#pragma unroll
+        for (int n = 1; n < 64; n <<= 1) dslope += __shfl_xor(dslope, n);
+        __syncthreads();
+        if (lane == 0) sums[wave] = dslope;
+        __syncthreads();
+        if (threadIdx.x == 0)
+            g.dslope[(int64_t)rest * a.heads + h] = (float)(sums[0] + sums[1] + sums[2] + sums[3]);
+    }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_attention_dkv(const AttnArgs a, const BwdArgs g) {
+    constexpr int QB = BwdTile<T>::kOther, LD = DP + Elem<T>::kPad;
+    typedef typename Elem<T>::frag frag;
+    __shared__ __align__(16) T sq[2][QB * LD];
+    __shared__ __align__(16) T sdo[2][QB * LD];
+    __shared__ __align__(16) float srow[2][5 * QB];  // x, y, z, log sum, D
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
+    const int s = rest % a.scenes, slot = rest / a.scenes;
+    const Scene c = scene_rows(a, s);
+    const int nq = c.q1 - c.q0, nk = c.k1 - c.k0, off = nk - nq;
+    const int group = a.heads / a.kv_heads;
+    const int tiles = (nk + kRows - 1) / kRows;
+    const bool far = a.slopes != nullptr, capped = a.cap > 0.f;
+    const float unit = capped ? kLog2e : a.scale * kLog2e;
+    const float in_cap = capped ? a.scale / a.cap : 0.f;
+
+    for (int tile = slot; tile < tiles; tile += a.slots) {
+        const int first = tile * kRows;
+        const int j = first + wave * 32 + (lane & 31);
+        const int64_t kj = c.k0 + j;
+        const bool live = j < nk && kept(a, kj);
+        frag k[DP / 16], v[DP / 16];
+        load_column<T, DP>(k, static_cast<const T *>(a.k) + kj * a.k_row + hk * a.k_head, a.dim,
+                           live, lane);
+        load_column<T, DP>(v, static_cast<const T *>(a.v) + kj * a.v_row + hk * a.v_head, a.dim,
+                           live, lane);
+        float x = 0.f, y = 0.f, z = 0.f;
+        if (far && live) {
+            const float *p = a.k_pos + kj * a.k_pos_row;
+            x = p[0], y = p[1], z = p[2];
+        }
+        // the first query row that sees this key; one that no row sees
+        const int from = !live ? INT32_MAX : a.causal && j >= c.prefix ? j - off : 0;
+        const bool dead_here = __any(!live);
+        const int wave_from = a.causal && first + wave * 32 >= c.prefix ? first + wave * 32 - off : 0;
+        const int wave_all = dead_here ? INT32_MAX
+                             : a.causal && first + wave * 32 + 31 >= c.prefix
+                                 ? first + wave * 32 + 31 - off : 0;
+        const int q_from =
+            a.causal && first >= c.prefix ? max(first - off, 0) / QB * QB : 0;
+        const int per_head = q_from < nq ? (nq - q_from + QB - 1) / QB : 0;
+        const int steps = per_head * group;
+        f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
+
+        Staged<T, DP, QB> gq, gd;
+        float gr[2] = {};
+        auto fetch = [&](int step) {
+            const int h = hk * group + step / per_head, i0 = q_from + step % per_head * QB;
+            const int64_t q0 = c.q0 + i0;
+            auto inside = [&](int r) { return i0 + r < nq; };
+            gq.load(static_cast<const T *>(a.q) + q0 * a.q_row + h * a.q_head, a.q_row, a.dim, inside);
+            gd.load(static_cast<const T *>(g.dout) + q0 * g.dout_row + h * g.dout_head, g.dout_row,
+                    a.dim, inside);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int at = n * 256 + threadIdx.x, r = at % QB, what = at / QB;
+                gr[n] = what == 3 ? INFINITY : 0.f;
+                if (what < 5 && i0 + r < nq) {
+                    if (what < 3) {
+                        if (far) gr[n] = a.q_pos[(q0 + r) * a.q_pos_row + what];
+                    } else {
+                        gr[n] = (what == 3 ? g.lse : g.delta)[(int64_t)h * a.q_tokens + q0 + r];
+                    }
+                }
+            }
+        };
+        auto put = [&](int b) {
+            gq.store(sq[b]);
+            gd.store(sdo[b]);
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+                if (n * 256 + threadIdx.x < 5 * QB) srow[b][n * 256 + threadIdx.x] = gr[n];
+        };
+        __syncthreads();
+        if (steps > 0) {
+            fetch(0);
+            put(0);
+        }
+        __syncthreads();
+        int b = 0;
+        for (int step = 0; step < steps; ++step, b ^= 1) {
+            const bool more = step + 1 < steps;
+            if (more) fetch(step + 1);
+            const int i0 = q_from + step % per_head * QB;
+            if (i0 + QB > wave_from && first + wave * 32 < nk) {
+                const float slope = slope_of(a, hk * group + step / per_head);
+                const float far_unit = capped ? slope : slope / a.scale;
+                const bool masked = i0 < wave_all;
+#pragma unroll
+                for (int qb = 0; qb < QB / 32; ++qb) {
+                    f32x16 d = {}, w = {}, u = {}, dp, lse;
+                    if (far) d = distances(srow[b], QB, qb * 32, lane, x, y, z);
+                    if (far && !capped)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) w[r] = -far_unit * d[r];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const float *p = srow[b] + 3 * QB + qb * 32 + 8 * n + 4 * (lane >> 5);
+                        const f32x4 ls = *reinterpret_cast<const f32x4 *>(p);
+                        const f32x4 de = *reinterpret_cast<const f32x4 *>(p + QB);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) lse[4 * n + e] = ls[e], dp[4 * n + e] = -de[e];
+                    }
+                    const int at0 = (qb * 32 + (lane & 31)) * LD + 8 * (lane >> 5);
+#pragma unroll
+                    for (int st = 0; st < DP / 16; ++st) {
+                        w = mma(row_frag(sq[b] + at0 + st * 16), k[st], w);
+                        dp = mma(row_frag(sdo[b] + at0 + st * 16), v[st], dp);
+                    }
+                    weigh<T>(w, u, d, capped, far, in_cap, a.cap, far_unit);
+                    if (masked) {
+                        const int lo = from == INT32_MAX ? from : from - i0 - qb * 32 - 4 * (lane >> 5);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (8 * (r >> 2) + (r & 3) < lo) w[r] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        w[r] = fast_exp2(fmaf(w[r], unit, -lse[r]));
+                        dp[r] *= w[r];
+                        if (capped) dp[r] *= fmaf(-u[r], u[r], 1.f);
+                    }
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const frag p = to_frag<T>(w, half), ds = to_frag<T>(dp, half);
+                        const int at = (qb * 32 + half * 16) * LD;
+#pragma unroll
+                        for (int n = 0; n < DP / 32; ++n) {
+                            dv[n] = mma(tr_frag<LD>(sdo[b] + at + n * 32, lane), p, dv[n]);
+                            dk[n] = mma(tr_frag<LD>(sq[b] + at + n * 32, lane), ds, dk[n]);
+                        }
+                    }
+                }
+            }
+            if (more) put(b ^ 1);
+            __syncthreads();
+        }
+        if (j < nk) {
+            const int64_t at = (kj * a.kv_heads + hk) * a.dim;
+            store_column<T, DP>(static_cast<T *>(g.dk) + at, dk, a.scale, a.dim, lane);
+            store_column<T, DP>(static_cast<T *>(g.dv) + at, dv, 1.f, a.dim, lane);
+        }
+    }
+}
+
+// The workgroups' sums of each head, in order.
+__global__ __launch_bounds__(64) void k_slope_sum(const float *__restrict__ part, int n, int heads,
+                                                  void *__restrict__ out, int f32) {
+    const int h = blockIdx.x;
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < n; i += 64) sum += part[(int64_t)i * heads + h];
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k);
+    if (threadIdx.x) return;
+    if (f32) static_cast<float *>(out)[h] = (float)sum;
+    else static_cast<bf16 *>(out)[h] = (bf16)(float)sum;
+}
+
+template <typename T, int DP> void launch_bwd(AttnArgs a, const BwdArgs &g, int kslots, hipStream_t st) {
+    const dim3 block(256);
+    if (a.q_tokens > 0)
+        hipLaunchKernelGGL((k_attention_dq<T, DP>), dim3((unsigned)a.slots * a.scenes * a.heads),
+                           block, 0, st, a, g);
+    a.slots = kslots;
+    if (a.k_tokens > 0)
+        hipLaunchKernelGGL((k_attention_dkv<T, DP>), dim3((unsigned)a.slots * a.scenes * a.kv_heads),
+                           block, 0, st, a, g);
+}
+template <typename T> void launch_bwd(const AttnArgs &a, const BwdArgs &g, int kslots, hipStream_t st) {
+    if (a.dim <= 32) launch_bwd<T, 32>(a, g, kslots, st);
+    else if (a.dim <= 64) launch_bwd<T, 64>(a, g, kslots, st);
+    else launch_bwd<T, 128>(a, g, kslots, st);
+}
+
+size_t delta_bytes(const AttnArgs &a) {
+    return ((size_t)a.heads * a.q_tokens * sizeof(float) + 255) / 256 * 256;
+}
+
+int bwd_plan(const gsv_attention *args, AttnArgs *a, int *kslots) {
+    int lq, lk;
+    const int st = attention_args(args, a, &lq, &lk);
+    if (st != GSV_OK) return st;
+    if (!attention_slots(a, lk, kRows, a->kv_heads)) return GSV_ERR_SIZE_OVERFLOW;
+    *kslots = a->slots;
+    return attention_slots(a, lq, kRows, a->heads) ? GSV_OK : GSV_ERR_SIZE_OVERFLOW;
+}
+
+}  // namespace
+}  // namespace gsv
+
+using namespace gsv;
+
+extern "C" int gsv_attention_bwd_workspace_bytes(const gsv_attention *args, size_t *bytes) {
+    AttnArgs a;
+    int kslots;
+    if (!bytes) return GSV_ERR_INVALID_ARGUMENT;
+    const int st = bwd_plan(args, &a, &kslots);
+    if (st != GSV_OK) return st;
+    *bytes = delta_bytes(a) + (a.slopes ? sizeof(float) * a.slots * a.scenes * a.heads : 0);
+    return GSV_OK;
+}
+
+extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, const float *lse,
+                                 const void *dout, int64_t dout_row, int64_t dout_head, void *dq,
+                                 void *dk, void *dv, void *dslopes, void *workspace,
+                                 size_t workspace_bytes, void *stream) {
+    AttnArgs a;
+    int kslots;
+    size_t need;
+    int st = bwd_plan(args, &a, &kslots);
+    if (st != GSV_OK) return st;
+    if ((st = gsv_attention_bwd_workspace_bytes(args, &need)) != GSV_OK) return st;
+    if (need > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
+    const int64_t chunk = args->dtype == GSV_BF16 ? 8 : 4;
+    if (dout_row % chunk || dout_head % chunk) return GSV_ERR_INVALID_ARGUMENT;
+    if (a.q_tokens > 0 && (!out || !lse || !dout || !dq || !workspace)) return GSV_ERR_INVALID_ARGUMENT;
+    if ((a.k_tokens > 0 && (!dk || !dv)) || (a.slopes && !dslopes)) return GSV_ERR_INVALID_ARGUMENT;
+    const void *ptrs[] = {out, dout, dq, dk, dv, workspace};
+    for (const void *p : ptrs)
+        if (reinterpret_cast<uintptr_t>(p) % 16) return GSV_ERR_INVALID_ARGUMENT;
+    float *delta = static_cast<float *>(workspace);
+    float *part = reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(a));
+    const BwdArgs g{out, dout, dout_row, dout_head, lse, delta, part, dq, dk, dv};
+    hipStream_t s = as_stream(stream);
+    if (args->dtype == GSV_BF16) launch_bwd<bf16>(a, g, kslots, s);
+    else launch_bwd<float>(a, g, kslots, s);
+    if (a.slopes)
+        hipLaunchKernelGGL(k_slope_sum, dim3(a.heads), dim3(64), 0, s, part,
+                           a.q_tokens > 0 ? a.slots * a.scenes : 0, a.heads, dslopes, a.slopes_f32);
+    return check_launch();
+}

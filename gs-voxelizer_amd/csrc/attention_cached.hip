@@ -1,0 +1,323 @@
+// attention_cached.hip — one query token a scene against a cache of keys and values.
+//
+// Same scores as attention_fwd.hip.  The bytes of the cache are the floor: each is read
+// once, by coalesced 16-byte loads, and serves all query heads of its key head, which
+// are the columns of a matrix product (32, those past the group idle: the matrix units
+// have an order of magnitude to spare here).  A cache is split over workgroups, a split over
+// four waves that never wait for each other; a second kernel joins the splits.
+#include "gsv_attention.h"
+
+namespace gsv {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kKeys = 32;   // keys of a wave's step
+constexpr int kHeads = 32;  // query heads of a workgroup
+constexpr float kSlack = 8.f;
+
+struct CacheArgs {
+    const int *lengths;
+    int64_t k_scene, v_scene, k_pos_scene, keep_scene;
+    int splits, head_tiles;
+    float *part_o;   // (scenes, heads, splits, dim): sums of weights times values
+    float2 *part_ms; // (scenes, heads, splits): maximum (log2) and sum of weights
+};
+
+// 32 rows of a head on their way to one wave's LDS: 64 lanes, 16-byte chunks.
+template <typename T, int DP> struct WaveStaged {
+    static constexpr int kCh = Elem<T>::kChunk, kPerRow = DP / kCh, kN = kKeys * kPerRow / 64;
+    uint4 r[kN];
+    template <typename Live>
+    __device__ __forceinline__ void load(const T *base, int64_t stride, int dim, int lane, Live live) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int c = i * 64 + lane, row = c / kPerRow, col = (c % kPerRow) * kCh;
+            r[i] = make_uint4(0, 0, 0, 0);
+            if (col < dim && live(row))
+                r[i] = *reinterpret_cast<const uint4 *>(base + row * stride + col);
+        }
+    }
+    __device__ __forceinline__ void store(T *tile, int lane) const {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int c = i * 64 + lane, row = c / kPerRow, col = (c % kPerRow) * kCh;
+            *reinterpret_cast<uint4 *>(tile + row * (DP + Elem<T>::kPad) + col) = r[i];
+        }
+    }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, const CacheArgs c,
+                                                          T *__restrict__ out) {
+    constexpr int LD = DP + Elem<T>::kPad;
+    typedef typename Elem<T>::frag frag;
+    static_assert(2 * kKeys * LD * sizeof(T) >= kHeads * DP * sizeof(float), "sums reuse the tiles");
+    __shared__ __align__(16) T tiles[4][2 * kKeys * LD];
+    __shared__ __align__(16) float spos[4][3 * kKeys];
+    __shared__ float sm[4][kHeads], ss[4][kHeads];
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int group = a.heads / a.kv_heads;
+    int n = blockIdx.x;
+    const int hk = n % a.kv_heads;
+    n /= a.kv_heads;
+    const int ht = n % c.head_tiles;
+    n /= c.head_tiles;
+    const int split = n % c.splits, s = n / c.splits;
+    const int len = min(max(c.lengths[s], 0), a.k_tokens);
+    const int per = ((len + c.splits - 1) / c.splits + kKeys - 1) / kKeys * kKeys;
+    const int j_begin = min((int64_t)split * per, (int64_t)len), j_end = min(j_begin + per, len);
+    const int col = ht * kHeads + (lane & 31);  // query head within the group
+    const bool head = col < group;
+    const int h = hk * group + (head ? col : 0);
+
+    const bool far = a.slopes != nullptr, capped = a.cap > 0.f;
+    const float slope = slope_of(a, h);
+    const float unit = capped ? kLog2e : a.scale * kLog2e;
+    const float far_unit = capped ? slope : slope / a.scale;
+    const float in_cap = capped ? a.scale / a.cap : 0.f;
+    frag q[DP / 16];
+    load_column<T, DP>(q, static_cast<const T *>(a.q) + s * a.q_row + h * a.q_head, a.dim, head, lane);
+    float x = 0.f, y = 0.f, z = 0.f;
+    if (far) {
+        const float *p = a.q_pos + s * a.q_pos_row;
+        x = p[0], y = p[1], z = p[2];
+    }
+    const T *kbase = static_cast<const T *>(a.k) + s * c.k_scene + hk * a.k_head;
+    const T *vbase = static_cast<const T *>(a.v) + s * c.v_scene + hk * a.v_head;
+    T *sk = tiles[wave], *sv = sk + kKeys * LD;
+    auto keep_at = [&](int j) {
+        if (!a.keep) return true;
+        const int64_t at = s * c.keep_scene + j;
+        return a.keep_bytes == 1 ? static_cast<const uint8_t *>(a.keep)[at] != 0
+                                 : static_cast<const int *>(a.keep)[at] != 0;
+    };
+
+    f32x16 o[DP / 32] = {};
+    float m = -INFINITY, sum = 0.f;
+    WaveStaged<T, DP> gk, gv;
+    float gp[2] = {};
+    auto fetch = [&](int j0) {
+        auto live = [&](int r) { return j0 + r < j_end && keep_at(j0 + r); };
+        gk.load(kbase + (int64_t)j0 * a.k_row, a.k_row, a.dim, lane, live);
+        gv.load(vbase + (int64_t)j0 * a.v_row, a.v_row, a.dim, lane, live);
+        if (far)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int at = i * 64 + lane, r = at % kKeys, ax = at / kKeys;
+                gp[i] = ax < 3 && j0 + r < j_end
+                            ? a.k_pos[s * c.k_pos_scene + (int64_t)(j0 + r) * a.k_pos_row + ax] : 0.f;
+            }
+    };
+    int j0 = j_begin + wave * kKeys;
+    if (j0 < j_end) fetch(j0);
+    for (; j0 < j_end; j0 += 4 * kKeys) {
+        gk.store(sk, lane);
+        gv.store(sv, lane);
+        if (far) {
+            spos[wave][lane] = gp[0];
+            if (lane < kKeys) spos[wave][64 + lane] = gp[1];
+        }
+        // the tile is this wave's own: its LDS accesses complete in order, only the
+        // compiler has to keep them so
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const uint32_t live = (uint32_t)__ballot(lane < kKeys && j0 + lane < j_end &&
+                                                 keep_at(min(j0 + lane, j_end - 1)));
+        if (j0 + 4 * kKeys < j_end) fetch(j0 + 4 * kKeys);
+        f32x16 d = {}, w = {};
+        if (far) d = distances(spos[wave], kKeys, 0, lane, x, y, z);
+        if (far && !capped)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) w[r] = -far_unit * d[r];
+        const T *krow = sk + (lane & 31) * LD + 8 * (lane >> 5);
+#pragma unroll
+        for (int st = 0; st < DP / 16; ++st) w = mma(row_frag(krow + st * 16), q[st], w);
+        if (capped)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                w[r] = a.cap * tanh_of<T>(w[r] * in_cap);
+                if (far) w[r] = fmaf(-far_unit, d[r], w[r]);
+            }
+        if (live != 0xffffffffu) {
+            const uint32_t bits = live >> (4 * (lane >> 5));
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (!((bits >> (8 * (r >> 2) + (r & 3))) & 1)) w[r] = -INFINITY;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, w[r]);
+        top *= unit;
+        if (__any(top > m + kSlack)) {
+            const float next = fmaxf(m, fmaxf(top, other_half(top)));
+            const float by = next == -INFINITY ? 1.f : fast_exp2(m - next);
+            m = next;
+            sum *= by;
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b) o[b] *= by;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            w[r] = fast_exp2(fmaf(w[r], unit, -ref));
+            sum += w[r];
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const frag p = to_frag<T>(w, half);
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b)
+                o[b] = mma(tr_frag<LD>(sv + half * 16 * LD + b * 32, lane), p, o[b]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    sum += other_half(sum);
+    // the waves' sums, joined
+    if (lane < 32) sm[wave][lane] = m, ss[wave][lane] = sum;
+    float *so = reinterpret_cast<float *>(tiles[wave]);
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                so[(lane & 31) * DP + b * 32 + 8 * g + 4 * (lane >> 5) + e] = o[b][4 * g + e];
+    __syncthreads();
+    const int heads = min(group - ht * kHeads, kHeads);
+    for (int i = threadIdx.x; i < heads * DP; i += 256) {
+        const int r = i / DP, dd = i % DP;
+        float top = -INFINITY, total = 0.f, val = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w][r]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            // a wave without keys has the maximum -inf and the sum 0; NaN sums pass
+            const float by = sm[w][r] == -INFINITY ? 1.f : fast_exp2(sm[w][r] - top);
+            total = fmaf(by, ss[w][r], total);
+            val = fmaf(by, reinterpret_cast<const float *>(tiles[w])[i], val);
+        }
+        if (dd >= a.dim) continue;
+        const int hh = hk * group + ht * kHeads + r;
+        if (c.splits == 1) {
+            out[((int64_t)s * a.heads + hh) * a.dim + dd] = (T)(total == 0.f ? 0.f : val / total);
+        } else {
+            const int64_t at = ((int64_t)s * a.heads + hh) * c.splits + split;
+            c.part_o[at * a.dim + dd] = val;
+            if (dd == 0) c.part_ms[at] = make_float2(top, total);
+        }
+    }
+}
+
+// One wave a scene and head: its splits, joined in order.
+template <typename T>
+__global__ __launch_bounds__(64) void k_cached_join(const float *__restrict__ part_o,
+                                                    const float2 *__restrict__ part_ms, int splits,
+                                                    int dim, T *__restrict__ out) {
+    const int64_t row = blockIdx.x;
+    const float2 *ms = part_ms + row * splits;
+    float top = -INFINITY;
+    for (int p = threadIdx.x; p < splits; p += 64) top = fmaxf(top, ms[p].x);
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+    float total = 0.f, v0 = 0.f, v1 = 0.f;
+    const int d0 = threadIdx.x, d1 = threadIdx.x + 64;
+    for (int p = 0; p < splits; ++p) {
+        const float2 e = ms[p];
+        const float by = e.x == -INFINITY ? 1.f : fast_exp2(e.x - top);
+        total = fmaf(by, e.y, total);
+        const float *o = part_o + (row * splits + p) * dim;
+        if (d0 < dim) v0 = fmaf(by, o[d0], v0);
+        if (d1 < dim) v1 = fmaf(by, o[d1], v1);
+    }
+    const float by = total == 0.f ? 0.f : 1.f / total;
+    if (d0 < dim) out[row * dim + d0] = (T)(v0 * by);
+    if (d1 < dim) out[row * dim + d1] = (T)(v1 * by);
+}
+
+// Splits of a cache: enough workgroups for two rounds on 256 CUs, each with at least a step
+// for all its waves.
+int cache_splits(const AttnArgs &a, int head_tiles) {
+    const int64_t each = (int64_t)a.scenes * a.kv_heads * head_tiles;
+    const int64_t want = (1024 + each - 1) / each, most = (a.k_tokens + 4 * kKeys - 1) / (4 * kKeys);
+    return (int)imax64(1, imin64(want, most));
+}
+
+template <typename T>
+int launch_cached(const AttnArgs &a, const CacheArgs &c, void *out, hipStream_t st) {
+    const dim3 grid((unsigned)(a.scenes * a.kv_heads * c.head_tiles * c.splits)), block(256);
+    T *o = static_cast<T *>(out);
+    if (a.dim <= 32)
+        hipLaunchKernelGGL((k_attention_cached<T, 32>), grid, block, 0, st, a, c, o);
+    else if (a.dim <= 64)
+        hipLaunchKernelGGL((k_attention_cached<T, 64>), grid, block, 0, st, a, c, o);
+    else
+        hipLaunchKernelGGL((k_attention_cached<T, 128>), grid, block, 0, st, a, c, o);
+    if (c.splits > 1)
+        hipLaunchKernelGGL(k_cached_join<T>, dim3((unsigned)(a.scenes * a.heads)), dim3(64), 0, st,
+                           c.part_o, c.part_ms, c.splits, a.dim, o);
+    return check_launch();
+}
+
+int cached_plan(const gsv_attention *args, AttnArgs *a, int *head_tiles, int *splits) {
+    int lq, lk;
+    if (!args || args->causal || args->prefix || args->q_starts || args->k_starts ||
+        args->scenes < 0 || args->scenes != args->q_tokens)
+        return GSV_ERR_INVALID_ARGUMENT;
+    gsv_attention one = *args;
+    one.scenes = 1;  // rows are addressed by scene here, not packed
+    const int st = attention_args(&one, a, &lq, &lk);
+    if (st != GSV_OK) return st;
+    a->scenes = args->scenes;
+    const int64_t tiles = (a->heads / a->kv_heads + kHeads - 1) / kHeads;
+    if ((int64_t)a->scenes * a->kv_heads * tiles > (1 << 22) || (int64_t)a->scenes * a->heads > (1 << 24))
+        return GSV_ERR_SIZE_OVERFLOW;
+    *head_tiles = (int)tiles;
+    *splits = a->scenes ? cache_splits(*a, (int)tiles) : 1;
+    return GSV_OK;
+}
+
+size_t part_o_bytes(const AttnArgs &a, int splits) {
+    return sizeof(float) * a.scenes * a.heads * splits * a.dim;  // a multiple of 32 bytes
+}
+
+}  // namespace
+}  // namespace gsv
+
+using namespace gsv;
+
+extern "C" int gsv_attention_cached_workspace_bytes(const gsv_attention *args, size_t *bytes) {
+    AttnArgs a;
+    int tiles, splits;
+    if (!bytes) return GSV_ERR_INVALID_ARGUMENT;
+    const int st = cached_plan(args, &a, &tiles, &splits);
+    if (st != GSV_OK) return st;
+    *bytes = splits > 1 ? part_o_bytes(a, splits) + sizeof(float2) * a.scenes * a.heads * splits : 0;
+    return GSV_OK;
+}
+
+extern "C" int gsv_attention_cached(const gsv_attention *args, const int32_t *lengths,
+                                    int64_t k_scene, int64_t v_scene, int64_t k_pos_scene,
+                                    int64_t keep_scene, void *out, void *workspace,
+                                    size_t workspace_bytes, void *stream) {
+    AttnArgs a;
+    int tiles, splits;
+    size_t need;
+    int st = cached_plan(args, &a, &tiles, &splits);
+    if (st != GSV_OK) return st;
+    if (a.scenes == 0) return GSV_OK;
+    if ((st = gsv_attention_cached_workspace_bytes(args, &need)) != GSV_OK) return st;
+    if (need > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
+    const int64_t chunk = args->dtype == GSV_BF16 ? 8 : 4;
+    if (!lengths || !out || (need && !workspace) || k_scene % chunk || v_scene % chunk ||
+        reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16)
+        return GSV_ERR_INVALID_ARGUMENT;
+    float *po = static_cast<float *>(workspace);
+    const CacheArgs c{lengths, k_scene, v_scene, k_pos_scene, keep_scene, splits, tiles, po,
+                      reinterpret_cast<float2 *>(static_cast<char *>(workspace) + part_o_bytes(a, splits))};
+    hipStream_t s = as_stream(stream);
+    return args->dtype == GSV_BF16 ? launch_cached<bf16>(a, c, out, s) : launch_cached<float>(a, c, out, s);
+}

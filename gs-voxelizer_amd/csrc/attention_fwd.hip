@@ -1,0 +1,241 @@
+// attention_fwd.hip — attention inside packed scenes, forward.
+//
+//   t_ij = cap tanh(scale q_i.k_j / cap) - slope_h |p_i - p_j|   (cap, slope optional)
+//   o_i = sum_j softmax_j(t_ij) v_j     over the keys j that row i sees; 0 if it sees none
+//
+// A workgroup of four waves takes 128 query rows of one head; a wave 32 of them, one in
+// each lane pair (l, l + 32).  Keys pass through LDS in tiles, the scores are formed
+// transposed (K Q^T), so a row's running maximum and sum stay with its lanes.
+#include "gsv_attention.h"
+
+namespace gsv {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kRows = 128;  // query rows of a workgroup
+// The maximum follows the scores only when one exceeds it by 2^8: weights then stay
+// below 2^8, and a rescale of the sums (one multiply a register) is rare.
+constexpr float kSlack = 8.f;
+
+template <typename T> struct FwdTile { static constexpr int kKeys = sizeof(T) == 2 ? 64 : 32; };
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_attention_fwd(const AttnArgs a, T *__restrict__ out,
+                                                       float *__restrict__ lse) {
+    constexpr int KB = FwdTile<T>::kKeys, LD = DP + Elem<T>::kPad;
+    typedef typename Elem<T>::frag frag;
+    __shared__ __align__(16) T sk[2][KB * LD];
+    __shared__ __align__(16) T sv[2][KB * LD];
+    __shared__ __align__(16) float spos[2][3 * KB];
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // heads vary fastest: with eight (or a multiple) of them each XCD's L2 holds the keys
+    // of its own heads
+    const int h = blockIdx.x % a.heads, rest = blockIdx.x / a.heads;
+    const int s = rest % a.scenes, slot = rest / a.scenes;
+    const Scene c = scene_rows(a, s);
+    const int nq = c.q1 - c.q0, nk = c.k1 - c.k0;
+    const int tiles = (nq + kRows - 1) / kRows;
+    const int hk = h / (a.heads / a.kv_heads);
+    const T *kbase = static_cast<const T *>(a.k) + (int64_t)c.k0 * a.k_row + hk * a.k_head;
+    const T *vbase = static_cast<const T *>(a.v) + (int64_t)c.k0 * a.v_row + hk * a.v_head;
+    const bool far = a.slopes != nullptr, capped = a.cap > 0.f;
+    const float slope = slope_of(a, h);
+    // scores leave the matrix product in units of 1 / scale (or 1 where they are capped);
+    // unit turns them into powers of two
+    const float unit = capped ? kLog2e : a.scale * kLog2e;
+    const float far_unit = capped ? slope : slope / a.scale;
+    const float in_cap = capped ? a.scale / a.cap : 0.f;
+
+    for (int tile = slot; tile < tiles; tile += a.slots) {
+        // the last rows of a causal scene see the most keys: they start first
+        const int first = (tiles - 1 - tile) * kRows;
+        const int i = first + wave * 32 + (lane & 31);
+        const bool row = i < nq;
+        const int64_t qi = c.q0 + i;
+        frag q[DP / 16];
+        load_column<T, DP>(q, static_cast<const T *>(a.q) + qi * a.q_row + h * a.q_head, a.dim, row,
+                           lane);
+        float x = 0.f, y = 0.f, z = 0.f;
+        if (far && row) {
+            const float *p = a.q_pos + qi * a.q_pos_row;
+            x = p[0], y = p[1], z = p[2];
+        }
+        const int limit = row ? key_limit(a, c, i) : 0;
+        const int all = first + wave * 32 + 31 < nq ? key_limit(a, c, first + wave * 32) : 0;
+        const int most = key_limit(a, c, min(first + kRows, nq) - 1);  // of the workgroup
+        const int mine = first + wave * 32 < nq
+                             ? key_limit(a, c, min(first + wave * 32 + 32, nq) - 1) : 0;
+        f32x16 o[DP / 32] = {};
+        float m = -INFINITY, sum = 0.f;
+
+        Staged<T, DP, KB> gk, gv;
+        float gp = 0.f;
+        auto fetch = [&](int j0) {
+            auto live = [&](int r) { return j0 + r < most && kept(a, c.k0 + j0 + r); };
+            gk.load(kbase + j0 * a.k_row, a.k_row, a.dim, live);
+            gv.load(vbase + j0 * a.v_row, a.v_row, a.dim, live);
+            if (far && threadIdx.x < 3 * KB) {
+                const int r = threadIdx.x % KB, ax = threadIdx.x / KB;
+                gp = j0 + r < most ? a.k_pos[(int64_t)(c.k0 + j0 + r) * a.k_pos_row + ax] : 0.f;
+            }
+        };
+        auto put = [&](int b) {
+            gk.store(sk[b]);
+            gv.store(sv[b]);
+            if (far && threadIdx.x < 3 * KB) spos[b][threadIdx.x] = gp;
+        };
+        __syncthreads();  // the previous tile's last reads
+        if (most > 0) {
+            fetch(0);
+            put(0);
+        }
+        __syncthreads();
+        int b = 0;
+        for (int j0 = 0; j0 < most; j0 += KB, b ^= 1) {
+            const bool more = j0 + KB < most;
+            if (more) fetch(j0 + KB);
+            if (j0 < mine) {
+                // keys of the tile that are inside and kept, a bit each
+                uint64_t live = ~0ull;
+                if (a.keep || j0 + KB > all)
+                    live = __ballot(j0 + lane < nk && lane < KB && kept(a, c.k0 + min(j0 + lane, nk - 1)));
+                const bool masked = j0 + KB > all || (KB == 64 ? ~live : (~live & 0xffffffffull)) != 0;
+                f32x16 t[KB / 32];
+                float top = -INFINITY;
+#pragma unroll
+                for (int kb = 0; kb < KB / 32; ++kb) {
+                    f32x16 d = {};
+                    if (far) d = distances(spos[b], KB, kb * 32, lane, x, y, z);
+                    f32x16 w = {};
+                    if (far && !capped)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) w[r] = -far_unit * d[r];
+                    const T *krow = sk[b] + (kb * 32 + (lane & 31)) * LD + 8 * (lane >> 5);
+#pragma unroll
+                    for (int st = 0; st < DP / 16; ++st) w = mma(row_frag(krow + st * 16), q[st], w);
+                    if (capped)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            w[r] = a.cap * tanh_of<T>(w[r] * in_cap);
+                            if (far) w[r] = fmaf(-far_unit, d[r], w[r]);
+                        }
+                    if (masked) {
+                        const uint32_t bits = (uint32_t)(live >> (kb * 32)) >> (4 * (lane >> 5));
+                        const int lim = limit - j0 - kb * 32 - 4 * (lane >> 5);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int at = 8 * (r >> 2) + (r & 3);
+                            if (at >= lim || !((bits >> at) & 1)) w[r] = -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) top = fmaxf(top, w[r]);
+                    t[kb] = w;
+                }
+                top *= unit;
+                if (__any(top > m + kSlack)) {
+                    const float next = fmaxf(m, fmaxf(top, other_half(top)));
+                    const float by = next == -INFINITY ? 1.f : fast_exp2(m - next);
+                    m = next;
+                    sum *= by;
+#pragma unroll
+                    for (int n = 0; n < DP / 32; ++n) o[n] *= by;
+                }
+                const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int kb = 0; kb < KB / 32; ++kb) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        t[kb][r] = fast_exp2(fmaf(t[kb][r], unit, -ref));
+                        sum += t[kb][r];
+                    }
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const frag p = to_frag<T>(t[kb], half);
+#pragma unroll
+                        for (int n = 0; n < DP / 32; ++n)
+                            o[n] = mma(tr_frag<LD>(sv[b] + (kb * 32 + half * 16) * LD + n * 32, lane),
+                                       p, o[n]);
+                    }
+                }
+            }
+            if (more) put(b ^ 1);
+            __syncthreads();
+        }
+        sum += other_half(sum);
+        if (row) {
+            store_column<T, DP>(out + (qi * a.heads + h) * a.dim, o, sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum),
+                                a.dim, lane);
+            // log2 of the row's sum of exponentials; +inf for an empty row, whose weights
+            // in the backward are exp2(-inf)
+            if (lse && lane < 32)
+                lse[(int64_t)h * a.q_tokens + qi] = sum == 0.f ? INFINITY : m + log2f(sum);
+        }
+    }
+}
+
+template <typename T> int launch_fwd(const AttnArgs &a, void *out, float *lse, hipStream_t st) {
+    const dim3 grid((unsigned)a.slots * a.scenes * a.heads), block(256);
+    T *o = static_cast<T *>(out);
+    if (a.dim <= 32)
+        hipLaunchKernelGGL((k_attention_fwd<T, 32>), grid, block, 0, st, a, o, lse);
+    else if (a.dim <= 64)
+        hipLaunchKernelGGL((k_attention_fwd<T, 64>), grid, block, 0, st, a, o, lse);
+    else
+        hipLaunchKernelGGL((k_attention_fwd<T, 128>), grid, block, 0, st, a, o, lse);
+    return check_launch();
+}
+
+}  // namespace
+
+int attention_args(const gsv_attention *in, AttnArgs *a, int *longest_q, int *longest_k) {
+    if (!in) return GSV_ERR_INVALID_ARGUMENT;
+    const gsv_attention &g = *in;
+    if (g.dtype != GSV_F32 && g.dtype != GSV_BF16) return GSV_ERR_INVALID_ARGUMENT;
+    if (g.q_tokens < 0 || g.k_tokens < 0 || g.heads < 1 || g.kv_heads < 1 ||
+        g.heads % g.kv_heads || g.dim < 8 || g.dim > 128 || g.dim % 8 || g.scenes < 1)
+        return GSV_ERR_INVALID_ARGUMENT;
+    const int64_t chunk = g.dtype == GSV_BF16 ? 8 : 4;
+    const int64_t strides[] = {g.q_row, g.q_head, g.k_row, g.k_head, g.v_row, g.v_head};
+    for (int64_t x : strides)
+        if (x % chunk) return GSV_ERR_INVALID_ARGUMENT;
+    const void *ptrs[] = {g.q, g.k, g.v};
+    for (const void *p : ptrs)
+        if (reinterpret_cast<uintptr_t>(p) % 16) return GSV_ERR_INVALID_ARGUMENT;
+    if ((g.q_tokens > 0 && !g.q) || (g.k_tokens > 0 && (!g.k || !g.v)))
+        return GSV_ERR_INVALID_ARGUMENT;
+    if (g.scenes > 1 && (!g.q_starts || !g.k_starts)) return GSV_ERR_INVALID_ARGUMENT;
+    if (!(g.scale > 0.f) || !(g.cap >= 0.f)) return GSV_ERR_INVALID_ARGUMENT;
+    if (g.slopes && ((!g.q_positions && g.q_tokens > 0) || (!g.k_positions && g.k_tokens > 0) ||
+                     (g.slopes_dtype != GSV_F32 && g.slopes_dtype != GSV_BF16)))
+        return GSV_ERR_INVALID_ARGUMENT;
+    if (g.keep && g.keep_bytes != 1 && g.keep_bytes != 4) return GSV_ERR_INVALID_ARGUMENT;
+    *a = AttnArgs{g.q, g.k, g.v, g.q_row, g.q_head, g.k_row, g.k_head, g.v_row, g.v_head,
+                  g.q_tokens, g.k_tokens, g.heads, g.kv_heads, g.dim, g.scenes, g.q_starts,
+                  g.k_starts, g.prefix, g.causal, g.scale, g.cap, g.q_positions, g.k_positions,
+                  g.q_pos_row, g.k_pos_row, g.slopes, g.slopes_dtype == GSV_F32, g.keep,
+                  g.keep_bytes, 1};
+    const auto longest = [](int hint, int tokens) {
+        return hint < 1 || hint > tokens ? (tokens > 1 ? tokens : 1) : hint;
+    };
+    *longest_q = longest(g.longest_q, g.q_tokens);
+    *longest_k = longest(g.longest_k, g.k_tokens);
+    return GSV_OK;
+}
+
+}  // namespace gsv
+
+using namespace gsv;
+
+extern "C" int gsv_attention_fwd(const gsv_attention *args, void *out, float *lse, void *stream) {
+    AttnArgs a;
+    int lq, lk;
+    const int st = attention_args(args, &a, &lq, &lk);
+    if (st != GSV_OK) return st;
+    if (a.q_tokens == 0) return GSV_OK;
+    if (!out || reinterpret_cast<uintptr_t>(out) % 16) return GSV_ERR_INVALID_ARGUMENT;
+    if (!attention_slots(&a, lq, kRows, a.heads)) return GSV_ERR_SIZE_OVERFLOW;
+    hipStream_t s = as_stream(stream);
+    return args->dtype == GSV_BF16 ? launch_fwd<bf16>(a, out, lse, s) : launch_fwd<float>(a, out, lse, s);
+}

@@ -1,0 +1,455 @@
+// gated_norm.hip — the norms around a block, fused with its gate and residual scale.
+//
+//   n = branch rstd(branch) branch_weight   (or branch)
+//   y = x + gate scale n                    h = y rstd(y) weight
+// with rstd(v) = 1 / sqrt(mean(v^2) + eps).  Bytes bound both directions: a row passes
+// through registers once, in float32 throughout.  The backward forms y again from x and
+// branch rather than reading it (the same bytes, and nothing rounded between), and
+// sums two things over rows, from which every parameter's gradient follows:
+//   A[c] = sum dy' branch_hat,  B[c] = sum dh y_hat    (dy': the whole gradient at y)
+//   dgate = scale branch_weight A (a scene's), dscale = sum_s gate branch_weight A,
+//   dbranch_weight = sum_s gate scale A, dweight = B
+// first over each workgroup's rows of one scene, then over workgroups, in a fixed order.
+#include "gsv_device.h"
+
+namespace gsv {
+namespace {
+
+typedef __bf16 bf16;
+
+struct NormArgs {
+    const void *x, *branch, *gate;
+    const float *weight, *branch_weight, *scale;
+    const int *starts;
+    int64_t x_row, branch_row, gate_row;
+    int tokens, channels, scenes, per_token, f32_gate;
+    float eps;
+    // forward
+    void *y, *h;
+    // backward
+    const void *dy, *dh;
+    int64_t dy_row, dh_row;
+    void *dx, *dbranch, *dgate;
+    float *part_a, *part_b;  // (scenes, slots, channels)
+    int slots, rows;         // workgroups a scene, rows of a workgroup
+};
+
+template <typename T, int N> struct __align__(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) Pack {
+    T v[N];
+};
+
+// One row's channels of a lane: item i covers VEC channels from (i * LANES + lane) * VEC.
+template <int VEC, int E, int LANES> struct Lane {
+    static constexpr int kItems = E / VEC;
+    template <typename T>
+    static __device__ __forceinline__ void load(float (&f)[E], const T *row, int lane, int channels,
+                                                float other = 0.f) {
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const int c = (i * LANES + lane) * VEC;
+            Pack<T, VEC> p;
+            if (c < channels) p = *reinterpret_cast<const Pack<T, VEC> *>(row + c);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) f[i * VEC + e] = c < channels ? (float)p.v[e] : other;
+        }
+    }
+    template <typename T>
+    static __device__ __forceinline__ void store(const float (&f)[E], T *row, int lane, int channels) {
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const int c = (i * LANES + lane) * VEC;
+            Pack<T, VEC> p;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) p.v[e] = (T)f[i * VEC + e];
+            if (c < channels) *reinterpret_cast<Pack<T, VEC> *>(row + c) = p;
+        }
+    }
+};
+
+// The sum over a row's lanes: one wave, or four of them through LDS.
+template <int WAVES> __device__ __forceinline__ float row_sum(float v, float *lds) {
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) v += __shfl_xor(v, k);
+    if constexpr (WAVES > 1) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) v += lds[w];
+    }
+    return v;
+}
+
+__device__ __forceinline__ int start_of(const NormArgs &a, int s) {
+    if (s <= 0) return 0;
+    if (s >= a.scenes) return a.tokens;
+    return min(max(a.starts[s], 0), a.tokens);
+}
+
+// The scene of a row: how many scenes after the first start at or before it.
+__device__ __forceinline__ int scene_of(const NormArgs &a, int row) {
+    int n = 0;
+    for (int s = 1 + (threadIdx.x & 63); s - (int)(threadIdx.x & 63) < a.scenes; s += 64)
+        n += __popcll(__ballot(s < a.scenes && a.starts[min(s, a.scenes)] <= row));
+    return n;
+}
+
+template <typename TF, typename L, int E>
+__device__ __forceinline__ void load_gate(const NormArgs &a, float (&f)[E], int64_t row, int lane) {
+    if (a.f32_gate)
+        L::load(f, static_cast<const float *>(a.gate) + row * a.gate_row, lane, a.channels);
+    else
+        L::load(f, static_cast<const TF *>(a.gate) + row * a.gate_row, lane, a.channels);
+}
+
+template <typename TX, typename TF, int VEC, int E, int WAVES>
+__global__ __launch_bounds__(256) void k_norm_fwd(const NormArgs a) {
+    typedef Lane<VEC, E, 64 * WAVES> L;
+    __shared__ float lds[4];
+    const int lane = threadIdx.x % (64 * WAVES);
+    constexpr int kPer = 4 / WAVES;  // rows of a workgroup at a time
+    const float inv = 1.f / a.channels;
+    float w[E];
+    L::load(w, a.weight, lane, a.channels);
+    const int stride = gridDim.x * kPer;
+    for (int row = blockIdx.x * kPer + (threadIdx.x >> 6) / WAVES; row < a.tokens; row += stride) {
+        float x[E], f[E];
+        L::load(f, static_cast<const TF *>(a.branch) + row * a.branch_row, lane, a.channels);
+        L::load(x, static_cast<const TX *>(a.x) + row * a.x_row, lane, a.channels);
+        float by[E];
+        if (a.gate) {
+            load_gate<TF, L>(a, by, a.per_token ? row : a.scenes > 1 ? scene_of(a, row) : 0, lane);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) by[e] = 1.f;
+        }
+        if (a.scale) {
+            float t[E];
+            L::load(t, a.scale, lane, a.channels);
+#pragma unroll
+            for (int e = 0; e < E; ++e) by[e] *= t[e];
+        }
+        if (a.branch_weight) {
+            float t[E], sq = 0.f;
+            L::load(t, a.branch_weight, lane, a.channels);
+#pragma unroll
+            for (int e = 0; e < E; ++e) sq = fmaf(f[e], f[e], sq);
+            const float r = rsqrtf(row_sum<WAVES>(sq, lds) * inv + a.eps);
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[e] *= r * t[e];
+        }
+        float sq = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = fmaf(by[e], f[e], x[e]), sq = fmaf(x[e], x[e], sq);
+        const float r = rsqrtf(row_sum<WAVES>(sq, lds) * inv + a.eps);
+        L::store(x, static_cast<TX *>(a.y) + (int64_t)row * a.channels, lane, a.channels);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] *= r * w[e];
+        L::store(x, static_cast<TF *>(a.h) + (int64_t)row * a.channels, lane, a.channels);
+    }
+}
+
+template <typename TX, typename TF, int VEC, int E, int WAVES>
+__global__ __launch_bounds__(256) void k_norm_bwd(const NormArgs a) {
+    typedef Lane<VEC, E, 64 * WAVES> L;
+    __shared__ float lds[4];
+    __shared__ float sums[WAVES == 1 ? 3 * 64 * E : 1];
+    const int lane = threadIdx.x % (64 * WAVES), wave = threadIdx.x >> 6;
+    constexpr int kPer = 4 / WAVES;
+    const float inv = 1.f / a.channels;
+    const int s = blockIdx.x / a.slots, slot = blockIdx.x % a.slots;
+    const int r0 = start_of(a, s), r1 = max(start_of(a, s + 1), r0);
+    float wgt[E], gs[E], bw[E], sum_a[E], sum_b[E];
+    L::load(wgt, a.weight, lane, a.channels);
+#pragma unroll
+    for (int e = 0; e < E; ++e) gs[e] = bw[e] = 1.f, sum_a[e] = sum_b[e] = 0.f;
+    if (a.branch_weight) L::load(bw, a.branch_weight, lane, a.channels);
+    if (a.scale) L::load(gs, a.scale, lane, a.channels);
+    if (a.gate && !a.per_token) {
+        float g[E];
+        load_gate<TF, L>(a, g, s, lane);
+#pragma unroll
+        for (int e = 0; e < E; ++e) gs[e] *= g[e];
+    }
+    for (int64_t base = r0 + (int64_t)slot * a.rows; base < r1; base += (int64_t)a.slots * a.rows)
+        for (int64_t row = base + wave / WAVES; row < min(base + a.rows, (int64_t)r1); row += kPer) {
+            float x[E], f[E], dy[E], dh[E], g[E];
+            L::load(f, static_cast<const TF *>(a.branch) + row * a.branch_row, lane, a.channels);
+            L::load(x, static_cast<const TX *>(a.x) + row * a.x_row, lane, a.channels);
+#pragma unroll
+            for (int e = 0; e < E; ++e) dy[e] = dh[e] = 0.f;
+            if (a.dh) L::load(dh, static_cast<const TF *>(a.dh) + row * a.dh_row, lane, a.channels);
+            if (a.dy) L::load(dy, static_cast<const TX *>(a.dy) + row * a.dy_row, lane, a.channels);
+            if (a.per_token) load_gate<TF, L>(a, g, row, lane);
+            float rb = 1.f;
+            if (a.branch_weight) {
+                float sq = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) sq = fmaf(f[e], f[e], sq);
+                rb = rsqrtf(row_sum<WAVES>(sq, lds) * inv + a.eps);
+            }
+            float sq = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                f[e] *= rb;  // branch_hat
+                const float by = a.per_token ? gs[e] * g[e] : gs[e];
+                x[e] = fmaf(by * bw[e], f[e], x[e]);
+                sq = fmaf(x[e], x[e], sq);
+            }
+            const float ry = rsqrtf(row_sum<WAVES>(sq, lds) * inv + a.eps);
+            float m1 = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                x[e] *= ry;  // y_hat
+                sum_b[e] = fmaf(dh[e], x[e], sum_b[e]);
+                dh[e] *= wgt[e];
+                m1 = fmaf(dh[e], x[e], m1);
+            }
+            m1 = row_sum<WAVES>(m1, lds) * inv;
+            float m2 = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                dy[e] = fmaf(ry, dh[e] - x[e] * m1, dy[e]);
+                const float by = a.per_token ? gs[e] * g[e] : gs[e];
+                const float t = dy[e] * f[e];  // of A
+                sum_a[e] += a.per_token ? t * g[e] : t;
+                if (a.per_token) g[e] = t * gs[e] * bw[e];
+                x[e] = dy[e] * by * bw[e];
+                m2 = fmaf(x[e], f[e], m2);
+            }
+            L::store(dy, static_cast<TX *>(a.dx) + row * a.channels, lane, a.channels);
+            if (a.per_token) {
+                if (a.f32_gate) L::store(g, static_cast<float *>(a.dgate) + row * a.channels, lane, a.channels);
+                else L::store(g, static_cast<TF *>(a.dgate) + row * a.channels, lane, a.channels);
+            }
+            if (a.branch_weight) {
+                m2 = row_sum<WAVES>(m2, lds) * inv;
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = rb * (x[e] - f[e] * m2);
+            }
+            L::store(x, static_cast<TF *>(a.dbranch) + row * a.channels, lane, a.channels);
+        }
+    // the workgroup's sums
+    if constexpr (WAVES == 1) {
+#pragma unroll
+        for (int turn = 0; turn < 2; ++turn) {
+            float(&v)[E] = turn ? sum_b : sum_a;
+            __syncthreads();
+            if (wave)
+#pragma unroll
+                for (int e = 0; e < E; ++e) sums[((wave - 1) * E + e) * 64 + lane] = v[e];
+            __syncthreads();
+            if (!wave)
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    v[e] += sums[e * 64 + lane] + sums[(E + e) * 64 + lane] + sums[(2 * E + e) * 64 + lane];
+        }
+        if (wave) return;
+    }
+    L::store(sum_a, a.part_a + (int64_t)blockIdx.x * a.channels, lane, a.channels);
+    L::store(sum_b, a.part_b + (int64_t)blockIdx.x * a.channels, lane, a.channels);
+}
+
+constexpr int kCols = 16, kGroups = 16;  // columns and row groups of a summing workgroup
+
+// Each scene's sums over its workgroups, into the first of them; a scene's gate gradient.
+__global__ __launch_bounds__(256) void k_norm_scene_sums(const NormArgs a, int f32_gate) {
+    __shared__ float la[kGroups][kCols], lb[kGroups][kCols];
+    const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+    const int c = blockIdx.x * kCols + col, s = blockIdx.y;
+    float sa = 0.f, sb = 0.f;
+    if (c < a.channels)
+        for (int p = grp; p < a.slots; p += kGroups) {
+            const int64_t at = ((int64_t)s * a.slots + p) * a.channels + c;
+            sa += a.part_a[at], sb += a.part_b[at];
+        }
+    la[grp][col] = sa, lb[grp][col] = sb;
+    __syncthreads();
+    if (grp || c >= a.channels) return;
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g) sa += la[g][col], sb += lb[g][col];
+    // no other workgroup reads these columns of this scene
+    const int64_t at = (int64_t)s * a.slots * a.channels + c;
+    a.part_a[at] = sa, a.part_b[at] = sb;
+    if (a.dgate && !a.per_token) {
+        const float g = sa * (a.scale ? a.scale[c] : 1.f) * (a.branch_weight ? a.branch_weight[c] : 1.f);
+        if (f32_gate) static_cast<float *>(a.dgate)[(int64_t)s * a.channels + c] = g;
+        else static_cast<bf16 *>(a.dgate)[(int64_t)s * a.channels + c] = (bf16)g;
+    }
+}
+
+// The parameters' gradients from the scenes' sums.
+__global__ __launch_bounds__(256) void k_norm_sums(const NormArgs a, float *dweight,
+                                                   float *dbranch_weight, float *dscale) {
+    __shared__ float la[kGroups][kCols], lb[kGroups][kCols];
+    const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+    const int c = blockIdx.x * kCols + col;
+    float sa = 0.f, sb = 0.f;
+    if (c < a.channels)
+        for (int s = grp; s < a.scenes; s += kGroups) {
+            const int64_t at = (int64_t)s * a.slots * a.channels + c;
+            float g = 1.f;
+            if (a.gate && !a.per_token)
+                g = a.f32_gate ? static_cast<const float *>(a.gate)[s * a.gate_row + c]
+                               : (float)static_cast<const bf16 *>(a.gate)[s * a.gate_row + c];
+            sa = fmaf(a.part_a[at], g, sa), sb += a.part_b[at];
+        }
+    la[grp][col] = sa, lb[grp][col] = sb;
+    __syncthreads();
+    if (grp || c >= a.channels) return;
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g) sa += la[g][col], sb += lb[g][col];
+    dweight[c] = sb;
+    if (dscale) dscale[c] = sa * (a.branch_weight ? a.branch_weight[c] : 1.f);
+    if (dbranch_weight) dbranch_weight[c] = sa * (a.scale ? a.scale[c] : 1.f);
+}
+
+template <typename TX, typename TF, int VEC, int E, int WAVES>
+void launch_one(const NormArgs &a, bool backward, hipStream_t s) {
+    if (backward) {
+        hipLaunchKernelGGL((k_norm_bwd<TX, TF, VEC, E, WAVES>), dim3((unsigned)(a.scenes * a.slots)),
+                           dim3(256), 0, s, a);
+    } else {
+        // 16 waves a SIMD's worth of rows at most; a wave keeps the weights over its rows
+        const int64_t want = ((int64_t)a.tokens * WAVES + 3) / 4;
+        hipLaunchKernelGGL((k_norm_fwd<TX, TF, VEC, E, WAVES>), dim3((unsigned)imin64(want, 8192)),
+                           dim3(256), 0, s, a);
+    }
+}
+template <typename TX, typename TF, int VEC>
+void launch_width(const NormArgs &a, bool backward, hipStream_t s) {
+    // channels of a lane: a row of a wave up to 2048 channels, of four waves up to 8192
+    if (a.channels <= 512) launch_one<TX, TF, VEC, 8, 1>(a, backward, s);
+    else if (a.channels <= 1024) launch_one<TX, TF, VEC, 16, 1>(a, backward, s);
+    else if (a.channels <= 2048) launch_one<TX, TF, VEC, 32, 1>(a, backward, s);
+    else launch_one<TX, TF, VEC, 32, 4>(a, backward, s);
+}
+template <typename TX, typename TF> void launch_types(const NormArgs &a, int vec, bool backward, hipStream_t s) {
+    if (vec == 8) launch_width<TX, TF, 8>(a, backward, s);
+    else if (vec == 4) launch_width<TX, TF, 4>(a, backward, s);
+    else launch_width<TX, TF, 1>(a, backward, s);
+}
+void launch(const gsv_norm *n, const NormArgs &a, int vec, bool backward, hipStream_t s) {
+    if (n->branch_dtype == GSV_F32) launch_types<float, float>(a, vec, backward, s);
+    else if (n->dtype == GSV_F32) launch_types<float, bf16>(a, vec, backward, s);
+    else launch_types<bf16, bf16>(a, vec, backward, s);
+}
+
+int norm_args(const gsv_norm *n, NormArgs *a) {
+    if (!n) return GSV_ERR_INVALID_ARGUMENT;
+    const auto type = [](int t) { return t == GSV_F32 || t == GSV_BF16; };
+    if (!type(n->dtype) || !type(n->branch_dtype) || n->dtype > n->branch_dtype) return GSV_ERR_INVALID_ARGUMENT;
+    if (n->tokens < 0 || n->channels < 1 || n->channels > 8192 || n->scenes < 1 || !(n->eps >= 0.f))
+        return GSV_ERR_INVALID_ARGUMENT;
+    if (n->scenes > 1 && !n->starts) return GSV_ERR_INVALID_ARGUMENT;
+    if (n->gate && (!type(n->gate_dtype) || (n->gate_dtype == GSV_BF16 && n->branch_dtype == GSV_F32)))
+        return GSV_ERR_INVALID_ARGUMENT;
+    if (n->gate && n->gate_per_token && n->scenes != 1) return GSV_ERR_INVALID_ARGUMENT;
+    if (n->tokens > 0 && (!n->x || !n->branch || !n->weight)) return GSV_ERR_INVALID_ARGUMENT;
+    *a = NormArgs{};
+    a->x = n->x, a->branch = n->branch, a->gate = n->gate, a->weight = n->weight;
+    a->branch_weight = n->branch_weight, a->scale = n->scale, a->starts = n->starts;
+    a->x_row = n->x_row, a->branch_row = n->branch_row, a->gate_row = n->gate_row;
+    a->tokens = n->tokens, a->channels = n->channels, a->scenes = n->scenes;
+    a->per_token = n->gate && n->gate_per_token, a->f32_gate = n->gate_dtype == GSV_F32;
+    a->eps = n->eps;
+    return GSV_OK;
+}
+
+// Channels of one access: 8, or 4, where every row and vector starts aligned for it (16 bytes,
+// or what 4 or 8 channels take where that is less).
+int norm_vec(const gsv_norm *n, const void *const *ptrs, const int *f32, const int64_t *rows, int count) {
+    for (int vec : {8, 4}) {
+        bool ok = n->channels % vec == 0;
+        for (int i = 0; i < count && ok; ++i) {
+            const int size = f32[i] ? 4 : 2, need = vec * size > 16 ? 16 : vec * size;
+            ok = reinterpret_cast<uintptr_t>(ptrs[i]) % need == 0 && (rows[i] * size) % need == 0;
+        }
+        if (ok) return vec;
+    }
+    return 1;
+}
+
+// Rows and workgroups of the backward: about 1024 workgroups, at least 16 rows each.
+bool norm_slots(const gsv_norm *n, NormArgs *a) {
+    const int64_t longest = n->longest > 0 && n->longest < n->tokens ? n->longest : imax64(n->tokens, 1);
+    a->rows = (int)imax64(16, (n->tokens + 1023) / 1024);
+    a->slots = (int)((longest + a->rows - 1) / a->rows);
+    if (a->scenes > (1 << 22)) return false;
+    a->slots = (int)imin64(a->slots, imax64(1, 16384 / a->scenes));
+    return true;
+}
+
+}  // namespace
+}  // namespace gsv
+
+using namespace gsv;
+
+extern "C" int gsv_gated_norm_fwd(const gsv_norm *n, void *y, void *h, void *stream) {
+    NormArgs a;
+    const int st = norm_args(n, &a);
+    if (st != GSV_OK) return st;
+    if (a.tokens == 0) return GSV_OK;
+    if (!y || !h) return GSV_ERR_INVALID_ARGUMENT;
+    a.y = y, a.h = h;
+    const int xf = n->dtype == GSV_F32, bf = n->branch_dtype == GSV_F32;
+    const void *ptrs[] = {n->x, n->branch, n->gate, n->weight, n->branch_weight, n->scale, y, h};
+    const int f32[] = {xf, bf, a.f32_gate, 1, 1, 1, xf, bf};
+    const int64_t rows[] = {n->x_row, n->branch_row, n->gate ? n->gate_row : 0, 0, 0, 0, n->channels, n->channels};
+    launch(n, a, norm_vec(n, ptrs, f32, rows, 8), false, as_stream(stream));
+    return check_launch();
+}
+
+extern "C" int gsv_gated_norm_bwd_workspace_bytes(const gsv_norm *n, size_t *bytes) {
+    NormArgs a;
+    if (!bytes) return GSV_ERR_INVALID_ARGUMENT;
+    const int st = norm_args(n, &a);
+    if (st != GSV_OK) return st;
+    if (!norm_slots(n, &a)) return GSV_ERR_SIZE_OVERFLOW;
+    const size_t one = ((size_t)a.scenes * a.slots * a.channels * sizeof(float) + 255) / 256 * 256;
+    *bytes = 2 * one;
+    return GSV_OK;
+}
+
+extern "C" int gsv_gated_norm_bwd(const gsv_norm *n, const void *dy, int64_t dy_row, const void *dh,
+                                  int64_t dh_row, void *dx, void *dbranch, float *dweight,
+                                  float *dbranch_weight, float *dscale, void *dgate,
+                                  void *workspace, size_t workspace_bytes, void *stream) {
+    NormArgs a;
+    int st = norm_args(n, &a);
+    if (st != GSV_OK) return st;
+    if (!norm_slots(n, &a)) return GSV_ERR_SIZE_OVERFLOW;
+    size_t need;
+    if ((st = gsv_gated_norm_bwd_workspace_bytes(n, &need)) != GSV_OK) return st;
+    if (need > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
+    if (!dweight || !workspace || (a.tokens > 0 && (!dx || !dbranch)) || (a.gate && !dgate) ||
+        (a.branch_weight && !dbranch_weight) || (a.scale && !dscale) ||
+        reinterpret_cast<uintptr_t>(workspace) % 256)
+        return GSV_ERR_INVALID_ARGUMENT;
+    a.dy = dy, a.dh = dh, a.dy_row = dy_row, a.dh_row = dh_row;
+    a.dx = dx, a.dbranch = dbranch, a.dgate = a.gate ? dgate : nullptr;
+    a.part_a = static_cast<float *>(workspace);
+    a.part_b = reinterpret_cast<float *>(static_cast<char *>(workspace) + need / 2);
+    const int xf = n->dtype == GSV_F32, bf = n->branch_dtype == GSV_F32;
+    const int64_t C = n->channels;
+    const void *ptrs[] = {n->x, n->branch, n->gate, n->weight, n->branch_weight, n->scale, dy, dh, dx, dbranch,
+                          a.per_token ? dgate : nullptr};
+    const int f32[] = {xf, bf, a.f32_gate, 1, 1, 1, xf, bf, xf, bf, a.f32_gate};
+    const int64_t rows[] = {n->x_row, n->branch_row, n->gate ? n->gate_row : 0, 0, 0, 0, dy ? dy_row : 0,
+                            dh ? dh_row : 0, C, C, C};
+    hipStream_t s = as_stream(stream);
+    launch(n, a, norm_vec(n, ptrs, f32, rows, 11), true, s);
+    const dim3 cols((unsigned)((C + kCols - 1) / kCols), 1);
+    // scenes are the y axis of the grid, 65535 at most: the rest in further launches
+    for (int s0 = 0; s0 < a.scenes; s0 += 65535) {
+        NormArgs part = a;
+        part.part_a += (int64_t)s0 * a.slots * C, part.part_b += (int64_t)s0 * a.slots * C;
+        if (a.dgate && !a.per_token)
+            part.dgate = static_cast<char *>(a.dgate) + (int64_t)s0 * C * (a.f32_gate ? 4 : 2);
+        hipLaunchKernelGGL(k_norm_scene_sums, dim3(cols.x, (unsigned)imin64(a.scenes - s0, 65535)),
+                           dim3(256), 0, s, part, a.f32_gate);
+    }
+    hipLaunchKernelGGL(k_norm_sums, cols, dim3(256), 0, s, a, dweight, dbranch_weight, dscale);
+    return check_launch();
+}

@@ -14,6 +14,30 @@ _c_int, _c_i64, _c_float, _c_void_p, _c_size_t = (ctypes.c_int32, ctypes.c_int64
                                                    ctypes.c_void_p, ctypes.c_size_t)
 _P = _c_void_p
 
+
+def _struct(name, fields):
+    """A C structure of include/gsvox.h: (type, "names in order") runs."""
+    return type(name, (ctypes.Structure,), {
+        "_fields_": [(n, t) for t, names in fields for n in names.split()]})
+
+
+Attention = _struct("Attention", (
+    (_P, "q k v"), (_c_i64, "q_row q_head k_row k_head v_row v_head"),
+    (_P, "q_starts k_starts prefix q_positions k_positions"), (_c_i64, "q_pos_row k_pos_row"),
+    (_P, "slopes keep"), (_c_int, "dtype slopes_dtype keep_bytes causal q_tokens k_tokens heads "
+                                  "kv_heads dim scenes longest_q longest_k"),
+    (_c_float, "scale cap")))
+Rotary = _struct("Rotary", (
+    (_P, "q k"), (_c_i64, "q_row q_head k_row k_head"), (_P, "positions frequencies"),
+    (_c_i64, "pos_row pos_axis"),
+    (_c_int, "dtype tokens heads kv_heads dim pairs axes interleaved")))
+Norm = _struct("Norm", (
+    (_P, "x branch gate weight branch_weight scale starts"), (_c_i64, "x_row branch_row gate_row"),
+    (_c_int, "dtype branch_dtype gate_dtype gate_per_token tokens channels scenes longest"),
+    (_c_float, "eps")))
+_ATT, _ROT, _NORM = (ctypes.POINTER(t) for t in (Attention, Rotary, Norm))
+_BYTES = ctypes.POINTER(_c_size_t)
+
 # name -> argument types, in the order of include/gsvox.h
 SIGNATURES = {
     "gsv_version": [],
@@ -51,6 +75,16 @@ SIGNATURES = {
     "gsv_voxelize_bwd_l1": [_c_int, _c_int, _c_int, _c_int, _c_int, _c_i64, _P, _P, _P, _P, _P,
                             _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _c_int, _P,
                             _c_size_t, _P],
+    "gsv_rotary": [_ROT, _P, _P, _c_int, _P],
+    "gsv_gated_norm_fwd": [_NORM, _P, _P, _P],
+    "gsv_gated_norm_bwd_workspace_bytes": [_NORM, _BYTES],
+    "gsv_gated_norm_bwd": [_NORM, _P, _c_i64, _P, _c_i64, _P, _P, _P, _P, _P, _P, _P, _c_size_t,
+                           _P],
+    "gsv_attention_fwd": [_ATT, _P, _P, _P],
+    "gsv_attention_bwd_workspace_bytes": [_ATT, _BYTES],
+    "gsv_attention_bwd": [_ATT, _P, _P, _P, _c_i64, _c_i64, _P, _P, _P, _P, _P, _c_size_t, _P],
+    "gsv_attention_cached_workspace_bytes": [_ATT, _BYTES],
+    "gsv_attention_cached": [_ATT, _P, _c_i64, _c_i64, _c_i64, _c_i64, _P, _P, _c_size_t, _P],
     "gsv_kernel_timing_enable": [_c_int],
     "gsv_kernel_timing_collect": [_c_int, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_c_int)],
     "gsv_wave_timeline": [_c_int, _P, _c_int],

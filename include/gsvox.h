@@ -339,6 +339,115 @@ int gsv_kernel_timing_collect(int32_t kernel, double *total_ms, int32_t *count);
  */
 int gsv_wave_timeline(int32_t kernel, uint64_t *records, int32_t capacity);
 
+/*
+ * Operators on packed tokens (no counterpart in the reference): rotary positions,
+ * attention inside scenes, one-token attention over a cache, and the gated residual
+ * norm of a model whose tokens are Gaussians.  Element types are float32 and bfloat16
+ * (GSV_F32, GSV_BF16); sums, softmax statistics and norms are held in float32.
+ * Strides count elements; the last axis of every tensor is contiguous.
+ */
+#define GSV_F32 0
+#define GSV_BF16 1
+
+/*
+ * Attention inside the scenes of a packed batch.  q (q_tokens, heads, dim), k and v
+ * (k_tokens, kv_heads, dim) with the given row and head strides; heads a multiple of
+ * kv_heads, query head h reads key head h / (heads / kv_heads); dim a multiple of 8,
+ * 8 .. 128; pointers and strides multiples of 16 bytes.
+ *   t_ij = scale q_i.k_j, with cap > 0: cap tanh(scale q_i.k_j / cap);
+ *   with slopes: - slopes[h] |q_positions[i] - k_positions[j]|
+ * over the keys j that row i sees: those of its own scene, kept ones (keep NULL, or
+ * keep[j] != 0; keep_bytes 1 or 4), and with causal those below the larger of
+ * prefix[scene] and i + 1 + keys - queries (rows counted in the scene, which so end
+ * where its keys end).  A row that sees no key gives 0.
+ * q_starts, k_starts: (scenes + 1) first rows of the scenes, ascending; the first scene
+ * begins at row 0 and the last one ends with the arrays (entries 0 and `scenes` are not
+ * read).  NULL only for one scene.  longest_q, longest_k: rows of the longest scene, 0 if
+ * unknown; they only size the launch.  positions: rows of float x, y, z.
+ */
+typedef struct gsv_attention {
+    const void *q, *k, *v;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    const int32_t *q_starts, *k_starts, *prefix;
+    const float *q_positions, *k_positions;
+    int64_t q_pos_row, k_pos_row;
+    const void *slopes, *keep;
+    int32_t dtype, slopes_dtype, keep_bytes, causal;
+    int32_t q_tokens, k_tokens, heads, kv_heads, dim, scenes, longest_q, longest_k;
+    float scale, cap;
+} gsv_attention;
+
+/* out (q_tokens, heads, dim) contiguous; lse (heads, q_tokens), optional, receives what
+ * the backward needs (log2 of each row's sum of exponentials, +inf for an empty row). */
+int gsv_attention_fwd(const gsv_attention *args, void *out, float *lse, void *stream);
+
+/* Gradients: dq, dk, dv contiguous like q, k, v's shapes, dslopes (heads) in the slopes'
+ * type (only with slopes).  out and lse from the forward; dout with its strides.  The
+ * sums run in a fixed order (no atomics): the same inputs give the same bits. */
+int gsv_attention_bwd_workspace_bytes(const gsv_attention *args, size_t *bytes);
+int gsv_attention_bwd(const gsv_attention *args, const void *out, const float *lse,
+                      const void *dout, int64_t dout_row, int64_t dout_head, void *dq, void *dk,
+                      void *dv, void *dslopes, void *workspace, size_t workspace_bytes,
+                      void *stream);
+
+/*
+ * The same attention for one query token a scene over a cache: q (scenes, heads, dim), k
+ * and v (scenes, k_tokens = capacity, kv_heads, dim) with scene strides k_scene and
+ * v_scene; rows [0, lengths[s]) of scene s are live (lengths are clamped to 0 ..
+ * capacity), the rest is never read.  In args q_tokens = scenes, causal 0, prefix and
+ * starts NULL; k_positions (scenes, capacity) rows of x, y, z with k_pos_scene; keep
+ * (scenes, capacity) with keep_scene.  A scene without live keys gives 0.
+ */
+int gsv_attention_cached_workspace_bytes(const gsv_attention *args, size_t *bytes);
+int gsv_attention_cached(const gsv_attention *args, const int32_t *lengths, int64_t k_scene,
+                         int64_t v_scene, int64_t k_pos_scene, int64_t keep_scene, void *out,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Rotary positions: theta[t, p] = sum_a positions[t, a] frequencies[a, p] for `pairs`
+ * channel pairs of every head of q (tokens, heads, dim) and k (tokens, kv_heads, dim);
+ * pair p is channels (p, pairs + p), or (2 p, 2 p + 1) where interleaved; channels from
+ * 2 pairs on pass through.  inverse != 0 turns by -theta (the gradient).  Outputs are
+ * contiguous; heads or kv_heads may be 0.  frequencies (axes, pairs) contiguous.
+ */
+typedef struct gsv_rotary_args {
+    const void *q, *k;
+    int64_t q_row, q_head, k_row, k_head;
+    const float *positions, *frequencies;
+    int64_t pos_row, pos_axis;
+    int32_t dtype, tokens, heads, kv_heads, dim, pairs, axes, interleaved;
+} gsv_rotary_args;
+int gsv_rotary(const gsv_rotary_args *args, void *q_out, void *k_out, int32_t inverse, void *stream);
+
+/*
+ * The norms around a block with its gate and residual scale, rows of `channels` (1 .. 8192):
+ *   n = branch rstd(branch) branch_weight    (branch_weight NULL: n = branch)
+ *   y = x + gate scale n                     h = y rstd(y) weight
+ *   rstd(v) = 1 / sqrt(mean(v^2) + eps)
+ * x and y have dtype, branch and h branch_dtype (float32 x with either, bfloat16 x with
+ * bfloat16), the weights and scale float32, gate float32 or branch_dtype.  gate (NULL: 1)
+ * has a row for each scene (starts as for gsv_attention) or, gate_per_token, for each token.
+ * y and h are contiguous.
+ */
+typedef struct gsv_norm {
+    const void *x, *branch, *gate;
+    const float *weight, *branch_weight, *scale;
+    const int32_t *starts;
+    int64_t x_row, branch_row, gate_row;
+    int32_t dtype, branch_dtype, gate_dtype, gate_per_token;
+    int32_t tokens, channels, scenes, longest;
+    float eps;
+} gsv_norm;
+int gsv_gated_norm_fwd(const gsv_norm *args, void *y, void *h, void *stream);
+
+/* Gradients from dy and dh (either may be NULL: zero).  dgate has the gate's rows and type.
+ * Sums run in a fixed order. */
+int gsv_gated_norm_bwd_workspace_bytes(const gsv_norm *args, size_t *bytes);
+int gsv_gated_norm_bwd(const gsv_norm *args, const void *dy, int64_t dy_row, const void *dh,
+                       int64_t dh_row, void *dx, void *dbranch, float *dweight,
+                       float *dbranch_weight, float *dscale, void *dgate, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
