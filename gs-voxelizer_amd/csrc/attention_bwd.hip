@@ -41,8 +41,8 @@ __device__ __forceinline__ void weigh(f32x16 &w, f32x16 &u, const f32x16 &d, boo
     }
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(256) void k_attention_dq(const AttnArgs a, const BwdArgs g) {
+template <typename T, int DP, bool FAR, bool CAPPED>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const AttnArgs a, const BwdArgs g) {
     constexpr int KB = BwdTile<T>::kOther, LD = DP + Elem<T>::kPad;
     typedef typename Elem<T>::frag frag;
     __shared__ __align__(16) T sk[2][KB * LD];
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void k_attention_dq(const AttnArgs a, const Bw
     const int hk = h / (a.heads / a.kv_heads);
     const T *kbase = static_cast<const T *>(a.k) + (int64_t)c.k0 * a.k_row + hk * a.k_head;
     const T *vbase = static_cast<const T *>(a.v) + (int64_t)c.k0 * a.v_row + hk * a.v_head;
-    const bool far = a.slopes != nullptr, capped = a.cap > 0.f;
+    constexpr bool far = FAR, capped = CAPPED;
     const float slope = slope_of(a, h);
     const float unit = capped ? kLog2e : a.scale * kLog2e;
     const float far_unit = capped ? slope : slope / a.scale;
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(256) void k_attention_dq(const AttnArgs a, const Bw
                     live = __ballot(j0 + lane < nk && lane < KB && kept(a, c.k0 + min(j0 + lane, nk - 1)));
                 const bool masked = j0 + KB > all || (KB == 64 ? ~live : (~live & 0xffffffffull)) != 0;
                 float here = 0.f;
-#pragma unroll
+#pragma unroll 1
                 for (int kb = 0; kb < KB / 32; ++kb) {
                     f32x16 d = {}, w = {}, u = {}, dp;
                     if (far) d = distances(spos[b], KB, kb * 32, lane, x, y, z);
@@ -200,8 +200,8 @@ __global__ __launch_bounds__(256) void k_attention_dq(const AttnArgs a, const Bw
     }
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(256) void k_attention_dkv(const AttnArgs a, const BwdArgs g) {
+template <typename T, int DP, bool FAR, bool CAPPED>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const AttnArgs a, const BwdArgs g) {
     constexpr int QB = BwdTile<T>::kOther, LD = DP + Elem<T>::kPad;
     typedef typename Elem<T>::frag frag;
     __shared__ __align__(16) T sq[2][QB * LD];
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(256) void k_attention_dkv(const AttnArgs a, const B
     const int nq = c.q1 - c.q0, nk = c.k1 - c.k0, off = nk - nq;
     const int group = a.heads / a.kv_heads;
     const int tiles = (nk + kRows - 1) / kRows;
-    const bool far = a.slopes != nullptr, capped = a.cap > 0.f;
+    constexpr bool far = FAR, capped = CAPPED;
     const float unit = capped ? kLog2e : a.scale * kLog2e;
     const float in_cap = capped ? a.scale / a.cap : 0.f;
 
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(256) void k_attention_dkv(const AttnArgs a, const B
                 const float slope = slope_of(a, hk * group + step / per_head);
                 const float far_unit = capped ? slope : slope / a.scale;
                 const bool masked = i0 < wave_all;
-#pragma unroll
+#pragma unroll 1
                 for (int qb = 0; qb < QB / 32; ++qb) {
                     f32x16 d = {}, w = {}, u = {}, dp, lse;
                     if (far) d = distances(srow[b], QB, qb * 32, lane, x, y, z);
@@ -361,21 +361,22 @@ __global__ __launch_bounds__(64) void k_slope_sum(const float *__restrict__ part
     else static_cast<bf16 *>(out)[h] = (bf16)(float)sum;
 }
 
-template <typename T, int DP> void launch_bwd(AttnArgs a, const BwdArgs &g, int kslots, hipStream_t st) {
-    const dim3 block(256);
-    if (a.q_tokens > 0)
-        hipLaunchKernelGGL((k_attention_dq<T, DP>), dim3((unsigned)a.slots * a.scenes * a.heads),
-                           block, 0, st, a, g);
-    a.slots = kslots;
-    if (a.k_tokens > 0)
-        hipLaunchKernelGGL((k_attention_dkv<T, DP>), dim3((unsigned)a.slots * a.scenes * a.kv_heads),
-                           block, 0, st, a, g);
-}
-template <typename T> void launch_bwd(const AttnArgs &a, const BwdArgs &g, int kslots, hipStream_t st) {
-    if (a.dim <= 32) launch_bwd<T, 32>(a, g, kslots, st);
-    else if (a.dim <= 64) launch_bwd<T, 64>(a, g, kslots, st);
-    else launch_bwd<T, 128>(a, g, kslots, st);
-}
+struct Backward {
+    const AttnArgs &a;
+    const BwdArgs &g;
+    int kslots;
+    hipStream_t st;
+    template <typename T, int DP, bool FAR, bool CAPPED> void run() const {
+        if (a.q_tokens > 0)
+            hipLaunchKernelGGL((k_attention_dq<T, DP, FAR, CAPPED>),
+                               dim3((unsigned)a.slots * a.scenes * a.heads), dim3(256), 0, st, a, g);
+        AttnArgs k = a;
+        k.slots = kslots;
+        if (a.k_tokens > 0)
+            hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED>),
+                               dim3((unsigned)kslots * a.scenes * a.kv_heads), dim3(256), 0, st, k, g);
+    }
+};
 
 size_t delta_bytes(const AttnArgs &a) {
     return ((size_t)a.heads * a.q_tokens * sizeof(float) + 255) / 256 * 256;
@@ -427,8 +428,7 @@ extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, con
     float *part = reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(a));
     const BwdArgs g{out, dout, dout_row, dout_head, lse, delta, part, dq, dk, dv};
     hipStream_t s = as_stream(stream);
-    if (args->dtype == GSV_BF16) launch_bwd<bf16>(a, g, kslots, s);
-    else launch_bwd<float>(a, g, kslots, s);
+    attention_variant(a, args->dtype, Backward{a, g, kslots, s});
     if (a.slopes)
         hipLaunchKernelGGL(k_slope_sum, dim3(a.heads), dim3(64), 0, s, part,
                            a.q_tokens > 0 ? a.slots * a.scenes : 0, a.heads, dslopes, a.slopes_f32);

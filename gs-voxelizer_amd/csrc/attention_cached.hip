@@ -46,7 +46,7 @@ template <typename T, int DP> struct WaveStaged {
     }
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool FAR, bool CAPPED>
 __global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, const CacheArgs c,
                                                           T *__restrict__ out) {
     constexpr int LD = DP + Elem<T>::kPad;
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, cons
     const bool head = col < group;
     const int h = hk * group + (head ? col : 0);
 
-    const bool far = a.slopes != nullptr, capped = a.cap > 0.f;
+    constexpr bool far = FAR, capped = CAPPED;
     const float slope = slope_of(a, h);
     const float unit = capped ? kLog2e : a.scale * kLog2e;
     const float far_unit = capped ? slope : slope / a.scale;
@@ -246,21 +246,21 @@ int cache_splits(const AttnArgs &a, int head_tiles) {
     return (int)imax64(1, imin64(want, most));
 }
 
-template <typename T>
-int launch_cached(const AttnArgs &a, const CacheArgs &c, void *out, hipStream_t st) {
-    const dim3 grid((unsigned)(a.scenes * a.kv_heads * c.head_tiles * c.splits)), block(256);
-    T *o = static_cast<T *>(out);
-    if (a.dim <= 32)
-        hipLaunchKernelGGL((k_attention_cached<T, 32>), grid, block, 0, st, a, c, o);
-    else if (a.dim <= 64)
-        hipLaunchKernelGGL((k_attention_cached<T, 64>), grid, block, 0, st, a, c, o);
-    else
-        hipLaunchKernelGGL((k_attention_cached<T, 128>), grid, block, 0, st, a, c, o);
-    if (c.splits > 1)
-        hipLaunchKernelGGL(k_cached_join<T>, dim3((unsigned)(a.scenes * a.heads)), dim3(64), 0, st,
-                           c.part_o, c.part_ms, c.splits, a.dim, o);
-    return check_launch();
-}
+struct Cached {
+    const AttnArgs &a;
+    const CacheArgs &c;
+    void *out;
+    hipStream_t st;
+    template <typename T, int DP, bool FAR, bool CAPPED> void run() const {
+        T *o = static_cast<T *>(out);
+        hipLaunchKernelGGL((k_attention_cached<T, DP, FAR, CAPPED>),
+                           dim3((unsigned)(a.scenes * a.kv_heads * c.head_tiles * c.splits)),
+                           dim3(256), 0, st, a, c, o);
+        if (c.splits > 1)
+            hipLaunchKernelGGL(k_cached_join<T>, dim3((unsigned)(a.scenes * a.heads)), dim3(64), 0,
+                               st, c.part_o, c.part_ms, c.splits, a.dim, o);
+    }
+};
 
 int cached_plan(const gsv_attention *args, AttnArgs *a, int *head_tiles, int *splits) {
     int lq, lk;
@@ -318,6 +318,6 @@ extern "C" int gsv_attention_cached(const gsv_attention *args, const int32_t *le
     float *po = static_cast<float *>(workspace);
     const CacheArgs c{lengths, k_scene, v_scene, k_pos_scene, keep_scene, splits, tiles, po,
                       reinterpret_cast<float2 *>(static_cast<char *>(workspace) + part_o_bytes(a, splits))};
-    hipStream_t s = as_stream(stream);
-    return args->dtype == GSV_BF16 ? launch_cached<bf16>(a, c, out, s) : launch_cached<float>(a, c, out, s);
+    attention_variant(a, args->dtype, Cached{a, c, out, as_stream(stream)});
+    return check_launch();
 }

@@ -19,8 +19,8 @@ constexpr float kSlack = 8.f;
 
 template <typename T> struct FwdTile { static constexpr int kKeys = sizeof(T) == 2 ? 64 : 32; };
 
-template <typename T, int DP>
-__global__ __launch_bounds__(256) void k_attention_fwd(const AttnArgs a, T *__restrict__ out,
+template <typename T, int DP, bool FAR, bool CAPPED>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const AttnArgs a, T *__restrict__ out,
                                                        float *__restrict__ lse) {
     constexpr int KB = FwdTile<T>::kKeys, LD = DP + Elem<T>::kPad;
     typedef typename Elem<T>::frag frag;
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256) void k_attention_fwd(const AttnArgs a, T *__re
     const int hk = h / (a.heads / a.kv_heads);
     const T *kbase = static_cast<const T *>(a.k) + (int64_t)c.k0 * a.k_row + hk * a.k_head;
     const T *vbase = static_cast<const T *>(a.v) + (int64_t)c.k0 * a.v_row + hk * a.v_head;
-    const bool far = a.slopes != nullptr, capped = a.cap > 0.f;
+    constexpr bool far = FAR, capped = CAPPED;
     const float slope = slope_of(a, h);
     // scores leave the matrix product in units of 1 / scale (or 1 where they are capped);
     // unit turns them into powers of two
@@ -101,13 +101,10 @@ __global__ __launch_bounds__(256) void k_attention_fwd(const AttnArgs a, T *__re
                 if (a.keep || j0 + KB > all)
                     live = __ballot(j0 + lane < nk && lane < KB && kept(a, c.k0 + min(j0 + lane, nk - 1)));
                 const bool masked = j0 + KB > all || (KB == 64 ? ~live : (~live & 0xffffffffull)) != 0;
-                f32x16 t[KB / 32];
-                float top = -INFINITY;
-#pragma unroll
+#pragma unroll 1
                 for (int kb = 0; kb < KB / 32; ++kb) {
-                    f32x16 d = {};
+                    f32x16 d = {}, w = {};
                     if (far) d = distances(spos[b], KB, kb * 32, lane, x, y, z);
-                    f32x16 w = {};
                     if (far && !capped)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) w[r] = -far_unit * d[r];
@@ -129,30 +126,27 @@ __global__ __launch_bounds__(256) void k_attention_fwd(const AttnArgs a, T *__re
                             if (at >= lim || !((bits >> at) & 1)) w[r] = -INFINITY;
                         }
                     }
+                    float top = -INFINITY;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) top = fmaxf(top, w[r]);
-                    t[kb] = w;
-                }
-                top *= unit;
-                if (__any(top > m + kSlack)) {
-                    const float next = fmaxf(m, fmaxf(top, other_half(top)));
-                    const float by = next == -INFINITY ? 1.f : fast_exp2(m - next);
-                    m = next;
-                    sum *= by;
+                    top *= unit;
+                    if (__any(top > m + kSlack)) {
+                        const float next = fmaxf(m, fmaxf(top, other_half(top)));
+                        const float by = next == -INFINITY ? 1.f : fast_exp2(m - next);
+                        m = next;
+                        sum *= by;
 #pragma unroll
-                    for (int n = 0; n < DP / 32; ++n) o[n] *= by;
-                }
-                const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-                for (int kb = 0; kb < KB / 32; ++kb) {
+                        for (int n = 0; n < DP / 32; ++n) o[n] *= by;
+                    }
+                    const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        t[kb][r] = fast_exp2(fmaf(t[kb][r], unit, -ref));
-                        sum += t[kb][r];
+                        w[r] = fast_exp2(fmaf(w[r], unit, -ref));
+                        sum += w[r];
                     }
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const frag p = to_frag<T>(t[kb], half);
+                        const frag p = to_frag<T>(w, half);
 #pragma unroll
                         for (int n = 0; n < DP / 32; ++n)
                             o[n] = mma(tr_frag<LD>(sv[b] + (kb * 32 + half * 16) * LD + n * 32, lane),
@@ -175,17 +169,17 @@ __global__ __launch_bounds__(256) void k_attention_fwd(const AttnArgs a, T *__re
     }
 }
 
-template <typename T> int launch_fwd(const AttnArgs &a, void *out, float *lse, hipStream_t st) {
-    const dim3 grid((unsigned)a.slots * a.scenes * a.heads), block(256);
-    T *o = static_cast<T *>(out);
-    if (a.dim <= 32)
-        hipLaunchKernelGGL((k_attention_fwd<T, 32>), grid, block, 0, st, a, o, lse);
-    else if (a.dim <= 64)
-        hipLaunchKernelGGL((k_attention_fwd<T, 64>), grid, block, 0, st, a, o, lse);
-    else
-        hipLaunchKernelGGL((k_attention_fwd<T, 128>), grid, block, 0, st, a, o, lse);
-    return check_launch();
-}
+struct Forward {
+    const AttnArgs &a;
+    void *out;
+    float *lse;
+    hipStream_t st;
+    template <typename T, int DP, bool FAR, bool CAPPED> void run() const {
+        hipLaunchKernelGGL((k_attention_fwd<T, DP, FAR, CAPPED>),
+                           dim3((unsigned)a.slots * a.scenes * a.heads), dim3(256), 0, st, a,
+                           static_cast<T *>(out), lse);
+    }
+};
 
 }  // namespace
 
@@ -236,6 +230,6 @@ extern "C" int gsv_attention_fwd(const gsv_attention *args, void *out, float *ls
     if (a.q_tokens == 0) return GSV_OK;
     if (!out || reinterpret_cast<uintptr_t>(out) % 16) return GSV_ERR_INVALID_ARGUMENT;
     if (!attention_slots(&a, lq, kRows, a.heads)) return GSV_ERR_SIZE_OVERFLOW;
-    hipStream_t s = as_stream(stream);
-    return args->dtype == GSV_BF16 ? launch_fwd<bf16>(a, out, lse, s) : launch_fwd<float>(a, out, lse, s);
+    attention_variant(a, args->dtype, Forward{a, out, lse, as_stream(stream)});
+    return check_launch();
 }

@@ -117,6 +117,25 @@ struct AttnArgs {
 // Checks the C arguments and lays them out for a launch; longest_*: rows of the longest scene.
 int attention_args(const gsv_attention *in, AttnArgs *a, int *longest_q, int *longest_k);
 
+// The kernel variant of a call: element type, channels (up to 32, 64 or 128; the columns past
+// dim are zeros), distance bias, score cap.
+template <typename T, int DP, typename F> void attention_options(const AttnArgs &a, const F &f) {
+    const bool far = a.slopes, capped = a.cap > 0.f;
+    if (far && capped) f.template run<T, DP, true, true>();
+    else if (far) f.template run<T, DP, true, false>();
+    else if (capped) f.template run<T, DP, false, true>();
+    else f.template run<T, DP, false, false>();
+}
+template <typename T, typename F> void attention_channels(const AttnArgs &a, const F &f) {
+    if (a.dim <= 32) attention_options<T, 32>(a, f);
+    else if (a.dim <= 64) attention_options<T, 64>(a, f);
+    else attention_options<T, 128>(a, f);
+}
+template <typename F> void attention_variant(const AttnArgs &a, int dtype, const F &f) {
+    if (dtype == GSV_BF16) attention_channels<bf16>(a, f);
+    else attention_channels<float>(a, f);
+}
+
 // Workgroups for each scene and head: one for each tile of the longest scene, fewer where the
 // launch would pass a million (they take the tiles in turn, so any number is right).
 inline bool attention_slots(AttnArgs *a, int longest, int rows, int heads) {
