@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
     __shared__ __align__(16) float spos[2][3 * KB];
     __shared__ double sums[4];
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = blockIdx.x % a.heads, rest = blockIdx.x / a.heads;
     const int s = rest % a.scenes, slot = rest / a.scenes;
     const Scene c = scene_rows(a, s);
@@ -65,6 +65,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
     const float far_unit = capped ? slope : slope / a.scale;
     const float in_cap = capped ? a.scale / a.cap : 0.f;
     double dslope = 0.0;
+
+    Staged<T, DP, KB> gk, gv;
+    gk.plan(a.k_row, a.dim);
+    gv.plan(a.v_row, a.dim);
 
     for (int tile = slot; tile < tiles; tile += a.slots) {
         const int first = (tiles - 1 - tile) * kRows;
@@ -98,6 +102,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
                 x = p[0], y = p[1], z = p[2];
             }
         }
+        x = own_side(x, lane), y = own_side(y, lane), z = own_side(z, lane);
         const int limit = row ? key_limit(a, c, i) : 0;
         const int all = first + wave * 32 + 31 < nq ? key_limit(a, c, first + wave * 32) : 0;
         const int most = key_limit(a, c, min(first + kRows, nq) - 1);
@@ -105,18 +110,24 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
                              ? key_limit(a, c, min(first + wave * 32 + 32, nq) - 1) : 0;
         f32x16 dq[DP / 32] = {};
 
-        Staged<T, DP, KB> gk, gv;
         float gp = 0.f;
+        bool gl = true;
+        uint64_t live = ~0ull;
         auto fetch = [&](int j0) {
-            auto live = [&](int r) { return j0 + r < most && kept(a, c.k0 + j0 + r); };
-            gk.load(kbase + j0 * a.k_row, a.k_row, a.dim, live);
-            gv.load(vbase + j0 * a.v_row, a.v_row, a.dim, live);
-            if (far && threadIdx.x < 3 * KB) {
-                const int r = threadIdx.x % KB, ax = threadIdx.x / KB;
-                gp = j0 + r < most ? a.k_pos[(int64_t)(c.k0 + j0 + r) * a.k_pos_row + ax] : 0.f;
-            }
+            const int left = most - j0;
+            gk.load(kbase + j0 * a.k_row, a.k_row, a.dim, left);
+            gv.load(vbase + j0 * a.v_row, a.v_row, a.dim, left);
+            if (far && threadIdx.x < 3 * KB)
+                gp = a.k_pos[(c.k0 + j0 + min((int)threadIdx.x % KB, left - 1)) * a.k_pos_row +
+                             threadIdx.x / KB];
+            if (a.keep) gl = lane < KB && lane < left && kept(a, c.k0 + j0 + lane);
         };
         auto put = [&](int b) {
+            if (a.keep) {
+                live = __ballot(gl);
+                gk.keep(live);
+                gv.keep(live);
+            }
             gk.store(sk[b]);
             gv.store(sv[b]);
             if (far && threadIdx.x < 3 * KB) spos[b][threadIdx.x] = gp;
@@ -132,10 +143,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
             const bool more = j0 + KB < most;
             if (more) fetch(j0 + KB);
             if (j0 < mine) {
-                uint64_t live = ~0ull;
-                if (a.keep || j0 + KB > all)
-                    live = __ballot(j0 + lane < nk && lane < KB && kept(a, c.k0 + min(j0 + lane, nk - 1)));
-                const bool masked = j0 + KB > all || (KB == 64 ? ~live : (~live & 0xffffffffull)) != 0;
+                const bool masked = j0 + KB > all || (KB == 64 ? ~live : (uint32_t)~live) != 0;
                 float here = 0.f;
 #pragma unroll 1
                 for (int kb = 0; kb < KB / 32; ++kb) {
@@ -208,7 +216,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
     __shared__ __align__(16) T sdo[2][QB * LD];
     __shared__ __align__(16) float srow[2][5 * QB];  // x, y, z, log sum, D
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
     const int s = rest % a.scenes, slot = rest / a.scenes;
     const Scene c = scene_rows(a, s);
@@ -218,6 +226,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
     constexpr bool far = FAR, capped = CAPPED;
     const float unit = capped ? kLog2e : a.scale * kLog2e;
     const float in_cap = capped ? a.scale / a.cap : 0.f;
+
+    Staged<T, DP, QB> gq, gd;
+    gq.plan(a.q_row, a.dim);
+    gd.plan(g.dout_row, a.dim);
 
     for (int tile = slot; tile < tiles; tile += a.slots) {
         const int first = tile * kRows;
@@ -234,6 +246,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
             const float *p = a.k_pos + kj * a.k_pos_row;
             x = p[0], y = p[1], z = p[2];
         }
+        x = own_side(x, lane), y = own_side(y, lane), z = own_side(z, lane);
         // the first query row that sees this key; one that no row sees
         const int from = !live ? INT32_MAX : a.causal && j >= c.prefix ? j - off : 0;
         const bool dead_here = __any(!live);
@@ -247,26 +260,25 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
         const int steps = per_head * group;
         f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
 
-        Staged<T, DP, QB> gq, gd;
         float gr[2] = {};
         auto fetch = [&](int step) {
             const int h = hk * group + step / per_head, i0 = q_from + step % per_head * QB;
             const int64_t q0 = c.q0 + i0;
-            auto inside = [&](int r) { return i0 + r < nq; };
-            gq.load(static_cast<const T *>(a.q) + q0 * a.q_row + h * a.q_head, a.q_row, a.dim, inside);
+            const int left = nq - i0;
+            gq.load(static_cast<const T *>(a.q) + q0 * a.q_row + h * a.q_head, a.q_row, a.dim, left);
             gd.load(static_cast<const T *>(g.dout) + q0 * g.dout_row + h * g.dout_head, g.dout_row,
-                    a.dim, inside);
+                    a.dim, left);
+            // positions, log sums and D of the rows, five arrays in turn
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const int at = n * 256 + threadIdx.x, r = at % QB, what = at / QB;
-                gr[n] = what == 3 ? INFINITY : 0.f;
-                if (what < 5 && i0 + r < nq) {
-                    if (what < 3) {
-                        if (far) gr[n] = a.q_pos[(q0 + r) * a.q_pos_row + what];
-                    } else {
-                        gr[n] = (what == 3 ? g.lse : g.delta)[(int64_t)h * a.q_tokens + q0 + r];
-                    }
-                }
+                if (what >= 5) continue;
+                const int64_t row = q0 + min(r, left - 1);
+                if (what >= 3)
+                    gr[n] = (what == 3 ? g.lse : g.delta)[(int64_t)h * a.q_tokens + row];
+                else if (far)
+                    gr[n] = a.q_pos[row * a.q_pos_row + what];
+                if (what == 3 && r >= left) gr[n] = INFINITY;  // no weights past the last row
             }
         };
         auto put = [&](int b) {
@@ -418,7 +430,9 @@ extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, con
     if ((st = gsv_attention_bwd_workspace_bytes(args, &need)) != GSV_OK) return st;
     if (need > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
     const int64_t chunk = args->dtype == GSV_BF16 ? 8 : 4;
-    if (dout_row % chunk || dout_head % chunk) return GSV_ERR_INVALID_ARGUMENT;
+    if (dout_row % chunk || dout_head % chunk || dout_row < 0 ||
+        dout_row * (16 / chunk) > kMaxRowBytes)
+        return GSV_ERR_INVALID_ARGUMENT;
     if (a.q_tokens > 0 && (!out || !lse || !dout || !dq || !workspace)) return GSV_ERR_INVALID_ARGUMENT;
     if ((a.k_tokens > 0 && (!dk || !dv)) || (a.slopes && !dslopes)) return GSV_ERR_INVALID_ARGUMENT;
     const void *ptrs[] = {out, dout, dq, dk, dv, workspace};

@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, cons
     __shared__ __align__(16) float spos[4][3 * kKeys];
     __shared__ float sm[4][kHeads], ss[4][kHeads];
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int group = a.heads / a.kv_heads;
     int n = blockIdx.x;
     const int hk = n % a.kv_heads;
@@ -83,6 +83,7 @@ __global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, cons
         const float *p = a.q_pos + s * a.q_pos_row;
         x = p[0], y = p[1], z = p[2];
     }
+    x = own_side(x, lane), y = own_side(y, lane), z = own_side(z, lane);
     const T *kbase = static_cast<const T *>(a.k) + s * c.k_scene + hk * a.k_head;
     const T *vbase = static_cast<const T *>(a.v) + s * c.v_scene + hk * a.v_head;
     T *sk = tiles[wave], *sv = sk + kKeys * LD;

@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const A
     __shared__ __align__(16) T sv[2][KB * LD];
     __shared__ __align__(16) float spos[2][3 * KB];
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // heads vary fastest: with eight (or a multiple) of them each XCD's L2 holds the keys
     // of its own heads
     const int h = blockIdx.x % a.heads, rest = blockIdx.x / a.heads;
@@ -47,6 +47,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const A
     const float far_unit = capped ? slope : slope / a.scale;
     const float in_cap = capped ? a.scale / a.cap : 0.f;
 
+    Staged<T, DP, KB> gk, gv;
+    gk.plan(a.k_row, a.dim);
+    gv.plan(a.v_row, a.dim);
+
     for (int tile = slot; tile < tiles; tile += a.slots) {
         // the last rows of a causal scene see the most keys: they start first
         const int first = (tiles - 1 - tile) * kRows;
@@ -61,6 +65,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const A
             const float *p = a.q_pos + qi * a.q_pos_row;
             x = p[0], y = p[1], z = p[2];
         }
+        x = own_side(x, lane), y = own_side(y, lane), z = own_side(z, lane);
         const int limit = row ? key_limit(a, c, i) : 0;
         const int all = first + wave * 32 + 31 < nq ? key_limit(a, c, first + wave * 32) : 0;
         const int most = key_limit(a, c, min(first + kRows, nq) - 1);  // of the workgroup
@@ -69,18 +74,24 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const A
         f32x16 o[DP / 32] = {};
         float m = -INFINITY, sum = 0.f;
 
-        Staged<T, DP, KB> gk, gv;
         float gp = 0.f;
+        bool gl = true;
+        uint64_t live = ~0ull;
         auto fetch = [&](int j0) {
-            auto live = [&](int r) { return j0 + r < most && kept(a, c.k0 + j0 + r); };
-            gk.load(kbase + j0 * a.k_row, a.k_row, a.dim, live);
-            gv.load(vbase + j0 * a.v_row, a.v_row, a.dim, live);
-            if (far && threadIdx.x < 3 * KB) {
-                const int r = threadIdx.x % KB, ax = threadIdx.x / KB;
-                gp = j0 + r < most ? a.k_pos[(int64_t)(c.k0 + j0 + r) * a.k_pos_row + ax] : 0.f;
-            }
+            const int left = most - j0;
+            gk.load(kbase + j0 * a.k_row, a.k_row, a.dim, left);
+            gv.load(vbase + j0 * a.v_row, a.v_row, a.dim, left);
+            if (far && threadIdx.x < 3 * KB)
+                gp = a.k_pos[(c.k0 + j0 + min((int)threadIdx.x % KB, left - 1)) * a.k_pos_row +
+                             threadIdx.x / KB];
+            if (a.keep) gl = lane < KB && lane < left && kept(a, c.k0 + j0 + lane);
         };
         auto put = [&](int b) {
+            if (a.keep) {
+                live = __ballot(gl);
+                gk.keep(live);
+                gv.keep(live);
+            }
             gk.store(sk[b]);
             gv.store(sv[b]);
             if (far && threadIdx.x < 3 * KB) spos[b][threadIdx.x] = gp;
@@ -96,11 +107,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const A
             const bool more = j0 + KB < most;
             if (more) fetch(j0 + KB);
             if (j0 < mine) {
-                // keys of the tile that are inside and kept, a bit each
-                uint64_t live = ~0ull;
-                if (a.keep || j0 + KB > all)
-                    live = __ballot(j0 + lane < nk && lane < KB && kept(a, c.k0 + min(j0 + lane, nk - 1)));
-                const bool masked = j0 + KB > all || (KB == 64 ? ~live : (~live & 0xffffffffull)) != 0;
+                const bool masked = j0 + KB > all || (KB == 64 ? ~live : (uint32_t)~live) != 0;
 #pragma unroll 1
                 for (int kb = 0; kb < KB / 32; ++kb) {
                     f32x16 d = {}, w = {};
@@ -194,6 +201,8 @@ int attention_args(const gsv_attention *in, AttnArgs *a, int *longest_q, int *lo
     const int64_t strides[] = {g.q_row, g.q_head, g.k_row, g.k_head, g.v_row, g.v_head};
     for (int64_t x : strides)
         if (x % chunk) return GSV_ERR_INVALID_ARGUMENT;
+    for (int64_t x : {g.q_row, g.k_row, g.v_row})
+        if (x < 0 || x * (16 / chunk) > kMaxRowBytes) return GSV_ERR_INVALID_ARGUMENT;
     const void *ptrs[] = {g.q, g.k, g.v};
     for (const void *p : ptrs)
         if (reinterpret_cast<uintptr_t>(p) % 16) return GSV_ERR_INVALID_ARGUMENT;

@@ -182,30 +182,45 @@ __device__ __forceinline__ float slope_of(const AttnArgs &a, int h) {
                         : (float)static_cast<const bf16 *>(a.slopes)[h];
 }
 
-// A tile of ROWS rows of one head on its way from global memory to LDS: 256 threads,
-// 16-byte chunks, columns from dim up to DP zero, rows that are not live zero (so that
-// no value of theirs, NaN among them, meets a weight of 0).
+// The widest row stride: 64 rows have to lie within a buffer descriptor's 2^31 bytes.
+constexpr int64_t kMaxRowBytes = 1 << 24;
+
+// A tile of ROWS rows of one head on its way from global memory to LDS: 256 threads, 16-byte
+// chunks through a buffer descriptor that ends with the last live row, so that rows past it and
+// columns from dim up to DP arrive as zeros without a branch.  Rows of a mask are zeroed
+// as they are stored: no value of theirs, NaN among them, meets a weight of 0.
 template <typename T, int DP, int ROWS> struct Staged {
-    static constexpr int kCh = Elem<T>::kChunk, kPerRow = DP / kCh;
-    static constexpr int kN = (ROWS * kPerRow + 255) / 256;
-    uint4 r[kN];
-    template <typename Live>
-    __device__ __forceinline__ void load(const T *base, int64_t stride, int dim, Live live) {
+    static constexpr int kCh = Elem<T>::kChunk, kPerRow = DP / kCh, LD = DP + Elem<T>::kPad;
+    static constexpr int kN = ROWS * kPerRow / 256;
+    static_assert(ROWS * kPerRow % 256 == 0, "whole chunks for each thread");
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 r[kN];
+    int at[kN];  // byte offsets in the tile
+    __device__ __forceinline__ void plan(int64_t stride, int dim) {
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
             const int c = i * 256 + threadIdx.x, row = c / kPerRow, col = (c % kPerRow) * kCh;
-            r[i] = make_uint4(0, 0, 0, 0);
-            if (row < ROWS && col < dim && live(row))
-                r[i] = *reinterpret_cast<const uint4 *>(base + row * stride + col);
+            at[i] = col < dim ? (row * (int)stride + col) * (int)sizeof(T) : INT32_MAX - 15;
         }
     }
+    // rows: live rows from base on, 1 at least
+    __device__ __forceinline__ void load(const T *base, int64_t stride, int dim, int rows) {
+        const int bytes = ((min(rows, ROWS) - 1) * (int)stride + dim) * (int)sizeof(T);
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, bytes, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) r[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at[i], 0, 0);
+    }
     __device__ __forceinline__ void store(T *tile) const {
-        constexpr int LD = DP + Elem<T>::kPad;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
             const int c = i * 256 + threadIdx.x, row = c / kPerRow, col = (c % kPerRow) * kCh;
-            if (row < ROWS) *reinterpret_cast<uint4 *>(tile + row * LD + col) = r[i];
+            *reinterpret_cast<u32x4 *>(tile + row * LD + col) = r[i];
         }
+    }
+    __device__ __forceinline__ void keep(uint64_t live) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            if (!((live >> ((i * 256 + threadIdx.x) / kPerRow)) & 1)) r[i] = u32x4{};
     }
 };
 
@@ -239,23 +254,29 @@ __device__ __forceinline__ void store_column(T *row, const f32x16 (&o)[DP / 32],
         }
 }
 
-// Distances of one lane's row (x, y, z) to the 16 rows of its results' registers;
-// xyz: three arrays of `n` floats in LDS, `first` the block's first row in them.
+// What a lane adds to the products below: 1 for the other side's coordinate, or minus its own.
+__device__ __forceinline__ float own_side(float x, int lane) { return lane < 32 ? 1.f : -x; }
+
+// Distances of the lanes' columns (own_side of x, y, z) to the 32 rows of a block, in the result's
+// layout; xyz: three arrays of `n` floats in LDS, `first` the block's first row in them.  A
+// difference is a product of two terms, x_row * 1 + 1 * -x_column, one v_mfma_f32_32x32x2_f32 an
+// axis: the rounding of a subtraction, but 48 vector instructions a block fewer and one LDS word a
+// lane and axis instead of four times four.
 __device__ __forceinline__ f32x16 distances(const float *xyz, int n, int first, int lane, float x,
                                             float y, float z) {
+    const float *p = xyz + first + (lane & 31);
+    const float c[3] = {x, y, z};
     f32x16 d;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        const float *p = xyz + first + 8 * g + 4 * (lane >> 5);
-        const f32x4 px = *reinterpret_cast<const f32x4 *>(p);
-        const f32x4 py = *reinterpret_cast<const f32x4 *>(p + n);
-        const f32x4 pz = *reinterpret_cast<const f32x4 *>(p + 2 * n);
+    for (int ax = 0; ax < 3; ++ax) {
+        const float at = p[ax * n];
+        const f32x16 e =
+            __builtin_amdgcn_mfma_f32_32x32x2f32(lane < 32 ? at : 1.f, c[ax], f32x16{}, 0, 0, 0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float dx = px[e] - x, dy = py[e] - y, dz = pz[e] - z;
-            d[4 * g + e] = __builtin_amdgcn_sqrtf(fmaf(dx, dx, fmaf(dy, dy, dz * dz)));
-        }
+        for (int r = 0; r < 16; ++r) d[r] = ax ? fmaf(e[r], e[r], d[r]) : e[r] * e[r];
     }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) d[r] = __builtin_amdgcn_sqrtf(d[r]);
     return d;
 }
 

@@ -52,11 +52,15 @@ def activations(t, what, dims, like=None):
     return t
 
 
+MAX_ROW_BYTES = 1 << 24
+
+
 def rows16(t):
-    """`t`, or a contiguous copy where its last axis is strided or a row is not 16-byte aligned."""
-    size = t.element_size()
-    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0 and all(
-            s * size % 16 == 0 for s in t.stride()[:-1]):
+    """`t`, or a contiguous copy where its last axis is strided, a row is not 16-byte aligned or
+    rows (the third axis from the end) lie 16 MB apart or more."""
+    size, strides = t.element_size(), t.stride()
+    if (strides[-1] == 1 and t.data_ptr() % 16 == 0 and strides[-3] * size <= MAX_ROW_BYTES
+            and all(s * size % 16 == 0 for s in strides[:-1])):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
