@@ -47,14 +47,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
     typedef typename Elem<T>::frag frag;
     __shared__ __align__(16) T sk[2][KB * LD];
     __shared__ __align__(16) T sv[2][KB * LD];
-    __shared__ __align__(16) float spos[2][3 * KB];
+    __shared__ __align__(16) typename Places<T>::Row spos[2][3 * KB];
     __shared__ double sums[4];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = blockIdx.x % a.heads, rest = blockIdx.x / a.heads;
     const int s = rest % a.scenes, slot = rest / a.scenes;
     const Scene c = scene_rows(a, s);
-    const int nq = c.q1 - c.q0, nk = c.k1 - c.k0;
+    const int nq = c.q1 - c.q0;
     const int tiles = (nq + kRows - 1) / kRows;
     const int hk = h / (a.heads / a.kv_heads);
     const T *kbase = static_cast<const T *>(a.k) + (int64_t)c.k0 * a.k_row + hk * a.k_head;
@@ -102,7 +102,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
                 x = p[0], y = p[1], z = p[2];
             }
         }
-        x = own_side(x, lane), y = own_side(y, lane), z = own_side(z, lane);
+        Places<T> place;
+        place.set(x, y, z, lane);
         const int limit = row ? key_limit(a, c, i) : 0;
         const int all = first + wave * 32 + 31 < nq ? key_limit(a, c, first + wave * 32) : 0;
         const int most = key_limit(a, c, min(first + kRows, nq) - 1);
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
             }
             gk.store(sk[b]);
             gv.store(sv[b]);
-            if (far && threadIdx.x < 3 * KB) spos[b][threadIdx.x] = gp;
+            if (far && threadIdx.x < 3 * KB) spos[b][threadIdx.x] = Places<T>::row(gp);
         };
         __syncthreads();
         if (most > 0) {
@@ -148,7 +149,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
 #pragma unroll 1
                 for (int kb = 0; kb < KB / 32; ++kb) {
                     f32x16 d = {}, w = {}, u = {}, dp;
-                    if (far) d = distances(spos[b], KB, kb * 32, lane, x, y, z);
+                    if (far) d = distances(place, spos[b], KB, kb * 32, lane);
                     if (far && !capped)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) w[r] = -far_unit * d[r];
@@ -214,7 +215,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
     typedef typename Elem<T>::frag frag;
     __shared__ __align__(16) T sq[2][QB * LD];
     __shared__ __align__(16) T sdo[2][QB * LD];
-    __shared__ __align__(16) float srow[2][5 * QB];  // x, y, z, log sum, D
+    __shared__ __align__(16) typename Places<T>::Row spos[2][3 * QB];
+    __shared__ __align__(16) float srow[2][2 * QB];  // log sums, D
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
@@ -246,7 +248,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
             const float *p = a.k_pos + kj * a.k_pos_row;
             x = p[0], y = p[1], z = p[2];
         }
-        x = own_side(x, lane), y = own_side(y, lane), z = own_side(z, lane);
+        Places<T> place;
+        place.set(x, y, z, lane);
         // the first query row that sees this key; one that no row sees
         const int from = !live ? INT32_MAX : a.causal && j >= c.prefix ? j - off : 0;
         const bool dead_here = __any(!live);
@@ -268,17 +271,17 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
             gq.load(static_cast<const T *>(a.q) + q0 * a.q_row + h * a.q_head, a.q_row, a.dim, left);
             gd.load(static_cast<const T *>(g.dout) + q0 * g.dout_row + h * g.dout_head, g.dout_row,
                     a.dim, left);
-            // positions, log sums and D of the rows, five arrays in turn
+            // log sums, D and positions of the rows, five arrays in turn
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const int at = n * 256 + threadIdx.x, r = at % QB, what = at / QB;
                 if (what >= 5) continue;
                 const int64_t row = q0 + min(r, left - 1);
-                if (what >= 3)
-                    gr[n] = (what == 3 ? g.lse : g.delta)[(int64_t)h * a.q_tokens + row];
+                if (what < 2)
+                    gr[n] = (what ? g.delta : g.lse)[(int64_t)h * a.q_tokens + row];
                 else if (far)
-                    gr[n] = a.q_pos[row * a.q_pos_row + what];
-                if (what == 3 && r >= left) gr[n] = INFINITY;  // no weights past the last row
+                    gr[n] = a.q_pos[row * a.q_pos_row + what - 2];
+                if (what == 0 && r >= left) gr[n] = INFINITY;  // no weights past the last row
             }
         };
         auto put = [&](int b) {
@@ -286,7 +289,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
             gd.store(sdo[b]);
 #pragma unroll
             for (int n = 0; n < 2; ++n)
-                if (n * 256 + threadIdx.x < 5 * QB) srow[b][n * 256 + threadIdx.x] = gr[n];
+                if (const int at = n * 256 + threadIdx.x; at >= 2 * QB && at < 5 * QB) {
+                    if (far) spos[b][at - 2 * QB] = Places<T>::row(gr[n]);
+                } else if (at < 2 * QB) {
+                    srow[b][at] = gr[n];
+                }
         };
         __syncthreads();
         if (steps > 0) {
@@ -306,13 +313,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
 #pragma unroll 1
                 for (int qb = 0; qb < QB / 32; ++qb) {
                     f32x16 d = {}, w = {}, u = {}, dp, lse;
-                    if (far) d = distances(srow[b], QB, qb * 32, lane, x, y, z);
+                    if (far) d = distances(place, spos[b], QB, qb * 32, lane);
                     if (far && !capped)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) w[r] = -far_unit * d[r];
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
-                        const float *p = srow[b] + 3 * QB + qb * 32 + 8 * n + 4 * (lane >> 5);
+                        const float *p = srow[b] + qb * 32 + 8 * n + 4 * (lane >> 5);
                         const f32x4 ls = *reinterpret_cast<const f32x4 *>(p);
                         const f32x4 de = *reinterpret_cast<const f32x4 *>(p + QB);
 #pragma unroll

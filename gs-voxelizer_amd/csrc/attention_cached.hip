@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, cons
     typedef typename Elem<T>::frag frag;
     static_assert(2 * kKeys * LD * sizeof(T) >= kHeads * DP * sizeof(float), "sums reuse the tiles");
     __shared__ __align__(16) T tiles[4][2 * kKeys * LD];
-    __shared__ __align__(16) float spos[4][3 * kKeys];
+    __shared__ __align__(16) typename Places<T>::Row spos[4][3 * kKeys];
     __shared__ float sm[4][kHeads], ss[4][kHeads];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -83,7 +83,8 @@ __global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, cons
         const float *p = a.q_pos + s * a.q_pos_row;
         x = p[0], y = p[1], z = p[2];
     }
-    x = own_side(x, lane), y = own_side(y, lane), z = own_side(z, lane);
+    Places<T> place;
+        place.set(x, y, z, lane);
     const T *kbase = static_cast<const T *>(a.k) + s * c.k_scene + hk * a.k_head;
     const T *vbase = static_cast<const T *>(a.v) + s * c.v_scene + hk * a.v_head;
     T *sk = tiles[wave], *sv = sk + kKeys * LD;
@@ -116,8 +117,8 @@ __global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, cons
         gk.store(sk, lane);
         gv.store(sv, lane);
         if (far) {
-            spos[wave][lane] = gp[0];
-            if (lane < kKeys) spos[wave][64 + lane] = gp[1];
+            spos[wave][lane] = Places<T>::row(gp[0]);
+            if (lane < kKeys) spos[wave][64 + lane] = Places<T>::row(gp[1]);
         }
         // the tile is this wave's own: its LDS accesses complete in order, only the
         // compiler has to keep them so
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, cons
                                                  keep_at(min(j0 + lane, j_end - 1)));
         if (j0 + 4 * kKeys < j_end) fetch(j0 + 4 * kKeys);
         f32x16 d = {}, w = {};
-        if (far) d = distances(spos[wave], kKeys, 0, lane, x, y, z);
+        if (far) d = distances(place, spos[wave], kKeys, 0, lane);
         if (far && !capped)
 #pragma unroll
             for (int r = 0; r < 16; ++r) w[r] = -far_unit * d[r];

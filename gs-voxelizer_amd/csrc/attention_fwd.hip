@@ -17,39 +17,52 @@ constexpr int kRows = 128;  // query rows of a workgroup
 // below 2^8, and a rescale of the sums (one multiply a register) is rare.
 constexpr float kSlack = 8.f;
 
-template <typename T> struct FwdTile { static constexpr int kKeys = sizeof(T) == 2 ? 64 : 32; };
+// HEADS query heads of a wave share its distances (a third of the vector work of one head: 2
+// multiply-adds, a multiply and a root an element, at the matrix units' differences).  With one
+// key head for both (SHARED) they share the tiles too.
+template <typename T, int DP, int HEADS> struct FwdTile {
+    static constexpr int kKeys = HEADS * DP * sizeof(T) >= 256 ? 32 : 64;
+};
 
-template <typename T, int DP, bool FAR, bool CAPPED>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const AttnArgs a, T *__restrict__ out,
-                                                       float *__restrict__ lse) {
-    constexpr int KB = FwdTile<T>::kKeys, LD = DP + Elem<T>::kPad;
+template <typename T, int DP, bool FAR, bool CAPPED, int HEADS, bool SHARED>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const AttnArgs a,
+                                                                         T *__restrict__ out,
+                                                                         float *__restrict__ lse) {
+    constexpr int KB = FwdTile<T, DP, HEADS>::kKeys, LD = DP + Elem<T>::kPad;
+    constexpr int KV = SHARED ? 1 : HEADS;  // key heads of the workgroup
+    constexpr bool far = FAR, capped = CAPPED;
     typedef typename Elem<T>::frag frag;
-    __shared__ __align__(16) T sk[2][KB * LD];
-    __shared__ __align__(16) T sv[2][KB * LD];
-    __shared__ __align__(16) float spos[2][3 * KB];
+    __shared__ __align__(16) T sk[2][KV][KB * LD];
+    __shared__ __align__(16) T sv[2][KV][KB * LD];
+    __shared__ __align__(16) typename Places<T>::Row spos[2][3 * KB];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // heads vary fastest: with eight (or a multiple) of them each XCD's L2 holds the keys
     // of its own heads
-    const int h = blockIdx.x % a.heads, rest = blockIdx.x / a.heads;
+    const int sets = a.heads / HEADS;
+    const int h0 = blockIdx.x % sets * HEADS, rest = blockIdx.x / sets;
     const int s = rest % a.scenes, slot = rest / a.scenes;
     const Scene c = scene_rows(a, s);
-    const int nq = c.q1 - c.q0, nk = c.k1 - c.k0;
+    const int nq = c.q1 - c.q0;
     const int tiles = (nq + kRows - 1) / kRows;
-    const int hk = h / (a.heads / a.kv_heads);
-    const T *kbase = static_cast<const T *>(a.k) + (int64_t)c.k0 * a.k_row + hk * a.k_head;
-    const T *vbase = static_cast<const T *>(a.v) + (int64_t)c.k0 * a.v_row + hk * a.v_head;
-    constexpr bool far = FAR, capped = CAPPED;
-    const float slope = slope_of(a, h);
+    const int group = a.heads / a.kv_heads;
+    const T *kbase[KV], *vbase[KV];
+#pragma unroll
+    for (int n = 0; n < KV; ++n) {
+        const int hk = (h0 + n) / group;
+        kbase[n] = static_cast<const T *>(a.k) + (int64_t)c.k0 * a.k_row + hk * a.k_head;
+        vbase[n] = static_cast<const T *>(a.v) + (int64_t)c.k0 * a.v_row + hk * a.v_head;
+    }
     // scores leave the matrix product in units of 1 / scale (or 1 where they are capped);
     // unit turns them into powers of two
     const float unit = capped ? kLog2e : a.scale * kLog2e;
-    const float far_unit = capped ? slope : slope / a.scale;
     const float in_cap = capped ? a.scale / a.cap : 0.f;
-
-    Staged<T, DP, KB> gk, gv;
-    gk.plan(a.k_row, a.dim);
-    gv.plan(a.v_row, a.dim);
+    float far_unit[HEADS];
+#pragma unroll
+    for (int n = 0; n < HEADS; ++n) far_unit[n] = slope_of(a, h0 + n) / (capped ? 1.f : a.scale);
+    Staged<T, DP, KB> gk[KV], gv[KV];
+#pragma unroll
+    for (int n = 0; n < KV; ++n) gk[n].plan(a.k_row, a.dim), gv[n].plan(a.v_row, a.dim);
 
     for (int tile = slot; tile < tiles; tile += a.slots) {
         // the last rows of a causal scene see the most keys: they start first
@@ -57,44 +70,54 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const A
         const int i = first + wave * 32 + (lane & 31);
         const bool row = i < nq;
         const int64_t qi = c.q0 + i;
-        frag q[DP / 16];
-        load_column<T, DP>(q, static_cast<const T *>(a.q) + qi * a.q_row + h * a.q_head, a.dim, row,
-                           lane);
-        float x = 0.f, y = 0.f, z = 0.f;
-        if (far && row) {
-            const float *p = a.q_pos + qi * a.q_pos_row;
-            x = p[0], y = p[1], z = p[2];
+        frag q[HEADS][DP / 16];
+#pragma unroll
+        for (int n = 0; n < HEADS; ++n)
+            load_column<T, DP>(q[n], static_cast<const T *>(a.q) + qi * a.q_row + (h0 + n) * a.q_head,
+                               a.dim, row, lane);
+        Places<T> place;
+        if (far) {
+            float x = 0.f, y = 0.f, z = 0.f;
+            if (row) {
+                const float *p = a.q_pos + qi * a.q_pos_row;
+                x = p[0], y = p[1], z = p[2];
+            }
+            place.set(x, y, z, lane);
         }
-        x = own_side(x, lane), y = own_side(y, lane), z = own_side(z, lane);
         const int limit = row ? key_limit(a, c, i) : 0;
         const int all = first + wave * 32 + 31 < nq ? key_limit(a, c, first + wave * 32) : 0;
         const int most = key_limit(a, c, min(first + kRows, nq) - 1);  // of the workgroup
         const int mine = first + wave * 32 < nq
                              ? key_limit(a, c, min(first + wave * 32 + 32, nq) - 1) : 0;
-        f32x16 o[DP / 32] = {};
-        float m = -INFINITY, sum = 0.f;
+        f32x16 o[HEADS][DP / 32] = {};
+        float m[HEADS], sum[HEADS];
+#pragma unroll
+        for (int n = 0; n < HEADS; ++n) m[n] = -INFINITY, sum[n] = 0.f;
 
         float gp = 0.f;
         bool gl = true;
         uint64_t live = ~0ull;
         auto fetch = [&](int j0) {
             const int left = most - j0;
-            gk.load(kbase + j0 * a.k_row, a.k_row, a.dim, left);
-            gv.load(vbase + j0 * a.v_row, a.v_row, a.dim, left);
+#pragma unroll
+            for (int n = 0; n < KV; ++n) {
+                gk[n].load(kbase[n] + j0 * a.k_row, a.k_row, a.dim, left);
+                gv[n].load(vbase[n] + j0 * a.v_row, a.v_row, a.dim, left);
+            }
             if (far && threadIdx.x < 3 * KB)
                 gp = a.k_pos[(c.k0 + j0 + min((int)threadIdx.x % KB, left - 1)) * a.k_pos_row +
                              threadIdx.x / KB];
             if (a.keep) gl = lane < KB && lane < left && kept(a, c.k0 + j0 + lane);
         };
         auto put = [&](int b) {
-            if (a.keep) {
-                live = __ballot(gl);
-                gk.keep(live);
-                gv.keep(live);
+            if (a.keep) live = __ballot(gl);
+#pragma unroll
+            for (int n = 0; n < KV; ++n) {
+                if (a.keep) gk[n].keep(live), gv[n].keep(live);
+                gk[n].store(sk[b][n]);
+                gv[n].store(sv[b][n]);
             }
-            gk.store(sk[b]);
-            gv.store(sv[b]);
-            if (far && threadIdx.x < 3 * KB) spos[b][threadIdx.x] = gp;
+            if (far && threadIdx.x < 3 * KB) spos[b][threadIdx.x] = Places<T>::row(gp);
         };
         __syncthreads();  // the previous tile's last reads
         if (most > 0) {
@@ -110,68 +133,88 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const A
                 const bool masked = j0 + KB > all || (KB == 64 ? ~live : (uint32_t)~live) != 0;
 #pragma unroll 1
                 for (int kb = 0; kb < KB / 32; ++kb) {
-                    f32x16 d = {}, w = {};
-                    if (far) d = distances(spos[b], KB, kb * 32, lane, x, y, z);
-                    if (far && !capped)
+                    f32x16 d = {}, w[HEADS] = {};
+                    if (far) d = distances<T>(place, spos[b], KB, kb * 32, lane);
+                    const int at0 = (kb * 32 + (lane & 31)) * LD + 8 * (lane >> 5);
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) w[r] = -far_unit * d[r];
-                    const T *krow = sk[b] + (kb * 32 + (lane & 31)) * LD + 8 * (lane >> 5);
+                    for (int n = 0; n < HEADS; ++n) {
+                        if (far && !capped)
 #pragma unroll
-                    for (int st = 0; st < DP / 16; ++st) w = mma(row_frag(krow + st * 16), q[st], w);
-                    if (capped)
+                            for (int r = 0; r < 16; ++r) w[n][r] = -far_unit[n] * d[r];
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            w[r] = a.cap * tanh_of<T>(w[r] * in_cap);
-                            if (far) w[r] = fmaf(-far_unit, d[r], w[r]);
-                        }
+                        for (int st = 0; st < DP / 16; ++st)
+                            w[n] = mma(row_frag(sk[b][SHARED ? 0 : n] + at0 + st * 16), q[n][st], w[n]);
+                        if (capped)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                w[n][r] = a.cap * tanh_of<T>(w[n][r] * in_cap);
+                                if (far) w[n][r] = fmaf(-far_unit[n], d[r], w[n][r]);
+                            }
+                    }
                     if (masked) {
                         const uint32_t bits = (uint32_t)(live >> (kb * 32)) >> (4 * (lane >> 5));
                         const int lim = limit - j0 - kb * 32 - 4 * (lane >> 5);
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const int at = 8 * (r >> 2) + (r & 3);
-                            if (at >= lim || !((bits >> at) & 1)) w[r] = -INFINITY;
+                            if (at >= lim || !((bits >> at) & 1))
+#pragma unroll
+                                for (int n = 0; n < HEADS; ++n) w[n][r] = -INFINITY;
                         }
                     }
-                    float top = -INFINITY;
+                    float top[HEADS];
+                    bool grown = false;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) top = fmaxf(top, w[r]);
-                    top *= unit;
-                    if (__any(top > m + kSlack)) {
-                        const float next = fmaxf(m, fmaxf(top, other_half(top)));
-                        const float by = next == -INFINITY ? 1.f : fast_exp2(m - next);
-                        m = next;
-                        sum *= by;
+                    for (int n = 0; n < HEADS; ++n) {
+                        top[n] = -INFINITY;
 #pragma unroll
-                        for (int n = 0; n < DP / 32; ++n) o[n] *= by;
+                        for (int r = 0; r < 16; ++r) top[n] = fmaxf(top[n], w[n][r]);
+                        top[n] *= unit;
+                        grown |= top[n] > m[n] + kSlack;
                     }
-                    const float ref = m == -INFINITY ? 0.f : m;
+                    if (__any(grown)) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        w[r] = fast_exp2(fmaf(w[r], unit, -ref));
-                        sum += w[r];
+                        for (int n = 0; n < HEADS; ++n) {
+                            const float next = fmaxf(m[n], fmaxf(top[n], other_half(top[n])));
+                            const float by = next == -INFINITY ? 1.f : fast_exp2(m[n] - next);
+                            m[n] = next;
+                            sum[n] *= by;
+#pragma unroll
+                            for (int e = 0; e < DP / 32; ++e) o[n][e] *= by;
+                        }
                     }
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const frag p = to_frag<T>(w, half);
+                    for (int n = 0; n < HEADS; ++n) {
+                        const float ref = m[n] == -INFINITY ? 0.f : m[n];
 #pragma unroll
-                        for (int n = 0; n < DP / 32; ++n)
-                            o[n] = mma(tr_frag<LD>(sv[b] + (kb * 32 + half * 16) * LD + n * 32, lane),
-                                       p, o[n]);
+                        for (int r = 0; r < 16; ++r) {
+                            w[n][r] = fast_exp2(fmaf(w[n][r], unit, -ref));
+                            sum[n] += w[n][r];
+                        }
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const frag p = to_frag<T>(w[n], half);
+                            const T *vt = sv[b][SHARED ? 0 : n] + (kb * 32 + half * 16) * LD;
+#pragma unroll
+                            for (int e = 0; e < DP / 32; ++e)
+                                o[n][e] = mma(tr_frag<LD>(vt + e * 32, lane), p, o[n][e]);
+                        }
                     }
                 }
             }
             if (more) put(b ^ 1);
             __syncthreads();
         }
-        sum += other_half(sum);
-        if (row) {
-            store_column<T, DP>(out + (qi * a.heads + h) * a.dim, o, sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum),
-                                a.dim, lane);
+#pragma unroll
+        for (int n = 0; n < HEADS; ++n) {
+            sum[n] += other_half(sum[n]);
+            if (!row) continue;
+            store_column<T, DP>(out + (qi * a.heads + h0 + n) * a.dim, o[n],
+                                sum[n] == 0.f ? 0.f : 1.f / sum[n], a.dim, lane);
             // log2 of the row's sum of exponentials; +inf for an empty row, whose weights
             // in the backward are exp2(-inf)
             if (lse && lane < 32)
-                lse[(int64_t)h * a.q_tokens + qi] = sum == 0.f ? INFINITY : m + log2f(sum);
+                lse[(int64_t)(h0 + n) * a.q_tokens + qi] = sum[n] == 0.f ? INFINITY : m[n] + log2f(sum[n]);
         }
     }
 }
@@ -181,10 +224,20 @@ struct Forward {
     void *out;
     float *lse;
     hipStream_t st;
+    template <typename T, int DP, bool FAR, bool CAPPED, int HEADS, bool SHARED> void start() const {
+        hipLaunchKernelGGL((k_attention_fwd<T, DP, FAR, CAPPED, HEADS, SHARED>),
+                           dim3((unsigned)a.slots * a.scenes * (a.heads / HEADS)), dim3(256), 0, st,
+                           a, static_cast<T *>(out), lse);
+    }
     template <typename T, int DP, bool FAR, bool CAPPED> void run() const {
-        hipLaunchKernelGGL((k_attention_fwd<T, DP, FAR, CAPPED>),
-                           dim3((unsigned)a.slots * a.scenes * a.heads), dim3(256), 0, st, a,
-                           static_cast<T *>(out), lse);
+        if constexpr (FAR && sizeof(T) == 2 && DP <= 64) {
+            if (attention_pairs(a)) {
+                if (a.heads / a.kv_heads % 2 == 0) start<T, DP, FAR, CAPPED, 2, true>();
+                else start<T, DP, FAR, CAPPED, 2, false>();
+                return;
+            }
+        }
+        start<T, DP, FAR, CAPPED, 1, true>();
     }
 };
 

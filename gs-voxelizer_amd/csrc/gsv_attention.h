@@ -136,6 +136,9 @@ template <typename F> void attention_variant(const AttnArgs &a, int dtype, const
     else attention_channels<float>(a, f);
 }
 
+// Whether a wave takes two heads (for their distances): an even number of them.
+inline bool attention_pairs(const AttnArgs &a) { return a.heads % 2 == 0; }
+
 // Workgroups for each scene and head: one for each tile of the longest scene, fewer where the
 // launch would pass a million (they take the tiles in turn, so any number is right).
 inline bool attention_slots(AttnArgs *a, int longest, int rows, int heads) {
@@ -254,24 +257,60 @@ __device__ __forceinline__ void store_column(T *row, const f32x16 (&o)[DP / 32],
         }
 }
 
-// What a lane adds to the products below: 1 for the other side's coordinate, or minus its own.
-__device__ __forceinline__ float own_side(float x, int lane) { return lane < 32 ? 1.f : -x; }
+// Positions for distances: differences of two sides' coordinates formed by the matrix units.
+// float32: x_row * 1 + 1 * -x_column, one v_mfma_f32_32x32x2_f32 an axis, the rounding of a
+// subtraction.  bfloat16: each coordinate as the exact sum of three bfloat16 (24 bits), so a
+// difference is six exact products with one, in one v_mfma_f32_32x32x16_bf16 an axis; the
+// products' sum is rounded like a binary32 sum of six terms.  That form runs beside the vector
+// instructions, where 48 subtractions a block would queue with them (the float32 matrix
+// instructions do not: they share the vector units, measured).
+template <typename T> struct Places;
 
-// Distances of the lanes' columns (own_side of x, y, z) to the 32 rows of a block, in the result's
-// layout; xyz: three arrays of `n` floats in LDS, `first` the block's first row in them.  A
-// difference is a product of two terms, x_row * 1 + 1 * -x_column, one v_mfma_f32_32x32x2_f32 an
-// axis: the rounding of a subtraction, but 48 vector instructions a block fewer and one LDS word a
-// lane and axis instead of four times four.
-__device__ __forceinline__ f32x16 distances(const float *xyz, int n, int first, int lane, float x,
-                                            float y, float z) {
-    const float *p = xyz + first + (lane & 31);
-    const float c[3] = {x, y, z};
+template <> struct Places<float> {
+    typedef float Row;
+    float own[3];
+    static __device__ __forceinline__ Row row(float x) { return x; }
+    __device__ __forceinline__ void set(float x, float y, float z, int lane) {
+        own[0] = lane < 32 ? 1.f : -x, own[1] = lane < 32 ? 1.f : -y, own[2] = lane < 32 ? 1.f : -z;
+    }
+    __device__ __forceinline__ f32x16 minus(Row r, int ax, int lane) const {
+        return __builtin_amdgcn_mfma_f32_32x32x2f32(lane < 32 ? r : 1.f, own[ax], f32x16{}, 0, 0, 0);
+    }
+};
+
+template <> struct Places<bf16> {
+    typedef bf16x8 Row;
+    bf16x8 own[3];
+    static __device__ __forceinline__ Row row(float x) {
+        const bf16 a = (bf16)x;
+        x -= (float)a;
+        const bf16 b = (bf16)x, c = (bf16)(x - (float)b), one = (bf16)1.f, no = (bf16)0.f;
+        return bf16x8{a, b, c, one, one, one, no, no};
+    }
+    // the upper lanes' contraction indices meet zeros
+    __device__ __forceinline__ void set(float x, float y, float z, int lane) {
+        const float c[3] = {x, y, z};
+#pragma unroll
+        for (int ax = 0; ax < 3; ++ax) {
+            const bf16x8 r = row(-c[ax]);
+            own[ax] = lane < 32 ? bf16x8{r[3], r[4], r[5], r[0], r[1], r[2], r[6], r[7]} : bf16x8{};
+        }
+    }
+    __device__ __forceinline__ f32x16 minus(Row r, int ax, int) const {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(r, own[ax], f32x16{}, 0, 0, 0);
+    }
+};
+
+// Distances of the lanes' columns to the 32 rows of a block, in the result's layout; xyz: three
+// arrays of `n` rows in LDS, `first` the block's first row in them.
+template <typename T>
+__device__ __forceinline__ f32x16 distances(const Places<T> &to, const typename Places<T>::Row *xyz,
+                                            int n, int first, int lane) {
+    const typename Places<T>::Row *p = xyz + first + (lane & 31);
     f32x16 d;
 #pragma unroll
     for (int ax = 0; ax < 3; ++ax) {
-        const float at = p[ax * n];
-        const f32x16 e =
-            __builtin_amdgcn_mfma_f32_32x32x2f32(lane < 32 ? at : 1.f, c[ax], f32x16{}, 0, 0, 0);
+        const f32x16 e = to.minus(p[ax * n], ax, lane);
 #pragma unroll
         for (int r = 0; r < 16; ++r) d[r] = ax ? fmaf(e[r], e[r], d[r]) : e[r] * e[r];
     }
