@@ -16,7 +16,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRows = 128;  // rows (dq) or keys (dk, dv) of a workgroup, 32 a wave
 
-template <typename T> struct BwdTile { static constexpr int kOther = sizeof(T) == 2 ? 64 : 32; };
+// Rows of the other side in a tile.
+template <typename T> constexpr int kOther = sizeof(T) == 2 ? 64 : 32;
 
 struct BwdArgs {
     const void *out, *dout;
@@ -27,26 +28,29 @@ struct BwdArgs {
     void *dq, *dk, *dv;
 };
 
-// dt (before the cap's factor) and ds of a block from its scores w, as the matrix product
-// leaves them, and dp - D.
-template <typename T>
-__device__ __forceinline__ void weigh(f32x16 &w, f32x16 &u, const f32x16 &d, bool capped, bool far,
-                                      float in_cap, float cap, float far_unit) {
-    if (!capped) return;
+// A block's scores from the matrix product: capped (u: the tanh), with their bias.
+template <typename T, bool FAR, bool CAPPED>
+__device__ __forceinline__ void finish_scores(f32x16 &w, f32x16 &u, const f32x16 &d, float in_cap,
+                                              float cap, float far_unit) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        u[r] = tanh_of<T>(w[r] * in_cap);
-        w[r] = cap * u[r];
-        if (far) w[r] = fmaf(-far_unit, d[r], w[r]);
+        if (CAPPED) {
+            u[r] = tanh_of<T>(w[r] * in_cap);
+            w[r] = cap * u[r];
+        }
+        if (FAR) w[r] = fmaf(-far_unit, d[r], w[r]);
     }
 }
 
+// dq, D and dslope.  A wave's lanes are query rows, as in the forward.
 template <typename T, int DP, bool FAR, bool CAPPED>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const AttnArgs a, const BwdArgs g) {
-    constexpr int KB = BwdTile<T>::kOther, LD = DP + Elem<T>::kPad;
+__global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_attention_dq(
+    const AttnArgs a, const BwdArgs g) {
+    constexpr int KB = kOther<T>, WAVES = 4;
+    constexpr bool far = FAR, capped = CAPPED;
     typedef typename Elem<T>::frag frag;
-    __shared__ __align__(16) T sk[2][KB * LD];
-    __shared__ __align__(16) T sv[2][KB * LD];
+    __shared__ __align__(1024) T sk[2][KB * DP];
+    __shared__ __align__(1024) T sv[2][KB * DP];
     __shared__ __align__(16) typename Places<T>::Row spos[2][3 * KB];
     __shared__ double sums[4];
 
@@ -59,16 +63,15 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
     const int hk = h / (a.heads / a.kv_heads);
     const T *kbase = static_cast<const T *>(a.k) + (int64_t)c.k0 * a.k_row + hk * a.k_head;
     const T *vbase = static_cast<const T *>(a.v) + (int64_t)c.k0 * a.v_row + hk * a.v_head;
-    constexpr bool far = FAR, capped = CAPPED;
-    const float slope = slope_of(a, h);
     const float unit = capped ? kLog2e : a.scale * kLog2e;
-    const float far_unit = capped ? slope : slope / a.scale;
     const float in_cap = capped ? a.scale / a.cap : 0.f;
+    const float far_unit = slope_of(a, h) / (capped ? 1.f : a.scale);
     double dslope = 0.0;
-
-    Staged<T, DP, KB> gk, gv;
-    gk.plan(a.k_row, a.dim);
-    gv.plan(a.v_row, a.dim);
+    Tile<T, DP> at;
+    at.plan(lane);
+    Copy<T, DP, KB, WAVES> ck, cv;
+    ck.plan(a.k_row, a.dim, wave, lane);
+    cv.plan(a.v_row, a.dim, wave, lane);
 
     for (int tile = slot; tile < tiles; tile += a.slots) {
         const int first = (tiles - 1 - tile) * kRows;
@@ -80,30 +83,29 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
                            lane);
         load_column<T, DP>(dO, static_cast<const T *>(g.dout) + qi * g.dout_row + h * g.dout_head,
                            a.dim, row, lane);
-        float delta = 0.f, lse = INFINITY, x = 0.f, y = 0.f, z = 0.f;
-        {
-            const T *o = static_cast<const T *>(g.out) + (qi * a.heads + h) * a.dim;
+        const T *o = static_cast<const T *>(g.out) + (qi * a.heads + h) * a.dim;
+        float delta = 0.f;
 #pragma unroll
-            for (int st = 0; st < DP / 16; ++st) {
-                const int d = st * 16 + 8 * (lane >> 5);
-                if (row && d < a.dim) {
-                    const frag f = row_frag(o + d);
+        for (int st = 0; st < DP / 16; ++st) {
+            const int d = st * 16 + 8 * (lane >> 5);
+            if (row && d < a.dim) {
+                const frag f = row_frag(o + d);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) delta = fmaf((float)f[e], (float)dO[st][e], delta);
-                }
+                for (int e = 0; e < 8; ++e) delta = fmaf((float)f[e], (float)dO[st][e], delta);
             }
         }
         delta += other_half(delta);
-        if (row) {
-            if (lane < 32) g.delta[(int64_t)h * a.q_tokens + qi] = delta;
-            lse = g.lse[(int64_t)h * a.q_tokens + qi];
-            if (far) {
+        if (row && lane < 32) g.delta[(int64_t)h * a.q_tokens + qi] = delta;
+        const float lse = row ? g.lse[(int64_t)h * a.q_tokens + qi] : INFINITY;
+        Places<T> place;
+        if (far) {
+            float x = 0.f, y = 0.f, z = 0.f;
+            if (row) {
                 const float *p = a.q_pos + qi * a.q_pos_row;
                 x = p[0], y = p[1], z = p[2];
             }
+            place.set(x, y, z, lane);
         }
-        Places<T> place;
-        place.set(x, y, z, lane);
         const int limit = row ? key_limit(a, c, i) : 0;
         const int all = first + wave * 32 + 31 < nq ? key_limit(a, c, first + wave * 32) : 0;
         const int most = key_limit(a, c, min(first + kRows, nq) - 1);
@@ -112,71 +114,67 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
         f32x16 dq[DP / 32] = {};
 
         float gp = 0.f;
-        bool gl = true;
-        uint64_t live = ~0ull;
-        auto fetch = [&](int j0) {
+        int raw = 0;
+        uint64_t live = ~0ull, next_live = ~0ull;
+        auto look = [&](int j0) {  // the mask of a tile
+            if (a.keep && j0 < most) raw = keep_raw(a, c.k0 + min(j0 + lane, most - 1));
+        };
+        auto fetch = [&](int b, int j0) {
             const int left = most - j0;
-            gk.load(kbase + j0 * a.k_row, a.k_row, a.dim, left);
-            gv.load(vbase + j0 * a.v_row, a.v_row, a.dim, left);
+            if (a.keep) next_live = __ballot(raw != 0);
+            look(j0 + KB);
+            ck.start(sk[b], kbase + j0 * a.k_row, a.k_row, a.dim, left, a.keep, next_live, wave, lane);
+            cv.start(sv[b], vbase + j0 * a.v_row, a.v_row, a.dim, left, a.keep, next_live, wave, lane);
             if (far && threadIdx.x < 3 * KB)
                 gp = a.k_pos[(c.k0 + j0 + min((int)threadIdx.x % KB, left - 1)) * a.k_pos_row +
                              threadIdx.x / KB];
-            if (a.keep) gl = lane < KB && lane < left && kept(a, c.k0 + j0 + lane);
         };
         auto put = [&](int b) {
-            if (a.keep) {
-                live = __ballot(gl);
-                gk.keep(live);
-                gv.keep(live);
-            }
-            gk.store(sk[b]);
-            gv.store(sv[b]);
             if (far && threadIdx.x < 3 * KB) spos[b][threadIdx.x] = Places<T>::row(gp);
+            tile_wait();
         };
         __syncthreads();
         if (most > 0) {
-            fetch(0);
+            look(0);
+            fetch(0, 0);
             put(0);
         }
         __syncthreads();
         int b = 0;
         for (int j0 = 0; j0 < most; j0 += KB, b ^= 1) {
             const bool more = j0 + KB < most;
-            if (more) fetch(j0 + KB);
+            live = next_live;
+            if (more) fetch(b ^ 1, j0 + KB);
             if (j0 < mine) {
                 const bool masked = j0 + KB > all || (KB == 64 ? ~live : (uint32_t)~live) != 0;
                 float here = 0.f;
 #pragma unroll 1
                 for (int kb = 0; kb < KB / 32; ++kb) {
-                    f32x16 d = {}, w = {}, u = {}, dp;
-                    if (far) d = distances(place, spos[b], KB, kb * 32, lane);
-                    if (far && !capped)
+                    f32x16 d = {};
+                    uint32_t seen = 0;
+                    if (far) d = distances<T>(place, spos[b], KB, kb * 32, lane);
+                    if (masked) {
+                        seen = seen_rows(live, kb, limit - j0 - kb * 32, lane);
+                        if (far)  // a masked key's position may be anything
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) w[r] = -far_unit * d[r];
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) dp[r] = -delta;
-                    const int at0 = (kb * 32 + (lane & 31)) * LD + 8 * (lane >> 5);
+                            for (int r = 0; r < 16; ++r)
+                                if (!(seen & (1u << result_row(r)))) d[r] = 0.f;
+                    }
+                    f32x16 w = {}, u = {}, dp = {};
+                    const T *kt = sk[b] + kb * 32 * DP, *vt = sv[b] + kb * 32 * DP;
 #pragma unroll
                     for (int st = 0; st < DP / 16; ++st) {
-                        w = mma(row_frag(sk[b] + at0 + st * 16), q[st], w);
-                        dp = mma(row_frag(sv[b] + at0 + st * 16), dO[st], dp);
+                        w = mma(at.rows(kt, st), q[st], w);
+                        dp = mma(at.rows(vt, st), dO[st], dp);
                     }
-                    weigh<T>(w, u, d, capped, far, in_cap, a.cap, far_unit);
-                    if (masked) {
-                        const uint32_t bits = (uint32_t)(live >> (kb * 32)) >> (4 * (lane >> 5));
-                        const int lim = limit - j0 - kb * 32 - 4 * (lane >> 5);
+                    finish_scores<T, FAR, CAPPED>(w, u, d, in_cap, a.cap, far_unit);
+                    if (masked)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int at = 8 * (r >> 2) + (r & 3);
-                            if (at >= lim || !((bits >> at) & 1)) {
-                                w[r] = -INFINITY;
-                                if (far) d[r] = 0.f;  // a masked key's position may be anything
-                            }
-                        }
-                    }
+                        for (int r = 0; r < 16; ++r)
+                            if (!(seen & (1u << result_row(r)))) w[r] = -INFINITY;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        dp[r] *= fast_exp2(fmaf(w[r], unit, -lse));
+                        dp[r] = (dp[r] - delta) * fast_exp2(fmaf(w[r], unit, -lse));
                         if (far) here = fmaf(dp[r], d[r], here);
                         if (capped) dp[r] *= fmaf(-u[r], u[r], 1.f);
                     }
@@ -184,9 +182,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
                     for (int half = 0; half < 2; ++half) {
                         const frag ds = to_frag<T>(dp, half);
 #pragma unroll
-                        for (int n = 0; n < DP / 32; ++n)
-                            dq[n] = mma(tr_frag<LD>(sk[b] + (kb * 32 + half * 16) * LD + n * 32, lane),
-                                        ds, dq[n]);
+                        for (int e = 0; e < DP / 32; ++e)
+                            dq[e] = mma(at.columns(kt + half * 16 * DP, e, lane), ds, dq[e]);
                     }
                 }
                 dslope -= here;
@@ -195,26 +192,25 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dq(const At
             __syncthreads();
         }
         if (row)
-            store_column<T, DP>(static_cast<T *>(g.dq) + (qi * a.heads + h) * a.dim, dq, a.scale,
-                                a.dim, lane);
+            store_column<T, DP>(static_cast<T *>(g.dq) + (qi * a.heads + h) * a.dim, dq, a.scale, a.dim,
+                                lane);
     }
-    if (far) {
+    if (!far) return;
 #pragma unroll
-        for (int n = 1; n < 64; n <<= 1) dslope += __shfl_xor(dslope, n);
-        __syncthreads();
-        if (lane == 0) sums[wave] = dslope;
-        __syncthreads();
-        if (threadIdx.x == 0)
-            g.dslope[(int64_t)rest * a.heads + h] = (float)(sums[0] + sums[1] + sums[2] + sums[3]);
-    }
+    for (int k = 1; k < 64; k <<= 1) dslope += __shfl_xor(dslope, k);
+    if (lane == 0) sums[wave] = dslope;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        g.dslope[(int64_t)rest * a.heads + h] = (float)(sums[0] + sums[1] + sums[2] + sums[3]);
 }
 
+// dk and dv.  A wave's lanes are keys; the rows of all query heads of the key head pass by.
 template <typename T, int DP, bool FAR, bool CAPPED>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const AttnArgs a, const BwdArgs g) {
-    constexpr int QB = BwdTile<T>::kOther, LD = DP + Elem<T>::kPad;
+    constexpr int QB = kOther<T>, WAVES = 4;
     typedef typename Elem<T>::frag frag;
-    __shared__ __align__(16) T sq[2][QB * LD];
-    __shared__ __align__(16) T sdo[2][QB * LD];
+    __shared__ __align__(1024) T sq[2][QB * DP];
+    __shared__ __align__(1024) T sdo[2][QB * DP];
     __shared__ __align__(16) typename Places<T>::Row spos[2][3 * QB];
     __shared__ __align__(16) float srow[2][2 * QB];  // log sums, D
 
@@ -229,9 +225,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
     const float unit = capped ? kLog2e : a.scale * kLog2e;
     const float in_cap = capped ? a.scale / a.cap : 0.f;
 
-    Staged<T, DP, QB> gq, gd;
-    gq.plan(a.q_row, a.dim);
-    gd.plan(g.dout_row, a.dim);
+    Tile<T, DP> tl;
+    tl.plan(lane);
+    Copy<T, DP, QB, WAVES> cq, cd;
+    cq.plan(a.q_row, a.dim, wave, lane);
+    cd.plan(g.dout_row, a.dim, wave, lane);
 
     for (int tile = slot; tile < tiles; tile += a.slots) {
         const int first = tile * kRows;
@@ -264,13 +262,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
         f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
 
         float gr[2] = {};
-        auto fetch = [&](int step) {
-            const int h = hk * group + step / per_head, i0 = q_from + step % per_head * QB;
+        auto fetch = [&](int b, int step) {
+            const int h = hk * group + step % group, i0 = q_from + step / group * QB;
             const int64_t q0 = c.q0 + i0;
             const int left = nq - i0;
-            gq.load(static_cast<const T *>(a.q) + q0 * a.q_row + h * a.q_head, a.q_row, a.dim, left);
-            gd.load(static_cast<const T *>(g.dout) + q0 * g.dout_row + h * g.dout_head, g.dout_row,
-                    a.dim, left);
+            cq.start(sq[b], static_cast<const T *>(a.q) + q0 * a.q_row + h * a.q_head, a.q_row, a.dim,
+                     left, false, 0, wave, lane);
+            cd.start(sdo[b], static_cast<const T *>(g.dout) + q0 * g.dout_row + h * g.dout_head,
+                     g.dout_row, a.dim, left, false, 0, wave, lane);
             // log sums, D and positions of the rows, five arrays in turn
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
@@ -285,8 +284,6 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
             }
         };
         auto put = [&](int b) {
-            gq.store(sq[b]);
-            gd.store(sdo[b]);
 #pragma unroll
             for (int n = 0; n < 2; ++n)
                 if (const int at = n * 256 + threadIdx.x; at >= 2 * QB && at < 5 * QB) {
@@ -294,29 +291,27 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
                 } else if (at < 2 * QB) {
                     srow[b][at] = gr[n];
                 }
+            tile_wait();
         };
         __syncthreads();
         if (steps > 0) {
-            fetch(0);
+            fetch(0, 0);
             put(0);
         }
         __syncthreads();
         int b = 0;
         for (int step = 0; step < steps; ++step, b ^= 1) {
             const bool more = step + 1 < steps;
-            if (more) fetch(step + 1);
-            const int i0 = q_from + step % per_head * QB;
+            if (more) fetch(b ^ 1, step + 1);
+            const int i0 = q_from + step / group * QB;
             if (i0 + QB > wave_from && first + wave * 32 < nk) {
-                const float slope = slope_of(a, hk * group + step / per_head);
+                const float slope = slope_of(a, hk * group + step % group);
                 const float far_unit = capped ? slope : slope / a.scale;
                 const bool masked = i0 < wave_all;
 #pragma unroll 1
                 for (int qb = 0; qb < QB / 32; ++qb) {
                     f32x16 d = {}, w = {}, u = {}, dp, lse;
-                    if (far) d = distances(place, spos[b], QB, qb * 32, lane);
-                    if (far && !capped)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) w[r] = -far_unit * d[r];
+                    if (far) d = distances<T>(place, spos[b], QB, qb * 32, lane);
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
                         const float *p = srow[b] + qb * 32 + 8 * n + 4 * (lane >> 5);
@@ -325,18 +320,17 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
 #pragma unroll
                         for (int e = 0; e < 4; ++e) lse[4 * n + e] = ls[e], dp[4 * n + e] = -de[e];
                     }
-                    const int at0 = (qb * 32 + (lane & 31)) * LD + 8 * (lane >> 5);
 #pragma unroll
                     for (int st = 0; st < DP / 16; ++st) {
-                        w = mma(row_frag(sq[b] + at0 + st * 16), k[st], w);
-                        dp = mma(row_frag(sdo[b] + at0 + st * 16), v[st], dp);
+                        w = mma(tl.rows(sq[b] + qb * 32 * DP, st), k[st], w);
+                        dp = mma(tl.rows(sdo[b] + qb * 32 * DP, st), v[st], dp);
                     }
-                    weigh<T>(w, u, d, capped, far, in_cap, a.cap, far_unit);
+                    finish_scores<T, FAR, CAPPED>(w, u, d, in_cap, a.cap, far_unit);
                     if (masked) {
                         const int lo = from == INT32_MAX ? from : from - i0 - qb * 32 - 4 * (lane >> 5);
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
-                            if (8 * (r >> 2) + (r & 3) < lo) w[r] = -INFINITY;
+                            if (result_row(r) < lo) w[r] = -INFINITY;
                     }
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
@@ -347,11 +341,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const frag p = to_frag<T>(w, half), ds = to_frag<T>(dp, half);
-                        const int at = (qb * 32 + half * 16) * LD;
+                        const int at = (qb * 32 + half * 16) * DP;
 #pragma unroll
                         for (int n = 0; n < DP / 32; ++n) {
-                            dv[n] = mma(tr_frag<LD>(sdo[b] + at + n * 32, lane), p, dv[n]);
-                            dk[n] = mma(tr_frag<LD>(sq[b] + at + n * 32, lane), ds, dk[n]);
+                            dv[n] = mma(tl.columns(sdo[b] + at, n, lane), p, dv[n]);
+                            dk[n] = mma(tl.columns(sq[b] + at, n, lane), ds, dk[n]);
                         }
                     }
                 }
@@ -449,7 +443,8 @@ extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, con
     float *part = reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(a));
     const BwdArgs g{out, dout, dout_row, dout_head, lse, delta, part, dq, dk, dv};
     hipStream_t s = as_stream(stream);
-    attention_variant(a, args->dtype, Backward{a, g, kslots, s});
+    Backward f{a, g, kslots, s};
+    attention_variant(a, args->dtype, f);
     if (a.slopes)
         hipLaunchKernelGGL(k_slope_sum, dim3(a.heads), dim3(64), 0, s, part,
                            a.q_tokens > 0 ? a.slots * a.scenes : 0, a.heads, dslopes, a.slopes_f32);

@@ -23,38 +23,18 @@ struct CacheArgs {
     float2 *part_ms; // (scenes, heads, splits): maximum (log2) and sum of weights
 };
 
-// 32 rows of a head on their way to one wave's LDS: 64 lanes, 16-byte chunks.
-template <typename T, int DP> struct WaveStaged {
-    static constexpr int kCh = Elem<T>::kChunk, kPerRow = DP / kCh, kN = kKeys * kPerRow / 64;
-    uint4 r[kN];
-    template <typename Live>
-    __device__ __forceinline__ void load(const T *base, int64_t stride, int dim, int lane, Live live) {
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            const int c = i * 64 + lane, row = c / kPerRow, col = (c % kPerRow) * kCh;
-            r[i] = make_uint4(0, 0, 0, 0);
-            if (col < dim && live(row))
-                r[i] = *reinterpret_cast<const uint4 *>(base + row * stride + col);
-        }
-    }
-    __device__ __forceinline__ void store(T *tile, int lane) const {
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            const int c = i * 64 + lane, row = c / kPerRow, col = (c % kPerRow) * kCh;
-            *reinterpret_cast<uint4 *>(tile + row * (DP + Elem<T>::kPad) + col) = r[i];
-        }
-    }
-};
+// Waves of a workgroup: four, two where their tiles would pass the LDS of a CU.
+template <typename T, int DP> constexpr int kWaves = DP * sizeof(T) > 256 ? 2 : 4;
 
 template <typename T, int DP, bool FAR, bool CAPPED>
-__global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, const CacheArgs c,
+__global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const AttnArgs a, const CacheArgs c,
                                                           T *__restrict__ out) {
-    constexpr int LD = DP + Elem<T>::kPad;
     typedef typename Elem<T>::frag frag;
-    static_assert(2 * kKeys * LD * sizeof(T) >= kHeads * DP * sizeof(float), "sums reuse the tiles");
-    __shared__ __align__(16) T tiles[4][2 * kKeys * LD];
-    __shared__ __align__(16) typename Places<T>::Row spos[4][3 * kKeys];
-    __shared__ float sm[4][kHeads], ss[4][kHeads];
+    constexpr int W = kWaves<T, DP>;
+    static_assert(4 * kKeys * DP * sizeof(T) >= kHeads * DP * sizeof(float), "sums reuse the tiles");
+    __shared__ __align__(1024) T tiles[W][4 * kKeys * DP];  // a wave's keys and values, two buffers
+    __shared__ __align__(16) typename Places<T>::Row spos[W][2][3 * kKeys];
+    __shared__ float sm[W][kHeads], ss[W][kHeads];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int group = a.heads / a.kv_heads;
@@ -87,55 +67,67 @@ __global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, cons
         place.set(x, y, z, lane);
     const T *kbase = static_cast<const T *>(a.k) + s * c.k_scene + hk * a.k_head;
     const T *vbase = static_cast<const T *>(a.v) + s * c.v_scene + hk * a.v_head;
-    T *sk = tiles[wave], *sv = sk + kKeys * LD;
-    auto keep_at = [&](int j) {
-        if (!a.keep) return true;
-        const int64_t at = s * c.keep_scene + j;
-        return a.keep_bytes == 1 ? static_cast<const uint8_t *>(a.keep)[at] != 0
-                                 : static_cast<const int *>(a.keep)[at] != 0;
-    };
-
+    T *const sk = tiles[wave], *const sv = sk + 2 * kKeys * DP;
+    Tile<T, DP> at;
+    at.plan(lane);
+    Copy<T, DP, kKeys, 1> ck, cv;
+    ck.plan(a.k_row, a.dim, 0, lane);
+    cv.plan(a.v_row, a.dim, 0, lane);
     f32x16 o[DP / 32] = {};
     float m = -INFINITY, sum = 0.f;
-    WaveStaged<T, DP> gk, gv;
     float gp[2] = {};
-    auto fetch = [&](int j0) {
-        auto live = [&](int r) { return j0 + r < j_end && keep_at(j0 + r); };
-        gk.load(kbase + (int64_t)j0 * a.k_row, a.k_row, a.dim, lane, live);
-        gv.load(vbase + (int64_t)j0 * a.v_row, a.v_row, a.dim, lane, live);
+    int raw = 0;
+    uint32_t live = ~0u, next_live = ~0u;
+    const int step = W * kKeys;
+    auto look = [&](int j0) {
+        if (a.keep && j0 < j_end)
+            raw = keep_raw(a, s * c.keep_scene + min(j0 + (lane & 31), j_end - 1));
+    };
+    auto fetch = [&](int b, int j0) {
+        if (a.keep) next_live = (uint32_t)__ballot(raw != 0);
+        look(j0 + step);
+        const int left = j_end - j0;
+        ck.start(sk + b * kKeys * DP, kbase + (int64_t)j0 * a.k_row, a.k_row, a.dim, left, a.keep,
+                 next_live, 0, lane);
+        cv.start(sv + b * kKeys * DP, vbase + (int64_t)j0 * a.v_row, a.v_row, a.dim, left, a.keep,
+                 next_live, 0, lane);
         if (far)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int at = i * 64 + lane, r = at % kKeys, ax = at / kKeys;
-                gp[i] = ax < 3 && j0 + r < j_end
-                            ? a.k_pos[s * c.k_pos_scene + (int64_t)(j0 + r) * a.k_pos_row + ax] : 0.f;
+                const int r = min((i * 64 + lane) % kKeys, left - 1), ax = min((i * 64 + lane) / kKeys, 2);
+                gp[i] = a.k_pos[s * c.k_pos_scene + (int64_t)(j0 + r) * a.k_pos_row + ax];
             }
     };
-    int j0 = j_begin + wave * kKeys;
-    if (j0 < j_end) fetch(j0);
-    for (; j0 < j_end; j0 += 4 * kKeys) {
-        gk.store(sk, lane);
-        gv.store(sv, lane);
+    // the tiles are this wave's own: its copies and LDS accesses need no barrier, only waits
+    auto put = [&](int b) {
         if (far) {
-            spos[wave][lane] = Places<T>::row(gp[0]);
-            if (lane < kKeys) spos[wave][64 + lane] = Places<T>::row(gp[1]);
+            spos[wave][b][lane] = Places<T>::row(gp[0]);
+            if (lane < kKeys) spos[wave][b][64 + lane] = Places<T>::row(gp[1]);
         }
-        // the tile is this wave's own: its LDS accesses complete in order, only the
-        // compiler has to keep them so
+        tile_wait();
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        const uint32_t live = (uint32_t)__ballot(lane < kKeys && j0 + lane < j_end &&
-                                                 keep_at(min(j0 + lane, j_end - 1)));
-        if (j0 + 4 * kKeys < j_end) fetch(j0 + 4 * kKeys);
+    };
+    int b = 0;
+    if (j_begin + wave * kKeys < j_end) {
+        look(j_begin + wave * kKeys);
+        fetch(0, j_begin + wave * kKeys);
+        put(0);
+    }
+    for (int j0 = j_begin + wave * kKeys; j0 < j_end; j0 += step, b ^= 1) {
+        const bool more = j0 + step < j_end;
+        live = next_live;
+        if (j_end - j0 < kKeys) live &= (1u << (j_end - j0)) - 1;
+        if (more) fetch(b ^ 1, j0 + step);
+        const T *kt = sk + b * kKeys * DP, *vt = sv + b * kKeys * DP;
         f32x16 d = {}, w = {};
-        if (far) d = distances(place, spos[wave], kKeys, 0, lane);
+        if (far) d = distances<T>(place, spos[wave][b], kKeys, 0, lane);
         if (far && !capped)
 #pragma unroll
             for (int r = 0; r < 16; ++r) w[r] = -far_unit * d[r];
-        const T *krow = sk + (lane & 31) * LD + 8 * (lane >> 5);
 #pragma unroll
-        for (int st = 0; st < DP / 16; ++st) w = mma(row_frag(krow + st * 16), q[st], w);
+        for (int st = 0; st < DP / 16; ++st) w = mma(at.rows(kt, st), q[st], w);
         if (capped)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -143,10 +135,10 @@ __global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, cons
                 if (far) w[r] = fmaf(-far_unit, d[r], w[r]);
             }
         if (live != 0xffffffffu) {
-            const uint32_t bits = live >> (4 * (lane >> 5));
+            const uint32_t seen = live >> (4 * (lane >> 5));
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if (!((bits >> (8 * (r >> 2) + (r & 3))) & 1)) w[r] = -INFINITY;
+                if (!(seen & (1u << result_row(r)))) w[r] = -INFINITY;
         }
         float top = -INFINITY;
 #pragma unroll
@@ -170,12 +162,10 @@ __global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, cons
         for (int half = 0; half < 2; ++half) {
             const frag p = to_frag<T>(w, half);
 #pragma unroll
-            for (int b = 0; b < DP / 32; ++b)
-                o[b] = mma(tr_frag<LD>(sv + half * 16 * LD + b * 32, lane), p, o[b]);
+            for (int e = 0; e < DP / 32; ++e)
+                o[e] = mma(at.columns(vt + half * 16 * DP, e, lane), p, o[e]);
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (more) put(b ^ 1);
     }
     sum += other_half(sum);
     // the waves' sums, joined
@@ -190,13 +180,13 @@ __global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, cons
                 so[(lane & 31) * DP + b * 32 + 8 * g + 4 * (lane >> 5) + e] = o[b][4 * g + e];
     __syncthreads();
     const int heads = min(group - ht * kHeads, kHeads);
-    for (int i = threadIdx.x; i < heads * DP; i += 256) {
+    for (int i = threadIdx.x; i < heads * DP; i += 64 * W) {
         const int r = i / DP, dd = i % DP;
         float top = -INFINITY, total = 0.f, val = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w][r]);
+        for (int w = 0; w < W; ++w) top = fmaxf(top, sm[w][r]);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < W; ++w) {
             // a wave without keys has the maximum -inf and the sum 0; NaN sums pass
             const float by = sm[w][r] == -INFINITY ? 1.f : fast_exp2(sm[w][r] - top);
             total = fmaf(by, ss[w][r], total);
@@ -214,30 +204,39 @@ __global__ __launch_bounds__(256) void k_attention_cached(const AttnArgs a, cons
     }
 }
 
-// One wave a scene and head: its splits, joined in order.
+// One workgroup a scene and head: four waves take the splits in turn, then their sums are joined,
+// always in the same order.
 template <typename T>
-__global__ __launch_bounds__(64) void k_cached_join(const float *__restrict__ part_o,
-                                                    const float2 *__restrict__ part_ms, int splits,
-                                                    int dim, T *__restrict__ out) {
+__global__ __launch_bounds__(256) void k_cached_join(const float *__restrict__ part_o,
+                                                     const float2 *__restrict__ part_ms, int splits,
+                                                     int dim, T *__restrict__ out) {
+    __shared__ float so[4][128], ss[4];
     const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float2 *ms = part_ms + row * splits;
     float top = -INFINITY;
-    for (int p = threadIdx.x; p < splits; p += 64) top = fmaxf(top, ms[p].x);
+    for (int p = lane; p < splits; p += 64) top = fmaxf(top, ms[p].x);
 #pragma unroll
     for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
     float total = 0.f, v0 = 0.f, v1 = 0.f;
-    const int d0 = threadIdx.x, d1 = threadIdx.x + 64;
-    for (int p = 0; p < splits; ++p) {
+    const int d0 = min(lane, dim - 1), d1 = min(lane + 64, dim - 1);
+#pragma unroll 4
+    for (int p = wave; p < splits; p += 4) {
         const float2 e = ms[p];
         const float by = e.x == -INFINITY ? 1.f : fast_exp2(e.x - top);
         total = fmaf(by, e.y, total);
         const float *o = part_o + (row * splits + p) * dim;
-        if (d0 < dim) v0 = fmaf(by, o[d0], v0);
-        if (d1 < dim) v1 = fmaf(by, o[d1], v1);
+        v0 = fmaf(by, o[d0], v0);
+        v1 = fmaf(by, o[d1], v1);
     }
-    const float by = total == 0.f ? 0.f : 1.f / total;
-    if (d0 < dim) out[row * dim + d0] = (T)(v0 * by);
-    if (d1 < dim) out[row * dim + d1] = (T)(v1 * by);
+    so[wave][lane] = v0, so[wave][64 + lane] = v1;
+    if (lane == 0) ss[wave] = total;
+    __syncthreads();
+    if (threadIdx.x >= (unsigned)dim) return;
+    const int d = threadIdx.x;
+    total = ss[0] + ss[1] + ss[2] + ss[3];
+    const float v = so[0][d] + so[1][d] + so[2][d] + so[3][d];
+    out[row * dim + d] = (T)(total == 0.f ? 0.f : v / total);
 }
 
 // Splits of a cache: enough workgroups for two rounds on 256 CUs, each with at least a step
@@ -257,9 +256,9 @@ struct Cached {
         T *o = static_cast<T *>(out);
         hipLaunchKernelGGL((k_attention_cached<T, DP, FAR, CAPPED>),
                            dim3((unsigned)(a.scenes * a.kv_heads * c.head_tiles * c.splits)),
-                           dim3(256), 0, st, a, c, o);
+                           dim3(64 * kWaves<T, DP>), 0, st, a, c, o);
         if (c.splits > 1)
-            hipLaunchKernelGGL(k_cached_join<T>, dim3((unsigned)(a.scenes * a.heads)), dim3(64), 0,
+            hipLaunchKernelGGL(k_cached_join<T>, dim3((unsigned)(a.scenes * a.heads)), dim3(256), 0,
                                st, c.part_o, c.part_ms, c.splits, a.dim, o);
     }
 };
@@ -320,6 +319,7 @@ extern "C" int gsv_attention_cached(const gsv_attention *args, const int32_t *le
     float *po = static_cast<float *>(workspace);
     const CacheArgs c{lengths, k_scene, v_scene, k_pos_scene, keep_scene, splits, tiles, po,
                       reinterpret_cast<float2 *>(static_cast<char *>(workspace) + part_o_bytes(a, splits))};
-    attention_variant(a, args->dtype, Cached{a, c, out, as_stream(stream)});
+    Cached f{a, c, out, as_stream(stream)};
+    attention_variant(a, args->dtype, f);
     return check_launch();
 }

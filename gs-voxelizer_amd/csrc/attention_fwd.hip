@@ -12,7 +12,7 @@ namespace gsv {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kRows = 128;  // query rows of a workgroup
+constexpr int WAVES = 4, kRows = 32 * WAVES;  // a workgroup's waves and query rows
 // The maximum follows the scores only when one exceeds it by 2^8: weights then stay
 // below 2^8, and a rescale of the sums (one multiply a register) is rare.
 constexpr float kSlack = 8.f;
@@ -20,20 +20,15 @@ constexpr float kSlack = 8.f;
 // HEADS query heads of a wave share its distances (a third of the vector work of one head: 2
 // multiply-adds, a multiply and a root an element, at the matrix units' differences).  With one
 // key head for both (SHARED) they share the tiles too.
-template <typename T, int DP, int HEADS> struct FwdTile {
-    static constexpr int kKeys = HEADS * DP * sizeof(T) >= 256 ? 32 : 64;
-};
-
 template <typename T, int DP, bool FAR, bool CAPPED, int HEADS, bool SHARED>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const AttnArgs a,
-                                                                         T *__restrict__ out,
-                                                                         float *__restrict__ lse) {
-    constexpr int KB = FwdTile<T, DP, HEADS>::kKeys, LD = DP + Elem<T>::kPad;
-    constexpr int KV = SHARED ? 1 : HEADS;  // key heads of the workgroup
+__global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_attention_fwd(
+    const AttnArgs a, T *__restrict__ out, float *__restrict__ lse) {
+    constexpr int KB = sizeof(T) == 2 ? 64 : 32;  // keys of a tile
+    constexpr int KV = SHARED ? 1 : HEADS;        // key heads of the workgroup
     constexpr bool far = FAR, capped = CAPPED;
     typedef typename Elem<T>::frag frag;
-    __shared__ __align__(16) T sk[2][KV][KB * LD];
-    __shared__ __align__(16) T sv[2][KV][KB * LD];
+    __shared__ __align__(1024) T sk[2][KV][KB * DP];
+    __shared__ __align__(1024) T sv[2][KV][KB * DP];
     __shared__ __align__(16) typename Places<T>::Row spos[2][3 * KB];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -60,9 +55,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const A
     float far_unit[HEADS];
 #pragma unroll
     for (int n = 0; n < HEADS; ++n) far_unit[n] = slope_of(a, h0 + n) / (capped ? 1.f : a.scale);
-    Staged<T, DP, KB> gk[KV], gv[KV];
-#pragma unroll
-    for (int n = 0; n < KV; ++n) gk[n].plan(a.k_row, a.dim), gv[n].plan(a.v_row, a.dim);
+    Tile<T, DP> at;
+    at.plan(lane);
+    Copy<T, DP, KB, WAVES> ck, cv;
+    ck.plan(a.k_row, a.dim, wave, lane);
+    cv.plan(a.v_row, a.dim, wave, lane);
 
     for (int tile = slot; tile < tiles; tile += a.slots) {
         // the last rows of a causal scene see the most keys: they start first
@@ -95,72 +92,68 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const A
         for (int n = 0; n < HEADS; ++n) m[n] = -INFINITY, sum[n] = 0.f;
 
         float gp = 0.f;
-        bool gl = true;
-        uint64_t live = ~0ull;
-        auto fetch = [&](int j0) {
+        int raw = 0;
+        uint64_t live = ~0ull, next_live = ~0ull;
+        auto look = [&](int j0) {  // the mask of a tile
+            if (a.keep && j0 < most) raw = keep_raw(a, c.k0 + min(j0 + lane, most - 1));
+        };
+        auto fetch = [&](int b, int j0) {
             const int left = most - j0;
+            if (a.keep) next_live = __ballot(raw != 0);
+            look(j0 + KB);
 #pragma unroll
             for (int n = 0; n < KV; ++n) {
-                gk[n].load(kbase[n] + j0 * a.k_row, a.k_row, a.dim, left);
-                gv[n].load(vbase[n] + j0 * a.v_row, a.v_row, a.dim, left);
+                ck.start(sk[b][n], kbase[n] + j0 * a.k_row, a.k_row, a.dim, left, a.keep, next_live,
+                         wave, lane);
+                cv.start(sv[b][n], vbase[n] + j0 * a.v_row, a.v_row, a.dim, left, a.keep, next_live,
+                         wave, lane);
             }
             if (far && threadIdx.x < 3 * KB)
                 gp = a.k_pos[(c.k0 + j0 + min((int)threadIdx.x % KB, left - 1)) * a.k_pos_row +
                              threadIdx.x / KB];
-            if (a.keep) gl = lane < KB && lane < left && kept(a, c.k0 + j0 + lane);
         };
         auto put = [&](int b) {
-            if (a.keep) live = __ballot(gl);
-#pragma unroll
-            for (int n = 0; n < KV; ++n) {
-                if (a.keep) gk[n].keep(live), gv[n].keep(live);
-                gk[n].store(sk[b][n]);
-                gv[n].store(sv[b][n]);
-            }
             if (far && threadIdx.x < 3 * KB) spos[b][threadIdx.x] = Places<T>::row(gp);
+            tile_wait();
         };
         __syncthreads();  // the previous tile's last reads
         if (most > 0) {
-            fetch(0);
+            look(0);
+            fetch(0, 0);
             put(0);
         }
         __syncthreads();
         int b = 0;
         for (int j0 = 0; j0 < most; j0 += KB, b ^= 1) {
             const bool more = j0 + KB < most;
-            if (more) fetch(j0 + KB);
+            live = next_live;
+            if (more) fetch(b ^ 1, j0 + KB);
             if (j0 < mine) {
                 const bool masked = j0 + KB > all || (KB == 64 ? ~live : (uint32_t)~live) != 0;
 #pragma unroll 1
                 for (int kb = 0; kb < KB / 32; ++kb) {
                     f32x16 d = {}, w[HEADS] = {};
+#pragma unroll
+                    for (int st = 0; st < DP / 16; ++st)
+#pragma unroll
+                        for (int n = 0; n < HEADS; ++n)
+                            w[n] = mma(at.rows(sk[b][SHARED ? 0 : n] + kb * 32 * DP, st), q[n][st], w[n]);
+                    // the distances' vector work runs while the products above do
                     if (far) d = distances<T>(place, spos[b], KB, kb * 32, lane);
-                    const int at0 = (kb * 32 + (lane & 31)) * LD + 8 * (lane >> 5);
 #pragma unroll
-                    for (int n = 0; n < HEADS; ++n) {
-                        if (far && !capped)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) w[n][r] = -far_unit[n] * d[r];
-#pragma unroll
-                        for (int st = 0; st < DP / 16; ++st)
-                            w[n] = mma(row_frag(sk[b][SHARED ? 0 : n] + at0 + st * 16), q[n][st], w[n]);
-                        if (capped)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) {
-                                w[n][r] = a.cap * tanh_of<T>(w[n][r] * in_cap);
-                                if (far) w[n][r] = fmaf(-far_unit[n], d[r], w[n][r]);
-                            }
-                    }
-                    if (masked) {
-                        const uint32_t bits = (uint32_t)(live >> (kb * 32)) >> (4 * (lane >> 5));
-                        const int lim = limit - j0 - kb * 32 - 4 * (lane >> 5);
+                    for (int n = 0; n < HEADS; ++n)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
-                            const int at = 8 * (r >> 2) + (r & 3);
-                            if (at >= lim || !((bits >> at) & 1))
-#pragma unroll
-                                for (int n = 0; n < HEADS; ++n) w[n][r] = -INFINITY;
+                            if (capped) w[n][r] = a.cap * tanh_of<T>(w[n][r] * in_cap);
+                            if (far) w[n][r] = fmaf(-far_unit[n], d[r], w[n][r]);
                         }
+                    if (masked) {
+                        const uint32_t seen = seen_rows(live, kb, limit - j0 - kb * 32, lane);
+#pragma unroll
+                        for (int n = 0; n < HEADS; ++n)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                if (!(seen & (1u << result_row(r)))) w[n][r] = -INFINITY;
                     }
                     float top[HEADS];
                     bool grown = false;
@@ -194,10 +187,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const A
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             const frag p = to_frag<T>(w[n], half);
-                            const T *vt = sv[b][SHARED ? 0 : n] + (kb * 32 + half * 16) * LD;
+                            const T *vt = sv[b][SHARED ? 0 : n] + (kb * 32 + half * 16) * DP;
 #pragma unroll
                             for (int e = 0; e < DP / 32; ++e)
-                                o[n][e] = mma(tr_frag<LD>(vt + e * 32, lane), p, o[n][e]);
+                                o[n][e] = mma(at.columns(vt, e, lane), p, o[n][e]);
                         }
                     }
                 }
@@ -220,16 +213,23 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_fwd(const A
 }
 
 struct Forward {
-    const AttnArgs &a;
+    AttnArgs a;
+    int longest;
     void *out;
     float *lse;
     hipStream_t st;
-    template <typename T, int DP, bool FAR, bool CAPPED, int HEADS, bool SHARED> void start() const {
+    int status;
+    template <typename T, int DP, bool FAR, bool CAPPED, int HEADS, bool SHARED> void start() {
+        if (!attention_slots(&a, longest, kRows, a.heads)) {
+            status = GSV_ERR_SIZE_OVERFLOW;
+            return;
+        }
         hipLaunchKernelGGL((k_attention_fwd<T, DP, FAR, CAPPED, HEADS, SHARED>),
-                           dim3((unsigned)a.slots * a.scenes * (a.heads / HEADS)), dim3(256), 0, st,
-                           a, static_cast<T *>(out), lse);
+                           dim3((unsigned)a.slots * a.scenes * (a.heads / HEADS)), dim3(256), 0,
+                           st, a, static_cast<T *>(out), lse);
+        status = check_launch();
     }
-    template <typename T, int DP, bool FAR, bool CAPPED> void run() const {
+    template <typename T, int DP, bool FAR, bool CAPPED> void run() {
         if constexpr (FAR && sizeof(T) == 2 && DP <= 64) {
             if (attention_pairs(a)) {
                 if (a.heads / a.kv_heads % 2 == 0) start<T, DP, FAR, CAPPED, 2, true>();
@@ -291,7 +291,7 @@ extern "C" int gsv_attention_fwd(const gsv_attention *args, void *out, float *ls
     if (st != GSV_OK) return st;
     if (a.q_tokens == 0) return GSV_OK;
     if (!out || reinterpret_cast<uintptr_t>(out) % 16) return GSV_ERR_INVALID_ARGUMENT;
-    if (!attention_slots(&a, lq, kRows, a.heads)) return GSV_ERR_SIZE_OVERFLOW;
-    attention_variant(a, args->dtype, Forward{a, out, lse, as_stream(stream)});
-    return check_launch();
+    Forward f{a, lq, out, lse, as_stream(stream), GSV_OK};
+    attention_variant(a, args->dtype, f);
+    return f.status;
 }

@@ -15,6 +15,9 @@
 
 #include "gsv_device.h"
 
+// m0 is named as written by the copies below; the compiler warns that it is a reserved register
+#pragma clang diagnostic ignored "-Winline-asm"
+
 namespace gsv {
 
 typedef __bf16 bf16;
@@ -28,12 +31,10 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 template <typename T> struct Elem;
 template <> struct Elem<bf16> {
     typedef bf16x8 frag;
-    static constexpr int kPad = 8;    // LDS row padding, elements
     static constexpr int kChunk = 8;  // elements of a 16-byte chunk
 };
 template <> struct Elem<float> {
     typedef f32x8 frag;
-    static constexpr int kPad = 4;
     static constexpr int kChunk = 4;
 };
 
@@ -64,26 +65,62 @@ __device__ __forceinline__ f32x8 row_frag(const float *p) {
     return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-// The transposed left operand: column l % 32 of 32 columns, rows 4 g .. 4 g + 3 and
-// 8 + 4 g .. 8 + 4 g + 3 of 16 rows.  `tile` points at the first row and column.  For 16-bit
-// elements ds_read_b64_tr_b16 does it: of 16 lanes, lane i gives the address of
-// row i / 4, columns 4 (i % 4) .. + 3, and receives column i of the four rows.
-template <int LD> __device__ __forceinline__ bf16x8 tr_frag(const bf16 *tile, int lane) {
-    const int i = lane & 15, g = lane >> 5;
-    const bf16 *p = tile + (4 * g + (i >> 2)) * LD + (lane & 16) + 4 * (i & 3);
-    typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * LD));
-    const bf16x4 x = __builtin_bit_cast(bf16x4, a), y = __builtin_bit_cast(bf16x4, b);
-    return bf16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-}
-template <int LD> __device__ __forceinline__ f32x8 tr_frag(const float *tile, int lane) {
-    const float *p = tile + 4 * (lane >> 5) * LD + (lane & 31);
-    f32x8 f;
+// A tile of one head in LDS: rows of DP elements, no padding (the copies below fill 1024
+// bytes in lane order), chunk c of row r at place c ^ turn(r).  turn spreads what one access reads over
+// all 64 banks: chunk c of eight rows in sequence, and four chunks of four rows in sequence.  It
+// depends on the row's low four bits.
+template <typename T, int DP> struct Tile {
+    static constexpr int kPerRow = DP / Elem<T>::kChunk, kRowBytes = kPerRow * 16;
+    static __device__ __forceinline__ int turn(int r) {
+        if constexpr (kPerRow == 4) return (r >> 2) & 3;
+        if constexpr (kPerRow == 8) return (r & 2) << 1 | (r & 4) >> 1 | (r & 8) >> 3;
+        return (r & 3) << 2 | ((r >> 2) & 3);
+    }
+    int row_at, col_at;  // byte offsets of the lane's parts below
+    __device__ __forceinline__ void plan(int lane) {
+        const int r = lane & 31, g = lane >> 5;
+        row_at = r * kRowBytes + (((sizeof(T) == 2 ? g : 2 * g) ^ turn(r)) << 4);
+        const int i = lane & 15, r4 = 4 * g + (i >> 2);
+        col_at = r4 * kRowBytes + ((((lane >> 3) & 2) + ((i & 3) >> 1)) ^ turn(r4)) * 16 + (i & 1) * 8;
+    }
+    static __device__ __forceinline__ const T *at(const T *tile, int bytes) {
+        return reinterpret_cast<const T *>(reinterpret_cast<const char *>(tile) + bytes);
+    }
+    // Columns 16 st + 8 (lane / 32) .. + 7 of row lane % 32; the tile from a multiple of 16 rows on.
+    __device__ __forceinline__ typename Elem<T>::frag rows(const T *tile, int st) const {
+        if constexpr (sizeof(T) == 2) {
+            return *reinterpret_cast<const bf16x8 *>(at(tile, row_at ^ (st << 5)));
+        } else {
+            const int x = row_at ^ (st << 6);
+            const f32x4 a = *reinterpret_cast<const f32x4 *>(at(tile, x));
+            const f32x4 b = *reinterpret_cast<const f32x4 *>(at(tile, x ^ 16));
+            return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        }
+    }
+    // The transposed left operand: column 32 block + lane % 32, rows 4 g .. 4 g + 3 and 8 + 4 g ..
+    // 8 + 4 g + 3.  For 16-bit elements ds_read_b64_tr_b16 does it: of 16 lanes, lane i gives the
+    // address of row i / 4, columns 4 (i % 4) .. + 3, and receives column i of the four rows.
+    __device__ __forceinline__ typename Elem<T>::frag columns(const T *tile, int block, int lane) const {
+        if constexpr (sizeof(T) == 2) {
+            typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
+            const int x = col_at ^ (block << 6);
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at(tile, x));
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_ptr)at(tile, (x ^ (turn(8) << 4)) + 8 * kRowBytes));
+            const bf16x4 u = __builtin_bit_cast(bf16x4, a), v = __builtin_bit_cast(bf16x4, b);
+            return bf16x8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+        } else {
+            f32x8 f;
+            const int chunk = 8 * block + ((lane & 31) >> 2);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = p[e * LD], f[4 + e] = p[(8 + e) * LD];
-    return f;
-}
+            for (int e = 0; e < 8; ++e) {
+                const int r = 4 * (lane >> 5) + (e & 3) + 8 * (e >> 2);
+                f[e] = *at(tile, r * kRowBytes + ((chunk ^ turn(r)) << 4) + (lane & 3) * 4);
+            }
+            return f;
+        }
+    }
+};
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -119,19 +156,19 @@ int attention_args(const gsv_attention *in, AttnArgs *a, int *longest_q, int *lo
 
 // The kernel variant of a call: element type, channels (up to 32, 64 or 128; the columns past
 // dim are zeros), distance bias, score cap.
-template <typename T, int DP, typename F> void attention_options(const AttnArgs &a, const F &f) {
+template <typename T, int DP, typename F> void attention_options(const AttnArgs &a, F &f) {
     const bool far = a.slopes, capped = a.cap > 0.f;
     if (far && capped) f.template run<T, DP, true, true>();
     else if (far) f.template run<T, DP, true, false>();
     else if (capped) f.template run<T, DP, false, true>();
     else f.template run<T, DP, false, false>();
 }
-template <typename T, typename F> void attention_channels(const AttnArgs &a, const F &f) {
+template <typename T, typename F> void attention_channels(const AttnArgs &a, F &f) {
     if (a.dim <= 32) attention_options<T, 32>(a, f);
     else if (a.dim <= 64) attention_options<T, 64>(a, f);
     else attention_options<T, 128>(a, f);
 }
-template <typename F> void attention_variant(const AttnArgs &a, int dtype, const F &f) {
+template <typename F> void attention_variant(const AttnArgs &a, int dtype, F &f) {
     if (dtype == GSV_BF16) attention_channels<bf16>(a, f);
     else attention_channels<float>(a, f);
 }
@@ -188,44 +225,60 @@ __device__ __forceinline__ float slope_of(const AttnArgs &a, int h) {
 // The widest row stride: 64 rows have to lie within a buffer descriptor's 2^31 bytes.
 constexpr int64_t kMaxRowBytes = 1 << 24;
 
-// A tile of ROWS rows of one head on its way from global memory to LDS: 256 threads, 16-byte
-// chunks through a buffer descriptor that ends with the last live row, so that rows past it and
-// columns from dim up to DP arrive as zeros without a branch.  Rows of a mask are zeroed
-// as they are stored: no value of theirs, NaN among them, meets a weight of 0.
-template <typename T, int DP, int ROWS> struct Staged {
-    static constexpr int kCh = Elem<T>::kChunk, kPerRow = DP / kCh, LD = DP + Elem<T>::kPad;
-    static constexpr int kN = ROWS * kPerRow / 256;
-    static_assert(ROWS * kPerRow % 256 == 0, "whole chunks for each thread");
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    u32x4 r[kN];
-    int at[kN];  // byte offsets in the tile
-    __device__ __forceinline__ void plan(int64_t stride, int dim) {
+// Copies ROWS rows of one head from global memory into a tile, asynchronously and past the
+// registers (buffer_load_dwordx4 ... lds: a wave's 64 chunks of 16 bytes, to LDS in lane order).
+// The buffer descriptor ends with the last live row: rows past it, columns from dim up to DP and
+// rows that a mask drops are given offsets past its end, where the hardware reads zeros, so that no
+// value of theirs, NaN among them, meets a weight of 0.  tile_wait() before the barrier behind
+// which the tile is read.
+template <typename T, int DP, int ROWS, int WAVES> struct Copy {
+    static constexpr int kPerRow = DP / Elem<T>::kChunk, kAll = ROWS * kPerRow / 64;
+    static constexpr int kN = (kAll + WAVES - 1) / WAVES;
+    static constexpr int kNowhere = INT32_MAX - 15;
+    int at[kN];
+    static __device__ __forceinline__ int row_of(int i, int wave, int lane) {
+        return ((i * WAVES + wave) * 64 + lane) / kPerRow;
+    }
+    __device__ __forceinline__ void plan(int64_t stride, int dim, int wave, int lane) {
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            const int c = i * 256 + threadIdx.x, row = c / kPerRow, col = (c % kPerRow) * kCh;
-            at[i] = col < dim ? (row * (int)stride + col) * (int)sizeof(T) : INT32_MAX - 15;
+            const int row = row_of(i, wave, lane);
+            const int col = ((lane % kPerRow) ^ Tile<T, DP>::turn(row)) * Elem<T>::kChunk;
+            at[i] = col < dim ? (row * (int)stride + col) * (int)sizeof(T) : kNowhere;
         }
     }
-    // rows: live rows from base on, 1 at least
-    __device__ __forceinline__ void load(const T *base, int64_t stride, int dim, int rows) {
+    // rows: live rows from base on, 1 at least; with `some`, those whose bit is set in `live`
+    __device__ __forceinline__ void start(T *tile, const T *base, int64_t stride, int dim, int rows,
+                                          bool some, uint64_t live, int wave, int lane) const {
         const int bytes = ((min(rows, ROWS) - 1) * (int)stride + dim) * (int)sizeof(T);
         const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, bytes, 0x00020000);
-#pragma unroll
-        for (int i = 0; i < kN; ++i) r[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at[i], 0, 0);
-    }
-    __device__ __forceinline__ void store(T *tile) const {
+        typedef __attribute__((address_space(3))) const void *lds_ptr;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            const int c = i * 256 + threadIdx.x, row = c / kPerRow, col = (c % kPerRow) * kCh;
-            *reinterpret_cast<u32x4 *>(tile + row * LD + col) = r[i];
+            if (kAll % WAVES && i * WAVES + wave >= kAll) break;
+            int x = at[i];
+            if (some && !((live >> row_of(i, wave, lane)) & 1)) x = kNowhere;
+            // As assembly, without register outputs: for the builtin the compiler waits before
+            // every read of LDS, also of the other buffer.  The only readers of this tile
+            // stand behind tile_wait() and a barrier.
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :
+                         : "s"((uint32_t)(uintptr_t)(lds_ptr)(tile + (i * WAVES + wave) * 64 *
+                                                                        Elem<T>::kChunk)),
+                           "v"(x), "s"(rsrc)
+                         : "m0", "memory");
         }
     }
-    __device__ __forceinline__ void keep(uint64_t live) {
-#pragma unroll
-        for (int i = 0; i < kN; ++i)
-            if (!((live >> ((i * 256 + threadIdx.x) / kPerRow)) & 1)) r[i] = u32x4{};
-    }
 };
+// Waits for this wave's copies (vmcnt 0, the other counters as they are).
+__device__ __forceinline__ void tile_wait() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
+// A key's mask value as it lies in memory; compared only where it is used, so that nothing
+// waits for it where it is loaded.
+__device__ __forceinline__ int keep_raw(const AttnArgs &a, int64_t row) {
+    return a.keep_bytes == 1 ? static_cast<const uint8_t *>(a.keep)[row]
+                             : static_cast<const int *>(a.keep)[row];
+}
 
 // A row of global memory as the right operand's column of one lane.
 template <typename T, int DP>
@@ -319,8 +372,14 @@ __device__ __forceinline__ f32x16 distances(const Places<T> &to, const typename 
     return d;
 }
 
-__device__ __forceinline__ int result_row(int r, int lane) {
-    return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+// The row of a block that result register r of a lane's half holds, less 4 (lane / 32).
+__device__ __forceinline__ constexpr int result_row(int r) { return 8 * (r >> 2) + (r & 3); }
+
+// The rows of a block that a lane sees, a bit each at result_row(r): those kept (bits of the tile)
+// below the lane's limit, counted from the block's first row.
+__device__ __forceinline__ uint32_t seen_rows(uint64_t live, int block, int limit, int lane) {
+    const uint32_t below = limit >= 32 ? ~0u : limit > 0 ? (1u << limit) - 1 : 0u;
+    return ((uint32_t)(live >> (32 * block)) & below) >> (4 * (lane >> 5));
 }
 
 }  // namespace gsv
