@@ -24,8 +24,10 @@ struct BwdArgs {
     int64_t dout_row, dout_head;
     const float *lse;
     float *delta;   // (heads, q_tokens)
-    float *dslope;  // (slots * scenes, heads) partial sums
+    double *dslope; // (slots * scenes, heads) partial sums
     void *dq, *dk, *dv;
+    int parts;             // workgroups that share a key tile's rows
+    float *part_k, *part_v;  // (parts, k_tokens, kv_heads, dim) partial sums, with parts > 1
 };
 
 // A block's scores from the matrix product: capped (u: the tanh), with their bias.
@@ -201,7 +203,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
     if (lane == 0) sums[wave] = dslope;
     __syncthreads();
     if (threadIdx.x == 0)
-        g.dslope[(int64_t)rest * a.heads + h] = (float)(sums[0] + sums[1] + sums[2] + sums[3]);
+        g.dslope[(int64_t)rest * a.heads + h] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
 // dk and dv.  A wave's lanes are keys; the rows of all query heads of the key head pass by.
@@ -215,7 +217,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
     __shared__ __align__(16) float srow[2][2 * QB];  // log sums, D
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
+    const int hk = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads % g.parts;
+    const int rest = blockIdx.x / a.kv_heads / g.parts;
     const int s = rest % a.scenes, slot = rest / a.scenes;
     const Scene c = scene_rows(a, s);
     const int nq = c.q1 - c.q0, nk = c.k1 - c.k0, off = nk - nq;
@@ -258,7 +261,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
         const int q_from =
             a.causal && first >= c.prefix ? max(first - off, 0) / QB * QB : 0;
         const int per_head = q_from < nq ? (nq - q_from + QB - 1) / QB : 0;
-        const int steps = per_head * group;
+        const int first_step = (int64_t)per_head * group * part / g.parts;
+        const int steps = (int64_t)per_head * group * (part + 1) / g.parts;
         f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
 
         float gr[2] = {};
@@ -294,13 +298,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
             tile_wait();
         };
         __syncthreads();
-        if (steps > 0) {
-            fetch(0, 0);
+        if (first_step < steps) {
+            fetch(0, first_step);
             put(0);
         }
         __syncthreads();
         int b = 0;
-        for (int step = 0; step < steps; ++step, b ^= 1) {
+        for (int step = first_step; step < steps; ++step, b ^= 1) {
             const bool more = step + 1 < steps;
             if (more) fetch(b ^ 1, step + 1);
             const int i0 = q_from + step / group * QB;
@@ -355,14 +359,40 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
         }
         if (j < nk) {
             const int64_t at = (kj * a.kv_heads + hk) * a.dim;
-            store_column<T, DP>(static_cast<T *>(g.dk) + at, dk, a.scale, a.dim, lane);
-            store_column<T, DP>(static_cast<T *>(g.dv) + at, dv, 1.f, a.dim, lane);
+            if (g.parts == 1) {
+                store_column<T, DP>(static_cast<T *>(g.dk) + at, dk, a.scale, a.dim, lane);
+                store_column<T, DP>(static_cast<T *>(g.dv) + at, dv, 1.f, a.dim, lane);
+            } else {
+                const int64_t all = (int64_t)a.k_tokens * a.kv_heads * a.dim * part;
+                store_column<float, DP>(g.part_k + all + at, dk, a.scale, a.dim, lane);
+                store_column<float, DP>(g.part_v + all + at, dv, 1.f, a.dim, lane);
+            }
         }
     }
 }
 
+// The parts' sums of dk and dv, in order: four values a thread, 16 bytes of each part.
+template <typename T>
+__global__ __launch_bounds__(256) void k_parts_sum(const float *__restrict__ pk,
+                                                   const float *__restrict__ pv, int parts,
+                                                   int64_t fours, T *__restrict__ dk,
+                                                   T *__restrict__ dv) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= 2 * fours) return;
+    const bool second = i >= fours;
+    const int64_t at = second ? i - fours : i;
+    const f32x4 *p = reinterpret_cast<const f32x4 *>(second ? pv : pk) + at;
+    f32x4 sum = p[0];
+    for (int n = 1; n < parts; ++n) sum += p[n * fours];
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = (T)sum[e];
+    reinterpret_cast<t4 *>(second ? dv : dk)[at] = r;
+}
+
 // The workgroups' sums of each head, in order.
-__global__ __launch_bounds__(64) void k_slope_sum(const float *__restrict__ part, int n, int heads,
+__global__ __launch_bounds__(64) void k_slope_sum(const double *__restrict__ part, int n, int heads,
                                                   void *__restrict__ out, int f32) {
     const int h = blockIdx.x;
     double sum = 0.0;
@@ -385,9 +415,15 @@ struct Backward {
                                dim3((unsigned)a.slots * a.scenes * a.heads), dim3(256), 0, st, a, g);
         AttnArgs k = a;
         k.slots = kslots;
-        if (a.k_tokens > 0)
-            hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED>),
-                               dim3((unsigned)kslots * a.scenes * a.kv_heads), dim3(256), 0, st, k, g);
+        if (a.k_tokens == 0) return;
+        hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED>),
+                           dim3((unsigned)kslots * a.scenes * a.kv_heads * g.parts), dim3(256), 0, st,
+                           k, g);
+        if (g.parts == 1) return;
+        const int64_t fours = (int64_t)a.k_tokens * a.kv_heads * a.dim / 4;
+        hipLaunchKernelGGL(k_parts_sum<T>, dim3((unsigned)((2 * fours + 255) / 256)), dim3(256), 0, st,
+                           g.part_k, g.part_v, g.parts, fours, static_cast<T *>(g.dk),
+                           static_cast<T *>(g.dv));
     }
 };
 
@@ -395,11 +431,30 @@ size_t delta_bytes(const AttnArgs &a) {
     return ((size_t)a.heads * a.q_tokens * sizeof(float) + 255) / 256 * 256;
 }
 
-int bwd_plan(const gsv_attention *args, AttnArgs *a, int *kslots) {
+// Parts of a key tile's rows: more workgroups where the tiles alone leave CUs idle or, as under a
+// causal mask, a few of them have most of the work.  About four rounds of workgroups at one a CU
+// (128 channels), one at two a CU; eight parts at most, each with four tiles of a mean scene's
+// rows at least (sizes alone decide: the longest scene's length is a hint that may change no bit).
+// Partial sums then pass through memory: 10,007 tokens of 4 causal scenes, 16 heads on 4, 128
+// channels take 945 us in one part and 770 in four; 8 heads of 64, 8,001 tokens gain nothing.
+int bwd_parts(const AttnArgs &a, int elem) {
+    const int64_t tiles = ((int64_t)a.k_tokens / kRows + a.scenes) * a.kv_heads;
+    const int64_t want = (a.dim > 64 ? 1024 : 512) / tiles + (a.dim > 64);
+    const int64_t rows = elem == GSV_BF16 ? kOther<bf16> : kOther<float>;
+    const int64_t most = (int64_t)a.q_tokens / a.scenes * (a.heads / a.kv_heads) / (4 * rows);
+    return (int)imax64(1, imin64(imin64(want, most), 8));
+}
+
+size_t parts_bytes(const AttnArgs &a, int parts) {
+    return parts == 1 ? 0 : sizeof(float) * parts * a.k_tokens * a.kv_heads * a.dim;  // of 32 bytes each
+}
+
+int bwd_plan(const gsv_attention *args, AttnArgs *a, int *kslots, int *parts) {
     int lq, lk;
     const int st = attention_args(args, a, &lq, &lk);
     if (st != GSV_OK) return st;
-    if (!attention_slots(a, lk, kRows, a->kv_heads)) return GSV_ERR_SIZE_OVERFLOW;
+    *parts = bwd_parts(*a, args->dtype);
+    if (!attention_slots(a, lk, kRows, a->kv_heads * *parts)) return GSV_ERR_SIZE_OVERFLOW;
     *kslots = a->slots;
     return attention_slots(a, lq, kRows, a->heads) ? GSV_OK : GSV_ERR_SIZE_OVERFLOW;
 }
@@ -411,11 +466,12 @@ using namespace gsv;
 
 extern "C" int gsv_attention_bwd_workspace_bytes(const gsv_attention *args, size_t *bytes) {
     AttnArgs a;
-    int kslots;
+    int kslots, parts;
     if (!bytes) return GSV_ERR_INVALID_ARGUMENT;
-    const int st = bwd_plan(args, &a, &kslots);
+    const int st = bwd_plan(args, &a, &kslots, &parts);
     if (st != GSV_OK) return st;
-    *bytes = delta_bytes(a) + (a.slopes ? sizeof(float) * a.slots * a.scenes * a.heads : 0);
+    *bytes = delta_bytes(a) + 2 * parts_bytes(a, parts) +
+             (a.slopes ? sizeof(double) * a.slots * a.scenes * a.heads : 0);
     return GSV_OK;
 }
 
@@ -424,9 +480,9 @@ extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, con
                                  void *dk, void *dv, void *dslopes, void *workspace,
                                  size_t workspace_bytes, void *stream) {
     AttnArgs a;
-    int kslots;
+    int kslots, parts;
     size_t need;
-    int st = bwd_plan(args, &a, &kslots);
+    int st = bwd_plan(args, &a, &kslots, &parts);
     if (st != GSV_OK) return st;
     if ((st = gsv_attention_bwd_workspace_bytes(args, &need)) != GSV_OK) return st;
     if (need > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
@@ -440,13 +496,16 @@ extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, con
     for (const void *p : ptrs)
         if (reinterpret_cast<uintptr_t>(p) % 16) return GSV_ERR_INVALID_ARGUMENT;
     float *delta = static_cast<float *>(workspace);
-    float *part = reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(a));
-    const BwdArgs g{out, dout, dout_row, dout_head, lse, delta, part, dq, dk, dv};
+    char *next = static_cast<char *>(workspace) + delta_bytes(a);
+    float *part_k = reinterpret_cast<float *>(next);
+    float *part_v = reinterpret_cast<float *>(next + parts_bytes(a, parts));
+    double *slopes = reinterpret_cast<double *>(next + 2 * parts_bytes(a, parts));
+    const BwdArgs g{out, dout, dout_row, dout_head, lse, delta, slopes, dq, dk, dv, parts, part_k, part_v};
     hipStream_t s = as_stream(stream);
     Backward f{a, g, kslots, s};
     attention_variant(a, args->dtype, f);
     if (a.slopes)
-        hipLaunchKernelGGL(k_slope_sum, dim3(a.heads), dim3(64), 0, s, part,
+        hipLaunchKernelGGL(k_slope_sum, dim3(a.heads), dim3(64), 0, s, slopes,
                            a.q_tokens > 0 ? a.slots * a.scenes : 0, a.heads, dslopes, a.slopes_f32);
     return check_launch();
 }

@@ -68,8 +68,7 @@ template <int VEC, int E, int LANES> struct Lane {
 
 // The sum over a row's lanes: one wave, or four of them through LDS.
 template <int WAVES> __device__ __forceinline__ float row_sum(float v, float *lds) {
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) v += __shfl_xor(v, k);
+    v = wave_sum(v);
     if constexpr (WAVES > 1) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;

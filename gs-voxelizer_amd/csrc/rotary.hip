@@ -21,6 +21,7 @@ struct RotaryArgs {
     int64_t pos_row, pos_axis;
     float sign;
     int block_tokens;
+    FastDiv by_pairs, by_items, by_heads;
 };
 
 template <typename T, int N> struct __align__(sizeof(T) * N) Pack {
@@ -38,7 +39,7 @@ __global__ __launch_bounds__(256) void k_rotary(const RotaryArgs a) {
     extern __shared__ float2 turns[];  // cos, sin of block_tokens x pairs
     const int t0 = blockIdx.x * a.block_tokens, nt = min(a.block_tokens, a.tokens - t0);
     for (int i = threadIdx.x; i < nt * a.pairs; i += 256) {
-        const int t = i / a.pairs, p = i % a.pairs;
+        const int t = fastdiv(i, a.by_pairs), p = i - t * a.pairs;
         // the angle in binary64, brought into -pi .. pi there: a binary32 product would lose
         // 2^-24 of an angle of some hundred radians
         double th = 0.0;
@@ -52,15 +53,25 @@ __global__ __launch_bounds__(256) void k_rotary(const RotaryArgs a) {
         turns[i] = make_float2(cs, a.sign * sn);
     }
     __syncthreads();
-    const int all = a.heads + a.kv_heads, items = a.pairs / VEC;
+    // a row's items: its pairs, then the channels past them, which pass through
+    constexpr int W = INTERLEAVED && VEC > 1 ? 2 * VEC : VEC;
+    const int all = a.heads + a.kv_heads, turning = a.pairs / VEC;
+    const int items = turning + (a.dim - 2 * a.pairs) / W;
     for (int i = threadIdx.x; i < nt * all * items; i += 256) {
-        const int row = i / items, p = i % items * VEC, t = row / all, h = row % all;
+        const int row = fastdiv(i, a.by_items), item = i - row * items, p = item * VEC;
+        const int t = fastdiv(row, a.by_heads), h = row - t * all;
         const bool is_q = h < a.heads;
         const int64_t token = t0 + t;
         const T *in = is_q ? static_cast<const T *>(a.q) + token * a.q_row + h * a.q_head
                            : static_cast<const T *>(a.k) + token * a.k_row + (h - a.heads) * a.k_head;
         T *out = is_q ? static_cast<T *>(a.q_out) + (token * a.heads + h) * a.dim
                       : static_cast<T *>(a.k_out) + (token * a.kv_heads + h - a.heads) * a.dim;
+        if (item >= turning) {
+            typedef Pack<T, W> P;
+            const int d = 2 * a.pairs + (item - turning) * W;
+            *reinterpret_cast<P *>(out + d) = *reinterpret_cast<const P *>(in + d);
+            continue;
+        }
         const float2 *tp = turns + t * a.pairs + p;
         if constexpr (INTERLEAVED && VEC == 1) {
             const float2 z = turned((float)in[2 * p], (float)in[2 * p + 1], *tp);
@@ -86,18 +97,6 @@ __global__ __launch_bounds__(256) void k_rotary(const RotaryArgs a) {
             *reinterpret_cast<P *>(out + p) = x;
             *reinterpret_cast<P *>(out + a.pairs + p) = z;
         }
-    }
-    // channels past the pairs pass through
-    const int rest = a.dim - 2 * a.pairs;
-    for (int i = threadIdx.x; i < nt * all * rest; i += 256) {
-        const int row = i / rest, d = 2 * a.pairs + i % rest, t = row / all, h = row % all;
-        const int64_t token = t0 + t;
-        if (h < a.heads)
-            static_cast<T *>(a.q_out)[(token * a.heads + h) * a.dim + d] =
-                static_cast<const T *>(a.q)[token * a.q_row + h * a.q_head + d];
-        else
-            static_cast<T *>(a.k_out)[(token * a.kv_heads + h - a.heads) * a.dim + d] =
-                static_cast<const T *>(a.k)[token * a.k_row + (h - a.heads) * a.k_head + d];
     }
 }
 
@@ -148,6 +147,7 @@ extern "C" int gsv_rotary(const gsv_rotary_args *r, void *q_out, void *k_out, in
         low |= (uint64_t)r->k_row * size | (uint64_t)r->k_head * size |
                reinterpret_cast<uintptr_t>(r->k) | reinterpret_cast<uintptr_t>(k_out);
     low |= (uint64_t)r->pairs * size * (r->interleaved ? 2 : 1);
+    low |= (uint64_t)(r->dim - 2 * r->pairs) * size;
     const int bytes = (int)(low & (0 - low));
     if (bytes < size) return GSV_ERR_INVALID_ARGUMENT;
     const int vec = r->interleaved && bytes > size ? bytes / size / 2 : bytes / size;
@@ -159,7 +159,11 @@ extern "C" int gsv_rotary(const gsv_rotary_args *r, void *q_out, void *k_out, in
     bt = imin64(bt, imax64(1, 2048 / r->pairs));
     const RotaryArgs a{r->q, r->k, q_out, k_out, r->q_row, r->q_head, r->k_row, r->k_head,
                        r->tokens, r->heads, r->kv_heads, r->dim, r->pairs, r->axes, r->positions,
-                       r->frequencies, r->pos_row, r->pos_axis, inverse ? -1.f : 1.f, (int)bt};
+                       r->frequencies, r->pos_row, r->pos_axis, inverse ? -1.f : 1.f, (int)bt,
+                       make_fastdiv(r->pairs),
+                       make_fastdiv(r->pairs / vec + (r->dim - 2 * r->pairs) /
+                                                         (r->interleaved && vec > 1 ? 2 * vec : vec)),
+                       make_fastdiv(r->heads + r->kv_heads)};
     hipStream_t s = as_stream(stream);
     if (r->dtype == GSV_BF16)
         r->interleaved ? launch_rotary<bf16, true>(a, vec, s) : launch_rotary<bf16, false>(a, vec, s);

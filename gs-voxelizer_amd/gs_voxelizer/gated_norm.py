@@ -35,7 +35,8 @@ def gated_residual_norm(x: Tensor, branch: Tensor, weight: Tensor, *,
         gate: a row for each scene (scenes, C) with scene_starts, for each token (T, C), or
             (1, C) for all of them; float32 or branch's type; or None.
         scene_starts: (scenes + 1,) int32 first rows of the scenes.
-        longest: rows of the longest scene, if known (sizes a launch, changes no value).
+        longest: rows of the longest scene, if known: it sizes a launch, and changes at most
+            the rounding of the sums over rows.
     Returns:
         y (T, C) of x's type and h (T, C) of branch's type.
     """

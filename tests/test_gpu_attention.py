@@ -453,3 +453,12 @@ def test_captured_cached_step(device):
         d = dict(c, lengths=torch.tensor([40 + step, 100 + step], dtype=torch.int32, device=device))
         assert torch.equal(got, _cached(d, 0.0)), step
         c["q"].copy_(q * (step + 2))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads", [(1, 1), (8, 1)], ids=str)
+def test_key_gradients_summed_over_parts(device, dtype, dim, heads):
+    """Few key tiles and many rows: several workgroups share a key tile's rows."""
+    _check(_case(device, dtype, [40, 1500], *heads, dim, bias=True, causal=True, prefix=True,
+                 key_lengths=[60, 900]), "parts")
