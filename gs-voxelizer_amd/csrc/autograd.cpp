@@ -36,7 +36,10 @@ using torch::autograd::variable_list;
     X(gsv_status_string) X(gsv_last_hip_error) X(gsv_project_fwd) X(gsv_project_bwd)               \
     X(gsv_cumsum_bin_workspace_bytes) X(gsv_cumsum_bin_and_sort_device_count) X(gsv_voxelize_fwd)  \
     X(gsv_voxelize_fwd_l1_workspace_bytes) X(gsv_voxelize_fwd_l1)                                  \
-    X(gsv_voxelize_bwd_workspace_bytes) X(gsv_voxelize_bwd) X(gsv_voxelize_bwd_l1)
+    X(gsv_voxelize_bwd_workspace_bytes) X(gsv_voxelize_bwd) X(gsv_voxelize_bwd_l1)                 \
+    X(gsv_rotary) X(gsv_gated_norm_fwd) X(gsv_gated_norm_bwd_workspace_bytes)                      \
+    X(gsv_gated_norm_bwd) X(gsv_attention_fwd) X(gsv_attention_bwd_workspace_bytes)                \
+    X(gsv_attention_bwd) X(gsv_attention_cached_workspace_bytes) X(gsv_attention_cached)
 struct Library {
 #define GSV_FIELD(name) decltype(&::name) name = nullptr;
     GSV_ENTRIES(GSV_FIELD)
@@ -470,9 +473,15 @@ std::tuple<int64_t, std::vector<Tensor>> voxelize(
 
 }  // namespace
 
+#include "autograd_tokens.h"
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.attr("torch_version") = GSV_TORCH_VERSION;  // the torch it was compiled against
     m.def("bind", &bind);
     m.def("project", &project, py::call_guard<py::gil_scoped_release>());
     m.def("voxelize", &voxelize, py::call_guard<py::gil_scoped_release>());
+    m.def("rotate", &rotate, py::call_guard<py::gil_scoped_release>());
+    m.def("gated_norm", &gated_norm, py::call_guard<py::gil_scoped_release>());
+    m.def("scene_attention", &scene_attention, py::call_guard<py::gil_scoped_release>());
+    m.def("cached_attention", &cached_attention, py::call_guard<py::gil_scoped_release>());
 }

@@ -66,19 +66,25 @@ template <int VEC, int E, int LANES> struct Lane {
     }
 };
 
-// The sum over a row's lanes: one wave, or four of them through LDS.
-template <int WAVES> __device__ __forceinline__ float row_sum(float v, float *lds) {
-    v = wave_sum(v);
-    if constexpr (WAVES > 1) {
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = 0.f;
+// The sum over a row's lanes: one wave, or several of them through LDS, in two places taken in turn:
+// a wave writes to a place again only behind the next sum's barrier, which all have read before.
+template <int WAVES> struct RowSum {
+    float (*lds)[4];
+    int turn = 0;
+    __device__ __forceinline__ float operator()(float v) {
+        v = wave_sum(v);
+        if constexpr (WAVES > 1) {
+            const int wave = threadIdx.x >> 6, first = wave / WAVES * WAVES;
+            if ((threadIdx.x & 63) == 0) lds[turn][wave] = v;
+            __syncthreads();
+            v = 0.f;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) v += lds[w];
+            for (int w = 0; w < WAVES; ++w) v += lds[turn][first + w];
+            turn ^= 1;
+        }
+        return v;
     }
-    return v;
-}
+};
 
 __device__ __forceinline__ int start_of(const NormArgs &a, int s) {
     if (s <= 0) return 0;
@@ -105,14 +111,17 @@ __device__ __forceinline__ void load_gate(const NormArgs &a, float (&f)[E], int6
 template <typename TX, typename TF, int VEC, int E, int WAVES>
 __global__ __launch_bounds__(256) void k_norm_fwd(const NormArgs a) {
     typedef Lane<VEC, E, 64 * WAVES> L;
-    __shared__ float lds[4];
+    __shared__ float lds[2][4];
+    RowSum<WAVES> row_sum{lds};
     const int lane = threadIdx.x % (64 * WAVES);
     constexpr int kPer = 4 / WAVES;  // rows of a workgroup at a time
     const float inv = 1.f / a.channels;
     float w[E];
     L::load(w, a.weight, lane, a.channels);
     const int stride = gridDim.x * kPer;
-    for (int row = blockIdx.x * kPer + (threadIdx.x >> 6) / WAVES; row < a.tokens; row += stride) {
+    for (int first = blockIdx.x * kPer; first < a.tokens; first += stride) {
+        // waves past the last row form it again and store nothing: all meet at the sums' barriers
+        const int mine = first + (threadIdx.x >> 6) / WAVES, row = min(mine, a.tokens - 1);
         float x[E], f[E];
         L::load(f, static_cast<const TF *>(a.branch) + row * a.branch_row, lane, a.channels);
         L::load(x, static_cast<const TX *>(a.x) + row * a.x_row, lane, a.channels);
@@ -134,69 +143,88 @@ __global__ __launch_bounds__(256) void k_norm_fwd(const NormArgs a) {
             L::load(t, a.branch_weight, lane, a.channels);
 #pragma unroll
             for (int e = 0; e < E; ++e) sq = fmaf(f[e], f[e], sq);
-            const float r = rsqrtf(row_sum<WAVES>(sq, lds) * inv + a.eps);
+            const float r = rsqrtf(row_sum(sq) * inv + a.eps);
 #pragma unroll
             for (int e = 0; e < E; ++e) f[e] *= r * t[e];
         }
         float sq = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) x[e] = fmaf(by[e], f[e], x[e]), sq = fmaf(x[e], x[e], sq);
-        const float r = rsqrtf(row_sum<WAVES>(sq, lds) * inv + a.eps);
-        L::store(x, static_cast<TX *>(a.y) + (int64_t)row * a.channels, lane, a.channels);
+        const float r = rsqrtf(row_sum(sq) * inv + a.eps);
+        if (mine == row) L::store(x, static_cast<TX *>(a.y) + (int64_t)row * a.channels, lane, a.channels);
 #pragma unroll
         for (int e = 0; e < E; ++e) x[e] *= r * w[e];
-        L::store(x, static_cast<TF *>(a.h) + (int64_t)row * a.channels, lane, a.channels);
+        if (mine == row) L::store(x, static_cast<TF *>(a.h) + (int64_t)row * a.channels, lane, a.channels);
     }
 }
 
-template <typename TX, typename TF, int VEC, int E, int WAVES>
+// TOKEN: a gate for each token.  What a lane keeps over its rows is weight, gate times scale times
+// branch_weight (TOKEN: without the gate) and the two sums.
+template <typename TX, typename TF, int VEC, int E, int WAVES, bool TOKEN>
 __global__ __launch_bounds__(256) void k_norm_bwd(const NormArgs a) {
     typedef Lane<VEC, E, 64 * WAVES> L;
-    __shared__ float lds[4];
-    __shared__ float sums[WAVES == 1 ? 3 * 64 * E : 1];
+    __shared__ float lds[2][4];
+    RowSum<WAVES> row_sum{lds};
+    constexpr int kPer = 4 / WAVES;  // rows of a workgroup at a time
+    __shared__ float sums[kPer > 1 ? (kPer - 1) * 64 * WAVES * E : 1];
     const int lane = threadIdx.x % (64 * WAVES), wave = threadIdx.x >> 6;
-    constexpr int kPer = 4 / WAVES;
     const float inv = 1.f / a.channels;
     const int s = blockIdx.x / a.slots, slot = blockIdx.x % a.slots;
     const int r0 = start_of(a, s), r1 = max(start_of(a, s + 1), r0);
-    float wgt[E], gs[E], bw[E], sum_a[E], sum_b[E];
+    float wgt[E], by[E], sum_a[E], sum_b[E];
     L::load(wgt, a.weight, lane, a.channels);
 #pragma unroll
-    for (int e = 0; e < E; ++e) gs[e] = bw[e] = 1.f, sum_a[e] = sum_b[e] = 0.f;
-    if (a.branch_weight) L::load(bw, a.branch_weight, lane, a.channels);
-    if (a.scale) L::load(gs, a.scale, lane, a.channels);
-    if (a.gate && !a.per_token) {
-        float g[E];
-        load_gate<TF, L>(a, g, s, lane);
+    for (int e = 0; e < E; ++e) by[e] = 1.f, sum_a[e] = sum_b[e] = 0.f;
+    if (a.branch_weight) L::load(by, a.branch_weight, lane, a.channels);
+    if (a.scale) {
+        float t[E];
+        L::load(t, a.scale, lane, a.channels);
 #pragma unroll
-        for (int e = 0; e < E; ++e) gs[e] *= g[e];
+        for (int e = 0; e < E; ++e) by[e] *= t[e];
+    }
+    if (!TOKEN && a.gate) {
+        float t[E];
+        load_gate<TF, L>(a, t, s, lane);
+#pragma unroll
+        for (int e = 0; e < E; ++e) by[e] *= t[e];
     }
     for (int64_t base = r0 + (int64_t)slot * a.rows; base < r1; base += (int64_t)a.slots * a.rows)
-        for (int64_t row = base + wave / WAVES; row < min(base + a.rows, (int64_t)r1); row += kPer) {
+        for (int64_t first = base, end = min(base + a.rows, (int64_t)r1); first < end; first += kPer) {
+            // waves past the last row take it with zero gradients and store nothing
+            const int64_t mine = first + wave / WAVES, row = min(mine, end - 1);
+            const bool live = mine == row;
             float x[E], f[E], dy[E], dh[E], g[E];
             L::load(f, static_cast<const TF *>(a.branch) + row * a.branch_row, lane, a.channels);
             L::load(x, static_cast<const TX *>(a.x) + row * a.x_row, lane, a.channels);
+            if (a.dh && live) {
+                L::load(dh, static_cast<const TF *>(a.dh) + row * a.dh_row, lane, a.channels);
+            } else {
 #pragma unroll
-            for (int e = 0; e < E; ++e) dy[e] = dh[e] = 0.f;
-            if (a.dh) L::load(dh, static_cast<const TF *>(a.dh) + row * a.dh_row, lane, a.channels);
-            if (a.dy) L::load(dy, static_cast<const TX *>(a.dy) + row * a.dy_row, lane, a.channels);
-            if (a.per_token) load_gate<TF, L>(a, g, row, lane);
+                for (int e = 0; e < E; ++e) dh[e] = 0.f;
+            }
+            if (a.dy && live) {
+                L::load(dy, static_cast<const TX *>(a.dy) + row * a.dy_row, lane, a.channels);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) dy[e] = 0.f;
+            }
+            if constexpr (TOKEN) load_gate<TF, L>(a, g, row, lane);
+            const auto weight = [&](int e) { return TOKEN ? by[e] * g[e] : by[e]; };
             float rb = 1.f;
             if (a.branch_weight) {
                 float sq = 0.f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) sq = fmaf(f[e], f[e], sq);
-                rb = rsqrtf(row_sum<WAVES>(sq, lds) * inv + a.eps);
+                rb = rsqrtf(row_sum(sq) * inv + a.eps);
             }
             float sq = 0.f;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 f[e] *= rb;  // branch_hat
-                const float by = a.per_token ? gs[e] * g[e] : gs[e];
-                x[e] = fmaf(by * bw[e], f[e], x[e]);
+                x[e] = fmaf(weight(e), f[e], x[e]);
                 sq = fmaf(x[e], x[e], sq);
             }
-            const float ry = rsqrtf(row_sum<WAVES>(sq, lds) * inv + a.eps);
+            const float ry = rsqrtf(row_sum(sq) * inv + a.eps);
             float m1 = 0.f;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
@@ -205,46 +233,52 @@ __global__ __launch_bounds__(256) void k_norm_bwd(const NormArgs a) {
                 dh[e] *= wgt[e];
                 m1 = fmaf(dh[e], x[e], m1);
             }
-            m1 = row_sum<WAVES>(m1, lds) * inv;
+            m1 = row_sum(m1) * inv;
             float m2 = 0.f;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 dy[e] = fmaf(ry, dh[e] - x[e] * m1, dy[e]);
-                const float by = a.per_token ? gs[e] * g[e] : gs[e];
-                const float t = dy[e] * f[e];  // of A
-                sum_a[e] += a.per_token ? t * g[e] : t;
-                if (a.per_token) g[e] = t * gs[e] * bw[e];
-                x[e] = dy[e] * by * bw[e];
+                x[e] = dy[e] * weight(e);
                 m2 = fmaf(x[e], f[e], m2);
+                const float t = dy[e] * f[e];  // of A
+                if constexpr (TOKEN) {
+                    sum_a[e] = fmaf(t, g[e], sum_a[e]);
+                    g[e] = t * by[e];
+                } else {
+                    sum_a[e] += t;
+                }
             }
-            L::store(dy, static_cast<TX *>(a.dx) + row * a.channels, lane, a.channels);
-            if (a.per_token) {
+            if (live) L::store(dy, static_cast<TX *>(a.dx) + row * a.channels, lane, a.channels);
+            if (TOKEN && live) {
                 if (a.f32_gate) L::store(g, static_cast<float *>(a.dgate) + row * a.channels, lane, a.channels);
                 else L::store(g, static_cast<TF *>(a.dgate) + row * a.channels, lane, a.channels);
             }
             if (a.branch_weight) {
-                m2 = row_sum<WAVES>(m2, lds) * inv;
+                m2 = row_sum(m2) * inv;
 #pragma unroll
                 for (int e = 0; e < E; ++e) x[e] = rb * (x[e] - f[e] * m2);
             }
-            L::store(x, static_cast<TF *>(a.dbranch) + row * a.channels, lane, a.channels);
+            if (live) L::store(x, static_cast<TF *>(a.dbranch) + row * a.channels, lane, a.channels);
         }
-    // the workgroup's sums
-    if constexpr (WAVES == 1) {
+    // the workgroup's sums: those of the first row's waves, then the other rows'
+    if constexpr (kPer > 1) {
+        constexpr int kLanes = 64 * WAVES;
+        const int group = wave / WAVES;
 #pragma unroll
         for (int turn = 0; turn < 2; ++turn) {
             float(&v)[E] = turn ? sum_b : sum_a;
             __syncthreads();
-            if (wave)
+            if (group)
 #pragma unroll
-                for (int e = 0; e < E; ++e) sums[((wave - 1) * E + e) * 64 + lane] = v[e];
+                for (int e = 0; e < E; ++e) sums[((group - 1) * E + e) * kLanes + lane] = v[e];
             __syncthreads();
-            if (!wave)
+            if (!group)
 #pragma unroll
                 for (int e = 0; e < E; ++e)
-                    v[e] += sums[e * 64 + lane] + sums[(E + e) * 64 + lane] + sums[(2 * E + e) * 64 + lane];
+#pragma unroll
+                    for (int o = 0; o < kPer - 1; ++o) v[e] += sums[(o * E + e) * kLanes + lane];
         }
-        if (wave) return;
+        if (group) return;
     }
     L::store(sum_a, a.part_a + (int64_t)blockIdx.x * a.channels, lane, a.channels);
     L::store(sum_b, a.part_b + (int64_t)blockIdx.x * a.channels, lane, a.channels);
@@ -305,24 +339,34 @@ __global__ __launch_bounds__(256) void k_norm_sums(const NormArgs a, float *dwei
 }
 
 template <typename TX, typename TF, int VEC, int E, int WAVES>
-void launch_one(const NormArgs &a, bool backward, hipStream_t s) {
-    if (backward) {
-        hipLaunchKernelGGL((k_norm_bwd<TX, TF, VEC, E, WAVES>), dim3((unsigned)(a.scenes * a.slots)),
-                           dim3(256), 0, s, a);
-    } else {
-        // 16 waves a SIMD's worth of rows at most; a wave keeps the weights over its rows
-        const int64_t want = ((int64_t)a.tokens * WAVES + 3) / 4;
-        hipLaunchKernelGGL((k_norm_fwd<TX, TF, VEC, E, WAVES>), dim3((unsigned)imin64(want, 8192)),
-                           dim3(256), 0, s, a);
-    }
+void launch_fwd(const NormArgs &a, hipStream_t s) {
+    // a wave keeps the weights over its rows
+    const int64_t want = ((int64_t)a.tokens * WAVES + 3) / 4;
+    hipLaunchKernelGGL((k_norm_fwd<TX, TF, VEC, E, WAVES>), dim3((unsigned)imin64(want, 8192)),
+                       dim3(256), 0, s, a);
 }
+template <typename TX, typename TF, int VEC, int E, int WAVES>
+void launch_bwd(const NormArgs &a, hipStream_t s) {
+    const dim3 grid((unsigned)(a.scenes * a.slots));
+    if (a.per_token) hipLaunchKernelGGL((k_norm_bwd<TX, TF, VEC, E, WAVES, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_norm_bwd<TX, TF, VEC, E, WAVES, false>), grid, dim3(256), 0, s, a);
+}
+// Channels of a lane and waves of a row.  The backward keeps eight vectors of them, so 8 channels a
+// lane (112 registers, four waves a SIMD) and more waves a row: 20,000 rows of 1024 take 88 us, with 16
+// channels a lane and one wave (190 registers) 140.
 template <typename TX, typename TF, int VEC>
 void launch_width(const NormArgs &a, bool backward, hipStream_t s) {
-    // channels of a lane: a row of a wave up to 2048 channels, of four waves up to 8192
-    if (a.channels <= 512) launch_one<TX, TF, VEC, 8, 1>(a, backward, s);
-    else if (a.channels <= 1024) launch_one<TX, TF, VEC, 16, 1>(a, backward, s);
-    else if (a.channels <= 2048) launch_one<TX, TF, VEC, 32, 1>(a, backward, s);
-    else launch_one<TX, TF, VEC, 32, 4>(a, backward, s);
+    if (!backward) {
+        if (a.channels <= 512) launch_fwd<TX, TF, VEC, 8, 1>(a, s);
+        else if (a.channels <= 1024) launch_fwd<TX, TF, VEC, 16, 1>(a, s);
+        else if (a.channels <= 2048) launch_fwd<TX, TF, VEC, 32, 1>(a, s);
+        else launch_fwd<TX, TF, VEC, 32, 4>(a, s);
+    } else {
+        if (a.channels <= 512) launch_bwd<TX, TF, VEC, 8, 1>(a, s);
+        else if (a.channels <= 1024) launch_bwd<TX, TF, VEC, 8, 2>(a, s);
+        else if (a.channels <= 2048) launch_bwd<TX, TF, VEC, 8, 4>(a, s);
+        else launch_bwd<TX, TF, VEC, 32, 4>(a, s);
+    }
 }
 template <typename TX, typename TF> void launch_types(const NormArgs &a, int vec, bool backward, hipStream_t s) {
     if (vec == 8) launch_width<TX, TF, 8>(a, backward, s);
@@ -373,7 +417,7 @@ int norm_vec(const gsv_norm *n, const void *const *ptrs, const int *f32, const i
 // Rows and workgroups of the backward: about 1024 workgroups, at least 16 rows each.
 bool norm_slots(const gsv_norm *n, NormArgs *a) {
     const int64_t longest = n->longest > 0 && n->longest < n->tokens ? n->longest : imax64(n->tokens, 1);
-    a->rows = (int)imax64(16, (n->tokens + 1023) / 1024);
+    a->rows = (int)imax64(16, ((int64_t)n->tokens + 1023) / 1024);
     a->slots = (int)((longest + a->rows - 1) / a->rows);
     if (a->scenes > (1 << 22)) return false;
     a->slots = (int)imin64(a->slots, imax64(1, 16384 / a->scenes));

@@ -1,7 +1,8 @@
 """The native autograd nodes (csrc/autograd.cpp) and which calls may take them.
 
 Plain calls of ``optim_to_render`` and ``voxelize_gaussians`` (ordinary tensors,
-no transform or mode active) go to ``project`` and ``voxelize``, which return
+no transform or mode active) go to ``project`` and ``voxelize``, those of the operators on
+packed tokens to ``rotate``, ``gated_norm``, ``scene_attention`` and ``cached_attention``; all return
 nothing for a call they do not take; the Python autograd classes then do it, and
 raise its errors.  Without a module built for this torch, or in a torch that no
 longer has one of the private names that `plain` asks, the classes do all calls
@@ -18,7 +19,10 @@ from . import _lib
 _ENTRIES = ("gsv_status_string", "gsv_last_hip_error", "gsv_project_fwd", "gsv_project_bwd",
             "gsv_cumsum_bin_workspace_bytes", "gsv_cumsum_bin_and_sort_device_count",
             "gsv_voxelize_fwd", "gsv_voxelize_fwd_l1_workspace_bytes", "gsv_voxelize_fwd_l1",
-            "gsv_voxelize_bwd_workspace_bytes", "gsv_voxelize_bwd", "gsv_voxelize_bwd_l1")
+            "gsv_voxelize_bwd_workspace_bytes", "gsv_voxelize_bwd", "gsv_voxelize_bwd_l1",
+            "gsv_rotary", "gsv_gated_norm_fwd", "gsv_gated_norm_bwd_workspace_bytes",
+            "gsv_gated_norm_bwd", "gsv_attention_fwd", "gsv_attention_bwd_workspace_bytes",
+            "gsv_attention_bwd", "gsv_attention_cached_workspace_bytes", "gsv_attention_cached")
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
@@ -50,6 +54,8 @@ _module, _why = _load()
 available = _module is not None
 if available:
     project, voxelize = _module.project, _module.voxelize
+    rotate, gated_norm = _module.rotate, _module.gated_norm
+    scene_attention, cached_attention = _module.scene_attention, _module.cached_attention
 else:
     warnings.warn(f"gs_voxelizer: no native autograd nodes ({_why}); every call takes the Python "
                   "classes. Build them with `python gs-voxelizer_amd/build.py`.", RuntimeWarning)

@@ -7,6 +7,7 @@ before anything is launched; outputs and workspaces are torch tensors, and
 every kernel is enqueued on torch's current stream of the tensors' device.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -113,6 +114,30 @@ def mask(t, what, shape, device):
     check(t.device == device, f"{what} must be on {device}, got {t.device}")
     check(tuple(t.shape) == shape, f"{what} must have shape {shape}, got {tuple(t.shape)}")
     return t if t.stride(-1) == 1 else t.contiguous()
+
+
+_ONCE = b"gs_voxelizer: this operator's gradients can be differentiated once only"
+
+
+def once(backward):
+    """A backward whose kernels have no gradients themselves: differentiating its results raises
+    (also where the incoming gradient is a constant, so that no second derivative is silently
+    left out)."""
+    @functools.wraps(backward)
+    def wrapped(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():  # no create_graph
+            return out
+        return tuple(g if g is None else
+                     torch._C._functions.DelayedError(_ONCE, 1)(g.detach().requires_grad_())
+                     for g in out)
+    return wrapped
+
+
+def present(*tensors):
+    """The optional arguments that are given."""
+    return [t for t in tensors if t is not None]
 
 
 def ptr(t):

@@ -17,9 +17,8 @@ from typing import Optional
 import torch
 from torch import Tensor
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
-from . import _lib, _tokens as _t
+from . import _lib, _native, _tokens as _t
 
 MAX_DIM = 128
 
@@ -81,6 +80,13 @@ def scene_attention(q: Tensor, k: Tensor, v: Tensor, *, scene_starts: Optional[T
     Returns:
         (T, H, D), contiguous.
     """
+    if scale != 0 and _native.plain(q, k, v, *_t.present(
+            scene_starts, key_starts, prefix, positions, key_positions, slopes, keep)):
+        out = _native.scene_attention(q, k, v, scene_starts, key_starts, int(longest or 0),
+                                      bool(causal), prefix, float(scale or 0.0), float(cap or 0.0),
+                                      positions, key_positions, slopes, keep)
+        if out:
+            return out[0]
     H, K, D = _heads(q, k, v, 3)
     dev, T, N = q.device, q.shape[0], k.shape[0]
     _t.check(T <= _t.INT32_MAX and N <= _t.INT32_MAX, "too many tokens")
@@ -154,7 +160,7 @@ class _SceneAttention(Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_t.once
     def backward(ctx, dout):
         q, k, v, slopes, out, lse, *held = ctx.saved_tensors
         a, dev = ctx.args, q.device
@@ -187,6 +193,12 @@ def cached_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tenso
     Returns:
         (S, H, D).
     """
+    if scale != 0 and _native.plain(q, k_cache, v_cache, lengths, *_t.present(
+            positions, key_positions, slopes, keep)):
+        out = _native.cached_attention(q, k_cache, v_cache, lengths, float(scale or 0.0),
+                                       float(cap or 0.0), positions, key_positions, slopes, keep)
+        if out:
+            return out[0]
     H, K, D = _heads(q, k_cache, v_cache, 4)
     dev, S, N = q.device, q.shape[0], k_cache.shape[1]
     _t.check(k_cache.shape[0] == S, f"k_cache holds {k_cache.shape[0]} scenes, q {S}")

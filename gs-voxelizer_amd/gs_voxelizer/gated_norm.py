@@ -13,9 +13,8 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
-from . import _lib, _tokens as _t
+from . import _lib, _native, _tokens as _t
 
 MAX_CHANNELS = 8192
 
@@ -40,6 +39,11 @@ def gated_residual_norm(x: Tensor, branch: Tensor, weight: Tensor, *,
     Returns:
         y (T, C) of x's type and h (T, C) of branch's type.
     """
+    if _native.plain(x, branch, weight, *_t.present(branch_weight, scale, gate, scene_starts)):
+        out = _native.gated_norm(x, branch, weight, branch_weight, scale, gate, scene_starts,
+                                 int(longest or 0), float(eps))
+        if out:
+            return tuple(out)
     _t.activations(x, "x", 2)
     _t.activations(branch, "branch", 2)
     dev, (T, C) = x.device, x.shape
@@ -113,7 +117,7 @@ class _GatedNorm(Function):
         return _forward(x, branch, weight, branch_weight, scale, gate, starts, opts)
 
     @staticmethod
-    @once_differentiable
+    @_t.once
     def backward(ctx, dy, dh):
         x, branch, weight, branch_weight, scale, gate, starts = ctx.saved_tensors
         if dy is None and dh is None:

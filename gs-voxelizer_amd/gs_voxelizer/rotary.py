@@ -12,9 +12,8 @@ from typing import Optional, Sequence, Tuple
 import torch
 from torch import Tensor
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
-from . import _lib, _tokens as _t
+from . import _lib, _native, _tokens as _t
 
 
 def axis_frequencies(pairs: Sequence[int], base: float = 1000.0, device=None) -> Tensor:
@@ -44,6 +43,10 @@ def rotate_qk(q: Tensor, k: Optional[Tensor], positions: Tensor, frequencies: Te
     Returns:
         the turned q and k, contiguous; channels from 2 P on pass through.
     """
+    if k is not None and _native.plain(q, k, positions, frequencies):
+        out = _native.rotate(q, k, positions, frequencies, bool(interleaved))
+        if out:
+            return tuple(out)
     _t.activations(q, "q", 3)
     dev = q.device
     if k is not None:
@@ -102,7 +105,7 @@ class _RotateQK(Function):
         return _turn(q, k, positions, frequencies, interleaved, False)
 
     @staticmethod
-    @once_differentiable
+    @_t.once
     def backward(ctx, dq, dk):
         dq, dk = (g if need else None for g, need in zip((dq, dk), ctx.needs_input_grad))
         if dq is None and dk is None:

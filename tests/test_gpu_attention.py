@@ -4,11 +4,20 @@ import pytest
 import torch
 
 import token_reference as R
-from gs_voxelizer import attention
+from gs_voxelizer import _native, attention
 
 pytestmark = pytest.mark.gpu
 
 F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(autouse=True, params=["native", "python"])
+def route(request, monkeypatch):
+    """Through the native autograd nodes where they take the call, and through the Python classes."""
+    if request.param == "python":
+        monkeypatch.setattr(_native, "available", False)
+    else:
+        assert _native.available
 NAMES = ("dq", "dk", "dv", "dslopes")
 
 
@@ -462,3 +471,20 @@ def test_key_gradients_summed_over_parts(device, dtype, dim, heads):
     """Few key tiles and many rows: several workgroups share a key tile's rows."""
     _check(_case(device, dtype, [40, 1500], *heads, dim, bias=True, causal=True, prefix=True,
                  key_lengths=[60, 900]), "parts")
+
+
+def test_gradients_are_not_differentiated_again(device):
+    c = _case(device, F32, [20], 2, 2, 32)
+    q = c["q"].requires_grad_()
+    g, = torch.autograd.grad(attention.scene_attention(q, c["k"], c["v"]).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate"):
+        g.sum().backward()
+
+
+def test_saved_tensor_hooks_may_move_what_is_saved(device):
+    c = _case(device, BF16, [150, 77], 4, 2, 64, bias=True, causal=True, prefix=True, culled=0.2)
+    want = _run(c)
+    with torch.autograd.graph.save_on_cpu():
+        got = _run(c)
+    for n in got:
+        assert torch.equal(got[n], want[n]), n

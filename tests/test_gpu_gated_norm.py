@@ -7,11 +7,20 @@ import pytest
 import torch
 
 import token_reference as R
-from gs_voxelizer import gated_norm
+from gs_voxelizer import _native, gated_norm
 
 pytestmark = pytest.mark.gpu
 
 F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(autouse=True, params=["native", "python"])
+def route(request, monkeypatch):
+    """Through the native autograd nodes where they take the call, and through the Python classes."""
+    if request.param == "python":
+        monkeypatch.setattr(_native, "available", False)
+    else:
+        assert _native.available
 LEAVES = ("x", "branch", "weight", "branch_weight", "scale", "gate")
 
 
@@ -261,3 +270,21 @@ def test_refusals(device):
     refused("eps", x, x, w, eps=-1.0)
     big = torch.zeros(1, 8193, device=device)
     refused("channels", big, big, big[0])
+
+
+def test_gradients_are_not_differentiated_again(device):
+    x = torch.ones(5, 32, device=device, requires_grad=True)
+    y, h = gated_norm.gated_residual_norm(x, torch.ones_like(x), torch.ones(32, device=device))
+    g, = torch.autograd.grad((y + h).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate"):
+        g.sum().backward()
+
+
+def test_saved_tensor_hooks_may_move_what_is_saved(device):
+    """Saved tensors kept in host memory between the passes: the same gradients."""
+    c = _case(device, 300, 128, [130, 170], (F32, BF16))
+    want = _run(c)
+    with torch.autograd.graph.save_on_cpu():
+        got = _run(c)
+    for n in got:
+        assert torch.equal(got[n], want[n]), n

@@ -5,11 +5,20 @@ import pytest
 import torch
 
 import token_reference as R
-from gs_voxelizer import rotary
+from gs_voxelizer import _native, rotary
 
 pytestmark = pytest.mark.gpu
 
 F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(autouse=True, params=["native", "python"])
+def route(request, monkeypatch):
+    """Through the native autograd nodes where they take the call, and through the Python classes."""
+    if request.param == "python":
+        monkeypatch.setattr(_native, "available", False)
+    else:
+        assert _native.available
 
 
 def _gen(device, seed=0):
@@ -159,3 +168,12 @@ def test_refusals(device):
     refused("detach", q, q, pos.clone().requires_grad_(), f)
     with pytest.raises(ValueError):
         rotary.axis_frequencies([])
+
+
+def test_gradients_are_not_differentiated_again(device):
+    q = torch.ones(5, 2, 8, device=device, requires_grad=True)
+    f = rotary.axis_frequencies((2, 1, 1), device=device)
+    a, b = rotary.rotate_qk(q, q, torch.ones(5, 3, device=device), f)
+    g, = torch.autograd.grad((a.sum() + b.sum()), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate"):
+        g.sum().backward()
