@@ -5,7 +5,9 @@
 //   dslope = - sum_ij dt_ij |p_i - p_j|
 //   ds_ij = dt_ij (1 - tanh^2)        dq_i = scale sum_j ds_ij k_j
 //                                     dk_j = scale sum_i ds_ij q_i
-// Two kernels form the scores twice, one with the rows' sums (dq, D, dslope) and one with
+// D_i is formed from o_i in two parts (out, and out_low, what its rounding took): where one key has
+// nearly all of a row's weight, do_i.v_j - D_i is a small difference, and 8 bits of o_i would leave
+// little of it.  Two kernels form the scores twice, one with the rows' sums (dq, D, dslope) and one with
 // the keys' (dk, dv): each sum stays in the registers of one wave, in a fixed order, with
 // no atomics and no partial gradients in memory.
 #include "gsv_attention.h"
@@ -20,7 +22,7 @@ constexpr int kRows = 128;  // rows (dq) or keys (dk, dv) of a workgroup, 32 a w
 template <typename T> constexpr int kOther = sizeof(T) == 2 ? 64 : 32;
 
 struct BwdArgs {
-    const void *out, *dout;
+    const void *out, *out_low, *dout;
     int64_t dout_row, dout_head;
     const float *lse;
     float *delta;   // (heads, q_tokens)
@@ -94,6 +96,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
                 const frag f = row_frag(o + d);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) delta = fmaf((float)f[e], (float)dO[st][e], delta);
+                if (g.out_low) {
+                    const frag w = row_frag(static_cast<const T *>(g.out_low) +
+                                            (qi * a.heads + h) * a.dim + d);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) delta = fmaf((float)w[e], (float)dO[st][e], delta);
+                }
             }
         }
         delta += other_half(delta);
@@ -114,6 +122,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
         const int mine = first + wave * 32 < nq
                              ? key_limit(a, c, min(first + wave * 32 + 32, nq) - 1) : 0;
         f32x16 dq[DP / 32] = {};
+        float mean = 0.f, rest = 0.f;
 
         float gp = 0.f;
         int raw = 0;
@@ -176,8 +185,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
                             if (!(seen & (1u << result_row(r)))) w[r] = -INFINITY;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        dp[r] = (dp[r] - delta) * fast_exp2(fmaf(w[r], unit, -lse));
-                        if (far) here = fmaf(dp[r], d[r], here);
+                        const float p = fast_exp2(fmaf(w[r], unit, -lse));
+                        dp[r] = (dp[r] - delta) * p;
+                        if (far) {
+                            here = fmaf(dp[r], d[r], here);
+                            if (sizeof(T) == 2) mean = fmaf(p, d[r], mean), rest += dp[r];
+                        }
                         if (capped) dp[r] *= fmaf(-u[r], u[r], 1.f);
                     }
 #pragma unroll
@@ -192,6 +205,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
             }
             if (more) put(b ^ 1);
             __syncthreads();
+        }
+        // D_i comes from an output whose weights were rounded to T.  dslope sums over all rows, and in
+        // it a row's rest, sum_j p_ij (do_i.v_j - D_i), which ought to be 0, would meet its mean
+        // distance: taken out, dslope is as good as float32 weights make it.
+        if (far && sizeof(T) == 2) {
+            rest += other_half(rest);
+            dslope += rest * mean;
         }
         if (row)
             store_column<T, DP>(static_cast<T *>(g.dq) + (qi * a.heads + h) * a.dim, dq, a.scale, a.dim,
@@ -475,8 +495,8 @@ extern "C" int gsv_attention_bwd_workspace_bytes(const gsv_attention *args, size
     return GSV_OK;
 }
 
-extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, const float *lse,
-                                 const void *dout, int64_t dout_row, int64_t dout_head, void *dq,
+extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, const void *out_low,
+                                 const float *lse, const void *dout, int64_t dout_row, int64_t dout_head, void *dq,
                                  void *dk, void *dv, void *dslopes, void *workspace,
                                  size_t workspace_bytes, void *stream) {
     AttnArgs a;
@@ -492,7 +512,7 @@ extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, con
         return GSV_ERR_INVALID_ARGUMENT;
     if (a.q_tokens > 0 && (!out || !lse || !dout || !dq || !workspace)) return GSV_ERR_INVALID_ARGUMENT;
     if ((a.k_tokens > 0 && (!dk || !dv)) || (a.slopes && !dslopes)) return GSV_ERR_INVALID_ARGUMENT;
-    const void *ptrs[] = {out, dout, dq, dk, dv, workspace};
+    const void *ptrs[] = {out, out_low, dout, dq, dk, dv, workspace};
     for (const void *p : ptrs)
         if (reinterpret_cast<uintptr_t>(p) % 16) return GSV_ERR_INVALID_ARGUMENT;
     float *delta = static_cast<float *>(workspace);
@@ -500,7 +520,7 @@ extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, con
     float *part_k = reinterpret_cast<float *>(next);
     float *part_v = reinterpret_cast<float *>(next + parts_bytes(a, parts));
     double *slopes = reinterpret_cast<double *>(next + 2 * parts_bytes(a, parts));
-    const BwdArgs g{out, dout, dout_row, dout_head, lse, delta, slopes, dq, dk, dv, parts, part_k, part_v};
+    const BwdArgs g{out, out_low, dout, dout_row, dout_head, lse, delta, slopes, dq, dk, dv, parts, part_k, part_v};
     hipStream_t s = as_stream(stream);
     Backward f{a, g, kslots, s};
     attention_variant(a, args->dtype, f);

@@ -156,11 +156,11 @@ __global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             w[r] = fast_exp2(fmaf(w[r], unit, -ref));
-            sum += w[r];
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const frag p = to_frag<T>(w, half);
+            sum = add_weights(p, sum);
 #pragma unroll
             for (int e = 0; e < DP / 32; ++e)
                 o[e] = mma(at.columns(vt + half * 16 * DP, e, lane), p, o[e]);

@@ -20,9 +20,10 @@ constexpr float kSlack = 8.f;
 // HEADS query heads of a wave share its distances (a third of the vector work of one head: 2
 // multiply-adds, a multiply and a root an element, at the matrix units' differences).  With one
 // key head for both (SHARED) they share the tiles too.
-template <typename T, int DP, bool FAR, bool CAPPED, int HEADS, bool SHARED>
+// TRAIN: the log sums and out_low are wanted.
+template <typename T, int DP, bool FAR, bool CAPPED, int HEADS, bool SHARED, bool TRAIN>
 __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_attention_fwd(
-    const AttnArgs a, T *__restrict__ out, float *__restrict__ lse) {
+    const AttnArgs a, T *__restrict__ out, T *__restrict__ out_low, float *__restrict__ lse) {
     constexpr int KB = sizeof(T) == 2 ? 64 : 32;  // keys of a tile
     constexpr int KV = SHARED ? 1 : HEADS;        // key heads of the workgroup
     constexpr bool far = FAR, capped = CAPPED;
@@ -87,9 +88,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
         const int mine = first + wave * 32 < nq
                              ? key_limit(a, c, min(first + wave * 32 + 32, nq) - 1) : 0;
         f32x16 o[HEADS][DP / 32] = {};
-        float m[HEADS], sum[HEADS];
+        // the weights' sums as the product takes them and, for the log sums, unrounded
+        float m[HEADS], sum[HEADS], exact[HEADS];
 #pragma unroll
-        for (int n = 0; n < HEADS; ++n) m[n] = -INFINITY, sum[n] = 0.f;
+        for (int n = 0; n < HEADS; ++n) m[n] = -INFINITY, sum[n] = exact[n] = 0.f;
 
         float gp = 0.f;
         int raw = 0;
@@ -171,7 +173,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
                             const float next = fmaxf(m[n], fmaxf(top[n], other_half(top[n])));
                             const float by = next == -INFINITY ? 1.f : fast_exp2(m[n] - next);
                             m[n] = next;
-                            sum[n] *= by;
+                            sum[n] *= by, exact[n] *= by;
 #pragma unroll
                             for (int e = 0; e < DP / 32; ++e) o[n][e] *= by;
                         }
@@ -182,11 +184,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             w[n][r] = fast_exp2(fmaf(w[n][r], unit, -ref));
-                            sum[n] += w[n][r];
+                            if (TRAIN) exact[n] += w[n][r];
                         }
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             const frag p = to_frag<T>(w[n], half);
+                            sum[n] = add_weights(p, sum[n]);
                             const T *vt = sv[b][SHARED ? 0 : n] + (kb * 32 + half * 16) * DP;
 #pragma unroll
                             for (int e = 0; e < DP / 32; ++e)
@@ -201,13 +204,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
 #pragma unroll
         for (int n = 0; n < HEADS; ++n) {
             sum[n] += other_half(sum[n]);
+            exact[n] += other_half(exact[n]);
             if (!row) continue;
-            store_column<T, DP>(out + (qi * a.heads + h0 + n) * a.dim, o[n],
-                                sum[n] == 0.f ? 0.f : 1.f / sum[n], a.dim, lane);
+            const int64_t at_out = (qi * a.heads + h0 + n) * a.dim;
+            store_column<T, DP>(out + at_out, o[n], sum[n] == 0.f ? 0.f : 1.f / sum[n], a.dim, lane,
+                                TRAIN && out_low ? out_low + at_out : nullptr);
             // log2 of the row's sum of exponentials; +inf for an empty row, whose weights
             // in the backward are exp2(-inf)
-            if (lse && lane < 32)
-                lse[(int64_t)(h0 + n) * a.q_tokens + qi] = sum[n] == 0.f ? INFINITY : m[n] + log2f(sum[n]);
+            if (TRAIN && lane < 32)
+                lse[(int64_t)(h0 + n) * a.q_tokens + qi] =
+                    exact[n] == 0.f ? INFINITY : m[n] + log2f(exact[n]);
         }
     }
 }
@@ -215,7 +221,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
 struct Forward {
     AttnArgs a;
     int longest;
-    void *out;
+    void *out, *out_low;
     float *lse;
     hipStream_t st;
     int status;
@@ -224,9 +230,14 @@ struct Forward {
             status = GSV_ERR_SIZE_OVERFLOW;
             return;
         }
-        hipLaunchKernelGGL((k_attention_fwd<T, DP, FAR, CAPPED, HEADS, SHARED>),
-                           dim3((unsigned)a.slots * a.scenes * (a.heads / HEADS)), dim3(256), 0,
-                           st, a, static_cast<T *>(out), lse);
+        const dim3 grid((unsigned)a.slots * a.scenes * (a.heads / HEADS));
+        T *o = static_cast<T *>(out), *low = static_cast<T *>(out_low);
+        if (lse)
+            hipLaunchKernelGGL((k_attention_fwd<T, DP, FAR, CAPPED, HEADS, SHARED, true>), grid,
+                               dim3(256), 0, st, a, o, low, lse);
+        else
+            hipLaunchKernelGGL((k_attention_fwd<T, DP, FAR, CAPPED, HEADS, SHARED, false>), grid,
+                               dim3(256), 0, st, a, o, low, lse);
         status = check_launch();
     }
     template <typename T, int DP, bool FAR, bool CAPPED> void run() {
@@ -284,14 +295,15 @@ int attention_args(const gsv_attention *in, AttnArgs *a, int *longest_q, int *lo
 
 using namespace gsv;
 
-extern "C" int gsv_attention_fwd(const gsv_attention *args, void *out, float *lse, void *stream) {
+extern "C" int gsv_attention_fwd(const gsv_attention *args, void *out, void *out_low, float *lse,
+                                 void *stream) {
     AttnArgs a;
     int lq, lk;
     const int st = attention_args(args, &a, &lq, &lk);
     if (st != GSV_OK) return st;
     if (a.q_tokens == 0) return GSV_OK;
-    if (!out || reinterpret_cast<uintptr_t>(out) % 16) return GSV_ERR_INVALID_ARGUMENT;
-    Forward f{a, lq, out, lse, as_stream(stream), GSV_OK};
+    if (!out || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(out_low) % 16) return GSV_ERR_INVALID_ARGUMENT;
+    Forward f{a, lq, out, out_low, lse, as_stream(stream), GSV_OK};
     attention_variant(a, args->dtype, f);
     return f.status;
 }

@@ -327,13 +327,16 @@ struct SceneAttention : public torch::autograd::Function<SceneAttention> {
         const gsv_attention a = c->args();
         Tensor out = empty(q.sizes(), q, q.scalar_type());
         Tensor lse = empty({q.size(1), q.size(0)}, q, at::kFloat);
-        check(lib.gsv_attention_fwd(&a, ptr<void>(out), ptr<float>(lse), stream_of(q)), "attention_fwd");
+        // what rounding took from the output: the backward needs it whole
+        Tensor low = q.scalar_type() == at::kBFloat16 ? empty(q.sizes(), q, q.scalar_type()) : Tensor();
+        check(lib.gsv_attention_fwd(&a, ptr<void>(out), ptr<void>(low), ptr<float>(lse), stream_of(q)),
+              "attention_fwd");
         ctx->saved_data["kept"] = std::vector<int64_t>{
             q.get_device(), q.size(0), q.size(1), q.size(2), k.size(0), k.size(1), c->scenes,
             c->longest, c->causal, type_code(q), slopes.defined() ? type_code(slopes) : -1};
         ctx->saved_data["scale"] = c->scale;
         ctx->saved_data["cap"] = c->cap;
-        ctx->save_for_backward({q, k, v, slopes, out, lse, c->q_starts, c->k_starts, c->prefix,
+        ctx->save_for_backward({q, k, v, slopes, out, low, lse, c->q_starts, c->k_starts, c->prefix,
                                 c->q_pos, c->k_pos, c->keep});
         ctx->set_materialize_grads(false);
         return out;
@@ -364,15 +367,16 @@ struct SceneAttention : public torch::autograd::Function<SceneAttention> {
             return t.stride(1) == 1 ? t : t.contiguous();
         };
         AttentionCall c{heads(s[0], T, H, "q"), heads(s[1], N, K, "k"), heads(s[2], N, K, "v"),
-                        s[3], ints(s[6], scenes + 1, "scene_starts"), ints(s[7], scenes + 1, "key_starts"),
-                        ints(s[8], scenes, "prefix"), places(s[9], T, "positions"),
-                        places(s[10], N, "key_positions"), s[11], scenes, m[7], m[8] != 0,
+                        s[3], ints(s[7], scenes + 1, "scene_starts"), ints(s[8], scenes + 1, "key_starts"),
+                        ints(s[9], scenes, "prefix"), places(s[10], T, "positions"),
+                        places(s[11], N, "key_positions"), s[12], scenes, m[7], m[8] != 0,
                         ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble()};
         if (c.slopes.defined())
             c.slopes = unpacked(c.slopes, m[10] == GSV_BF16 ? at::kBFloat16 : at::kFloat, dev, H, "slopes");
         TORCH_CHECK(!c.keep.defined() || is_mask(c.keep, {N}, dev), "keep: expected ", N, " values on ", dev);
         const Tensor out = heads(s[4], T, H, "out").contiguous();
-        const Tensor lse = unpacked(s[5], at::kFloat, dev, H * T, "the log sums");
+        const Tensor low = s[5].defined() ? heads(s[5], T, H, "out_low").contiguous() : s[5];
+        const Tensor lse = unpacked(s[6], at::kFloat, dev, H * T, "the log sums");
         const Tensor dout = heads(grads[0], T, H, "the gradient");
         const c10::DeviceGuard guard(dev);
         const gsv_attention a = c.args();
@@ -382,8 +386,8 @@ struct SceneAttention : public torch::autograd::Function<SceneAttention> {
         size_t bytes = 0;
         check(lib.gsv_attention_bwd_workspace_bytes(&a, &bytes), "attention_bwd_workspace_bytes");
         const Tensor ws = workspace(bytes, out);
-        check(lib.gsv_attention_bwd(&a, ptr<void>(out), ptr<float>(lse), ptr<void>(dout), dout.stride(0),
-                                    dout.stride(1), ptr<void>(dq), ptr<void>(dk), ptr<void>(dv),
+        check(lib.gsv_attention_bwd(&a, ptr<void>(out), ptr<void>(low), ptr<float>(lse), ptr<void>(dout),
+                                    dout.stride(0), dout.stride(1), ptr<void>(dq), ptr<void>(dk), ptr<void>(dv),
                                     ptr<void>(ds), ptr<void>(ws), bytes, stream_of(out)),
               "attention_bwd");
         return once({dq, dk, dv, ds, Tensor()});
@@ -423,7 +427,7 @@ std::vector<Tensor> scene_attention(const Tensor &q, const Tensor &k, const Tens
         return {SceneAttention::apply(q, k, v, maybe(c.slopes), (const AttentionCall *)&c)};
     const gsv_attention a = c.args();
     Tensor out = empty(q.sizes(), q, q.scalar_type());
-    check(lib.gsv_attention_fwd(&a, ptr<void>(out), nullptr, stream_of(q)), "attention_fwd");
+    check(lib.gsv_attention_fwd(&a, ptr<void>(out), nullptr, nullptr, stream_of(q)), "attention_fwd");
     return {out};
 }
 

@@ -122,6 +122,21 @@ template <typename T, int DP> struct Tile {
     }
 };
 
+// The sum of a fragment's weights as the product with V takes them, rounded: a row divided by this
+// sum is a mean of values, so that where one key has all the weight its value comes out exactly.
+__device__ __forceinline__ float add_weights(bf16x8 p, float sum) {
+    typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 one = {(bf16)1.f, (bf16)1.f};
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{p[e], p[e + 1]}, one, sum, false);
+    return sum;
+}
+__device__ __forceinline__ float add_weights(f32x8 p, float sum) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += p[e];
+    return sum;
+}
+
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // tanh.  For bfloat16 scores 1 - 2 / (exp(2 x) + 1): absolute error near 2^-23, far
@@ -292,10 +307,11 @@ __device__ __forceinline__ void load_column(typename Elem<T>::frag (&f)[DP / 16]
     }
 }
 
-// A 32 x DP result (columns of DP values) to one row of global memory, scaled.
+// A 32 x DP result (columns of DP values) to one row of global memory, scaled; with `low`, what the
+// rounding to T took away goes there.
 template <typename T, int DP>
 __device__ __forceinline__ void store_column(T *row, const f32x16 (&o)[DP / 32], float scale,
-                                             int dim, int lane) {
+                                             int dim, int lane, T *low = nullptr) {
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
@@ -303,10 +319,15 @@ __device__ __forceinline__ void store_column(T *row, const f32x16 (&o)[DP / 32],
             const int d = b * 32 + 8 * g + 4 * (lane >> 5);
             if (d >= dim) continue;
             typedef T t4 __attribute__((ext_vector_type(4)));
-            t4 v;
+            t4 v, w;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (T)(o[b][4 * g + e] * scale);
+            for (int e = 0; e < 4; ++e) {
+                const float x = o[b][4 * g + e] * scale;
+                v[e] = (T)x;
+                w[e] = (T)(x - (float)v[e]);
+            }
             *reinterpret_cast<t4 *>(row + d) = v;
+            if (low) *reinterpret_cast<t4 *>(low + d) = w;
         }
 }
 

@@ -80,9 +80,9 @@ SIGNATURES = {
     "gsv_gated_norm_bwd_workspace_bytes": [_NORM, _BYTES],
     "gsv_gated_norm_bwd": [_NORM, _P, _c_i64, _P, _c_i64, _P, _P, _P, _P, _P, _P, _P, _c_size_t,
                            _P],
-    "gsv_attention_fwd": [_ATT, _P, _P, _P],
+    "gsv_attention_fwd": [_ATT, _P, _P, _P, _P],
     "gsv_attention_bwd_workspace_bytes": [_ATT, _BYTES],
-    "gsv_attention_bwd": [_ATT, _P, _P, _P, _c_i64, _c_i64, _P, _P, _P, _P, _P, _c_size_t, _P],
+    "gsv_attention_bwd": [_ATT, _P, _P, _P, _P, _c_i64, _c_i64, _P, _P, _P, _P, _P, _c_size_t, _P],
     "gsv_attention_cached_workspace_bytes": [_ATT, _BYTES],
     "gsv_attention_cached": [_ATT, _P, _c_i64, _c_i64, _c_i64, _c_i64, _P, _P, _c_size_t, _P],
     "gsv_kernel_timing_enable": [_c_int],

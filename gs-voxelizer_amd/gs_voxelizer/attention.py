@@ -120,7 +120,7 @@ def scene_attention(q: Tensor, k: Tensor, v: Tensor, *, scene_starts: Optional[T
     q, k, v = _t.rows16(q), _t.rows16(k), _t.rows16(v)
     if not (torch.is_grad_enabled()
             and any(t is not None and t.requires_grad for t in (q, k, v, slopes))):
-        return _forward(a, q, k, v, slopes, held, None)
+        return _forward(a, q, k, v, slopes, held, None, None)
     return _SceneAttention.apply(q, k, v, slopes, a, *held)
 
 
@@ -142,11 +142,12 @@ def _point_packed(a, q, k, v, slopes, q_starts, k_starts, prefix, q_positions, k
         a.keep, a.keep_bytes = keep.data_ptr(), keep.element_size()
 
 
-def _forward(a, q, k, v, slopes, held, lse):
+def _forward(a, q, k, v, slopes, held, low, lse):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     _point_packed(a, q, k, v, slopes, *held)
     with torch.cuda.device(q.device):
-        _t.call("attention_fwd", ctypes.byref(a), out.data_ptr(), _t.ptr(lse), _t.stream(q.device))
+        _t.call("attention_fwd", ctypes.byref(a), out.data_ptr(), _t.ptr(low), _t.ptr(lse),
+                _t.stream(q.device))
     return out
 
 
@@ -154,15 +155,17 @@ class _SceneAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, a, *held):
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
-        out = _forward(a, q, k, v, slopes, held, lse)
+        # what rounding took from the output: the backward needs it whole
+        low = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q.dtype == torch.bfloat16 else None
+        out = _forward(a, q, k, v, slopes, held, low, lse)
         ctx.args = a
-        ctx.save_for_backward(q, k, v, slopes, out, lse, *held)
+        ctx.save_for_backward(q, k, v, slopes, out, low, lse, *held)
         return out
 
     @staticmethod
     @_t.once
     def backward(ctx, dout):
-        q, k, v, slopes, out, lse, *held = ctx.saved_tensors
+        q, k, v, slopes, out, low, lse, *held = ctx.saved_tensors
         a, dev = ctx.args, q.device
         _point_packed(a, q, k, v, slopes, *held)  # saved-tensor hooks may have moved them
         dout = _t.rows16(dout)
@@ -171,8 +174,8 @@ class _SceneAttention(Function):
         with torch.cuda.device(dev):
             n = _t.workspace_bytes("attention_bwd_workspace_bytes", a)
             ws = torch.empty(n, dtype=torch.uint8, device=dev)
-            _t.call("attention_bwd", ctypes.byref(a), out.data_ptr(), lse.data_ptr(),
-                    dout.data_ptr(), dout.stride(0), dout.stride(1), dq.data_ptr(), dk.data_ptr(),
+            _t.call("attention_bwd", ctypes.byref(a), out.data_ptr(), _t.ptr(low),
+                    lse.data_ptr(), dout.data_ptr(), dout.stride(0), dout.stride(1), dq.data_ptr(), dk.data_ptr(),
                     dv.data_ptr(), _t.ptr(ds), ws.data_ptr(), n, _t.stream(dev))
         return (dq, dk, dv, ds, None) + (None,) * 6
 

@@ -377,16 +377,18 @@ typedef struct gsv_attention {
     float scale, cap;
 } gsv_attention;
 
-/* out (q_tokens, heads, dim) contiguous; lse (heads, q_tokens), optional, receives what
- * the backward needs (log2 of each row's sum of exponentials, +inf for an empty row). */
-int gsv_attention_fwd(const gsv_attention *args, void *out, float *lse, void *stream);
+/* out (q_tokens, heads, dim) contiguous.  For a backward: lse (heads, q_tokens) receives log2
+ * of each row's sum of exponentials (+inf for an empty row), and out_low, of out's type and
+ * shape, what rounding took from out.  Both may be NULL; out_low is written with lse only, and
+ * is of use with bfloat16. */
+int gsv_attention_fwd(const gsv_attention *args, void *out, void *out_low, float *lse, void *stream);
 
 /* Gradients: dq, dk, dv contiguous like q, k, v's shapes, dslopes (heads) in the slopes'
- * type (only with slopes).  out and lse from the forward; dout with its strides.  The
+ * type (only with slopes).  out, out_low (or NULL) and lse from the forward; dout with its strides.  The
  * sums run in a fixed order (no atomics): the same inputs give the same bits. */
 int gsv_attention_bwd_workspace_bytes(const gsv_attention *args, size_t *bytes);
-int gsv_attention_bwd(const gsv_attention *args, const void *out, const float *lse,
-                      const void *dout, int64_t dout_row, int64_t dout_head, void *dq, void *dk,
+int gsv_attention_bwd(const gsv_attention *args, const void *out, const void *out_low,
+                      const float *lse, const void *dout, int64_t dout_row, int64_t dout_head, void *dq, void *dk,
                       void *dv, void *dslopes, void *workspace, size_t workspace_bytes,
                       void *stream);
 
