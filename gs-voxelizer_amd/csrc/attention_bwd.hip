@@ -184,12 +184,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
                         for (int r = 0; r < 16; ++r)
                             if (!(seen & (1u << result_row(r)))) w[r] = -INFINITY;
 #pragma unroll
+                    for (int r = 0; r < 16; ++r) w[r] = fast_exp2(fmaf(w[r], unit, -lse));
+#pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const float p = fast_exp2(fmaf(w[r], unit, -lse));
-                        dp[r] = (dp[r] - delta) * p;
+                        dp[r] = (dp[r] - delta) * w[r];
                         if (far) {
                             here = fmaf(dp[r], d[r], here);
-                            if (sizeof(T) == 2) mean = fmaf(p, d[r], mean), rest += dp[r];
+                            if (sizeof(T) == 2) mean = fmaf(w[r], d[r], mean), rest += dp[r];
                         }
                         if (capped) dp[r] *= fmaf(-u[r], u[r], 1.f);
                     }
