@@ -239,12 +239,18 @@ __global__ __launch_bounds__(256) void k_cached_join(const float *__restrict__ p
     out[row * dim + d] = (T)(total == 0.f ? 0.f : v / total);
 }
 
-// Splits of a cache: enough workgroups for two rounds on 256 CUs, each with at least a step
-// for all its waves.
-int cache_splits(const AttnArgs &a, int head_tiles) {
+// Splits of a cache: one round of workgroups, as many as the CUs hold at once (their tiles fill the
+// LDS), each with at least a step for all its waves.  Two caches of 200,003 rows, 4 heads of 128 (one
+// workgroup a CU): 70 us in one round, 75 in two, 90 in four; 16 of 4,096 rows, 2 heads of 64
+// (two a CU): 15 us in one round, 16 in half of one, 20 in two.
+int cache_splits(const AttnArgs &a, int head_tiles, int dtype) {
+    const int64_t size = dtype == GSV_BF16 ? 2 : 4, dp = a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : 128;
+    const int64_t waves = dp * size > 256 ? 2 : 4;
+    const int64_t lds = waves * (4 * kKeys * dp * size + (a.slopes ? 6 * kKeys * (size == 2 ? 16 : 4) : 0)) + 2048;
+    const int64_t round = 256 * imin64(163840 / lds, 4);
     const int64_t each = (int64_t)a.scenes * a.kv_heads * head_tiles;
-    const int64_t want = (1024 + each - 1) / each, most = (a.k_tokens + 4 * kKeys - 1) / (4 * kKeys);
-    return (int)imax64(1, imin64(want, most));
+    const int64_t most = (a.k_tokens + waves * kKeys - 1) / (waves * kKeys);
+    return (int)imax64(1, imin64(round / each, most));
 }
 
 struct Cached {
@@ -277,7 +283,7 @@ int cached_plan(const gsv_attention *args, AttnArgs *a, int *head_tiles, int *sp
     if ((int64_t)a->scenes * a->kv_heads * tiles > (1 << 22) || (int64_t)a->scenes * a->heads > (1 << 24))
         return GSV_ERR_SIZE_OVERFLOW;
     *head_tiles = (int)tiles;
-    *splits = a->scenes ? cache_splits(*a, (int)tiles) : 1;
+    *splits = a->scenes ? cache_splits(*a, (int)tiles, args->dtype) : 1;
     return GSV_OK;
 }
 
