@@ -26,7 +26,9 @@ struct BwdArgs {
     int64_t dout_row, dout_head;
     const float *lse;
     float *delta;   // (heads, q_tokens)
-    double *dslope; // (slots * scenes, heads) partial sums
+    double *dslope;  // (slots * scenes, heads) partial sums
+    void *dslopes;
+    int n_slopes;    // slots * scenes
     void *dq, *dk, *dv;
     int parts;             // workgroups that share a key tile's rows
     float *part_k, *part_v;  // (parts, k_tokens, kv_heads, dim) partial sums, with parts > 1
@@ -227,6 +229,216 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
         g.dslope[(int64_t)rest * a.heads + h] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
+// The same for few rows: 32 of them for a workgroup, whose waves take every W-th tile of 32 keys, as
+// k_attention_fwd_few does.
+template <typename T, int DP, bool FAR, bool CAPPED>
+__global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(const AttnArgs a,
+                                                                              const BwdArgs g) {
+    constexpr int W = kFewWaves<T, DP>, KB = 32;
+    constexpr bool far = FAR, capped = CAPPED;
+    typedef typename Elem<T>::frag frag;
+    static_assert(4 * KB * DP * sizeof(T) >= 32 * DP * sizeof(float), "sums reuse the tiles");
+    __shared__ __align__(1024) T tiles[W][4 * KB * DP];  // a wave's keys and values, two buffers
+    __shared__ __align__(16) typename Places<T>::Row spos[W][2][3 * KB];
+    __shared__ float srest[W][32], smean[W][32];
+    __shared__ double sums[W];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = blockIdx.x % a.heads, group_at = blockIdx.x / a.heads;
+    const int s = group_at % a.scenes, slot = group_at / a.scenes;
+    const Scene c = scene_rows(a, s);
+    const int nq = c.q1 - c.q0, row_tiles = (nq + 31) / 32;
+    const int hk = h / (a.heads / a.kv_heads);
+    const T *kbase = static_cast<const T *>(a.k) + (int64_t)c.k0 * a.k_row + hk * a.k_head;
+    const T *vbase = static_cast<const T *>(a.v) + (int64_t)c.k0 * a.v_row + hk * a.v_head;
+    const float unit = capped ? kLog2e : a.scale * kLog2e;
+    const float in_cap = capped ? a.scale / a.cap : 0.f;
+    const float far_unit = slope_of(a, h) / (capped ? 1.f : a.scale);
+    double dslope = 0.0;
+    T *const sk = tiles[wave], *const sv = sk + 2 * KB * DP;
+    Tile<T, DP> at;
+    at.plan(lane);
+    Copy<T, DP, KB, 1> ck, cv;
+    ck.plan(a.k_row, a.dim, 0, lane);
+    cv.plan(a.v_row, a.dim, 0, lane);
+
+    for (int tile = slot; tile < row_tiles; tile += a.slots) {
+        const int first = (row_tiles - 1 - tile) * 32, i = first + (lane & 31);
+        const bool row = i < nq;
+        const int64_t qi = c.q0 + i;
+        frag q[DP / 16], dO[DP / 16];
+        load_column<T, DP>(q, static_cast<const T *>(a.q) + qi * a.q_row + h * a.q_head, a.dim, row,
+                           lane);
+        load_column<T, DP>(dO, static_cast<const T *>(g.dout) + qi * g.dout_row + h * g.dout_head,
+                           a.dim, row, lane);
+        const T *o = static_cast<const T *>(g.out) + (qi * a.heads + h) * a.dim;
+        float delta = 0.f;
+#pragma unroll
+        for (int st = 0; st < DP / 16; ++st) {
+            const int d = st * 16 + 8 * (lane >> 5);
+            if (row && d < a.dim) {
+                const frag f = row_frag(o + d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) delta = fmaf((float)f[e], (float)dO[st][e], delta);
+                if (g.out_low) {
+                    const frag w = row_frag(static_cast<const T *>(g.out_low) +
+                                            (qi * a.heads + h) * a.dim + d);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) delta = fmaf((float)w[e], (float)dO[st][e], delta);
+                }
+            }
+        }
+        delta += other_half(delta);
+        if (row && threadIdx.x < 32) g.delta[(int64_t)h * a.q_tokens + qi] = delta;
+        const float lse = row ? g.lse[(int64_t)h * a.q_tokens + qi] : INFINITY;
+        Places<T> place;
+        if (far) {
+            float x = 0.f, y = 0.f, z = 0.f;
+            if (row) {
+                const float *p = a.q_pos + qi * a.q_pos_row;
+                x = p[0], y = p[1], z = p[2];
+            }
+            place.set(x, y, z, lane);
+        }
+        const int limit = row ? key_limit(a, c, i) : 0;
+        const int all = first + 31 < nq ? key_limit(a, c, first) : 0;
+        const int most = key_limit(a, c, min(first + 32, nq) - 1);
+        f32x16 dq[DP / 32] = {};
+        float mean = 0.f, rest = 0.f;
+
+        float gp[2] = {};
+        int raw = 0;
+        uint64_t live = ~0ull, next_live = ~0ull;
+        auto look = [&](int j0) {
+            if (a.keep && j0 < most) raw = keep_raw(a, c.k0 + min(j0 + (lane & 31), most - 1));
+        };
+        auto fetch = [&](int b, int j0) {
+            if (a.keep) next_live = __ballot(raw != 0);
+            look(j0 + W * KB);
+            const int left = most - j0;
+            ck.start(sk + b * KB * DP, kbase + j0 * a.k_row, a.k_row, a.dim, left, a.keep, next_live, 0, lane);
+            cv.start(sv + b * KB * DP, vbase + j0 * a.v_row, a.v_row, a.dim, left, a.keep, next_live, 0, lane);
+            if (far)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int r = min(lane & 31, left - 1), ax = min(2 * n + (lane >> 5), 2);
+                    gp[n] = a.k_pos[(c.k0 + j0 + r) * a.k_pos_row + ax];
+                }
+        };
+        auto put = [&](int b) {
+            if (far) {
+                spos[wave][b][lane] = Places<T>::row(gp[0]);
+                if (lane < KB) spos[wave][b][64 + lane] = Places<T>::row(gp[1]);
+            }
+            tile_wait();
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        };
+        __syncthreads();  // the previous rows' sums in the tiles have been read
+        int b = 0;
+        if (wave * KB < most) {
+            look(wave * KB);
+            fetch(0, wave * KB);
+            put(0);
+        }
+        for (int j0 = wave * KB; j0 < most; j0 += W * KB, b ^= 1) {
+            const bool more = j0 + W * KB < most;
+            live = next_live;
+            if (more) fetch(b ^ 1, j0 + W * KB);
+            const bool masked = j0 + KB > all || (uint32_t)~live;
+            const T *kt = sk + b * KB * DP, *vt = sv + b * KB * DP;
+            f32x16 d = {}, w = {}, u = {}, dp = {};
+            uint32_t seen = 0;
+            float here = 0.f;
+            if (far) d = distances<T>(place, spos[wave][b], KB, 0, lane);
+            if (masked) {
+                seen = seen_rows(live, 0, limit - j0, lane);
+                if (far)  // a masked key's position may be anything
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (!(seen & (1u << result_row(r)))) d[r] = 0.f;
+            }
+#pragma unroll
+            for (int st = 0; st < DP / 16; ++st) {
+                w = mma(at.rows(kt, st), q[st], w);
+                dp = mma(at.rows(vt, st), dO[st], dp);
+            }
+            finish_scores<T, FAR, CAPPED>(w, u, d, in_cap, a.cap, far_unit);
+            if (masked)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!(seen & (1u << result_row(r)))) w[r] = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float p = fast_exp2(fmaf(w[r], unit, -lse));
+                dp[r] = (dp[r] - delta) * p;
+                if (far) {
+                    here = fmaf(dp[r], d[r], here);
+                    if (sizeof(T) == 2) mean = fmaf(p, d[r], mean), rest += dp[r];
+                }
+                if (capped) dp[r] *= fmaf(-u[r], u[r], 1.f);
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const frag ds = to_frag<T>(dp, half);
+#pragma unroll
+                for (int e = 0; e < DP / 32; ++e)
+                    dq[e] = mma(at.columns(kt + half * 16 * DP, e, lane), ds, dq[e]);
+            }
+            dslope -= here;
+            if (more) put(b ^ 1);
+        }
+        if (far && sizeof(T) == 2) {  // a row's, over all waves (see k_attention_dq)
+            rest += other_half(rest);
+            mean += other_half(mean);
+            if (lane < 32) srest[wave][lane] = rest, smean[wave][lane] = mean;
+        }
+        // row r's channel d at d * 32 + r
+        float *so = reinterpret_cast<float *>(tiles[wave]);
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                so[(e * 32 + result_row(r) + 4 * (lane >> 5)) * 32 + (lane & 31)] = dq[e][r];
+        __syncthreads();
+        const int r = threadIdx.x & 31;
+        if (far && sizeof(T) == 2 && threadIdx.x < 32) {
+            float row_rest = 0.f, row_mean = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) row_rest += srest[w][r], row_mean += smean[w][r];
+            dslope += row_rest * row_mean;
+        }
+        if (first + r < nq) {
+            T *to = static_cast<T *>(g.dq) + ((int64_t)(c.q0 + first + r) * a.heads + h) * a.dim;
+            for (int d0 = (threadIdx.x >> 5) * 8; d0 < a.dim; d0 += 2 * W * 8) {
+                typedef T t8 __attribute__((ext_vector_type(8)));
+                t8 v;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int w = 0; w < W; ++w)
+                        x += reinterpret_cast<const float *>(tiles[w])[(d0 + e) * 32 + r];
+                    v[e] = (T)(x * a.scale);
+                }
+                *reinterpret_cast<t8 *>(to + d0) = v;
+            }
+        }
+    }
+    if (!far) return;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) dslope += __shfl_xor(dslope, k);
+    if (lane == 0) sums[wave] = dslope;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double sum = 0.0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) sum += sums[w];
+        g.dslope[(int64_t)group_at * a.heads + h] = sum;
+    }
+}
+
 // dk and dv.  A wave's lanes are keys; the rows of all query heads of the key head pass by.
 template <typename T, int DP, bool FAR, bool CAPPED>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const AttnArgs a, const BwdArgs g) {
@@ -254,6 +466,19 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
     Copy<T, DP, QB, WAVES> cq, cd;
     cq.plan(a.q_row, a.dim, wave, lane);
     cd.plan(g.dout_row, a.dim, wave, lane);
+
+    // the rows' kernel has ended: a head's partial sums of dslope, in order
+    if (far && rest == 0 && part == 0)
+        for (int h = hk * group + wave; h < (hk + 1) * group; h += WAVES) {
+            double sum = 0.0;
+            for (int n = lane; n < g.n_slopes; n += 64) sum += g.dslope[(int64_t)n * a.heads + h];
+#pragma unroll
+            for (int n = 1; n < 64; n <<= 1) sum += __shfl_xor(sum, n);
+            if (lane == 0) {
+                if (a.slopes_f32) static_cast<float *>(g.dslopes)[h] = (float)sum;
+                else static_cast<bf16 *>(g.dslopes)[h] = (bf16)(float)sum;
+            }
+        }
 
     for (int tile = slot; tile < tiles; tile += a.slots) {
         const int first = tile * kRows;
@@ -412,35 +637,24 @@ __global__ __launch_bounds__(256) void k_parts_sum(const float *__restrict__ pk,
     reinterpret_cast<t4 *>(second ? dv : dk)[at] = r;
 }
 
-// The workgroups' sums of each head, in order.
-__global__ __launch_bounds__(64) void k_slope_sum(const double *__restrict__ part, int n, int heads,
-                                                  void *__restrict__ out, int f32) {
-    const int h = blockIdx.x;
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < n; i += 64) sum += part[(int64_t)i * heads + h];
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k);
-    if (threadIdx.x) return;
-    if (f32) static_cast<float *>(out)[h] = (float)sum;
-    else static_cast<bf16 *>(out)[h] = (bf16)(float)sum;
-}
-
 struct Backward {
     const AttnArgs &a;
     const BwdArgs &g;
     int kslots;
     hipStream_t st;
     template <typename T, int DP, bool FAR, bool CAPPED> void run() const {
-        if (a.q_tokens > 0)
-            hipLaunchKernelGGL((k_attention_dq<T, DP, FAR, CAPPED>),
-                               dim3((unsigned)a.slots * a.scenes * a.heads), dim3(256), 0, st, a, g);
+        const dim3 grid((unsigned)a.slots * a.scenes * a.heads);
+        if (a.q_tokens > 0 && attention_few(a))
+            hipLaunchKernelGGL((k_attention_dq_few<T, DP, FAR, CAPPED>), grid,
+                               dim3(64 * kFewWaves<T, DP>), 0, st, a, g);
+        else if (a.q_tokens > 0)
+            hipLaunchKernelGGL((k_attention_dq<T, DP, FAR, CAPPED>), grid, dim3(256), 0, st, a, g);
         AttnArgs k = a;
         k.slots = kslots;
-        if (a.k_tokens == 0) return;
         hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED>),
                            dim3((unsigned)kslots * a.scenes * a.kv_heads * g.parts), dim3(256), 0, st,
                            k, g);
-        if (g.parts == 1) return;
+        if (g.parts == 1 || a.k_tokens == 0) return;
         const int64_t fours = (int64_t)a.k_tokens * a.kv_heads * a.dim / 4;
         hipLaunchKernelGGL(k_parts_sum<T>, dim3((unsigned)((2 * fours + 255) / 256)), dim3(256), 0, st,
                            g.part_k, g.part_v, g.parts, fours, static_cast<T *>(g.dk),
@@ -477,7 +691,8 @@ int bwd_plan(const gsv_attention *args, AttnArgs *a, int *kslots, int *parts) {
     *parts = bwd_parts(*a, args->dtype);
     if (!attention_slots(a, lk, kRows, a->kv_heads * *parts)) return GSV_ERR_SIZE_OVERFLOW;
     *kslots = a->slots;
-    return attention_slots(a, lq, kRows, a->heads) ? GSV_OK : GSV_ERR_SIZE_OVERFLOW;
+    const int rows = attention_few(*a) ? 32 : kRows;
+    return attention_slots(a, lq, rows, a->heads) ? GSV_OK : GSV_ERR_SIZE_OVERFLOW;
 }
 
 }  // namespace
@@ -521,12 +736,10 @@ extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, con
     float *part_k = reinterpret_cast<float *>(next);
     float *part_v = reinterpret_cast<float *>(next + parts_bytes(a, parts));
     double *slopes = reinterpret_cast<double *>(next + 2 * parts_bytes(a, parts));
-    const BwdArgs g{out, out_low, dout, dout_row, dout_head, lse, delta, slopes, dq, dk, dv, parts, part_k, part_v};
+    const BwdArgs g{out, out_low, dout, dout_row, dout_head, lse, delta, slopes, dslopes,
+                    a.q_tokens > 0 ? a.slots * a.scenes : 0, dq, dk, dv, parts, part_k, part_v};
     hipStream_t s = as_stream(stream);
     Backward f{a, g, kslots, s};
     attention_variant(a, args->dtype, f);
-    if (a.slopes)
-        hipLaunchKernelGGL(k_slope_sum, dim3(a.heads), dim3(64), 0, s, slopes,
-                           a.q_tokens > 0 ? a.slots * a.scenes : 0, a.heads, dslopes, a.slopes_f32);
     return check_launch();
 }

@@ -218,6 +218,191 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
     }
 }
 
+// The same for few rows: a workgroup takes 32 rows of one head, its waves every W-th tile of 32
+// keys each.  The tiles are a wave's own (its copies need no barrier, only waits); the waves' sums are
+// joined through LDS at the end.  Four times as many workgroups, each a quarter as long.
+template <typename T, int DP, bool FAR, bool CAPPED, bool TRAIN>
+__global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_fwd_few(
+    const AttnArgs a, T *__restrict__ out, T *__restrict__ out_low, float *__restrict__ lse) {
+    constexpr int W = kFewWaves<T, DP>, KB = 32;
+    constexpr bool far = FAR, capped = CAPPED;
+    typedef typename Elem<T>::frag frag;
+    static_assert(4 * KB * DP * sizeof(T) >= 32 * DP * sizeof(float), "sums reuse the tiles");
+    __shared__ __align__(1024) T tiles[W][4 * KB * DP];  // a wave's keys and values, two buffers
+    __shared__ __align__(16) typename Places<T>::Row spos[W][2][3 * KB];
+    __shared__ float sm[W][32], ss[W][32], se[W][32];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = blockIdx.x % a.heads, rest = blockIdx.x / a.heads;
+    const int s = rest % a.scenes, slot = rest / a.scenes;
+    const Scene c = scene_rows(a, s);
+    const int nq = c.q1 - c.q0, row_tiles = (nq + 31) / 32;
+    const int hk = h / (a.heads / a.kv_heads);
+    const T *kbase = static_cast<const T *>(a.k) + (int64_t)c.k0 * a.k_row + hk * a.k_head;
+    const T *vbase = static_cast<const T *>(a.v) + (int64_t)c.k0 * a.v_row + hk * a.v_head;
+    const float unit = capped ? kLog2e : a.scale * kLog2e;
+    const float in_cap = capped ? a.scale / a.cap : 0.f;
+    const float far_unit = slope_of(a, h) / (capped ? 1.f : a.scale);
+    T *const sk = tiles[wave], *const sv = sk + 2 * KB * DP;
+    Tile<T, DP> at;
+    at.plan(lane);
+    Copy<T, DP, KB, 1> ck, cv;
+    ck.plan(a.k_row, a.dim, 0, lane);
+    cv.plan(a.v_row, a.dim, 0, lane);
+
+    for (int tile = slot; tile < row_tiles; tile += a.slots) {
+        const int first = (row_tiles - 1 - tile) * 32, i = first + (lane & 31);
+        const bool row = i < nq;
+        const int64_t qi = c.q0 + i;
+        frag q[DP / 16];
+        load_column<T, DP>(q, static_cast<const T *>(a.q) + qi * a.q_row + h * a.q_head, a.dim, row, lane);
+        Places<T> place;
+        if (far) {
+            float x = 0.f, y = 0.f, z = 0.f;
+            if (row) {
+                const float *p = a.q_pos + qi * a.q_pos_row;
+                x = p[0], y = p[1], z = p[2];
+            }
+            place.set(x, y, z, lane);
+        }
+        const int limit = row ? key_limit(a, c, i) : 0;
+        const int all = first + 31 < nq ? key_limit(a, c, first) : 0;
+        const int most = key_limit(a, c, min(first + 32, nq) - 1);
+        f32x16 o[DP / 32] = {};
+        float m = -INFINITY, sum = 0.f, exact = 0.f;
+
+        float gp[2] = {};
+        int raw = 0;
+        uint64_t live = ~0ull, next_live = ~0ull;
+        auto look = [&](int j0) {
+            if (a.keep && j0 < most) raw = keep_raw(a, c.k0 + min(j0 + (lane & 31), most - 1));
+        };
+        auto fetch = [&](int b, int j0) {
+            if (a.keep) next_live = __ballot(raw != 0);
+            look(j0 + W * KB);
+            const int left = most - j0;
+            ck.start(sk + b * KB * DP, kbase + j0 * a.k_row, a.k_row, a.dim, left, a.keep, next_live, 0, lane);
+            cv.start(sv + b * KB * DP, vbase + j0 * a.v_row, a.v_row, a.dim, left, a.keep, next_live, 0, lane);
+            if (far)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int r = min(lane & 31, left - 1), ax = min(2 * n + (lane >> 5), 2);
+                    gp[n] = a.k_pos[(c.k0 + j0 + r) * a.k_pos_row + ax];
+                }
+        };
+        auto put = [&](int b) {
+            if (far) {
+                spos[wave][b][lane] = Places<T>::row(gp[0]);
+                if (lane < KB) spos[wave][b][64 + lane] = Places<T>::row(gp[1]);
+            }
+            tile_wait();
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        };
+        __syncthreads();  // the previous rows' sums in the tiles have been read
+        int b = 0;
+        if (wave * KB < most) {
+            look(wave * KB);
+            fetch(0, wave * KB);
+            put(0);
+        }
+        for (int j0 = wave * KB; j0 < most; j0 += W * KB, b ^= 1) {
+            const bool more = j0 + W * KB < most;
+            live = next_live;
+            if (more) fetch(b ^ 1, j0 + W * KB);
+            const T *kt = sk + b * KB * DP, *vt = sv + b * KB * DP;
+            f32x16 d = {}, w = {};
+#pragma unroll
+            for (int st = 0; st < DP / 16; ++st) w = mma(at.rows(kt, st), q[st], w);
+            if (far) d = distances<T>(place, spos[wave][b], KB, 0, lane);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                if (capped) w[r] = a.cap * tanh_of<T>(w[r] * in_cap);
+                if (far) w[r] = fmaf(-far_unit, d[r], w[r]);
+            }
+            if (j0 + KB > all || (uint32_t)~live) {
+                const uint32_t seen = seen_rows(live, 0, limit - j0, lane);
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!(seen & (1u << result_row(r)))) w[r] = -INFINITY;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, w[r]);
+            top *= unit;
+            if (__any(top > m + kSlack)) {
+                const float next = fmaxf(m, fmaxf(top, other_half(top)));
+                const float by = next == -INFINITY ? 1.f : fast_exp2(m - next);
+                m = next;
+                sum *= by, exact *= by;
+#pragma unroll
+                for (int e = 0; e < DP / 32; ++e) o[e] *= by;
+            }
+            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                w[r] = fast_exp2(fmaf(w[r], unit, -ref));
+                if (TRAIN) exact += w[r];
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const frag p = to_frag<T>(w, half);
+                sum = add_weights(p, sum);
+#pragma unroll
+                for (int e = 0; e < DP / 32; ++e)
+                    o[e] = mma(at.columns(vt + half * 16 * DP, e, lane), p, o[e]);
+            }
+            if (more) put(b ^ 1);
+        }
+        sum += other_half(sum);
+        exact += other_half(exact);
+        if (lane < 32) sm[wave][lane] = m, ss[wave][lane] = sum, se[wave][lane] = exact;
+        // the waves' sums: row r's channel d at d * 32 + r, so that lanes read and write in a line
+        float *so = reinterpret_cast<float *>(tiles[wave]);
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                so[(e * 32 + result_row(r) + 4 * (lane >> 5)) * 32 + (lane & 31)] = o[e][r];
+        __syncthreads();
+        float by[W], top = -INFINITY, total = 0.f, log_total = 0.f;
+        const int r = threadIdx.x & 31;
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = fmaxf(top, sm[w][r]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            by[w] = sm[w][r] == -INFINITY ? 1.f : fast_exp2(sm[w][r] - top);  // else its sum is 0
+            total = fmaf(by[w], ss[w][r], total);
+            log_total = fmaf(by[w], se[w][r], log_total);
+        }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        if (first + r < nq) {
+            const int64_t at_out = ((int64_t)(c.q0 + first + r) * a.heads + h) * a.dim;
+            // eight channels of a row at a time
+            for (int d0 = (threadIdx.x >> 5) * 8; d0 < a.dim; d0 += 2 * W * 8) {
+                typedef T t8 __attribute__((ext_vector_type(8)));
+                t8 v, low;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int w = 0; w < W; ++w)
+                        x = fmaf(by[w], reinterpret_cast<const float *>(tiles[w])[(d0 + e) * 32 + r], x);
+                    x *= inv;
+                    v[e] = (T)x;
+                    low[e] = (T)(x - (float)v[e]);
+                }
+                *reinterpret_cast<t8 *>(out + at_out + d0) = v;
+                if (TRAIN && out_low) *reinterpret_cast<t8 *>(out_low + at_out + d0) = low;
+            }
+            if (TRAIN && threadIdx.x < 32)
+                lse[(int64_t)h * a.q_tokens + c.q0 + first + r] =
+                    log_total == 0.f ? INFINITY : top + log2f(log_total);
+        }
+    }
+}
+
 struct Forward {
     AttnArgs a;
     int longest;
@@ -240,7 +425,21 @@ struct Forward {
                                dim3(256), 0, st, a, o, low, lse);
         status = check_launch();
     }
+    template <typename T, int DP, bool FAR, bool CAPPED> void few() {
+        if (!attention_slots(&a, longest, 32, a.heads)) {
+            status = GSV_ERR_SIZE_OVERFLOW;
+            return;
+        }
+        const dim3 grid((unsigned)a.slots * a.scenes * a.heads), block(64 * kFewWaves<T, DP>);
+        T *o = static_cast<T *>(out), *low = static_cast<T *>(out_low);
+        if (lse)
+            hipLaunchKernelGGL((k_attention_fwd_few<T, DP, FAR, CAPPED, true>), grid, block, 0, st, a, o, low, lse);
+        else
+            hipLaunchKernelGGL((k_attention_fwd_few<T, DP, FAR, CAPPED, false>), grid, block, 0, st, a, o, low, lse);
+        status = check_launch();
+    }
     template <typename T, int DP, bool FAR, bool CAPPED> void run() {
+        if (attention_few(a)) return few<T, DP, FAR, CAPPED>();
         if constexpr (FAR && sizeof(T) == 2 && DP <= 64) {
             if (attention_pairs(a)) {
                 if (a.heads / a.kv_heads % 2 == 0) start<T, DP, FAR, CAPPED, 2, true>();

@@ -200,8 +200,24 @@ template <typename F> void attention_variant(const AttnArgs &a, int dtype, F &f)
     else attention_channels<float>(a, f);
 }
 
-// Whether a wave takes two heads (for their distances): an even number of them.
-inline bool attention_pairs(const AttnArgs &a) { return a.heads % 2 == 0; }
+// Workgroups of 128 rows of one head, a mean scene's and all scenes' (sizes alone decide which kernel
+// runs: the longest scene's length is a hint that may change no bit).
+inline int64_t attention_tiles(const AttnArgs &a, bool mean) {
+    const int64_t each = (int64_t)a.q_tokens / a.scenes / 128 * a.heads;
+    return mean ? each : ((int64_t)a.q_tokens / 128 + a.scenes) * a.heads;
+}
+// Whether a wave takes two heads (for their distances): where a scene's workgroups fill two a CU
+// all the same.  One scene, 8 heads of 64: 16,000 tokens take 0.93 ms in pairs and 1.17 without, 6,000
+// 0.27 and 0.22; 8 scenes of 1,000, 16 heads 0.15 and 0.11.
+inline bool attention_pairs(const AttnArgs &a) {
+    return a.heads % 2 == 0 && attention_tiles(a, true) >= 2 * 448;
+}
+// Whether rows are so few that the waves of a workgroup share them and split the keys: below three
+// workgroups of 128 rows for four CUs.  8 heads of 64, one scene: 500 tokens forward 13 us so and 22
+// otherwise, 2,000 36 and 66, 4,000 118 and 110.
+inline bool attention_few(const AttnArgs &a) { return attention_tiles(a, false) < 192; }
+// The waves of such a workgroup: as many as the LDS holds their tiles.
+template <typename T, int DP> constexpr int kFewWaves = DP * sizeof(T) > 256 ? 2 : 4;
 
 // Workgroups for each scene and head: one for each tile of the longest scene, fewer where the
 // launch would pass a million (they take the tiles in turn, so any number is right).

@@ -488,3 +488,57 @@ def test_saved_tensor_hooks_may_move_what_is_saved(device):
         got = _run(c)
     for n in got:
         assert torch.equal(got[n], want[n]), n
+
+
+# ---- the kernels of larger calls: those above have few enough rows that the waves of a workgroup
+# share them; two hundred scenes of one token more, or long scenes of many heads, are past that
+
+
+MANY = [1] * 200
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("dim", [8, 24, 32, 40, 64, 72, 96, 128])
+@pytest.mark.parametrize("heads", [(1, 1), (4, 2)], ids=str)
+def test_many_scenes(device, dtype, dim, heads):
+    _check(_case(device, dtype, [33, 0, 140, 1] + MANY, *heads, dim, bias=True, causal=True, prefix=True,
+                 cap=20.0, culled=0.2), f"many {dim}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("causal", [False, True])
+def test_many_scenes_masks(device, dtype, bias, cap, causal):
+    _check(_case(device, dtype, [300, 129] + MANY, 2, 1, 64, bias=bias, causal=causal, cap=cap,
+                 culled=0.4), "masks")
+    _check(_case(device, dtype, [70, 9, 130] + MANY, 2, 2, 64, bias=bias, causal=causal, cap=cap,
+                 key_lengths=[200, 1, 40] + MANY), "other keys")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("junk", [float("nan"), float("inf")])
+def test_many_scenes_masked_keys_reach_nothing(device, dtype, junk):
+    c = _case(device, dtype, [150, 60] + MANY, 2, 2, 64, bias=True, culled=0.3, cap=8.0,
+              key_lengths=[90, 171] + MANY)
+    want = _run(c)
+    for n in ("k", "v", "k_positions"):
+        c[n] = c[n].clone()
+        c[n][c["keep"] == 0] = junk
+    got = _run(c)
+    for n in got:
+        assert torch.equal(got[n], want[n]), n
+    for longest in (1, 100, 400):
+        got = _run(c, longest=longest)
+        for n in got:
+            assert torch.equal(got[n], want[n]), (longest, n)
+
+
+@pytest.mark.parametrize("kv", [28, 14, 4], ids=lambda k: f"kv{k}")
+@pytest.mark.parametrize("dim,causal,cap,culled", [(64, False, 0.0, 0.1), (32, True, 9.0, 0.0)])
+def test_long_scene_of_many_heads(device, kv, dim, causal, cap, culled):
+    """Two heads of a wave share their distances, with one key head or two."""
+    c = _case(device, BF16, [4100], 28, kv, dim, bias=True, causal=causal, cap=cap, culled=culled)
+    _check(c, "pairs")
+    got, want = _run(c, train=False)["out"], _run(c)["out"]
+    assert torch.equal(got, want)
