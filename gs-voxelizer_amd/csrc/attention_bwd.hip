@@ -89,24 +89,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
                            lane);
         load_column<T, DP>(dO, static_cast<const T *>(g.dout) + qi * g.dout_row + h * g.dout_head,
                            a.dim, row, lane);
-        const T *o = static_cast<const T *>(g.out) + (qi * a.heads + h) * a.dim;
-        float delta = 0.f;
-#pragma unroll
-        for (int st = 0; st < DP / 16; ++st) {
-            const int d = st * 16 + 8 * (lane >> 5);
-            if (row && d < a.dim) {
-                const frag f = row_frag(o + d);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) delta = fmaf((float)f[e], (float)dO[st][e], delta);
-                if (g.out_low) {
-                    const frag w = row_frag(static_cast<const T *>(g.out_low) +
-                                            (qi * a.heads + h) * a.dim + d);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) delta = fmaf((float)w[e], (float)dO[st][e], delta);
-                }
-            }
+        // D_i: where the row sees one key, out is that key's value and D_i its do_i.v_j bit for bit, so
+        // that the row's gradients are exactly 0
+        frag o[DP / 16];
+        load_column<T, DP>(o, static_cast<const T *>(g.out) + (qi * a.heads + h) * a.dim, a.dim, row, lane);
+        float delta = own_product<T>(o, dO, lane);
+        if (g.out_low) {
+            load_column<T, DP>(o, static_cast<const T *>(g.out_low) + (qi * a.heads + h) * a.dim, a.dim,
+                               row, lane);
+            delta += own_product<T>(o, dO, lane);
         }
-        delta += other_half(delta);
         if (row && lane < 32) g.delta[(int64_t)h * a.q_tokens + qi] = delta;
         const float lse = row ? g.lse[(int64_t)h * a.q_tokens + qi] : INFINITY;
         Places<T> place;
@@ -271,24 +263,16 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
                            lane);
         load_column<T, DP>(dO, static_cast<const T *>(g.dout) + qi * g.dout_row + h * g.dout_head,
                            a.dim, row, lane);
-        const T *o = static_cast<const T *>(g.out) + (qi * a.heads + h) * a.dim;
-        float delta = 0.f;
-#pragma unroll
-        for (int st = 0; st < DP / 16; ++st) {
-            const int d = st * 16 + 8 * (lane >> 5);
-            if (row && d < a.dim) {
-                const frag f = row_frag(o + d);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) delta = fmaf((float)f[e], (float)dO[st][e], delta);
-                if (g.out_low) {
-                    const frag w = row_frag(static_cast<const T *>(g.out_low) +
-                                            (qi * a.heads + h) * a.dim + d);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) delta = fmaf((float)w[e], (float)dO[st][e], delta);
-                }
-            }
+        // D_i: where the row sees one key, out is that key's value and D_i its do_i.v_j bit for bit, so
+        // that the row's gradients are exactly 0
+        frag o[DP / 16];
+        load_column<T, DP>(o, static_cast<const T *>(g.out) + (qi * a.heads + h) * a.dim, a.dim, row, lane);
+        float delta = own_product<T>(o, dO, lane);
+        if (g.out_low) {
+            load_column<T, DP>(o, static_cast<const T *>(g.out_low) + (qi * a.heads + h) * a.dim, a.dim,
+                               row, lane);
+            delta += own_product<T>(o, dO, lane);
         }
-        delta += other_half(delta);
         if (row && threadIdx.x < 32) g.delta[(int64_t)h * a.q_tokens + qi] = delta;
         const float lse = row ? g.lse[(int64_t)h * a.q_tokens + qi] : INFINITY;
         Places<T> place;
@@ -560,7 +544,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
                 const bool masked = i0 < wave_all;
 #pragma unroll 1
                 for (int qb = 0; qb < QB / 32; ++qb) {
-                    f32x16 d = {}, w = {}, u = {}, dp, lse;
+                    f32x16 d = {}, w = {}, u = {}, dp = {}, lse, delta;
                     if (far) d = distances<T>(place, spos[b], QB, qb * 32, lane);
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
@@ -568,7 +552,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
                         const f32x4 ls = *reinterpret_cast<const f32x4 *>(p);
                         const f32x4 de = *reinterpret_cast<const f32x4 *>(p + QB);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) lse[4 * n + e] = ls[e], dp[4 * n + e] = -de[e];
+                        for (int e = 0; e < 4; ++e) lse[4 * n + e] = ls[e], delta[4 * n + e] = de[e];
                     }
 #pragma unroll
                     for (int st = 0; st < DP / 16; ++st) {
@@ -585,7 +569,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         w[r] = fast_exp2(fmaf(w[r], unit, -lse[r]));
-                        dp[r] *= w[r];
+                        dp[r] = (dp[r] - delta[r]) * w[r];
                         if (capped) dp[r] *= fmaf(-u[r], u[r], 1.f);
                     }
 #pragma unroll

@@ -8,6 +8,9 @@
 // transposed (K Q^T), so a row's running maximum and sum stay with its lanes.
 #include "gsv_attention.h"
 
+// (a product and a difference stay two roundings where they are written as two)
+#pragma clang fp contract(off)
+
 namespace gsv {
 namespace {
 
@@ -27,6 +30,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
     constexpr int KB = sizeof(T) == 2 ? 64 : 32;  // keys of a tile
     constexpr int KV = SHARED ? 1 : HEADS;        // key heads of the workgroup
     constexpr bool far = FAR, capped = CAPPED;
+    // float32: scores are rounded to powers of two before their maximum is taken off, so that the
+    // largest has the weight 1 exactly, as the rounding to bfloat16 gives it there
+    constexpr bool kExact = sizeof(T) == 4;
     typedef typename Elem<T>::frag frag;
     __shared__ __align__(1024) T sk[2][KV][KB * DP];
     __shared__ __align__(1024) T sv[2][KV][KB * DP];
@@ -157,6 +163,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
                             for (int r = 0; r < 16; ++r)
                                 if (!(seen & (1u << result_row(r)))) w[n][r] = -INFINITY;
                     }
+                    if constexpr (kExact)
+#pragma unroll
+                        for (int n = 0; n < HEADS; ++n)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) w[n][r] *= unit;
                     float top[HEADS];
                     bool grown = false;
 #pragma unroll
@@ -164,7 +175,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
                         top[n] = -INFINITY;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) top[n] = fmaxf(top[n], w[n][r]);
-                        top[n] *= unit;
+                        if (!kExact) top[n] *= unit;
                         grown |= top[n] > m[n] + kSlack;
                     }
                     if (__any(grown)) {
@@ -183,7 +194,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
                         const float ref = m[n] == -INFINITY ? 0.f : m[n];
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
-                            w[n][r] = fast_exp2(fmaf(w[n][r], unit, -ref));
+                            w[n][r] = fast_exp2(kExact ? w[n][r] - ref : fmaf(w[n][r], unit, -ref));
                             if (TRAIN) exact[n] += w[n][r];
                         }
 #pragma unroll
@@ -226,6 +237,9 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_fwd_few(
     const AttnArgs a, T *__restrict__ out, T *__restrict__ out_low, float *__restrict__ lse) {
     constexpr int W = kFewWaves<T, DP>, KB = 32;
     constexpr bool far = FAR, capped = CAPPED;
+    // float32: scores are rounded to powers of two before their maximum is taken off, so that the
+    // largest has the weight 1 exactly, as the rounding to bfloat16 gives it there
+    constexpr bool kExact = sizeof(T) == 4;
     typedef typename Elem<T>::frag frag;
     static_assert(4 * KB * DP * sizeof(T) >= 32 * DP * sizeof(float), "sums reuse the tiles");
     __shared__ __align__(1024) T tiles[W][4 * KB * DP];  // a wave's keys and values, two buffers
@@ -327,10 +341,13 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_fwd_few(
                 for (int r = 0; r < 16; ++r)
                     if (!(seen & (1u << result_row(r)))) w[r] = -INFINITY;
             }
+            if constexpr (kExact)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) w[r] *= unit;
             float top = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, w[r]);
-            top *= unit;
+            if (!kExact) top *= unit;
             if (__any(top > m + kSlack)) {
                 const float next = fmaxf(m, fmaxf(top, other_half(top)));
                 const float by = next == -INFINITY ? 1.f : fast_exp2(m - next);
@@ -342,7 +359,7 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_fwd_few(
             const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                w[r] = fast_exp2(fmaf(w[r], unit, -ref));
+                w[r] = fast_exp2(kExact ? w[r] - ref : fmaf(w[r], unit, -ref));
                 if (TRAIN) exact += w[r];
             }
 #pragma unroll

@@ -369,6 +369,24 @@ __device__ __forceinline__ void store_column(T *row, const f32x16 (&o)[DP / 32],
         }
 }
 
+// The row of a block that result register r of a lane's half holds, less 4 (lane / 32).
+__device__ __forceinline__ constexpr int result_row(int r) { return 8 * (r >> 2) + (r & 3); }
+
+// The product of each lane's own row with its column, the diagonal of a 32 x 32 product: formed by
+// the instructions and in the order of any other element, so that equal rows give equal bits.
+template <typename T, int N>
+__device__ __forceinline__ float own_product(const typename Elem<T>::frag (&row)[N],
+                                             const typename Elem<T>::frag (&column)[N], int lane) {
+    f32x16 w = {};
+#pragma unroll
+    for (int st = 0; st < N; ++st) w = mma(row[st], column[st], w);
+    float x = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        if (result_row(r) + 4 * (lane >> 5) == (lane & 31)) x = w[r];
+    return x + other_half(x);  // the other half's is 0
+}
+
 // Positions for distances: differences of two sides' coordinates formed by the matrix units.
 // float32: x_row * 1 + 1 * -x_column, one v_mfma_f32_32x32x2_f32 an axis, the rounding of a
 // subtraction.  bfloat16: each coordinate as the exact sum of three bfloat16 (24 bits), so a
@@ -430,9 +448,6 @@ __device__ __forceinline__ f32x16 distances(const Places<T> &to, const typename 
     for (int r = 0; r < 16; ++r) d[r] = __builtin_amdgcn_sqrtf(d[r]);
     return d;
 }
-
-// The row of a block that result register r of a lane's half holds, less 4 (lane / 32).
-__device__ __forceinline__ constexpr int result_row(int r) { return 8 * (r >> 2) + (r & 3); }
 
 // The rows of a block that a lane sees, a bit each at result_row(r): those kept (bits of the tile)
 // below the lane's limit, counted from the block's first row.

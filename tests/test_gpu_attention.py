@@ -542,3 +542,17 @@ def test_long_scene_of_many_heads(device, kv, dim, causal, cap, culled):
     _check(c, "pairs")
     got, want = _run(c, train=False)["out"], _run(c)["out"]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("dim", [8, 40, 64, 128])
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+@pytest.mark.parametrize("lengths", [[1, 1], [1] * 200], ids=["few", "many"])
+def test_rows_that_see_one_key(device, dtype, dim, cap, lengths):
+    """Their output is the key's value, and no gradient passes through their one weight: exactly."""
+    c = _case(device, dtype, lengths, 4, 2, dim, bias=True, causal=True, cap=cap)
+    got = _run(c)
+    assert torch.equal(got["out"], c["v"].repeat_interleave(2, 1))
+    for n in ("dq", "dk", "dslopes"):
+        assert not got[n].any(), n
+    R.assert_within(got["dv"], *(x["dv"] for x in R.attention(**c)), "dv")
