@@ -10,6 +10,12 @@
 // little of it.  Two kernels form the scores twice, one with the rows' sums (dq, D, dslope) and one with
 // the keys' (dk, dv): each sum stays in the registers of one wave, in a fixed order, with
 // no atomics and no partial gradients in memory.
+//
+// The rows' kernel does 6 dim operations an element in its products, the keys' 8 dim; both pay
+// the forward's vector instructions for an element's weight again and some for its gradient, and
+// two waves a SIMD (one at 128 channels, where dk and dv alone take 128 registers) overlap the two only
+// in part.  16,000 tokens, 8 heads of 64, bias, bfloat16: rows 1.36 ms (579 TFLOP/s), keys
+// 1.58 ms (665 TFLOP/s); 10,007 tokens in 4 causal scenes, 16 heads of 128 on 4, capped: 0.43 and 0.76 ms.
 #include "gsv_attention.h"
 
 namespace gsv {
@@ -228,6 +234,7 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
                                                                               const BwdArgs g) {
     constexpr int W = kFewWaves<T, DP>, KB = 32;
     constexpr bool far = FAR, capped = CAPPED;
+    constexpr bool kFine = sizeof(T) == 2;  // ds in two parts, as the forward's weights
     typedef typename Elem<T>::frag frag;
     static_assert(4 * KB * DP * sizeof(T) >= 32 * DP * sizeof(float), "sums reuse the tiles");
     __shared__ __align__(1024) T tiles[W][4 * KB * DP];  // a wave's keys and values, two buffers
@@ -363,12 +370,19 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
                 }
                 if (capped) dp[r] *= fmaf(-u[r], u[r], 1.f);
             }
+            f32x16 low;
+            if (kFine) low = remainders<T>(dp);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const frag ds = to_frag<T>(dp, half);
+                frag rest_ds;
+                if (kFine) rest_ds = to_frag<T>(low, half);
 #pragma unroll
-                for (int e = 0; e < DP / 32; ++e)
-                    dq[e] = mma(at.columns(kt + half * 16 * DP, e, lane), ds, dq[e]);
+                for (int e = 0; e < DP / 32; ++e) {
+                    const frag k = at.columns(kt + half * 16 * DP, e, lane);
+                    dq[e] = mma(k, ds, dq[e]);
+                    if (kFine) dq[e] = mma(k, rest_ds, dq[e]);
+                }
             }
             dslope -= here;
             if (more) put(b ^ 1);
@@ -423,9 +437,11 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
     }
 }
 
-// dk and dv.  A wave's lanes are keys; the rows of all query heads of the key head pass by.
-template <typename T, int DP, bool FAR, bool CAPPED>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const AttnArgs a, const BwdArgs g) {
+// dk and dv.  A wave's lanes are keys; the rows of all query heads of the key head pass by, so a shared
+// key head's gradient is summed in its wave's registers.
+// FINE: weights and ds enter the products in two parts (few bfloat16 rows, as in the forward).
+template <typename T, int DP, bool FAR, bool CAPPED, bool FINE>
+__global__ __launch_bounds__(256, DP <= 64 && !FINE ? 2 : 1) void k_attention_dkv(const AttnArgs a, const BwdArgs g) {
     constexpr int QB = kOther<T>, WAVES = 4;
     typedef typename Elem<T>::frag frag;
     __shared__ __align__(1024) T sq[2][QB * DP];
@@ -572,14 +588,22 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
                         dp[r] = (dp[r] - delta[r]) * w[r];
                         if (capped) dp[r] *= fmaf(-u[r], u[r], 1.f);
                     }
+                    f32x16 low_w, low_dp;
+                    if (FINE) low_w = remainders<T>(w), low_dp = remainders<T>(dp);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const frag p = to_frag<T>(w, half), ds = to_frag<T>(dp, half);
+                        frag rest_p, rest_ds;
+                        if (FINE) rest_p = to_frag<T>(low_w, half), rest_ds = to_frag<T>(low_dp, half);
                         const int at = (qb * 32 + half * 16) * DP;
 #pragma unroll
                         for (int n = 0; n < DP / 32; ++n) {
-                            dv[n] = mma(tl.columns(sdo[b] + at, n, lane), p, dv[n]);
-                            dk[n] = mma(tl.columns(sq[b] + at, n, lane), ds, dk[n]);
+                            const frag o = tl.columns(sdo[b] + at, n, lane);
+                            dv[n] = mma(o, p, dv[n]);
+                            if (FINE) dv[n] = mma(o, rest_p, dv[n]);
+                            const frag q = tl.columns(sq[b] + at, n, lane);
+                            dk[n] = mma(q, ds, dk[n]);
+                            if (FINE) dk[n] = mma(q, rest_ds, dk[n]);
                         }
                     }
                 }
@@ -601,7 +625,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
     }
 }
 
-// The parts' sums of dk and dv, in order: four values a thread, 16 bytes of each part.
+// The parts' sums of dk and dv, in order: four values a thread, 16 bytes of each part.  Bytes bound
+// it: four parts of 10,007 tokens, 4 heads of 128 (164 MB read, from the last-level cache in part) take 27 us.
 template <typename T>
 __global__ __launch_bounds__(256) void k_parts_sum(const float *__restrict__ pk,
                                                    const float *__restrict__ pv, int parts,
@@ -635,9 +660,15 @@ struct Backward {
             hipLaunchKernelGGL((k_attention_dq<T, DP, FAR, CAPPED>), grid, dim3(256), 0, st, a, g);
         AttnArgs k = a;
         k.slots = kslots;
-        hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED>),
-                           dim3((unsigned)kslots * a.scenes * a.kv_heads * g.parts), dim3(256), 0, st,
-                           k, g);
+        const dim3 keys((unsigned)kslots * a.scenes * a.kv_heads * g.parts);
+        if constexpr (sizeof(T) == 2) {
+            if (attention_few(a))
+                hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED, true>), keys, dim3(256), 0, st, k, g);
+            else
+                hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED, false>), keys, dim3(256), 0, st, k, g);
+        } else {
+            hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED, false>), keys, dim3(256), 0, st, k, g);
+        }
         if (g.parts == 1 || a.k_tokens == 0) return;
         const int64_t fours = (int64_t)a.k_tokens * a.kv_heads * a.dim / 4;
         hipLaunchKernelGGL(k_parts_sum<T>, dim3((unsigned)((2 * fours + 255) / 256)), dim3(256), 0, st,

@@ -10,6 +10,10 @@
 //   dgate = scale branch_weight A (a scene's), dscale = sum_s gate branch_weight A,
 //   dbranch_weight = sum_s gate scale A, dweight = B
 // first over each workgroup's rows of one scene, then over workgroups, in a fixed order.
+//
+// 20,000 rows of 1024, bfloat16 with a float32 residual (246 MB forward, 369 backward): 48 us (5.1 TB/s) and
+// 97 (3.8 TB/s) + 16 for the sums.  200,000 rows of 500, bfloat16 (0.8 and 1.2 GB): 216 us (3.7 TB/s)
+// and 357 (3.4 TB/s) + 18.
 #include "gsv_device.h"
 
 namespace gsv {

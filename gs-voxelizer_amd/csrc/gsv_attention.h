@@ -372,6 +372,14 @@ __device__ __forceinline__ void store_column(T *row, const f32x16 (&o)[DP / 32],
 // The row of a block that result register r of a lane's half holds, less 4 (lane / 32).
 __device__ __forceinline__ constexpr int result_row(int r) { return 8 * (r >> 2) + (r & 3); }
 
+// What the rounding to T takes from each value.
+template <typename T> __device__ __forceinline__ f32x16 remainders(const f32x16 &w) {
+    f32x16 low;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) low[r] = w[r] - (float)(T)w[r];
+    return low;
+}
+
 // The product of each lane's own row with its column, the diagonal of a 32 x 32 product: formed by
 // the instructions and in the order of any other element, so that equal rows give equal bits.
 template <typename T, int N>

@@ -556,3 +556,18 @@ def test_rows_that_see_one_key(device, dtype, dim, cap, lengths):
     for n in ("dq", "dk", "dslopes"):
         assert not got[n].any(), n
     R.assert_within(got["dv"], *(x["dv"] for x in R.attention(**c)), "dv")
+
+
+# The results' rounding to bfloat16 is at most 2^-9 of each value.  Weights, ds and out enter the products
+# with 16 bits: 2^-17 of each term, times what cancels in ds (2^4 here), times three.
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (50.0, True)])
+@pytest.mark.parametrize("lengths", [[2] * 9, [3, 1, 2, 0, 5], [14, 4, 5]], ids=str)
+def test_few_keys_average_no_rounding(device, dim, cap, bias, lengths):
+    """The gradients of tiny scenes are as exact as their own type."""
+    c = _case(device, BF16, lengths, 4, 2, dim, bias=bias, causal=True, cap=cap)
+    got = _run(c)
+    want = R.attention(**c)[0]
+    for n in ("out", "dq", "dk", "dv"):
+        w = want[n].double()
+        assert (got[n].double() - w).norm() <= (2.0 ** -9 + 2.0 ** -11) * w.norm(), n
