@@ -234,7 +234,7 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
                                                                               const BwdArgs g) {
     constexpr int W = kFewWaves<T, DP>, KB = 32;
     constexpr bool far = FAR, capped = CAPPED;
-    constexpr bool kFine = sizeof(T) == 2;  // ds in two parts, as the forward's weights
+    const bool fine = sizeof(T) == 2 && attention_fine(a);  // ds in two parts, as the forward's weights
     typedef typename Elem<T>::frag frag;
     static_assert(4 * KB * DP * sizeof(T) >= 32 * DP * sizeof(float), "sums reuse the tiles");
     __shared__ __align__(1024) T tiles[W][4 * KB * DP];  // a wave's keys and values, two buffers
@@ -370,18 +370,14 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
                 }
                 if (capped) dp[r] *= fmaf(-u[r], u[r], 1.f);
             }
-            f32x16 low;
-            if (kFine) low = remainders<T>(dp);
+            for (int part = 0; part <= (fine ? 1 : 0); ++part) {
+                if (part) dp = remainders<T>(dp);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const frag ds = to_frag<T>(dp, half);
-                frag rest_ds;
-                if (kFine) rest_ds = to_frag<T>(low, half);
+                for (int half = 0; half < 2; ++half) {
+                    const frag ds = to_frag<T>(dp, half);
 #pragma unroll
-                for (int e = 0; e < DP / 32; ++e) {
-                    const frag k = at.columns(kt + half * 16 * DP, e, lane);
-                    dq[e] = mma(k, ds, dq[e]);
-                    if (kFine) dq[e] = mma(k, rest_ds, dq[e]);
+                    for (int e = 0; e < DP / 32; ++e)
+                        dq[e] = mma(at.columns(kt + half * 16 * DP, e, lane), ds, dq[e]);
                 }
             }
             dslope -= here;
@@ -439,7 +435,7 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
 
 // dk and dv.  A wave's lanes are keys; the rows of all query heads of the key head pass by, so a shared
 // key head's gradient is summed in its wave's registers.
-// FINE: weights and ds enter the products in two parts (few bfloat16 rows, as in the forward).
+// FINE: weights and ds enter the products in two parts (attention_fine).
 template <typename T, int DP, bool FAR, bool CAPPED, bool FINE>
 __global__ __launch_bounds__(256, DP <= 64 && !FINE ? 2 : 1) void k_attention_dkv(const AttnArgs a, const BwdArgs g) {
     constexpr int QB = kOther<T>, WAVES = 4;
@@ -662,7 +658,7 @@ struct Backward {
         k.slots = kslots;
         const dim3 keys((unsigned)kslots * a.scenes * a.kv_heads * g.parts);
         if constexpr (sizeof(T) == 2) {
-            if (attention_few(a))
+            if (attention_few(a) && attention_fine(a))
                 hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED, true>), keys, dim3(256), 0, st, k, g);
             else
                 hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED, false>), keys, dim3(256), 0, st, k, g);

@@ -240,15 +240,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
 // tokens in 6 scenes, 4 heads of 32: 10 us): a workgroup takes 32 rows of one head, its waves every
 // W-th tile of 32 keys each.  The tiles are a wave's own (its copies need no barrier, only waits);
 // the waves' sums are joined through LDS at the end.  Four times as many workgroups, each a quarter as
-// long.  bfloat16 weights enter the product in two parts (kFine): few keys average no roundings, and
-// the matrix units have time to spare here.  Scores are rounded to powers of two before their
+// long.  Scores are rounded to powers of two before their
 // maximum is taken off, so that the largest weight is exactly a power of two.
 template <typename T, int DP, bool FAR, bool CAPPED, bool TRAIN>
 __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_fwd_few(
     const AttnArgs a, T *__restrict__ out, T *__restrict__ out_low, float *__restrict__ lse) {
     constexpr int W = kFewWaves<T, DP>, KB = 32;
     constexpr bool far = FAR, capped = CAPPED;
-    constexpr bool kFine = sizeof(T) == 2;
+    const bool fine = sizeof(T) == 2 && attention_fine(a);
     typedef typename Elem<T>::frag frag;
     static_assert(4 * KB * DP * sizeof(T) >= 32 * DP * sizeof(float), "sums reuse the tiles");
     __shared__ __align__(1024) T tiles[W][4 * KB * DP];  // a wave's keys and values, two buffers
@@ -369,19 +368,15 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_fwd_few(
                 w[r] = fast_exp2(w[r] - ref);
                 if (TRAIN) exact += w[r];
             }
-            f32x16 low;
-            if (kFine) low = remainders<T>(w);
+            for (int part = 0; part <= (fine ? 1 : 0); ++part) {
+                if (part) w = remainders<T>(w);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const frag p = to_frag<T>(w, half);
-                frag rest;
-                sum = add_weights(p, sum);
-                if (kFine) rest = to_frag<T>(low, half), sum = add_weights(rest, sum);
+                for (int half = 0; half < 2; ++half) {
+                    const frag p = to_frag<T>(w, half);
+                    sum = add_weights(p, sum);
 #pragma unroll
-                for (int e = 0; e < DP / 32; ++e) {
-                    const frag v = at.columns(vt + half * 16 * DP, e, lane);
-                    o[e] = mma(v, p, o[e]);
-                    if (kFine) o[e] = mma(v, rest, o[e]);
+                    for (int e = 0; e < DP / 32; ++e)
+                        o[e] = mma(at.columns(vt + half * 16 * DP, e, lane), p, o[e]);
                 }
             }
             if (more) put(b ^ 1);

@@ -214,8 +214,20 @@ inline bool attention_pairs(const AttnArgs &a) {
 }
 // Whether rows are so few that the waves of a workgroup share them and split the keys: below three
 // workgroups of 128 rows for four CUs.  8 heads of 64, one scene: 500 tokens forward 13 us so and 22
-// otherwise, 2,000 36 and 66, 4,000 118 and 110.
-inline bool attention_few(const AttnArgs &a) { return attention_tiles(a, false) < 192; }
+// otherwise, 2,000 36 and 66, 4,000 118 and 110.  And for scenes of 32 tokens and fewer while their
+// workgroups fit the CUs in one round, for attention_fine: 64 scenes, 8 heads take 40 us so (forward and
+// backward) and 27 otherwise, below what the call's own launches take.
+inline bool attention_few(const AttnArgs &a) {
+    return attention_tiles(a, false) < 192 ||
+           ((int64_t)a.q_tokens <= (int64_t)32 * a.scenes && (int64_t)a.scenes * a.heads <= 512);
+}
+// Whether bfloat16 weights and ds enter the products of few rows in two parts: where a row sees too few
+// keys to average their roundings.  The gradients of scenes of two tokens are 0.0018 off (2-norm,
+// the rounding of the results) so and 0.0031 otherwise, of long ones 0.0017 and 0.0024; one scene of 2,000
+// tokens, 8 heads of 64 takes 39 us (forward), 70 (rows) and 40 (keys) otherwise and 46, 73 and 77 so.
+__host__ __device__ inline bool attention_fine(const AttnArgs &a) {
+    return (int64_t)a.q_tokens < (int64_t)128 * a.scenes;
+}
 // The waves of such a workgroup: as many as the LDS holds their tiles.
 template <typename T, int DP> constexpr int kFewWaves = DP * sizeof(T) > 256 ? 2 : 4;
 

@@ -562,7 +562,7 @@ def test_rows_that_see_one_key(device, dtype, dim, cap, lengths):
 # with 16 bits: 2^-17 of each term, times what cancels in ds (2^4 here), times three.
 @pytest.mark.parametrize("dim", [32, 64, 128])
 @pytest.mark.parametrize("cap,bias", [(0.0, False), (50.0, True)])
-@pytest.mark.parametrize("lengths", [[2] * 9, [3, 1, 2, 0, 5], [14, 4, 5]], ids=str)
+@pytest.mark.parametrize("lengths", [[2] * 9, [3, 1, 2, 0, 5], [14, 4, 5], [2, 3] * 40], ids=str)
 def test_few_keys_average_no_rounding(device, dim, cap, bias, lengths):
     """The gradients of tiny scenes are as exact as their own type."""
     c = _case(device, BF16, lengths, 4, 2, dim, bias=bias, causal=True, cap=cap)
@@ -571,3 +571,15 @@ def test_few_keys_average_no_rounding(device, dim, cap, bias, lengths):
     for n in ("out", "dq", "dk", "dv"):
         w = want[n].double()
         assert (got[n].double() - w).norm() <= (2.0 ** -9 + 2.0 ** -11) * w.norm(), n
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("dim", [40, 64, 128])
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+@pytest.mark.parametrize("lengths", [[70, 33], [900] * 16], ids=["few", "many"])
+def test_first_causal_rows(device, dtype, dim, cap, lengths):
+    """A causal scene's first row sees its own key alone, whatever its tile's other rows see."""
+    c = _case(device, dtype, lengths, 4, 2, dim, bias=True, causal=True, cap=cap)
+    got, first = _run(c), torch.tensor([sum(lengths[:n]) for n in range(len(lengths))], device=device)
+    assert torch.equal(got["out"][first], c["v"][first].repeat_interleave(2, 1))
+    assert not got["dq"][first].any()
