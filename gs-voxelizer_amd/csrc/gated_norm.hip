@@ -356,7 +356,7 @@ void launch_bwd(const NormArgs &a, hipStream_t s) {
     else hipLaunchKernelGGL((k_norm_bwd<TX, TF, VEC, E, WAVES, false>), grid, dim3(256), 0, s, a);
 }
 // Channels of a lane and waves of a row.  The backward keeps eight vectors of them, so 8 channels a
-// lane (112 registers, four waves a SIMD) and more waves a row: 20,000 rows of 1024 take 88 us, with 16
+// lane (112 registers, four waves a SIMD) and more waves a row: 20,000 rows of 1024 take 97 us, with 16
 // channels a lane and one wave (190 registers) 140.
 template <typename TX, typename TF, int VEC>
 void launch_width(const NormArgs &a, bool backward, hipStream_t s) {
