@@ -734,6 +734,8 @@ extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, con
     if ((st = gsv_attention_bwd_workspace_bytes(args, &need)) != GSV_OK) return st;
     if (need > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
     const int64_t chunk = args->dtype == GSV_BF16 ? 8 : 4;
+    dout_row = used_stride(dout_row, a.q_tokens);
+    dout_head = used_stride(dout_head, a.heads);
     if (dout_row % chunk || dout_head % chunk || dout_row < 0 ||
         dout_row * (16 / chunk) > kMaxRowBytes)
         return GSV_ERR_INVALID_ARGUMENT;

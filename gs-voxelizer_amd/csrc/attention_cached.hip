@@ -323,6 +323,8 @@ extern "C" int gsv_attention_cached(const gsv_attention *args, const int32_t *le
     if ((st = gsv_attention_cached_workspace_bytes(args, &need)) != GSV_OK) return st;
     if (need > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
     const int64_t chunk = args->dtype == GSV_BF16 ? 8 : 4;
+    k_scene = used_stride(k_scene, a.scenes);
+    v_scene = used_stride(v_scene, a.scenes);
     if (!lengths || !out || (need && !workspace) || k_scene % chunk || v_scene % chunk ||
         reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16)
         return GSV_ERR_INVALID_ARGUMENT;

@@ -487,10 +487,12 @@ int attention_args(const gsv_attention *in, AttnArgs *a, int *longest_q, int *lo
         g.heads % g.kv_heads || g.dim < 8 || g.dim > 128 || g.dim % 8 || g.scenes < 1)
         return GSV_ERR_INVALID_ARGUMENT;
     const int64_t chunk = g.dtype == GSV_BF16 ? 8 : 4;
-    const int64_t strides[] = {g.q_row, g.q_head, g.k_row, g.k_head, g.v_row, g.v_head};
-    for (int64_t x : strides)
+    const int64_t q_row = used_stride(g.q_row, g.q_tokens), q_head = used_stride(g.q_head, g.heads);
+    const int64_t k_row = used_stride(g.k_row, g.k_tokens), k_head = used_stride(g.k_head, g.kv_heads);
+    const int64_t v_row = used_stride(g.v_row, g.k_tokens), v_head = used_stride(g.v_head, g.kv_heads);
+    for (int64_t x : {q_row, q_head, k_row, k_head, v_row, v_head})
         if (x % chunk) return GSV_ERR_INVALID_ARGUMENT;
-    for (int64_t x : {g.q_row, g.k_row, g.v_row})
+    for (int64_t x : {q_row, k_row, v_row})
         if (x < 0 || x * (16 / chunk) > kMaxRowBytes) return GSV_ERR_INVALID_ARGUMENT;
     const void *ptrs[] = {g.q, g.k, g.v};
     for (const void *p : ptrs)
@@ -503,7 +505,7 @@ int attention_args(const gsv_attention *in, AttnArgs *a, int *longest_q, int *lo
                      (g.slopes_dtype != GSV_F32 && g.slopes_dtype != GSV_BF16)))
         return GSV_ERR_INVALID_ARGUMENT;
     if (g.keep && g.keep_bytes != 1 && g.keep_bytes != 4) return GSV_ERR_INVALID_ARGUMENT;
-    *a = AttnArgs{g.q, g.k, g.v, g.q_row, g.q_head, g.k_row, g.k_head, g.v_row, g.v_head,
+    *a = AttnArgs{g.q, g.k, g.v, q_row, q_head, k_row, k_head, v_row, v_head,
                   g.q_tokens, g.k_tokens, g.heads, g.kv_heads, g.dim, g.scenes, g.q_starts,
                   g.k_starts, g.prefix, g.causal, g.scale, g.cap, g.q_positions, g.k_positions,
                   g.q_pos_row, g.k_pos_row, g.slopes, g.slopes_dtype == GSV_F32, g.keep,

@@ -31,12 +31,14 @@ bool is_tokens(const Tensor &t, int64_t dims, const at::Device &dev) {
     return t.defined() && t.layout() == at::kStrided && token_type(t) && t.device() == dev &&
            t.dim() == dims && t.stride(-1) == 1;
 }
-// Rows that start 16-byte aligned and lie within the attention kernels' reach.
+// Rows that start 16-byte aligned and lie within the attention kernels' reach; the stride of an axis
+// of one entry says nothing.
 bool is_aligned(const Tensor &t) {
     const int64_t size = t.element_size();
-    if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || t.stride(-3) * size > (1 << 24)) return false;
+    if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+    if (t.size(-3) > 1 && t.stride(-3) * size > (1 << 24)) return false;
     for (int64_t i = 0; i + 1 < t.dim(); ++i)
-        if (t.stride(i) * size % 16) return false;
+        if (t.size(i) > 1 && t.stride(i) * size % 16) return false;
     return true;
 }
 // Float32 rows of x, y, z.
@@ -352,9 +354,7 @@ struct SceneAttention : public torch::autograd::Function<SceneAttention> {
             TORCH_CHECK(t.defined() && t.device() == dev && t.scalar_type() == type && t.dim() == 3 &&
                             t.size(0) == n && t.size(1) == h && t.size(2) == D,
                         what, ": expected shape (", n, ", ", h, ", ", D, ") on ", dev);
-            if (t.stride(2) == 1 && is_aligned(t)) return t;
-            Tensor u = t.contiguous();
-            return is_aligned(u) ? u : u.clone();
+            return t.stride(2) == 1 && is_aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous);
         };
         const auto ints = [&](const Tensor &t, int64_t n, const char *what) {
             return t.defined() ? unpacked(t, at::kInt, dev, n, what) : t;

@@ -178,6 +178,9 @@ struct AttnArgs {
     int slots;  // workgroups a scene and head: they take its tiles in turn
 };
 
+// The stride of an axis of one entry is never used, whatever a caller's view holds there.
+inline int64_t used_stride(int64_t stride, int64_t entries) { return entries > 1 ? stride : 0; }
+
 // Checks the C arguments and lays them out for a launch; longest_*: rows of the longest scene.
 int attention_args(const gsv_attention *in, AttnArgs *a, int *longest_q, int *longest_k);
 

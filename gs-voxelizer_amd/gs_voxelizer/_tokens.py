@@ -58,13 +58,14 @@ MAX_ROW_BYTES = 1 << 24
 
 def rows16(t):
     """`t`, or a contiguous copy where its last axis is strided, a row is not 16-byte aligned or
-    rows (the third axis from the end) lie 16 MB apart or more."""
-    size, strides = t.element_size(), t.stride()
-    if (strides[-1] == 1 and t.data_ptr() % 16 == 0 and strides[-3] * size <= MAX_ROW_BYTES
-            and all(s * size % 16 == 0 for s in strides[:-1])):
+    rows (the third axis from the end) lie more than 16 MB apart.  The stride of an axis of one
+    entry says nothing and is not looked at; nor does the C side use it."""
+    size = t.element_size()
+    strides = [s * size if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
+    if (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and strides[-3] <= MAX_ROW_BYTES
+            and all(s % 16 == 0 for s in strides[:-1])):
         return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def rows(t):

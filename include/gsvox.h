@@ -353,7 +353,8 @@ int gsv_wave_timeline(int32_t kernel, uint64_t *records, int32_t capacity);
  * Attention inside the scenes of a packed batch.  q (q_tokens, heads, dim), k and v
  * (k_tokens, kv_heads, dim) with the given row and head strides; heads a multiple of
  * kv_heads, query head h reads key head h / (heads / kv_heads); dim a multiple of 8,
- * 8 .. 128; pointers and strides multiples of 16 bytes, row strides 0 .. 16 MB.
+ * 8 .. 128; pointers and strides multiples of 16 bytes, row strides 0 .. 16 MB (the stride
+ * of an axis of one entry is not looked at).
  *   t_ij = scale q_i.k_j, with cap > 0: cap tanh(scale q_i.k_j / cap);
  *   with slopes: - slopes[h] |q_positions[i] - k_positions[j]|
  * over the keys j that row i sees: those of its own scene, kept ones (keep NULL, or

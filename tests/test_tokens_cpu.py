@@ -1,0 +1,57 @@
+"""The operators on packed tokens without a GPU: what their host side accepts, copies and refuses."""
+import ctypes
+
+import pytest
+import torch
+
+from gs_voxelizer import _lib, _tokens
+
+OK, SIZE_OVERFLOW = 0, 4
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def _attention(**more):
+    a = dict(dtype=1, q_tokens=64, k_tokens=64, heads=4, kv_heads=4, dim=64, scenes=1, scale=0.125,
+             q=1024, k=1024, v=1024)
+    for n in "qkv":
+        a[n + "_row"], a[n + "_head"] = 256, 64
+    return _lib.Attention(**dict(a, **more))
+
+
+def _plan(name, a):
+    """The status of a call's host side: a workspace's size needs no device."""
+    return getattr(_lib.load(), f"gsv_attention_{name}_workspace_bytes")(
+        ctypes.byref(a), ctypes.byref(ctypes.c_size_t(0)))
+
+
+def _one_token(dtype=BF16):
+    """A scene's token sliced out of an array of 20,000: (1, H, D), its rows 40 MB apart."""
+    return torch.zeros(1, 20_000, 16, 64, dtype=dtype)[:, 7]
+
+
+def test_strides_of_one_entry_mean_nothing():
+    assert _plan("bwd", _attention()) == OK
+    for n in "qkv":
+        assert _plan("bwd", _attention(q_tokens=1, k_tokens=1, **{n + "_row": 20_480_000})) == OK
+        assert _plan("bwd", _attention(q_tokens=1, k_tokens=1, **{n + "_row": 7})) == OK
+        assert _plan("bwd", _attention(heads=1, kv_heads=1, **{n + "_head": 7})) == OK
+        assert _plan("bwd", _attention(**{n + "_row": 20_480_000})) != OK
+        assert _plan("bwd", _attention(**{n + "_row": 257})) != OK
+        assert _plan("bwd", _attention(**{n + "_head": 65})) != OK
+    assert _plan("cached", _attention(q_tokens=1, scenes=1, q_row=20_480_000)) == OK
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_views_are_taken_as_they_are_or_copied(dtype):
+    one = _one_token(dtype)
+    assert _tokens.rows16(one) is one
+    head = torch.zeros(5, 1, 67, dtype=dtype)[..., :64]
+    odd = head.as_strided((1, 1, 64), (7, 3, 1))
+    assert _tokens.rows16(odd) is odd
+    # rows off alignment, far rows, a strided last axis, a start off alignment: canonical copies
+    far = torch.zeros(2, 1 << 24, dtype=dtype)[:, :256].unflatten(1, (4, 64))
+    for t in (head, far, torch.zeros(5, 64, 4, dtype=dtype).transpose(1, 2),
+              torch.zeros(65, dtype=dtype)[1:].view(1, 1, 64)):
+        c = _tokens.rows16(t)
+        assert c is not t and c.is_contiguous() and c.stride() == (t.shape[1] * 64, 64, 1)
+        assert c.data_ptr() % 16 == 0 and torch.equal(c, t)
