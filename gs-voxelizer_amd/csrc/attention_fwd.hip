@@ -486,6 +486,7 @@ int attention_args(const gsv_attention *in, AttnArgs *a, int *longest_q, int *lo
     if (g.q_tokens < 0 || g.k_tokens < 0 || g.heads < 1 || g.kv_heads < 1 ||
         g.heads % g.kv_heads || g.dim < 8 || g.dim > 128 || g.dim % 8 || g.scenes < 1)
         return GSV_ERR_INVALID_ARGUMENT;
+    if (g.q_tokens > GSV_MAX_TOKENS || g.k_tokens > GSV_MAX_TOKENS) return GSV_ERR_SIZE_OVERFLOW;
     const int64_t chunk = g.dtype == GSV_BF16 ? 8 : 4;
     const int64_t q_row = used_stride(g.q_row, g.q_tokens), q_head = used_stride(g.q_head, g.heads);
     const int64_t k_row = used_stride(g.k_row, g.k_tokens), k_head = used_stride(g.k_head, g.kv_heads);

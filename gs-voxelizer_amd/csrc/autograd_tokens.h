@@ -136,7 +136,7 @@ std::vector<Tensor> rotate(const Tensor &q, const Tensor &k, const Tensor &posit
     const at::Device dev = q.device();
     if (!is_tokens(q, 3, dev) || !is_tokens(k, 3, dev) || k.scalar_type() != q.scalar_type()) return {};
     const int64_t T = q.size(0), D = q.size(2);
-    if (k.size(0) != T || k.size(2) != D || T < 1 || T > INT32_MAX || D > 1024 ||
+    if (k.size(0) != T || k.size(2) != D || T < 1 || T > GSV_MAX_TOKENS || D > 1024 ||
         q.size(1) + k.size(1) > 4096 || positions.dim() != 2 || frequencies.dim() != 2 ||
         positions.scalar_type() != at::kFloat || frequencies.scalar_type() != at::kFloat ||
         positions.device() != dev || frequencies.device() != dev || !frequencies.is_contiguous() ||
@@ -247,7 +247,7 @@ std::vector<Tensor> gated_norm(const Tensor &x, const Tensor &branch, const Tens
     const int64_t T = x.size(0), C = x.size(1);
     NormCall c{x, branch, weight, given(branch_weight), given(scale), given(gate), given(scene_starts),
                1, longest, false, eps};
-    if (T < 1 || T > INT32_MAX || C < 1 || C > 8192 || !(eps >= 0) ||
+    if (T < 1 || T > GSV_MAX_TOKENS || C < 1 || C > 8192 || !(eps >= 0) ||
         !weight.defined() || !is_parameter(weight, C, dev) || !is_parameter(c.branch_weight, C, dev) ||
         !is_parameter(c.scale, C, dev))
         return {};
@@ -311,7 +311,7 @@ struct AttentionCall {
             return false;
         const int64_t H = q.size(1), K = k.size(-2), D = q.size(2);
         if (k.size(-1) != D || D < 8 || D > 128 || D % 8 || H < 1 || K < 1 || H % K ||
-            q.size(0) < 1 || q.size(0) > INT32_MAX || k.size(-3) < 1 || k.size(-3) > INT32_MAX ||
+            q.size(0) < 1 || q.size(0) > GSV_MAX_TOKENS || k.size(-3) < 1 || k.size(-3) > GSV_MAX_TOKENS ||
             longest < 0 || longest > INT32_MAX)
             return false;
         if (!is_aligned(q) || !is_aligned(k) || !is_aligned(v)) return false;

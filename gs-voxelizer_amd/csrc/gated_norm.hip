@@ -389,6 +389,7 @@ int norm_args(const gsv_norm *n, NormArgs *a) {
     if (!type(n->dtype) || !type(n->branch_dtype) || n->dtype > n->branch_dtype) return GSV_ERR_INVALID_ARGUMENT;
     if (n->tokens < 0 || n->channels < 1 || n->channels > 8192 || n->scenes < 1 || !(n->eps >= 0.f))
         return GSV_ERR_INVALID_ARGUMENT;
+    if (n->tokens > GSV_MAX_TOKENS || n->scenes > GSV_MAX_TOKENS) return GSV_ERR_SIZE_OVERFLOW;
     if (n->scenes > 1 && !n->starts) return GSV_ERR_INVALID_ARGUMENT;
     if (n->gate && (!type(n->gate_dtype) || (n->gate_dtype == GSV_BF16 && n->branch_dtype == GSV_F32)))
         return GSV_ERR_INVALID_ARGUMENT;

@@ -267,7 +267,7 @@ __device__ __forceinline__ Scene scene_rows(const AttnArgs &a, int s) {
 __device__ __forceinline__ int key_limit(const AttnArgs &a, const Scene &c, int i) {
     const int n = c.k1 - c.k0;
     if (!a.causal) return n;
-    return min(max(c.prefix, i + n - (c.q1 - c.q0) + 1), n);
+    return min(max(c.prefix, n - (c.q1 - c.q0 - i) + 1), n);
 }
 __device__ __forceinline__ bool kept(const AttnArgs &a, int64_t row) {
     if (!a.keep) return true;

@@ -136,6 +136,7 @@ extern "C" int gsv_rotary(const gsv_rotary_args *r, void *q_out, void *k_out, in
         r->kv_heads < 0 || r->dim < 2 || r->dim > 1024 || r->pairs < 1 || 2 * r->pairs > r->dim ||
         r->axes < 1 || r->axes > 8)
         return GSV_ERR_INVALID_ARGUMENT;
+    if (r->tokens > GSV_MAX_TOKENS) return GSV_ERR_SIZE_OVERFLOW;
     if (r->tokens == 0 || r->heads + r->kv_heads == 0) return GSV_OK;
     if ((int64_t)r->heads + r->kv_heads > 4096) return GSV_ERR_INVALID_ARGUMENT;
     if ((r->heads && (!r->q || !q_out)) || (r->kv_heads && (!r->k || !k_out)) || !r->positions ||

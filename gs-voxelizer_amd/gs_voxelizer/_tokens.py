@@ -15,7 +15,7 @@ from . import _lib
 from .cuda import _status_error
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1}  # GSV_F32, GSV_BF16
-INT32_MAX = 2**31 - 1
+MAX_TOKENS = 2**31 - 2**16  # GSV_MAX_TOKENS
 
 _L = _lib.load()
 
@@ -87,7 +87,7 @@ def starts(t, what, device):
     if t is None:
         return None, 1
     t = int32s(t, what, None, device)
-    check(t.numel() >= 2, f"{what} must hold scenes + 1 values, got {t.numel()}")
+    check(2 <= t.numel() <= MAX_TOKENS, f"{what} must hold scenes + 1 values, got {t.numel()}")
     return t, t.numel() - 1
 
 

@@ -89,7 +89,7 @@ def scene_attention(q: Tensor, k: Tensor, v: Tensor, *, scene_starts: Optional[T
             return out[0]
     H, K, D = _heads(q, k, v, 3)
     dev, T, N = q.device, q.shape[0], k.shape[0]
-    _t.check(T <= _t.INT32_MAX and N <= _t.INT32_MAX, "too many tokens")
+    _t.check(T <= _t.MAX_TOKENS and N <= _t.MAX_TOKENS, "too many tokens")
     qs, scenes = _t.starts(scene_starts, "scene_starts", dev)
     if key_starts is None:
         _t.check(scenes == 1 or N == T, f"{N} keys for {T} queries need key_starts")
@@ -205,7 +205,7 @@ def cached_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tenso
     H, K, D = _heads(q, k_cache, v_cache, 4)
     dev, S, N = q.device, q.shape[0], k_cache.shape[1]
     _t.check(k_cache.shape[0] == S, f"k_cache holds {k_cache.shape[0]} scenes, q {S}")
-    _t.check(N <= _t.INT32_MAX, "too many tokens")
+    _t.check(N <= _t.MAX_TOKENS, "too many tokens")
     for t, what in ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache")):
         _t.fixed(t, what, "s")
     lengths = _t.int32s(lengths, "lengths", S, dev)

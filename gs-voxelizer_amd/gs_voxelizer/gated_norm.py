@@ -52,7 +52,7 @@ def gated_residual_norm(x: Tensor, branch: Tensor, weight: Tensor, *,
     _t.check(branch.dtype == x.dtype or x.dtype == torch.float32,
              f"branch must be bfloat16 where x is, got {branch.dtype}")
     _t.check(1 <= C <= MAX_CHANNELS, f"1 to {MAX_CHANNELS} channels, got {C}")
-    _t.check(T <= _t.INT32_MAX, "too many tokens")
+    _t.check(T <= _t.MAX_TOKENS, "too many tokens")
     for t, what in ((weight, "weight"), (branch_weight, "branch_weight"), (scale, "scale")):
         if t is None and what != "weight":
             continue

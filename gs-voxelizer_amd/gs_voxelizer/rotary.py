@@ -66,7 +66,7 @@ def rotate_qk(q: Tensor, k: Optional[Tensor], positions: Tensor, frequencies: Te
     _t.check(P >= 1 and 2 * P <= D, f"{P} channel pairs do not fit {D} channels")
     _t.check(D <= 1024, f"at most 1024 channels, got {D}")
     _t.check(q.shape[1] + (0 if k is None else k.shape[1]) <= 4096, "at most 4096 heads")
-    _t.check(T <= _t.INT32_MAX, "too many tokens")
+    _t.check(T <= _t.MAX_TOKENS, "too many tokens")
     frequencies = frequencies.contiguous()
     if not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
         return _turn(q, k, positions, frequencies, interleaved, False)

@@ -348,6 +348,9 @@ int gsv_wave_timeline(int32_t kernel, uint64_t *records, int32_t capacity);
  */
 #define GSV_F32 0
 #define GSV_BF16 1
+/* Rows of a batch or a cache, and scenes, that these operators take; more give
+ * GSV_ERR_SIZE_OVERFLOW.  (Kernels count rows in steps of up to 2^15 past the last one, in int32.) */
+#define GSV_MAX_TOKENS (INT32_MAX - 65535)
 
 /*
  * Attention inside the scenes of a packed batch.  q (q_tokens, heads, dim), k and v

@@ -55,3 +55,24 @@ def test_views_are_taken_as_they_are_or_copied(dtype):
         c = _tokens.rows16(t)
         assert c is not t and c.is_contiguous() and c.stride() == (t.shape[1] * 64, 64, 1)
         assert c.data_ptr() % 16 == 0 and torch.equal(c, t)
+
+
+@pytest.mark.parametrize("tokens", [2**31 - 2**16 + 1, 2**31 - 64, 2**31 - 1])
+def test_counts_that_would_pass_int32_are_refused(tokens):
+    """Kernels step past the last row by up to 2^15 rows: counts nearer to 2^31 would wrap there, and a
+    loop over keys would not end.  (No pointers: nothing could be launched.)"""
+    L = _lib.load()
+    assert _plan("bwd", _attention(q_tokens=tokens)) == SIZE_OVERFLOW
+    assert _plan("bwd", _attention(k_tokens=tokens)) == SIZE_OVERFLOW
+    assert _plan("cached", _attention(k_tokens=tokens, scenes=64)) == SIZE_OVERFLOW
+    n = _lib.Norm(dtype=0, branch_dtype=0, tokens=tokens, channels=1, scenes=1, eps=1e-6)
+    assert L.gsv_gated_norm_fwd(ctypes.byref(n), None, None, None) == SIZE_OVERFLOW
+    n.tokens, n.scenes = 5, tokens
+    assert L.gsv_gated_norm_fwd(ctypes.byref(n), None, None, None) == SIZE_OVERFLOW
+    r = _lib.Rotary(dtype=0, tokens=tokens, heads=1, kv_heads=0, dim=2, pairs=1, axes=1)
+    assert L.gsv_rotary(ctypes.byref(r), None, None, 0, None) == SIZE_OVERFLOW
+    # the most that is taken
+    assert _plan("bwd", _attention(k_tokens=_tokens.MAX_TOKENS)) == OK
+    assert _plan("cached", _attention(k_tokens=_tokens.MAX_TOKENS, scenes=64)) == OK
+    r.tokens = _tokens.MAX_TOKENS
+    assert L.gsv_rotary(ctypes.byref(r), None, None, 0, None) == 1  # its pointers are missing
