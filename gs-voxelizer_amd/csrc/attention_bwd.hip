@@ -72,6 +72,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
     const Scene c = scene_rows(a, s);
     const int nq = c.q1 - c.q0;
     const int tiles = (nq + kRows - 1) / kRows;
+    const bool fine = in_two_parts<T>(c.k1 - c.k0);
     const int hk = h / (a.heads / a.kv_heads);
     const T *kbase = static_cast<const T *>(a.k) + (int64_t)c.k0 * a.k_row + hk * a.k_head;
     const T *vbase = static_cast<const T *>(a.v) + (int64_t)c.k0 * a.v_row + hk * a.v_head;
@@ -194,12 +195,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
                         }
                         if (capped) dp[r] *= fmaf(-u[r], u[r], 1.f);
                     }
+                    for (int part = 0; part <= (fine ? 1 : 0); ++part) {
+                        if (part) dp = remainders<T>(dp);
+                        Tile<T, DP> cols = at;
+                        cols.forget();
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const frag ds = to_frag<T>(dp, half);
+                        for (int half = 0; half < 2; ++half) {
+                            const frag ds = to_frag<T>(dp, half);
 #pragma unroll
-                        for (int e = 0; e < DP / 32; ++e)
-                            dq[e] = mma(at.columns(kt + half * 16 * DP, e, lane), ds, dq[e]);
+                            for (int e = 0; e < DP / 32; ++e)
+                                dq[e] = mma(cols.columns(kt + half * 16 * DP, e, lane), ds, dq[e]);
+                        }
                     }
                 }
                 dslope -= here;
@@ -234,7 +240,6 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
                                                                               const BwdArgs g) {
     constexpr int W = kFewWaves<T, DP>, KB = 32;
     constexpr bool far = FAR, capped = CAPPED;
-    const bool fine = sizeof(T) == 2 && attention_fine(a);  // ds in two parts, as the forward's weights
     typedef typename Elem<T>::frag frag;
     static_assert(4 * KB * DP * sizeof(T) >= 32 * DP * sizeof(float), "sums reuse the tiles");
     __shared__ __align__(1024) T tiles[W][4 * KB * DP];  // a wave's keys and values, two buffers
@@ -247,6 +252,7 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
     const int s = group_at % a.scenes, slot = group_at / a.scenes;
     const Scene c = scene_rows(a, s);
     const int nq = c.q1 - c.q0, row_tiles = (nq + 31) / 32;
+    const bool fine = in_two_parts<T>(c.k1 - c.k0);  // ds, as the forward's weights
     const int hk = h / (a.heads / a.kv_heads);
     const T *kbase = static_cast<const T *>(a.k) + (int64_t)c.k0 * a.k_row + hk * a.k_head;
     const T *vbase = static_cast<const T *>(a.v) + (int64_t)c.k0 * a.v_row + hk * a.v_head;
@@ -435,9 +441,8 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
 
 // dk and dv.  A wave's lanes are keys; the rows of all query heads of the key head pass by, so a shared
 // key head's gradient is summed in its wave's registers.
-// FINE: weights and ds enter the products in two parts (attention_fine).
-template <typename T, int DP, bool FAR, bool CAPPED, bool FINE>
-__global__ __launch_bounds__(256, DP <= 64 && !FINE ? 2 : 1) void k_attention_dkv(const AttnArgs a, const BwdArgs g) {
+template <typename T, int DP, bool FAR, bool CAPPED>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const AttnArgs a, const BwdArgs g) {
     constexpr int QB = kOther<T>, WAVES = 4;
     typedef typename Elem<T>::frag frag;
     __shared__ __align__(1024) T sq[2][QB * DP];
@@ -453,6 +458,7 @@ __global__ __launch_bounds__(256, DP <= 64 && !FINE ? 2 : 1) void k_attention_dk
     const int nq = c.q1 - c.q0, nk = c.k1 - c.k0, off = nk - nq;
     const int group = a.heads / a.kv_heads;
     const int tiles = (nk + kRows - 1) / kRows;
+    const bool fine = in_two_parts<T>(nk);  // weights and ds
     constexpr bool far = FAR, capped = CAPPED;
     const float unit = capped ? kLog2e : a.scale * kLog2e;
     const float in_cap = capped ? a.scale / a.cap : 0.f;
@@ -584,22 +590,19 @@ __global__ __launch_bounds__(256, DP <= 64 && !FINE ? 2 : 1) void k_attention_dk
                         dp[r] = (dp[r] - delta[r]) * w[r];
                         if (capped) dp[r] *= fmaf(-u[r], u[r], 1.f);
                     }
-                    f32x16 low_w, low_dp;
-                    if (FINE) low_w = remainders<T>(w), low_dp = remainders<T>(dp);
+                    for (int part = 0; part <= (fine ? 1 : 0); ++part) {
+                        if (part) w = remainders<T>(w), dp = remainders<T>(dp);
+                        Tile<T, DP> cols = tl;
+                        cols.forget();
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const frag p = to_frag<T>(w, half), ds = to_frag<T>(dp, half);
-                        frag rest_p, rest_ds;
-                        if (FINE) rest_p = to_frag<T>(low_w, half), rest_ds = to_frag<T>(low_dp, half);
-                        const int at = (qb * 32 + half * 16) * DP;
+                        for (int half = 0; half < 2; ++half) {
+                            const frag p = to_frag<T>(w, half), ds = to_frag<T>(dp, half);
+                            const int at = (qb * 32 + half * 16) * DP;
 #pragma unroll
-                        for (int n = 0; n < DP / 32; ++n) {
-                            const frag o = tl.columns(sdo[b] + at, n, lane);
-                            dv[n] = mma(o, p, dv[n]);
-                            if (FINE) dv[n] = mma(o, rest_p, dv[n]);
-                            const frag q = tl.columns(sq[b] + at, n, lane);
-                            dk[n] = mma(q, ds, dk[n]);
-                            if (FINE) dk[n] = mma(q, rest_ds, dk[n]);
+                            for (int n = 0; n < DP / 32; ++n) {
+                                dv[n] = mma(cols.columns(sdo[b] + at, n, lane), p, dv[n]);
+                                dk[n] = mma(cols.columns(sq[b] + at, n, lane), ds, dk[n]);
+                            }
                         }
                     }
                 }
@@ -657,14 +660,7 @@ struct Backward {
         AttnArgs k = a;
         k.slots = kslots;
         const dim3 keys((unsigned)kslots * a.scenes * a.kv_heads * g.parts);
-        if constexpr (sizeof(T) == 2) {
-            if (attention_few(a) && attention_fine(a))
-                hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED, true>), keys, dim3(256), 0, st, k, g);
-            else
-                hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED, false>), keys, dim3(256), 0, st, k, g);
-        } else {
-            hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED, false>), keys, dim3(256), 0, st, k, g);
-        }
+        hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED>), keys, dim3(256), 0, st, k, g);
         if (g.parts == 1 || a.k_tokens == 0) return;
         const int64_t fours = (int64_t)a.k_tokens * a.kv_heads * a.dim / 4;
         hipLaunchKernelGGL(k_parts_sum<T>, dim3((unsigned)((2 * fours + 255) / 256)), dim3(256), 0, st,

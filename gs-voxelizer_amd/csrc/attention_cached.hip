@@ -11,6 +11,9 @@
 // launch to the first bytes and a wave's few steps one after the other bound it.
 #include "gsv_attention.h"
 
+// (a product and a difference stay two roundings where they are written as two)
+#pragma clang fp contract(off)
+
 namespace gsv {
 namespace {
 
@@ -57,7 +60,9 @@ __global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const
 
     constexpr bool far = FAR, capped = CAPPED;
     const float slope = slope_of(a, h);
+    const bool fine = in_two_parts<T>(len);
     const float unit = capped ? kLog2e : a.scale * kLog2e;
+    const float left_unit = fine ? 1.f : unit;  // two parts: the largest weight is a power of two exactly
     const float far_unit = capped ? slope : slope / a.scale;
     const float in_cap = capped ? a.scale / a.cap : 0.f;
     frag q[DP / 16];
@@ -144,10 +149,13 @@ __global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const
             for (int r = 0; r < 16; ++r)
                 if (!(seen & (1u << result_row(r)))) w[r] = -INFINITY;
         }
+        if (fine)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) w[r] *= unit;
         float top = -INFINITY;
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, w[r]);
-        top *= unit;
+        top *= left_unit;
         if (__any(top > m + kSlack)) {
             const float next = fmaxf(m, fmaxf(top, other_half(top)));
             const float by = next == -INFINITY ? 1.f : fast_exp2(m - next);
@@ -159,15 +167,18 @@ __global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const
         const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            w[r] = fast_exp2(fmaf(w[r], unit, -ref));
+            w[r] = fast_exp2(fmaf(w[r], left_unit, -ref));
         }
+        for (int part = 0; part <= (fine ? 1 : 0); ++part) {
+            if (part) w = remainders<T>(w);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const frag p = to_frag<T>(w, half);
-            sum = add_weights(p, sum);
+            for (int half = 0; half < 2; ++half) {
+                const frag p = to_frag<T>(w, half);
+                sum = add_weights(p, sum);
 #pragma unroll
-            for (int e = 0; e < DP / 32; ++e)
-                o[e] = mma(at.columns(vt + half * 16 * DP, e, lane), p, o[e]);
+                for (int e = 0; e < DP / 32; ++e)
+                    o[e] = mma(at.columns(vt + half * 16 * DP, e, lane), p, o[e]);
+            }
         }
         if (more) put(b ^ 1);
     }

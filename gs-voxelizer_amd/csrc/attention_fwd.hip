@@ -55,6 +55,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
     const int nq = c.q1 - c.q0;
     const int tiles = (nq + kRows - 1) / kRows;
     const int group = a.heads / a.kv_heads;
+    const bool fine = in_two_parts<T>(c.k1 - c.k0);
     const T *kbase[KV], *vbase[KV];
 #pragma unroll
     for (int n = 0; n < KV; ++n) {
@@ -65,6 +66,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
     // scores leave the matrix product in units of 1 / scale (or 1 where they are capped);
     // unit turns them into powers of two
     const float unit = capped ? kLog2e : a.scale * kLog2e;
+    const float left_unit = fine ? 1.f : unit;  // two parts: as for float32 (kExact)
     const float in_cap = capped ? a.scale / a.cap : 0.f;
     float far_unit[HEADS];
 #pragma unroll
@@ -170,7 +172,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
                             for (int r = 0; r < 16; ++r)
                                 if (!(seen & (1u << result_row(r)))) w[n][r] = -INFINITY;
                     }
-                    if constexpr (kExact)
+                    if (kExact || fine)
 #pragma unroll
                         for (int n = 0; n < HEADS; ++n)
 #pragma unroll
@@ -182,7 +184,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
                         top[n] = -INFINITY;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) top[n] = fmaxf(top[n], w[n][r]);
-                        if (!kExact) top[n] *= unit;
+                        if (!kExact) top[n] *= left_unit;
                         grown |= top[n] > m[n] + kSlack;
                     }
                     if (__any(grown)) {
@@ -201,17 +203,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
                         const float ref = m[n] == -INFINITY ? 0.f : m[n];
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
-                            w[n][r] = fast_exp2(kExact ? w[n][r] - ref : fmaf(w[n][r], unit, -ref));
+                            w[n][r] = fast_exp2(kExact ? w[n][r] - ref : fmaf(w[n][r], left_unit, -ref));
                             if (TRAIN) exact[n] += w[n][r];
                         }
+                        for (int part = 0; part <= (fine ? 1 : 0); ++part) {
+                            if (part) w[n] = remainders<T>(w[n]);
+                            Tile<T, DP> cols = at;
+                            cols.forget();
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const frag p = to_frag<T>(w[n], half);
-                            sum[n] = add_weights(p, sum[n]);
-                            const T *vt = sv[b][SHARED ? 0 : n] + (kb * 32 + half * 16) * DP;
+                            for (int half = 0; half < 2; ++half) {
+                                const frag p = to_frag<T>(w[n], half);
+                                sum[n] = add_weights(p, sum[n]);
+                                const T *vt = sv[b][SHARED ? 0 : n] + (kb * 32 + half * 16) * DP;
 #pragma unroll
-                            for (int e = 0; e < DP / 32; ++e)
-                                o[n][e] = mma(at.columns(vt, e, lane), p, o[n][e]);
+                                for (int e = 0; e < DP / 32; ++e)
+                                    o[n][e] = mma(cols.columns(vt, e, lane), p, o[n][e]);
+                            }
                         }
                     }
                 }
@@ -247,7 +254,6 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_fwd_few(
     const AttnArgs a, T *__restrict__ out, T *__restrict__ out_low, float *__restrict__ lse) {
     constexpr int W = kFewWaves<T, DP>, KB = 32;
     constexpr bool far = FAR, capped = CAPPED;
-    const bool fine = sizeof(T) == 2 && attention_fine(a);
     typedef typename Elem<T>::frag frag;
     static_assert(4 * KB * DP * sizeof(T) >= 32 * DP * sizeof(float), "sums reuse the tiles");
     __shared__ __align__(1024) T tiles[W][4 * KB * DP];  // a wave's keys and values, two buffers
@@ -259,6 +265,7 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_fwd_few(
     const int s = rest % a.scenes, slot = rest / a.scenes;
     const Scene c = scene_rows(a, s);
     const int nq = c.q1 - c.q0, row_tiles = (nq + 31) / 32;
+    const bool fine = in_two_parts<T>(c.k1 - c.k0);
     const int hk = h / (a.heads / a.kv_heads);
     const T *kbase = static_cast<const T *>(a.k) + (int64_t)c.k0 * a.k_row + hk * a.k_head;
     const T *vbase = static_cast<const T *>(a.v) + (int64_t)c.k0 * a.v_row + hk * a.v_head;

@@ -83,6 +83,9 @@ template <typename T, int DP> struct Tile {
         const int i = lane & 15, r4 = 4 * g + (i >> 2);
         col_at = r4 * kRowBytes + ((((lane >> 3) & 2) + ((i & 3) >> 1)) ^ turn(r4)) * 16 + (i & 1) * 8;
     }
+    // Lets the compiler know nothing of the columns' offset, in a loop over the parts of the weights: it
+    // would form all their addresses before the loop, and keep them in registers there are not.
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(col_at)); }
     // An address in LDS, as a number.  A tile starts at a multiple of 1024 bytes, so a lane's part
     // `bits` from its first is (base + at) ^ bits or base + (at ^ bits).  The first form keeps one
     // register, the second one for each part and saves an instruction a read: 16,000 tokens, 64
@@ -217,19 +220,15 @@ inline bool attention_pairs(const AttnArgs &a) {
 }
 // Whether rows are so few that the waves of a workgroup share them and split the keys: below three
 // workgroups of 128 rows for four CUs.  8 heads of 64, one scene: 500 tokens forward 13 us so and 22
-// otherwise, 2,000 36 and 66, 4,000 118 and 110.  And for scenes of 32 tokens and fewer while their
-// workgroups fit the CUs in one round, for attention_fine: 64 scenes, 8 heads take 40 us so (forward and
-// backward) and 27 otherwise, below what the call's own launches take.
-inline bool attention_few(const AttnArgs &a) {
-    return attention_tiles(a, false) < 192 ||
-           ((int64_t)a.q_tokens <= (int64_t)32 * a.scenes && (int64_t)a.scenes * a.heads <= 512);
-}
-// Whether bfloat16 weights and ds enter the products of few rows in two parts: where a row sees too few
-// keys to average their roundings.  The gradients of scenes of two tokens are 0.0018 off (2-norm,
-// the rounding of the results) so and 0.0031 otherwise, of long ones 0.0017 and 0.0024; one scene of 2,000
-// tokens, 8 heads of 64 takes 39 us (forward), 70 (rows) and 40 (keys) otherwise and 46, 73 and 77 so.
-__host__ __device__ inline bool attention_fine(const AttnArgs &a) {
-    return (int64_t)a.q_tokens < (int64_t)128 * a.scenes;
+// otherwise, 2,000 36 and 66, 4,000 118 and 110.
+inline bool attention_few(const AttnArgs &a) { return attention_tiles(a, false) < 192; }
+// Whether a scene's bfloat16 weights and ds enter the products in two parts (16 bits): where its rows see
+// too few keys to average their roundings.  The gradients of scenes of two tokens are 0.0017 off (2-norm:
+// the rounding of the results) so and 0.0025 in one part, of 64 tokens 0.0017 and 0.0024.  Its own keys alone
+// decide, so that no other scene of the batch changes how exact it is.  500 scenes of 120 tokens, 8 heads
+// of 64: 78 us (forward) and 461 (training), in one part 67 and 445.
+template <typename T> __device__ __forceinline__ bool in_two_parts(int keys) {
+    return sizeof(T) == 2 && keys < 128;
 }
 // The waves of such a workgroup: as many as the LDS holds their tiles.
 template <typename T, int DP> constexpr int kFewWaves = DP * sizeof(T) > 256 ? 2 : 4;

@@ -59,3 +59,98 @@ def test_one_head_of_an_odd_width(device, route, dtype):
     q, k, v = (t.as_strided((30, 1, 64), (72, 5, 1)) for t in wide)
     got = attention.scene_attention(q, k, v)
     assert torch.equal(got, attention.scene_attention(q.clone(), k.clone(), v.clone()))
+
+
+# ---- scenes of few keys: two parts of bfloat16 carry the weights and ds, whatever the batch holds
+
+
+def _case(device, dtype, lengths, H, K, D, key_lengths=None, bias=True, causal=False, cap=0.0, seed=0,
+          offset=0.0, spread=40.0):
+    g = _gen(device, seed)
+    T, N = sum(lengths), sum(key_lengths or lengths)
+
+    def normal(*shape):
+        return torch.randn(shape, generator=g, device=device).to(dtype)
+
+    def starts(ls):
+        return torch.tensor([0] + ls, device=device).cumsum(0).int()
+
+    c = dict(q=normal(T, H, D), k=normal(N, K, D), v=normal(N, K, D), dout=normal(T, H, D),
+             q_starts=starts(lengths), k_starts=starts(key_lengths) if key_lengths else None,
+             causal=causal, cap=cap)
+    if bias:
+        c["q_positions"] = offset + spread * torch.rand(T, 3, generator=g, device=device)
+        c["k_positions"] = (offset + spread * torch.rand(N, 3, generator=g, device=device)
+                            if key_lengths else c["q_positions"])
+        c["slopes"] = torch.tensor([2.0 ** -(h + 1) for h in range(H)], device=device).to(dtype)
+    return c
+
+
+def _run(c, **more):
+    names = [n for n in ("q", "k", "v", "slopes") if n in c]
+    v = {n: c[n].detach().clone().requires_grad_() for n in names}
+    out = attention.scene_attention(
+        v["q"], v["k"], v["v"], scene_starts=c["q_starts"], key_starts=c["k_starts"],
+        causal=c["causal"], prefix=c.get("prefix"), cap=c["cap"], positions=c.get("q_positions"),
+        key_positions=c.get("k_positions"), slopes=v.get("slopes"), keep=c.get("keep"), **more)
+    got = torch.autograd.grad(out, list(v.values()), c["dout"])
+    return {"out": out.detach(), **{"d" + n: g for n, g in zip(names, got)}}
+
+
+def _off(got, want):
+    """How far off in the 2-norm, against the value's."""
+    return float((got.double() - want).norm() / want.norm().clamp_min(1e-30))
+
+
+def _assert_rounded_once(got, want, what):
+    """As exact as its own type, in the 2-norm: what the rounding of the exact values to bfloat16 takes, and
+    a tenth of it (other values round elsewhere); weights, ds and out enter the products with 16 bits, 2^-17
+    of each term, times what cancels in ds (2^4 here).  One part of 8 bits there adds as much
+    again as the rounding, in quadrature: 1.4 of it."""
+    once = _off(want.to(BF16), want)
+    assert _off(got, want) <= 1.1 * once + 2.0 ** -13, (what, _off(got, want), once)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (50.0, True)])
+@pytest.mark.parametrize("lengths,key_lengths", [
+    ([2] * 64, None), ([2] * 65, None), ([2, 3] * 100, None), ([64] * 5, None), ([64] * 40, None),
+    ([127, 1] * 30, None), ([200] * 2, [2] * 2), ([400] * 20, [3, 100] * 10)],
+    ids=["2x64", "2x65", "2,3x100", "64x5", "64x40", "127,1x30", "200q2k", "400q3k"])
+def test_scenes_of_few_keys_in_any_batch(device, dim, cap, bias, lengths, key_lengths):
+    c = _case(device, BF16, lengths, 8, 2, dim, key_lengths=key_lengths, bias=bias, cap=cap)
+    got, want = _run(c), R.attention(**c)[0]
+    for n in ("out", "dq", "dk", "dv"):
+        _assert_rounded_once(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("others", [[], [5000], [300] * 30], ids=["alone", "long", "many"])
+def test_a_short_scene_is_as_exact_beside_any_others(device, dim, others):
+    c = _case(device, BF16, [2] * 9 + others, 8, 8, dim)
+    got, want = _run(c), R.attention(**c)[0]
+    for n in ("out", "dq", "dk", "dv"):
+        _assert_rounded_once(got[n][:18], want[n][:18], n)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (50.0, True)])
+def test_short_caches(device, dim, cap, bias):
+    """Caches of few live rows beside a long one; one row's value comes out as it is."""
+    g, lengths, N = _gen(device, 3), [1, 2, 3, 9, 60, 127, 3000], 3000
+    S, H, K = len(lengths), 8, 2
+    q = torch.randn(S, H, dim, generator=g, device=device).to(BF16)
+    k, v = (torch.randn(S, N, K, dim, generator=g, device=device).to(BF16) for _ in "kv")
+    more = {}
+    if bias:
+        more = dict(positions=40 * torch.rand(S, 3, generator=g, device=device),
+                    key_positions=40 * torch.rand(S, N, 3, generator=g, device=device),
+                    slopes=torch.tensor([2.0 ** -(h + 1) for h in range(H)], device=device).to(BF16))
+    got = attention.cached_attention(q, k, v, torch.tensor(lengths, dtype=torch.int32, device=device),
+                                     cap=cap, **more)
+    assert torch.equal(got[0], v[0, 0].repeat_interleave(H // K, 0))
+    for s, n in enumerate(lengths[:-1]):
+        ref = dict(q_positions=more["positions"][s:s + 1], k_positions=more["key_positions"][s, :n],
+                   slopes=more["slopes"]) if bias else {}
+        want = R.attention(q[s:s + 1], k[s, :n], v[s, :n], cap=cap, **ref)[0]["out"]
+        _assert_rounded_once(got[s:s + 1], want, n)
