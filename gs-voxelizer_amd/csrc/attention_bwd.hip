@@ -32,9 +32,9 @@ struct BwdArgs {
     int64_t dout_row, dout_head;
     const float *lse;
     float *delta;   // (heads, q_tokens)
-    double *dslope;  // (slots * scenes, heads) partial sums
+    double *dslope;  // (heads, n_slopes) partial sums
     void *dslopes;
-    int n_slopes;    // slots * scenes
+    int n_slopes;    // the rows' places
     void *dq, *dk, *dv;
     int parts;             // workgroups that share a key tile's rows
     float *part_k, *part_v;  // (parts, k_tokens, kv_heads, dim) partial sums, with parts > 1
@@ -67,9 +67,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
     __shared__ double sums[4];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = blockIdx.x % a.heads, rest = blockIdx.x / a.heads;
-    const int s = rest % a.scenes, slot = rest / a.scenes;
-    const Scene c = scene_rows(a, s);
+    const int h = blockIdx.x % a.heads, place_n = grid_place(a.heads);
+    if (place_n >= a.places) return;
+    const Place where = tile_place<kRows>(a.q_starts, a.scenes, a.q_tokens, place_n, a.slots);
+    const Scene c = scene_of(a, where.scene, true);
     const int nq = c.q1 - c.q0;
     const int tiles = (nq + kRows - 1) / kRows;
     const bool fine = in_two_parts<T>(c.k1 - c.k0);
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
     ck.plan(a.k_row, a.dim, wave, lane);
     cv.plan(a.v_row, a.dim, wave, lane);
 
-    for (int tile = slot; tile < tiles; tile += a.slots) {
+    for (int tile = where.tile; tile < tiles; tile += where.step) {
         const int first = (tiles - 1 - tile) * kRows;
         const int i = first + wave * 32 + (lane & 31);
         const bool row = i < nq;
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
     if (lane == 0) sums[wave] = dslope;
     __syncthreads();
     if (threadIdx.x == 0)
-        g.dslope[(int64_t)rest * a.heads + h] = sums[0] + sums[1] + sums[2] + sums[3];
+        g.dslope[(int64_t)h * a.places + place_n] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
 // The same for few rows: 32 of them for a workgroup, whose waves take every W-th tile of 32 keys, as
@@ -248,9 +249,10 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
     __shared__ double sums[W];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = blockIdx.x % a.heads, group_at = blockIdx.x / a.heads;
-    const int s = group_at % a.scenes, slot = group_at / a.scenes;
-    const Scene c = scene_rows(a, s);
+    const int h = blockIdx.x % a.heads, place_n = grid_place(a.heads);
+    if (place_n >= a.places) return;
+    const Place where = tile_place<32>(a.q_starts, a.scenes, a.q_tokens, place_n, a.slots);
+    const Scene c = scene_of(a, where.scene, true);
     const int nq = c.q1 - c.q0, row_tiles = (nq + 31) / 32;
     const bool fine = in_two_parts<T>(c.k1 - c.k0);  // ds, as the forward's weights
     const int hk = h / (a.heads / a.kv_heads);
@@ -267,7 +269,7 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
     ck.plan(a.k_row, a.dim, 0, lane);
     cv.plan(a.v_row, a.dim, 0, lane);
 
-    for (int tile = slot; tile < row_tiles; tile += a.slots) {
+    for (int tile = where.tile; tile < row_tiles; tile += where.step) {
         const int first = (row_tiles - 1 - tile) * 32, i = first + (lane & 31);
         const bool row = i < nq;
         const int64_t qi = c.q0 + i;
@@ -435,7 +437,7 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
         double sum = 0.0;
 #pragma unroll
         for (int w = 0; w < W; ++w) sum += sums[w];
-        g.dslope[(int64_t)group_at * a.heads + h] = sum;
+        g.dslope[(int64_t)h * a.places + place_n] = sum;
     }
 }
 
@@ -452,9 +454,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hk = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads % g.parts;
-    const int rest = blockIdx.x / a.kv_heads / g.parts;
-    const int s = rest % a.scenes, slot = rest / a.scenes;
-    const Scene c = scene_rows(a, s);
+    const int place_n = grid_place(a.kv_heads * g.parts);
+    if (place_n >= a.places) return;
+    const Place where = tile_place<kRows>(a.k_starts, a.scenes, a.k_tokens, place_n, a.slots);
+    const Scene c = scene_of(a, where.scene, false);
     const int nq = c.q1 - c.q0, nk = c.k1 - c.k0, off = nk - nq;
     const int group = a.heads / a.kv_heads;
     const int tiles = (nk + kRows - 1) / kRows;
@@ -470,10 +473,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
     cd.plan(g.dout_row, a.dim, wave, lane);
 
     // the rows' kernel has ended: a head's partial sums of dslope, in order
-    if (far && rest == 0 && part == 0)
+    if (far && place_n == 0 && part == 0)
         for (int h = hk * group + wave; h < (hk + 1) * group; h += WAVES) {
             double sum = 0.0;
-            for (int n = lane; n < g.n_slopes; n += 64) sum += g.dslope[(int64_t)n * a.heads + h];
+#pragma unroll 8
+            for (int n = lane; n < g.n_slopes; n += 64) sum += g.dslope[(int64_t)h * g.n_slopes + n];
 #pragma unroll
             for (int n = 1; n < 64; n <<= 1) sum += __shfl_xor(sum, n);
             if (lane == 0) {
@@ -482,7 +486,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
             }
         }
 
-    for (int tile = slot; tile < tiles; tile += a.slots) {
+    for (int tile = where.tile; tile < tiles; tile += where.step) {
         const int first = tile * kRows;
         const int j = first + wave * 32 + (lane & 31);
         const int64_t kj = c.k0 + j;
@@ -645,30 +649,6 @@ __global__ __launch_bounds__(256) void k_parts_sum(const float *__restrict__ pk,
     reinterpret_cast<t4 *>(second ? dv : dk)[at] = r;
 }
 
-struct Backward {
-    const AttnArgs &a;
-    const BwdArgs &g;
-    int kslots;
-    hipStream_t st;
-    template <typename T, int DP, bool FAR, bool CAPPED> void run() const {
-        const dim3 grid((unsigned)a.slots * a.scenes * a.heads);
-        if (a.q_tokens > 0 && attention_few(a))
-            hipLaunchKernelGGL((k_attention_dq_few<T, DP, FAR, CAPPED>), grid,
-                               dim3(64 * kFewWaves<T, DP>), 0, st, a, g);
-        else if (a.q_tokens > 0)
-            hipLaunchKernelGGL((k_attention_dq<T, DP, FAR, CAPPED>), grid, dim3(256), 0, st, a, g);
-        AttnArgs k = a;
-        k.slots = kslots;
-        const dim3 keys((unsigned)kslots * a.scenes * a.kv_heads * g.parts);
-        hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED>), keys, dim3(256), 0, st, k, g);
-        if (g.parts == 1 || a.k_tokens == 0) return;
-        const int64_t fours = (int64_t)a.k_tokens * a.kv_heads * a.dim / 4;
-        hipLaunchKernelGGL(k_parts_sum<T>, dim3((unsigned)((2 * fours + 255) / 256)), dim3(256), 0, st,
-                           g.part_k, g.part_v, g.parts, fours, static_cast<T *>(g.dk),
-                           static_cast<T *>(g.dv));
-    }
-};
-
 size_t delta_bytes(const AttnArgs &a) {
     return ((size_t)a.heads * a.q_tokens * sizeof(float) + 255) / 256 * 256;
 }
@@ -676,7 +656,7 @@ size_t delta_bytes(const AttnArgs &a) {
 // Parts of a key tile's rows: more workgroups where the tiles alone leave CUs idle or, as under a
 // causal mask, a few of them have most of the work.  About four rounds of workgroups at one a CU
 // (128 channels), one at two a CU; eight parts at most, each with four tiles of a mean scene's
-// rows at least (sizes alone decide: the longest scene's length is a hint that may change no bit).
+// rows at least (sizes alone decide: the longest scene's length is a hint that changes no sum of these).
 // Partial sums then pass through memory: 10,007 tokens of 4 causal scenes, 16 heads on 4, 128
 // channels take 945 us in one part and 770 in four; 8 heads of 64, 8,001 tokens gain nothing.
 int bwd_parts(const AttnArgs &a, int elem) {
@@ -691,16 +671,48 @@ size_t parts_bytes(const AttnArgs &a, int parts) {
     return parts == 1 ? 0 : sizeof(float) * parts * a.k_tokens * a.kv_heads * a.dim;  // of 32 bytes each
 }
 
-int bwd_plan(const gsv_attention *args, AttnArgs *a, int *kslots, int *parts) {
-    int lq, lk;
-    const int st = attention_args(args, a, &lq, &lk);
+// The two launches: of the rows' places (a->places, a->slots) and of the keys' in their parts.
+struct BwdPlan {
+    dim3 rows, keys;
+    int key_places, key_slots, parts;
+};
+int bwd_plan(const gsv_attention *args, AttnArgs *a, BwdPlan *p) {
+    const int st = attention_args(args, a);
     if (st != GSV_OK) return st;
-    *parts = bwd_parts(*a, args->dtype);
-    if (!attention_slots(a, lk, kRows, a->kv_heads * *parts)) return GSV_ERR_SIZE_OVERFLOW;
-    *kslots = a->slots;
+    p->parts = bwd_parts(*a, args->dtype);
     const int rows = attention_few(*a) ? 32 : kRows;
-    return attention_slots(a, lq, rows, a->heads) ? GSV_OK : GSV_ERR_SIZE_OVERFLOW;
+    const int64_t slots = attention_slots(*a, a->q_tokens, args->longest_q, rows);
+    const int64_t key_slots = attention_slots(*a, a->k_tokens, args->longest_k, kRows);
+    const int64_t places = attention_places(*a, a->q_tokens, rows, slots);
+    const int64_t key_places = attention_places(*a, a->k_tokens, kRows, key_slots);
+    a->slots = (int)slots, a->places = (int)places;
+    p->key_slots = (int)key_slots, p->key_places = (int)key_places;
+    return attention_grid(places, a->heads, &p->rows) &&
+                   attention_grid(key_places, (int64_t)a->kv_heads * p->parts, &p->keys)
+               ? GSV_OK : GSV_ERR_SIZE_OVERFLOW;
 }
+
+struct Backward {
+    const AttnArgs &a;
+    const BwdArgs &g;
+    const BwdPlan &plan;
+    hipStream_t st;
+    template <typename T, int DP, bool FAR, bool CAPPED> void run() const {
+        if (a.q_tokens > 0 && attention_few(a))
+            hipLaunchKernelGGL((k_attention_dq_few<T, DP, FAR, CAPPED>), plan.rows,
+                               dim3(64 * kFewWaves<T, DP>), 0, st, a, g);
+        else if (a.q_tokens > 0)
+            hipLaunchKernelGGL((k_attention_dq<T, DP, FAR, CAPPED>), plan.rows, dim3(256), 0, st, a, g);
+        AttnArgs k = a;
+        k.slots = plan.key_slots, k.places = plan.key_places;
+        hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED>), plan.keys, dim3(256), 0, st, k, g);
+        if (g.parts == 1 || a.k_tokens == 0) return;
+        const int64_t fours = (int64_t)a.k_tokens * a.kv_heads * a.dim / 4;
+        hipLaunchKernelGGL(k_parts_sum<T>, dim3((unsigned)((2 * fours + 255) / 256)), dim3(256), 0, st,
+                           g.part_k, g.part_v, g.parts, fours, static_cast<T *>(g.dk),
+                           static_cast<T *>(g.dv));
+    }
+};
 
 }  // namespace
 }  // namespace gsv
@@ -709,12 +721,12 @@ using namespace gsv;
 
 extern "C" int gsv_attention_bwd_workspace_bytes(const gsv_attention *args, size_t *bytes) {
     AttnArgs a;
-    int kslots, parts;
+    BwdPlan plan;
     if (!bytes) return GSV_ERR_INVALID_ARGUMENT;
-    const int st = bwd_plan(args, &a, &kslots, &parts);
+    const int st = bwd_plan(args, &a, &plan);
     if (st != GSV_OK) return st;
-    *bytes = delta_bytes(a) + 2 * parts_bytes(a, parts) +
-             (a.slopes ? sizeof(double) * a.slots * a.scenes * a.heads : 0);
+    *bytes = delta_bytes(a) + 2 * parts_bytes(a, plan.parts) +
+             (a.slopes ? sizeof(double) * a.places * a.heads : 0);
     return GSV_OK;
 }
 
@@ -723,9 +735,9 @@ extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, con
                                  void *dk, void *dv, void *dslopes, void *workspace,
                                  size_t workspace_bytes, void *stream) {
     AttnArgs a;
-    int kslots, parts;
+    BwdPlan plan;
     size_t need;
-    int st = bwd_plan(args, &a, &kslots, &parts);
+    int st = bwd_plan(args, &a, &plan);
     if (st != GSV_OK) return st;
     if ((st = gsv_attention_bwd_workspace_bytes(args, &need)) != GSV_OK) return st;
     if (need > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
@@ -743,12 +755,11 @@ extern "C" int gsv_attention_bwd(const gsv_attention *args, const void *out, con
     float *delta = static_cast<float *>(workspace);
     char *next = static_cast<char *>(workspace) + delta_bytes(a);
     float *part_k = reinterpret_cast<float *>(next);
-    float *part_v = reinterpret_cast<float *>(next + parts_bytes(a, parts));
-    double *slopes = reinterpret_cast<double *>(next + 2 * parts_bytes(a, parts));
+    float *part_v = reinterpret_cast<float *>(next + parts_bytes(a, plan.parts));
+    double *slopes = reinterpret_cast<double *>(next + 2 * parts_bytes(a, plan.parts));
     const BwdArgs g{out, out_low, dout, dout_row, dout_head, lse, delta, slopes, dslopes,
-                    a.q_tokens > 0 ? a.slots * a.scenes : 0, dq, dk, dv, parts, part_k, part_v};
-    hipStream_t s = as_stream(stream);
-    Backward f{a, g, kslots, s};
+                    a.q_tokens > 0 ? a.places : 0, dq, dk, dv, plan.parts, part_k, part_v};
+    Backward f{a, g, plan, as_stream(stream)};
     attention_variant(a, args->dtype, f);
     return check_launch();
 }

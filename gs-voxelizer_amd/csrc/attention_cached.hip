@@ -285,13 +285,12 @@ struct Cached {
 };
 
 int cached_plan(const gsv_attention *args, AttnArgs *a, int *head_tiles, int *splits) {
-    int lq, lk;
     if (!args || args->causal || args->prefix || args->q_starts || args->k_starts ||
         args->scenes < 0 || args->scenes != args->q_tokens)
         return GSV_ERR_INVALID_ARGUMENT;
     gsv_attention one = *args;
     one.scenes = 1;  // rows are addressed by scene here, not packed
-    const int st = attention_args(&one, a, &lq, &lk);
+    const int st = attention_args(&one, a);
     if (st != GSV_OK) return st;
     a->scenes = args->scenes;
     const int64_t tiles = (a->heads / a->kv_heads + kHeads - 1) / kHeads;

@@ -46,12 +46,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
     __shared__ __align__(16) typename Places<T>::Row spos[2][3 * KB];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // heads vary fastest: with eight (or a multiple) of them each XCD's L2 holds the keys
-    // of its own heads
     const int sets = a.heads / HEADS;
-    const int h0 = blockIdx.x % sets * HEADS, rest = blockIdx.x / sets;
-    const int s = rest % a.scenes, slot = rest / a.scenes;
-    const Scene c = scene_rows(a, s);
+    const int h0 = blockIdx.x % sets * HEADS, place_n = grid_place(sets);
+    if (place_n >= a.places) return;
+    const Place where = tile_place<kRows>(a.q_starts, a.scenes, a.q_tokens, place_n, a.slots);
+    const Scene c = scene_of(a, where.scene, true);
     const int nq = c.q1 - c.q0;
     const int tiles = (nq + kRows - 1) / kRows;
     const int group = a.heads / a.kv_heads;
@@ -77,7 +76,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
     ck.plan(a.k_row, a.dim, wave, lane);
     cv.plan(a.v_row, a.dim, wave, lane);
 
-    for (int tile = slot; tile < tiles; tile += a.slots) {
+    for (int tile = where.tile; tile < tiles; tile += where.step) {
         // the last rows of a causal scene see the most keys: they start first
         const int first = (tiles - 1 - tile) * kRows;
         const int i = first + wave * 32 + (lane & 31);
@@ -261,9 +260,10 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_fwd_few(
     __shared__ float sm[W][32], ss[W][32], se[W][32];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = blockIdx.x % a.heads, rest = blockIdx.x / a.heads;
-    const int s = rest % a.scenes, slot = rest / a.scenes;
-    const Scene c = scene_rows(a, s);
+    const int h = blockIdx.x % a.heads, place_n = grid_place(a.heads);
+    if (place_n >= a.places) return;
+    const Place where = tile_place<32>(a.q_starts, a.scenes, a.q_tokens, place_n, a.slots);
+    const Scene c = scene_of(a, where.scene, true);
     const int nq = c.q1 - c.q0, row_tiles = (nq + 31) / 32;
     const bool fine = in_two_parts<T>(c.k1 - c.k0);
     const int hk = h / (a.heads / a.kv_heads);
@@ -279,7 +279,7 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_fwd_few(
     ck.plan(a.k_row, a.dim, 0, lane);
     cv.plan(a.v_row, a.dim, 0, lane);
 
-    for (int tile = slot; tile < row_tiles; tile += a.slots) {
+    for (int tile = where.tile; tile < row_tiles; tile += where.step) {
         const int first = (row_tiles - 1 - tile) * 32, i = first + (lane & 31);
         const bool row = i < nq;
         const int64_t qi = c.q0 + i;
@@ -443,12 +443,16 @@ struct Forward {
     float *lse;
     hipStream_t st;
     int status;
+    bool plan(int rows, int heads, dim3 *grid) {
+        const int64_t slots = attention_slots(a, a.q_tokens, longest, rows);
+        const int64_t places = attention_places(a, a.q_tokens, rows, slots);
+        a.slots = (int)slots, a.places = (int)places;
+        status = attention_grid(places, heads, grid) ? GSV_OK : GSV_ERR_SIZE_OVERFLOW;
+        return status == GSV_OK;
+    }
     template <typename T, int DP, bool FAR, bool CAPPED, int HEADS, bool SHARED> void start() {
-        if (!attention_slots(&a, longest, kRows, a.heads)) {
-            status = GSV_ERR_SIZE_OVERFLOW;
-            return;
-        }
-        const dim3 grid((unsigned)a.slots * a.scenes * (a.heads / HEADS));
+        dim3 grid;
+        if (!plan(kRows, a.heads / HEADS, &grid)) return;
         T *o = static_cast<T *>(out), *low = static_cast<T *>(out_low);
         if (lse)
             hipLaunchKernelGGL((k_attention_fwd<T, DP, FAR, CAPPED, HEADS, SHARED, true>), grid,
@@ -459,11 +463,8 @@ struct Forward {
         status = check_launch();
     }
     template <typename T, int DP, bool FAR, bool CAPPED> void few() {
-        if (!attention_slots(&a, longest, 32, a.heads)) {
-            status = GSV_ERR_SIZE_OVERFLOW;
-            return;
-        }
-        const dim3 grid((unsigned)a.slots * a.scenes * a.heads), block(64 * kFewWaves<T, DP>);
+        dim3 grid, block(64 * kFewWaves<T, DP>);
+        if (!plan(32, a.heads, &grid)) return;
         T *o = static_cast<T *>(out), *low = static_cast<T *>(out_low);
         if (lse)
             hipLaunchKernelGGL((k_attention_fwd_few<T, DP, FAR, CAPPED, true>), grid, block, 0, st, a, o, low, lse);
@@ -486,14 +487,15 @@ struct Forward {
 
 }  // namespace
 
-int attention_args(const gsv_attention *in, AttnArgs *a, int *longest_q, int *longest_k) {
+int attention_args(const gsv_attention *in, AttnArgs *a) {
     if (!in) return GSV_ERR_INVALID_ARGUMENT;
     const gsv_attention &g = *in;
     if (g.dtype != GSV_F32 && g.dtype != GSV_BF16) return GSV_ERR_INVALID_ARGUMENT;
     if (g.q_tokens < 0 || g.k_tokens < 0 || g.heads < 1 || g.kv_heads < 1 ||
         g.heads % g.kv_heads || g.dim < 8 || g.dim > 128 || g.dim % 8 || g.scenes < 1)
         return GSV_ERR_INVALID_ARGUMENT;
-    if (g.q_tokens > GSV_MAX_TOKENS || g.k_tokens > GSV_MAX_TOKENS) return GSV_ERR_SIZE_OVERFLOW;
+    if (g.q_tokens > GSV_MAX_TOKENS || g.k_tokens > GSV_MAX_TOKENS || g.scenes > (1 << 29))
+        return GSV_ERR_SIZE_OVERFLOW;
     const int64_t chunk = g.dtype == GSV_BF16 ? 8 : 4;
     const int64_t q_row = used_stride(g.q_row, g.q_tokens), q_head = used_stride(g.q_head, g.heads);
     const int64_t k_row = used_stride(g.k_row, g.k_tokens), k_head = used_stride(g.k_head, g.kv_heads);
@@ -517,12 +519,7 @@ int attention_args(const gsv_attention *in, AttnArgs *a, int *longest_q, int *lo
                   g.q_tokens, g.k_tokens, g.heads, g.kv_heads, g.dim, g.scenes, g.q_starts,
                   g.k_starts, g.prefix, g.causal, g.scale, g.cap, g.q_positions, g.k_positions,
                   g.q_pos_row, g.k_pos_row, g.slopes, g.slopes_dtype == GSV_F32, g.keep,
-                  g.keep_bytes, 1};
-    const auto longest = [](int hint, int tokens) {
-        return hint < 1 || hint > tokens ? (tokens > 1 ? tokens : 1) : hint;
-    };
-    *longest_q = longest(g.longest_q, g.q_tokens);
-    *longest_k = longest(g.longest_k, g.k_tokens);
+                  g.keep_bytes, 0, 0};
     return GSV_OK;
 }
 
@@ -533,12 +530,11 @@ using namespace gsv;
 extern "C" int gsv_attention_fwd(const gsv_attention *args, void *out, void *out_low, float *lse,
                                  void *stream) {
     AttnArgs a;
-    int lq, lk;
-    const int st = attention_args(args, &a, &lq, &lk);
+    const int st = attention_args(args, &a);
     if (st != GSV_OK) return st;
     if (a.q_tokens == 0) return GSV_OK;
     if (!out || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(out_low) % 16) return GSV_ERR_INVALID_ARGUMENT;
-    Forward f{a, lq, out, out_low, lse, as_stream(stream), GSV_OK};
+    Forward f{a, args->longest_q, out, out_low, lse, as_stream(stream), GSV_OK};
     attention_variant(a, args->dtype, f);
     return f.status;
 }

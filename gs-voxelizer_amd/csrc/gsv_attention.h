@@ -178,14 +178,15 @@ struct AttnArgs {
     int slopes_f32;
     const void *keep;
     int keep_bytes;
-    int slots;  // workgroups a scene and head: they take its tiles in turn
+    int places;  // workgroups for each head
+    int slots;   // places a scene where they go by scene, 0 where they are tiles (tile_place)
 };
 
 // The stride of an axis of one entry is never used, whatever a caller's view holds there.
 inline int64_t used_stride(int64_t stride, int64_t entries) { return entries > 1 ? stride : 0; }
 
-// Checks the C arguments and lays them out for a launch; longest_*: rows of the longest scene.
-int attention_args(const gsv_attention *in, AttnArgs *a, int *longest_q, int *longest_k);
+// Checks the C arguments and lays them out for a launch.
+int attention_args(const gsv_attention *in, AttnArgs *a);
 
 // The kernel variant of a call: element type, channels (up to 32, 64 or 128; the columns past
 // dim are zeros), distance bias, score cap.
@@ -206,8 +207,7 @@ template <typename F> void attention_variant(const AttnArgs &a, int dtype, F &f)
     else attention_channels<float>(a, f);
 }
 
-// Workgroups of 128 rows of one head, a mean scene's and all scenes' (sizes alone decide which kernel
-// runs: the longest scene's length is a hint that may change no bit).
+// Workgroups of 128 rows of one head, a mean scene's and all scenes'.
 inline int64_t attention_tiles(const AttnArgs &a, bool mean) {
     const int64_t each = (int64_t)a.q_tokens / a.scenes / 128 * a.heads;
     return mean ? each : ((int64_t)a.q_tokens / 128 + a.scenes) * a.heads;
@@ -233,13 +233,27 @@ template <typename T> __device__ __forceinline__ bool in_two_parts(int keys) {
 // The waves of such a workgroup: as many as the LDS holds their tiles.
 template <typename T, int DP> constexpr int kFewWaves = DP * sizeof(T) > 256 ? 2 : 4;
 
-// Workgroups for each scene and head: one for each tile of the longest scene, fewer where the
-// launch would pass a million (they take the tiles in turn, so any number is right).
-inline bool attention_slots(AttnArgs *a, int longest, int rows, int heads) {
-    const int64_t each = (int64_t)a->scenes * heads;
-    if (each > (1 << 24) - 1) return false;
-    a->slots = (int)imin64((longest + rows - 1) / rows, imax64((1 << 20) / each, 1));
-    return true;
+// Places a scene of one side where fewer workgroups come of it than of its tiles (tile_place), else 0.
+// longest: rows of the longest scene, if known; places go by it, and no result.
+inline int64_t attention_slots(const AttnArgs &a, int tokens, int longest, int rows) {
+    if (longest < 1 || longest > tokens) return 0;
+    const int64_t slots = (longest + rows - 1) / rows;
+    return slots * a.scenes < (int64_t)tokens / rows + a.scenes ? slots : 0;
+}
+inline int64_t attention_places(const AttnArgs &a, int tokens, int rows, int64_t slots) {
+    return slots ? slots * a.scenes : (int64_t)tokens / rows + a.scenes;
+}
+// A launch of a workgroup for each place and `each` heads (or parts of them), which vary fastest: with
+// eight (or a multiple) of them each XCD's L2 holds the keys of its own heads.  The places past
+// four million workgroups are the grid's y axis.  False where that would pass its limit.
+inline bool attention_grid(int64_t places, int64_t each, dim3 *grid) {
+    if (each > (1 << 22)) return false;
+    const int64_t x = imin64(places, (1 << 22) / each), y = (places + x - 1) / x;
+    *grid = dim3((unsigned)(x * each), (unsigned)y);
+    return y <= 65535;
+}
+__device__ __forceinline__ int grid_place(int each) {
+    return blockIdx.y * (gridDim.x / each) + blockIdx.x / each;
 }
 
 // One scene's rows.  Starts are clamped to the arrays, the first scene begins at row 0
@@ -252,13 +266,57 @@ __device__ __forceinline__ int scene_start(const int *starts, int s, int scenes,
     if (s >= scenes) return tokens;
     return min(max(starts[s], 0), tokens);
 }
-__device__ __forceinline__ Scene scene_rows(const AttnArgs &a, int s) {
-    Scene c;
-    c.q0 = scene_start(a.q_starts, s, a.scenes, a.q_tokens);
-    c.q1 = max(scene_start(a.q_starts, s + 1, a.scenes, a.q_tokens), c.q0);
-    c.k0 = scene_start(a.k_starts, s, a.scenes, a.k_tokens);
-    c.k1 = max(scene_start(a.k_starts, s + 1, a.scenes, a.k_tokens), c.k0);
-    c.prefix = a.prefix ? min(max(a.prefix[s], 0), c.k1 - c.k0) : 0;
+// Scene s and its rows first .. last - 1 of one side.
+struct Span {
+    int s, first, last;
+};
+__device__ __forceinline__ Span span(const int *starts, int s, int scenes, int tokens) {
+    const int first = __builtin_amdgcn_readfirstlane(scene_start(starts, s, scenes, tokens));
+    return {s, first, max(__builtin_amdgcn_readfirstlane(scene_start(starts, s + 1, scenes, tokens)), first)};
+}
+// What a workgroup does on one side: of a scene's tiles of ROWS rows, `tile` and every `step` further.
+struct Place {
+    Span scene;
+    int tile, step;
+};
+// By tiles (slots 0), scene after scene: scene s has those from first / ROWS + s on.  That leaves it one
+// for each ROWS rows it begins, and often one without rows; a launch then needs to know nothing of the
+// scenes but their number, however their lengths differ, and a scene's longest rows start first.  The scene of
+// a place is looked for among the 64 around where it is if all have one length, by one load, and past
+// those by a search.  By slots, a scene has as many as its launch gives each.
+// Training, 8 heads of 64: 500 scenes of 128 tokens take 453 us in one slot each and 756 by tiles, of
+// which half are without rows (and 5,674 in slots for as many rows as there are); one scene of
+// 16,000 beside 999 of 10 takes 4.1 ms by tiles, and 20 in 125 slots each.
+template <int ROWS>
+__device__ __forceinline__ Place tile_place(const int *starts, int scenes, int tokens, int n, int slots) {
+    if (slots) return {span(starts, n % scenes, scenes, tokens), n / scenes, slots};
+    constexpr int kOnce = 1 << 30;
+    if (scenes == 1) return {{0, 0, tokens}, n, kOnce};
+    const int lane = threadIdx.x & 63;
+    const int guess = (int)((float)n * ((float)scenes / (float)(tokens / ROWS + scenes)));
+    const int lo = __builtin_amdgcn_readfirstlane(max(min(guess - 32, scenes - 64), 0));
+    const int start = scene_start(starts, lo + lane, scenes, tokens);
+    int at = __popcll(__ballot(lo + lane < scenes && start / ROWS + lo + lane <= n));
+    Span s;
+    if ((at == 0 && lo > 0) || (at == 64 && lo + 64 < scenes)) {
+        const auto before = [&](int s) { return scene_start(starts, s, scenes, tokens) / ROWS + s; };
+        s = span(starts, last_at_most(scenes, n, before), scenes, tokens);
+    } else {
+        at = __builtin_amdgcn_readfirstlane(max(at, 1));
+        const int first = __builtin_amdgcn_readlane(start, at - 1);
+        const int last = at < 64 ? __builtin_amdgcn_readlane(start, at) : tokens;
+        s = {lo + at - 1, first, max(last, first)};
+    }
+    const int tile = n - (s.first / ROWS + s.s);
+    return {s, tile >= 0 ? tile : kOnce, kOnce};  // (below 0 only where starts do not ascend)
+}
+// The scene whose rows of one side are known; the other side's are the same where both have the same starts.
+__device__ __forceinline__ Scene scene_of(const AttnArgs &a, const Span &p, bool queries) {
+    const bool same = a.q_starts == a.k_starts && a.q_tokens == a.k_tokens;
+    const Span q = queries || same ? p : span(a.q_starts, p.s, a.scenes, a.q_tokens);
+    const Span k = !queries || same ? p : span(a.k_starts, p.s, a.scenes, a.k_tokens);
+    Scene c{q.first, q.last, k.first, k.last, 0};
+    if (a.prefix) c.prefix = min(max(__builtin_amdgcn_readfirstlane(a.prefix[p.s]), 0), c.k1 - c.k0);
     return c;
 }
 // Keys of the scene that its query row i sees (those below the limit): with the causal mask
@@ -312,8 +370,12 @@ template <typename T, int DP, int ROWS, int WAVES> struct Copy {
     // rows: live rows from base on, 1 at least; with `some`, those whose bit is set in `live`
     __device__ __forceinline__ void start(T *tile, const T *base, int64_t stride, int dim, int rows,
                                           bool some, uint64_t live, int wave, int lane) const {
-        const int bytes = ((min(rows, ROWS) - 1) * (int)stride + dim) * (int)sizeof(T);
-        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, bytes, 0x00020000);
+        // (the same in all lanes, but loaded in a loop: said so, it lies in scalar registers)
+        const int bytes = __builtin_amdgcn_readfirstlane(((min(rows, ROWS) - 1) * (int)stride + dim) * (int)sizeof(T));
+        const uint64_t p = reinterpret_cast<uintptr_t>(base);
+        const uint64_t first_byte = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
+                                    (uint32_t)__builtin_amdgcn_readfirstlane((int)p);
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(first_byte), 0, bytes, 0x00020000);
         typedef __attribute__((address_space(3))) const void *lds_ptr;
         // the later rows' offsets and bits come from the first's here, not from registers kept all
         // along (at 128 channels those would not fit)

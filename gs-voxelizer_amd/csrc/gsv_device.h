@@ -87,6 +87,21 @@ __device__ __forceinline__ float wave_sum(float v) {
             __builtin_bit_cast(float, __builtin_amdgcn_readlane(row, 48)));
 }
 
+// The last of 0 .. n - 1 whose value is x or less, for values that ascend (that of 0 counts as such): a
+// wave looks at 64 of them at a time, so 4,096 take two loads one after the other.
+template <typename F> __device__ __forceinline__ int last_at_most(int n, int x, const F &value) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0;
+    while (n > 1) {
+        const int step = (n + 63) / 64, i = lane * step;
+        const uint64_t those = __ballot(i < n && value(lo + min(i, n - 1)) <= x);
+        const int last = __builtin_amdgcn_readfirstlane(max(__popcll(those) - 1, 0)) * step;
+        lo += last;
+        n = min(step, n - last);
+    }
+    return lo;
+}
+
 __host__ __device__ inline int64_t imin64(int64_t a, int64_t b) { return a < b ? a : b; }
 __host__ __device__ inline int64_t imax64(int64_t a, int64_t b) { return a > b ? a : b; }
 

@@ -65,8 +65,9 @@ def scene_attention(q: Tensor, k: Tensor, v: Tensor, *, scene_starts: Optional[T
         q: (T, H, D); k, v: (N, K, D), H a multiple of K, D a multiple of 8 up to 128.
         scene_starts: (scenes + 1,) int32 first token of each scene; None: one scene.
         key_starts: the same for the keys, where they are not the queries' tokens.
-        longest: rows of the longest scene, queries or keys, if known (sizes the
-            launches, changes no value).
+        longest: rows of the longest scene, queries or keys, if known: scenes of one length
+            then take fewer workgroups.  It changes no value, but how the slopes' gradient is
+            grouped in binary64.
         causal: a token sees the keys up to its own place; where a scene has more keys
             than queries, its queries are the last ones.
         prefix: (scenes,) int32, with causal: leading keys that all tokens of a scene see.

@@ -154,3 +154,40 @@ def test_short_caches(device, dim, cap, bias):
                    slopes=more["slopes"]) if bias else {}
         want = R.attention(q[s:s + 1], k[s, :n], v[s, :n], cap=cap, **ref)[0]["out"]
         _assert_rounded_once(got[s:s + 1], want, n)
+
+
+# ---- scenes are found from a workgroup's place
+
+
+PACKINGS = {
+    "long first": [2000] + [0] * 70 + [3] * 5 + [0] * 4000,
+    "long last": [0] * 4000 + [3] * 5 + [0] * 70 + [2000],
+    "far apart": ([0] * 99 + [40]) * 45,
+    "among empty": [0] * 5 + [129] + [0] * 5,
+    "even": [33] * 64,
+    "even, one more": [33] * 65,
+    "rising": list(range(0, 280, 4)),
+}
+
+
+@TYPES
+@pytest.mark.parametrize("packing", PACKINGS)
+@pytest.mark.parametrize("other_keys", [False, True], ids=["", "other keys"])
+def test_packings(device, dtype, packing, other_keys):
+    """Scenes of very different lengths, thousands of empty ones among them; with and without the longest
+    scene's length, a wrong one too, the same bits."""
+    lengths = PACKINGS[packing]
+    keys = [(n + 5) // 2 if n else 0 for n in lengths] if other_keys else None
+    c = _case(device, dtype, lengths, 2, 1, 32, key_lengths=keys, causal=True)
+    got = _run(c)
+    some = [n for n in lengths if n]
+    near = dict(c, q_starts=_case(device, dtype, some, 2, 1, 32)["q_starts"])
+    if keys:
+        near["k_starts"] = _case(device, dtype, [n for n in keys if n], 2, 1, 32)["q_starts"]
+    val, tol = R.attention(**near)  # a scene without rows has no part in the values
+    for n in got:
+        R.assert_within(got[n], val[n], tol[n], f"{packing} {n}")
+    for longest in (1, max(lengths), sum(lengths)):
+        again = _run(c, longest=longest)
+        for n in got:
+            assert torch.equal(again[n], got[n]), (longest, n)

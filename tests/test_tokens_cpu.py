@@ -76,3 +76,29 @@ def test_counts_that_would_pass_int32_are_refused(tokens):
     assert _plan("cached", _attention(k_tokens=_tokens.MAX_TOKENS, scenes=64)) == OK
     r.tokens = _tokens.MAX_TOKENS
     assert L.gsv_rotary(ctypes.byref(r), None, None, 0, None) == 1  # its pointers are missing
+
+
+def _bwd_bytes(**more):
+    n = ctypes.c_size_t(0)
+    a = _attention(**more)
+    assert _lib.load().gsv_attention_bwd_workspace_bytes(ctypes.byref(a), ctypes.byref(n)) == OK
+    return n.value
+
+
+@pytest.mark.parametrize("longest", [0, 1, 128, 16_000, 64_000, -5])
+def test_launches_go_by_the_rows_and_scenes_there_are(longest):
+    """The workspace holds a binary64 sum for each workgroup of the rows' kernel: their number is at most
+    a tile for each 128 rows and one for each scene, whatever is known of the longest scene."""
+    more = dict(q_tokens=64_000, k_tokens=64_000, heads=8, kv_heads=8, scenes=500, longest_q=longest,
+                longest_k=longest, q_starts=1024, k_starts=1024)
+    plain = _bwd_bytes(**more)
+    n = (_bwd_bytes(**more, slopes=1024, q_positions=1024, k_positions=1024) - plain) / (8 * 8)
+    assert 0 < n <= 64_000 // 128 + 500
+
+
+def test_more_scenes_than_a_launch_holds_are_refused():
+    more = dict(heads=64, kv_heads=64, q_starts=1024, k_starts=1024)
+    assert _plan("bwd", _attention(scenes=1 << 29, **more)) == OK
+    assert _plan("bwd", _attention(scenes=(1 << 29) + 1, **more)) == SIZE_OVERFLOW
+    more["heads"] = more["kv_heads"] = 1 << 14
+    assert _plan("bwd", _attention(scenes=1 << 29, **more)) == SIZE_OVERFLOW
