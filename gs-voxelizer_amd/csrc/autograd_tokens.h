@@ -153,7 +153,7 @@ std::vector<Tensor> rotate(const Tensor &q, const Tensor &k, const Tensor &posit
 
 struct NormCall {
     Tensor x, branch, weight, branch_weight, scale, gate, starts;
-    int64_t scenes, longest;
+    int64_t scenes;
     bool per_token;
     double eps;
 
@@ -168,7 +168,7 @@ struct NormCall {
         n.gate_dtype = gate.defined() ? type_code(gate) : 0;
         n.gate_per_token = per_token;
         n.tokens = (int)x.size(0), n.channels = (int)x.size(1), n.scenes = (int)scenes;
-        n.longest = (int)longest, n.eps = (float)eps;
+        n.eps = (float)eps;
         return n;
     }
     variable_list forward() const {
@@ -185,7 +185,7 @@ struct GatedNorm : public torch::autograd::Function<GatedNorm> {
                                  const NormCall *c) {
         const Tensor &branch_weight = c->branch_weight, &scale = c->scale, &gate = c->gate;
         ctx->saved_data["kept"] = std::vector<int64_t>{
-            x.size(0), x.size(1), x.get_device(), c->scenes, c->longest, c->per_token,
+            x.size(0), x.size(1), x.get_device(), c->scenes, c->per_token,
             gate.defined() ? gate.size(0) : 0, type_code(x), type_code(branch),
             gate.defined() ? type_code(gate) : 0};
         ctx->saved_data["eps"] = c->eps;
@@ -209,15 +209,15 @@ struct GatedNorm : public torch::autograd::Function<GatedNorm> {
         const auto vec = [&](const Tensor &t, const char *what) {
             return t.defined() ? unpacked(t, at::kFloat, dev, C, what) : t;
         };
-        NormCall c{rows(saved[0], k[7], T, "x"), rows(saved[1], k[8], T, "branch"),
+        NormCall c{rows(saved[0], k[6], T, "x"), rows(saved[1], k[7], T, "branch"),
                    vec(saved[2], "weight"), vec(saved[3], "branch_weight"), vec(saved[4], "scale"),
-                   saved[5].defined() ? rows(saved[5], k[9], k[6], "gate") : saved[5], saved[6],
-                   k[3], k[4], k[5] != 0, ctx->saved_data["eps"].toDouble()};
+                   saved[5].defined() ? rows(saved[5], k[8], k[5], "gate") : saved[5], saved[6],
+                   k[3], k[4] != 0, ctx->saved_data["eps"].toDouble()};
         if (c.starts.defined())
             c.starts = unpacked(c.starts, at::kInt, dev, c.scenes + 1, "scene_starts");
         const c10::DeviceGuard guard(dev);
-        const Tensor dy = grads[0].defined() ? rows(grads[0], k[7], T, "the gradient of y") : Tensor();
-        const Tensor dh = grads[1].defined() ? rows(grads[1], k[8], T, "the gradient of h") : Tensor();
+        const Tensor dy = grads[0].defined() ? rows(grads[0], k[6], T, "the gradient of y") : Tensor();
+        const Tensor dh = grads[1].defined() ? rows(grads[1], k[7], T, "the gradient of h") : Tensor();
         const gsv_norm n = c.args();
         const auto like = [&](const Tensor &t) {
             return t.defined() ? empty(t.sizes(), t, t.scalar_type()) : Tensor();
@@ -238,7 +238,7 @@ struct GatedNorm : public torch::autograd::Function<GatedNorm> {
 
 std::vector<Tensor> gated_norm(const Tensor &x, const Tensor &branch, const Tensor &weight,
                                const Maybe &branch_weight, const Maybe &scale, const Maybe &gate,
-                               const Maybe &scene_starts, int64_t longest, double eps) {
+                               const Maybe &scene_starts, double eps) {
     if (!x.defined() || !x.is_cuda()) return {};
     const at::Device dev = x.device();
     if (!is_tokens(x, 2, dev) || !is_tokens(branch, 2, dev) || branch.sizes() != x.sizes() ||
@@ -246,7 +246,7 @@ std::vector<Tensor> gated_norm(const Tensor &x, const Tensor &branch, const Tens
         return {};
     const int64_t T = x.size(0), C = x.size(1);
     NormCall c{x, branch, weight, given(branch_weight), given(scale), given(gate), given(scene_starts),
-               1, longest, false, eps};
+               1, false, eps};
     if (T < 1 || T > GSV_MAX_TOKENS || C < 1 || C > 8192 || !(eps >= 0) ||
         !weight.defined() || !is_parameter(weight, C, dev) || !is_parameter(c.branch_weight, C, dev) ||
         !is_parameter(c.scale, C, dev))
@@ -263,7 +263,6 @@ std::vector<Tensor> gated_norm(const Tensor &x, const Tensor &branch, const Tens
         if (!c.per_token && c.gate.size(0) != c.scenes) return {};
     }
     if (!c.gate.defined() || c.per_token) c.starts = Tensor(), c.scenes = 1;
-    if (!c.starts.defined()) c.longest = 0;
     const c10::DeviceGuard guard(dev);
     bool grad = false;
     for (const Tensor *t : {&c.x, &c.branch, &c.weight, &c.branch_weight, &c.scale, &c.gate})

@@ -34,14 +34,14 @@ def gated_residual_norm(x: Tensor, branch: Tensor, weight: Tensor, *,
         gate: a row for each scene (scenes, C) with scene_starts, for each token (T, C), or
             (1, C) for all of them; float32 or branch's type; or None.
         scene_starts: (scenes + 1,) int32 first rows of the scenes.
-        longest: rows of the longest scene, if known: it sizes a launch, and changes at most
-            the rounding of the sums over rows.
+        longest: rows of the longest scene, taken so that one packing's arguments serve all
+            operators; nothing here depends on it.
     Returns:
         y (T, C) of x's type and h (T, C) of branch's type.
     """
     if _native.plain(x, branch, weight, *_t.present(branch_weight, scale, gate, scene_starts)):
         out = _native.gated_norm(x, branch, weight, branch_weight, scale, gate, scene_starts,
-                                 int(longest or 0), float(eps))
+                                 float(eps))
         if out:
             return tuple(out)
     _t.activations(x, "x", 2)
@@ -72,7 +72,7 @@ def gated_residual_norm(x: Tensor, branch: Tensor, weight: Tensor, *,
     _t.check(eps >= 0, f"eps must not be negative, got {eps}")
     if gate is None or per_token:
         starts, scenes = None, 1  # no value depends on the scenes
-    opts = (per_token, scenes, int(longest or 0) if starts is not None else 0, float(eps))
+    opts = (per_token, scenes, float(eps))
     tensors = (x, branch, weight, branch_weight, scale, gate)
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)):
         return _forward(*tensors, starts, opts)
@@ -81,7 +81,7 @@ def gated_residual_norm(x: Tensor, branch: Tensor, weight: Tensor, *,
 
 def _args(x, branch, weight, branch_weight, scale, gate, starts, opts):
     """The native call's arguments, and the tensors they point into."""
-    per_token, scenes, longest, eps = opts
+    per_token, scenes, eps = opts
     x, branch = _t.rows(x), _t.rows(branch)
     held = [x, branch] + [t if t is None else t.contiguous() for t in (weight, branch_weight, scale)]
     if gate is not None:
@@ -90,7 +90,7 @@ def _args(x, branch, weight, branch_weight, scale, gate, starts, opts):
                   branch_weight=_t.ptr(held[3]), scale=_t.ptr(held[4]), starts=_t.ptr(starts),
                   x_row=x.stride(0), branch_row=branch.stride(0), dtype=_t.TYPES[x.dtype],
                   branch_dtype=_t.TYPES[branch.dtype], tokens=x.shape[0], channels=x.shape[1],
-                  scenes=scenes, longest=longest, eps=eps)
+                  scenes=scenes, eps=eps)
     if gate is not None:
         a.gate, a.gate_row, a.gate_dtype = gate.data_ptr(), gate.stride(0), _t.TYPES[gate.dtype]
         a.gate_per_token = per_token

@@ -433,7 +433,7 @@ int gsv_rotary(const gsv_rotary_args *args, void *q_out, void *k_out, int32_t in
  * x and y have dtype, branch and h branch_dtype (float32 x with either, bfloat16 x with
  * bfloat16), the weights and scale float32, gate float32 or branch_dtype.  gate (NULL: 1)
  * has a row for each scene (starts as for gsv_attention) or, gate_per_token, for each token.
- * y and h are contiguous.
+ * y and h are contiguous.  longest is not read.
  */
 typedef struct gsv_norm {
     const void *x, *branch, *gate;

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import test_gpu_gated_norm as norms
 import token_reference as R
 from gs_voxelizer import _native, attention, gated_norm, rotary
 
@@ -189,5 +190,19 @@ def test_packings(device, dtype, packing, other_keys):
         R.assert_within(got[n], val[n], tol[n], f"{packing} {n}")
     for longest in (1, max(lengths), sum(lengths)):
         again = _run(c, longest=longest)
+        for n in got:
+            assert torch.equal(again[n], got[n]), (longest, n)
+
+
+@pytest.mark.parametrize("types", norms.TYPES, ids=["f32", "mixed", "bf16"])
+@pytest.mark.parametrize("lengths", [
+    [3] * 1500, [1] * 5000, [2000] + [0] * 70 + [1] * 1100 + [0] * 2000, [0] * 4000 + [2000], list(range(90)),
+    [0] * 99 + [40] + [0] * 999 + [1]], ids=["3x1500", "1x5000", "long first", "long last", "rising", "far apart"])
+def test_norm_packings(device, types, lengths):
+    """Thousands of scenes: their gates and the sums over them; the longest scene's length changes nothing."""
+    c = norms._case(device, sum(lengths), 40, lengths, types)
+    got = norms._check(c)
+    for longest in (1, max(lengths)):
+        again = norms._run(c, longest=longest)
         for n in got:
             assert torch.equal(again[n], got[n]), (longest, n)

@@ -102,3 +102,12 @@ def test_more_scenes_than_a_launch_holds_are_refused():
     assert _plan("bwd", _attention(scenes=(1 << 29) + 1, **more)) == SIZE_OVERFLOW
     more["heads"] = more["kv_heads"] = 1 << 14
     assert _plan("bwd", _attention(scenes=1 << 29, **more)) == SIZE_OVERFLOW
+
+
+@pytest.mark.parametrize("longest", [0, 1, 2_900, 20_000])
+def test_the_norm_s_partial_sums_go_by_the_rows_and_scenes_there_are(longest):
+    n = ctypes.c_size_t(0)
+    a = _lib.Norm(dtype=0, branch_dtype=0, tokens=20_000, channels=1024, scenes=7, longest=longest, eps=1e-6,
+                  starts=1024, x=1024, branch=1024, weight=1024, x_row=1024, branch_row=1024)
+    assert _lib.load().gsv_gated_norm_bwd_workspace_bytes(ctypes.byref(a), ctypes.byref(n)) == OK
+    assert n.value <= 2 * 4 * 1024 * (1024 + 7)
