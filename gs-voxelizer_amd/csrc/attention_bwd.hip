@@ -41,13 +41,13 @@ struct BwdArgs {
 };
 
 // A block's scores from the matrix product: capped (u: the tanh), with their bias.
-template <typename T, bool FAR, bool CAPPED>
+template <typename T, bool FAR, int CAP>
 __device__ __forceinline__ void finish_scores(f32x16 &w, f32x16 &u, const f32x16 &d, float in_cap,
                                               float cap, float far_unit) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        if (CAPPED) {
-            u[r] = tanh_of<T>(w[r] * in_cap);
+        if (CAP != kNoCap) {
+            u[r] = tanh_of<T, CAP>(w[r] * in_cap);
             w[r] = cap * u[r];
         }
         if (FAR) w[r] = fmaf(-far_unit, d[r], w[r]);
@@ -55,11 +55,11 @@ __device__ __forceinline__ void finish_scores(f32x16 &w, f32x16 &u, const f32x16
 }
 
 // dq, D and dslope.  A wave's lanes are query rows, as in the forward.
-template <typename T, int DP, bool FAR, bool CAPPED>
+template <typename T, int DP, bool FAR, int CAP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_attention_dq(
     const AttnArgs a, const BwdArgs g) {
     constexpr int KB = kOther<T>, WAVES = 4;
-    constexpr bool far = FAR, capped = CAPPED;
+    constexpr bool far = FAR, capped = CAP != kNoCap;
     typedef typename Elem<T>::frag frag;
     __shared__ __align__(1024) T sk[2][KB * DP];
     __shared__ __align__(1024) T sv[2][KB * DP];
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
                         w = mma(at.rows(kt, st), q[st], w);
                         dp = mma(at.rows(vt, st), dO[st], dp);
                     }
-                    finish_scores<T, FAR, CAPPED>(w, u, d, in_cap, a.cap, far_unit);
+                    finish_scores<T, FAR, CAP>(w, u, d, in_cap, a.cap, far_unit);
                     if (masked)
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
@@ -236,11 +236,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void k_att
 
 // The same for few rows: 32 of them for a workgroup, whose waves take every W-th tile of 32 keys, as
 // k_attention_fwd_few does.
-template <typename T, int DP, bool FAR, bool CAPPED>
+template <typename T, int DP, bool FAR, int CAP>
 __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(const AttnArgs a,
                                                                               const BwdArgs g) {
     constexpr int W = kFewWaves<T, DP>, KB = 32;
-    constexpr bool far = FAR, capped = CAPPED;
+    constexpr bool far = FAR, capped = CAP != kNoCap;
     typedef typename Elem<T>::frag frag;
     static_assert(4 * KB * DP * sizeof(T) >= 32 * DP * sizeof(float), "sums reuse the tiles");
     __shared__ __align__(1024) T tiles[W][4 * KB * DP];  // a wave's keys and values, two buffers
@@ -363,7 +363,7 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
                 w = mma(at.rows(kt, st), q[st], w);
                 dp = mma(at.rows(vt, st), dO[st], dp);
             }
-            finish_scores<T, FAR, CAPPED>(w, u, d, in_cap, a.cap, far_unit);
+            finish_scores<T, FAR, CAP>(w, u, d, in_cap, a.cap, far_unit);
             if (masked)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
@@ -443,7 +443,7 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_dq_few(co
 
 // dk and dv.  A wave's lanes are keys; the rows of all query heads of the key head pass by, so a shared
 // key head's gradient is summed in its wave's registers.
-template <typename T, int DP, bool FAR, bool CAPPED>
+template <typename T, int DP, bool FAR, int CAP>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const AttnArgs a, const BwdArgs g) {
     constexpr int QB = kOther<T>, WAVES = 4;
     typedef typename Elem<T>::frag frag;
@@ -462,7 +462,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
     const int group = a.heads / a.kv_heads;
     const int tiles = (nk + kRows - 1) / kRows;
     const bool fine = in_two_parts<T>(nk);  // weights and ds
-    constexpr bool far = FAR, capped = CAPPED;
+    constexpr bool far = FAR, capped = CAP != kNoCap;
     const float unit = capped ? kLog2e : a.scale * kLog2e;
     const float in_cap = capped ? a.scale / a.cap : 0.f;
 
@@ -581,7 +581,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void k_attention_dkv(const A
                         w = mma(tl.rows(sq[b] + qb * 32 * DP, st), k[st], w);
                         dp = mma(tl.rows(sdo[b] + qb * 32 * DP, st), v[st], dp);
                     }
-                    finish_scores<T, FAR, CAPPED>(w, u, d, in_cap, a.cap, far_unit);
+                    finish_scores<T, FAR, CAP>(w, u, d, in_cap, a.cap, far_unit);
                     if (masked) {
                         const int lo = from == INT32_MAX ? from : from - i0 - qb * 32 - 4 * (lane >> 5);
 #pragma unroll
@@ -697,15 +697,15 @@ struct Backward {
     const BwdArgs &g;
     const BwdPlan &plan;
     hipStream_t st;
-    template <typename T, int DP, bool FAR, bool CAPPED> void run() const {
+    template <typename T, int DP, bool FAR, int CAP> void run() const {
         if (a.q_tokens > 0 && attention_few(a))
-            hipLaunchKernelGGL((k_attention_dq_few<T, DP, FAR, CAPPED>), plan.rows,
+            hipLaunchKernelGGL((k_attention_dq_few<T, DP, FAR, CAP>), plan.rows,
                                dim3(64 * kFewWaves<T, DP>), 0, st, a, g);
         else if (a.q_tokens > 0)
-            hipLaunchKernelGGL((k_attention_dq<T, DP, FAR, CAPPED>), plan.rows, dim3(256), 0, st, a, g);
+            hipLaunchKernelGGL((k_attention_dq<T, DP, FAR, CAP>), plan.rows, dim3(256), 0, st, a, g);
         AttnArgs k = a;
         k.slots = plan.key_slots, k.places = plan.key_places;
-        hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAPPED>), plan.keys, dim3(256), 0, st, k, g);
+        hipLaunchKernelGGL((k_attention_dkv<T, DP, FAR, CAP>), plan.keys, dim3(256), 0, st, k, g);
         if (g.parts == 1 || a.k_tokens == 0) return;
         const int64_t fours = (int64_t)a.k_tokens * a.kv_heads * a.dim / 4;
         hipLaunchKernelGGL(k_parts_sum<T>, dim3((unsigned)((2 * fours + 255) / 256)), dim3(256), 0, st,

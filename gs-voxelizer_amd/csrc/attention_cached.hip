@@ -33,7 +33,7 @@ struct CacheArgs {
 // Waves of a workgroup: four, two where their tiles would pass the LDS of a CU.
 template <typename T, int DP> constexpr int kWaves = DP * sizeof(T) > 256 ? 2 : 4;
 
-template <typename T, int DP, bool FAR, bool CAPPED>
+template <typename T, int DP, bool FAR, int CAP>
 __global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const AttnArgs a, const CacheArgs c,
                                                           T *__restrict__ out) {
     typedef typename Elem<T>::frag frag;
@@ -58,7 +58,7 @@ __global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const
     const bool head = col < group;
     const int h = hk * group + (head ? col : 0);
 
-    constexpr bool far = FAR, capped = CAPPED;
+    constexpr bool far = FAR, capped = CAP != kNoCap;
     const float slope = slope_of(a, h);
     const bool fine = in_two_parts<T>(len);
     const float unit = capped ? kLog2e : a.scale * kLog2e;
@@ -140,7 +140,7 @@ __global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const
         if (capped)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                w[r] = a.cap * tanh_of<T>(w[r] * in_cap);
+                w[r] = a.cap * tanh_of<T, CAP>(w[r] * in_cap);
                 if (far) w[r] = fmaf(-far_unit, d[r], w[r]);
             }
         if (live != 0xffffffffu) {
@@ -273,9 +273,9 @@ struct Cached {
     const CacheArgs &c;
     void *out;
     hipStream_t st;
-    template <typename T, int DP, bool FAR, bool CAPPED> void run() const {
+    template <typename T, int DP, bool FAR, int CAP> void run() const {
         T *o = static_cast<T *>(out);
-        hipLaunchKernelGGL((k_attention_cached<T, DP, FAR, CAPPED>),
+        hipLaunchKernelGGL((k_attention_cached<T, DP, FAR, CAP>),
                            dim3((unsigned)(a.scenes * a.kv_heads * c.head_tiles * c.splits)),
                            dim3(64 * kWaves<T, DP>), 0, st, a, c, o);
         if (c.splits > 1)

@@ -31,12 +31,12 @@ constexpr float kSlack = 8.f;
 // multiply-adds, a multiply and a root an element, at the matrix units' differences).  With one
 // key head for both (SHARED) they share the tiles too.
 // TRAIN: the log sums and out_low are wanted.
-template <typename T, int DP, bool FAR, bool CAPPED, int HEADS, bool SHARED, bool TRAIN>
+template <typename T, int DP, bool FAR, int CAP, int HEADS, bool SHARED, bool TRAIN>
 __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_attention_fwd(
     const AttnArgs a, T *__restrict__ out, T *__restrict__ out_low, float *__restrict__ lse) {
     constexpr int KB = sizeof(T) == 2 ? 64 : 32;  // keys of a tile
     constexpr int KV = SHARED ? 1 : HEADS;        // key heads of the workgroup
-    constexpr bool far = FAR, capped = CAPPED;
+    constexpr bool far = FAR, capped = CAP != kNoCap;
     // float32: scores are rounded to powers of two before their maximum is taken off, so that the
     // largest has the weight 1 exactly, as the rounding to bfloat16 gives it there
     constexpr bool kExact = sizeof(T) == 4;
@@ -160,7 +160,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
                     for (int n = 0; n < HEADS; ++n)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
-                            if (capped) w[n][r] = a.cap * tanh_of<T>(w[n][r] * in_cap);
+                            if (capped) w[n][r] = a.cap * tanh_of<T, CAP>(w[n][r] * in_cap);
                             if (far) w[n][r] = fmaf(-far_unit[n], d[r], w[n][r]);
                         }
                     if (masked) {
@@ -248,11 +248,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
 // the waves' sums are joined through LDS at the end.  Four times as many workgroups, each a quarter as
 // long.  Scores are rounded to powers of two before their
 // maximum is taken off, so that the largest weight is exactly a power of two.
-template <typename T, int DP, bool FAR, bool CAPPED, bool TRAIN>
+template <typename T, int DP, bool FAR, int CAP, bool TRAIN>
 __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_fwd_few(
     const AttnArgs a, T *__restrict__ out, T *__restrict__ out_low, float *__restrict__ lse) {
     constexpr int W = kFewWaves<T, DP>, KB = 32;
-    constexpr bool far = FAR, capped = CAPPED;
+    constexpr bool far = FAR, capped = CAP != kNoCap;
     typedef typename Elem<T>::frag frag;
     static_assert(4 * KB * DP * sizeof(T) >= 32 * DP * sizeof(float), "sums reuse the tiles");
     __shared__ __align__(1024) T tiles[W][4 * KB * DP];  // a wave's keys and values, two buffers
@@ -347,7 +347,7 @@ __global__ __launch_bounds__((64 * kFewWaves<T, DP>)) void k_attention_fwd_few(
             if (far) d = distances<T>(place, spos[wave][b], KB, 0, lane);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                if (capped) w[r] = a.cap * tanh_of<T>(w[r] * in_cap);
+                if (capped) w[r] = a.cap * tanh_of<T, CAP>(w[r] * in_cap);
                 if (far) w[r] = fmaf(-far_unit, d[r], w[r]);
             }
             if (j0 + KB > all || (uint32_t)~live) {
@@ -450,38 +450,38 @@ struct Forward {
         status = attention_grid(places, heads, grid) ? GSV_OK : GSV_ERR_SIZE_OVERFLOW;
         return status == GSV_OK;
     }
-    template <typename T, int DP, bool FAR, bool CAPPED, int HEADS, bool SHARED> void start() {
+    template <typename T, int DP, bool FAR, int CAP, int HEADS, bool SHARED> void start() {
         dim3 grid;
         if (!plan(kRows, a.heads / HEADS, &grid)) return;
         T *o = static_cast<T *>(out), *low = static_cast<T *>(out_low);
         if (lse)
-            hipLaunchKernelGGL((k_attention_fwd<T, DP, FAR, CAPPED, HEADS, SHARED, true>), grid,
+            hipLaunchKernelGGL((k_attention_fwd<T, DP, FAR, CAP, HEADS, SHARED, true>), grid,
                                dim3(256), 0, st, a, o, low, lse);
         else
-            hipLaunchKernelGGL((k_attention_fwd<T, DP, FAR, CAPPED, HEADS, SHARED, false>), grid,
+            hipLaunchKernelGGL((k_attention_fwd<T, DP, FAR, CAP, HEADS, SHARED, false>), grid,
                                dim3(256), 0, st, a, o, low, lse);
         status = check_launch();
     }
-    template <typename T, int DP, bool FAR, bool CAPPED> void few() {
+    template <typename T, int DP, bool FAR, int CAP> void few() {
         dim3 grid, block(64 * kFewWaves<T, DP>);
         if (!plan(32, a.heads, &grid)) return;
         T *o = static_cast<T *>(out), *low = static_cast<T *>(out_low);
         if (lse)
-            hipLaunchKernelGGL((k_attention_fwd_few<T, DP, FAR, CAPPED, true>), grid, block, 0, st, a, o, low, lse);
+            hipLaunchKernelGGL((k_attention_fwd_few<T, DP, FAR, CAP, true>), grid, block, 0, st, a, o, low, lse);
         else
-            hipLaunchKernelGGL((k_attention_fwd_few<T, DP, FAR, CAPPED, false>), grid, block, 0, st, a, o, low, lse);
+            hipLaunchKernelGGL((k_attention_fwd_few<T, DP, FAR, CAP, false>), grid, block, 0, st, a, o, low, lse);
         status = check_launch();
     }
-    template <typename T, int DP, bool FAR, bool CAPPED> void run() {
-        if (attention_few(a)) return few<T, DP, FAR, CAPPED>();
-        if constexpr (FAR && sizeof(T) == 2 && DP <= 64) {
+    template <typename T, int DP, bool FAR, int CAP> void run() {
+        if (attention_few(a)) return few<T, DP, FAR, CAP>();
+        if constexpr (FAR && sizeof(T) == 2 && DP <= 64 && CAP != kAnyCap) {
             if (attention_pairs(a)) {
-                if (a.heads / a.kv_heads % 2 == 0) start<T, DP, FAR, CAPPED, 2, true>();
-                else start<T, DP, FAR, CAPPED, 2, false>();
+                if (a.heads / a.kv_heads % 2 == 0) start<T, DP, FAR, CAP, 2, true>();
+                else start<T, DP, FAR, CAP, 2, false>();
                 return;
             }
         }
-        start<T, DP, FAR, CAPPED, 1, true>();
+        start<T, DP, FAR, CAP, 1, true>();
     }
 };
 

@@ -154,10 +154,13 @@ __device__ __forceinline__ float add_weights(f32x8 p, float sum) {
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// tanh.  For bfloat16 scores 1 - 2 / (exp(2 x) + 1): absolute error near 2^-23, far
-// below the 2^-9 of the operands; ends at +-1 where exp overflows or vanishes.
-template <typename T> __device__ __forceinline__ float tanh_of(float x) {
-    if constexpr (sizeof(T) == 4) return tanhf(x);
+// tanh.  For bfloat16 scores 1 - 2 / (exp(2 x) + 1): absolute error 2^-22.7, far
+// below the 2^-9 of the operands; ends at +-1 where exp overflows or vanishes.  Times a cap of
+// thousands that error is one of the scores (all near 0 then): past kWideCap, where it is 2^-12.7, tanhf.
+constexpr float kWideCap = 1024.f;
+enum Cap { kNoCap, kCap, kAnyCap };
+template <typename T, int CAP> __device__ __forceinline__ float tanh_of(float x) {
+    if constexpr (sizeof(T) == 4 || CAP == kAnyCap) return tanhf(x);
     const float e = fast_exp2(2.885390082f * x);  // 2 log2(e)
     return 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
 }
@@ -189,13 +192,16 @@ inline int64_t used_stride(int64_t stride, int64_t entries) { return entries > 1
 int attention_args(const gsv_attention *in, AttnArgs *a);
 
 // The kernel variant of a call: element type, channels (up to 32, 64 or 128; the columns past
-// dim are zeros), distance bias, score cap.
+// dim are zeros), distance bias, score cap (with another tanh past kWideCap for bfloat16).
 template <typename T, int DP, typename F> void attention_options(const AttnArgs &a, F &f) {
     const bool far = a.slopes, capped = a.cap > 0.f;
-    if (far && capped) f.template run<T, DP, true, true>();
-    else if (far) f.template run<T, DP, true, false>();
-    else if (capped) f.template run<T, DP, false, true>();
-    else f.template run<T, DP, false, false>();
+    if constexpr (sizeof(T) == 2)
+        if (a.cap > kWideCap)
+            return far ? f.template run<T, DP, true, kAnyCap>() : f.template run<T, DP, false, kAnyCap>();
+    if (far && capped) f.template run<T, DP, true, kCap>();
+    else if (far) f.template run<T, DP, true, kNoCap>();
+    else if (capped) f.template run<T, DP, false, kCap>();
+    else f.template run<T, DP, false, kNoCap>();
 }
 template <typename T, typename F> void attention_channels(const AttnArgs &a, F &f) {
     if (a.dim <= 32) attention_options<T, 32>(a, f);

@@ -206,3 +206,36 @@ def test_norm_packings(device, types, lengths):
         again = norms._run(c, longest=longest)
         for n in got:
             assert torch.equal(again[n], got[n]), (longest, n)
+
+
+# ---- caps far above the scores
+
+
+def _assert_rounded_twice(got, want, what):
+    """bfloat16 in the 2-norm: the rounding of the results and, in quadrature, as much from weights and ds of
+    8 bits (1.42 of the first), and a tenth of it."""
+    once = _off(want.to(BF16), want)
+    assert _off(got, want) <= 1.1 * 2 ** 0.5 * once + 2.0 ** -13, (what, _off(got, want), once)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("cap", [1000.0, 1e4, 1e5, 1e6])
+@pytest.mark.parametrize("lengths", [[300], [300] + [140] * 90], ids=["few", "many"])
+def test_large_caps(device, dim, bias, cap, lengths):
+    """The nearer a cap is to none, the nearer its results are to those without one."""
+    c = _case(device, BF16, lengths, 2, 2, dim, bias=bias, cap=cap)
+    got, want = _run(c), R.attention(**c)[0]
+    for n in ("out", "dq", "dk", "dv"):
+        _assert_rounded_twice(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("cap", [1000.0, 1e5, 1e6])
+def test_large_caps_over_a_cache(device, dim, cap):
+    g = _gen(device, 4)
+    q = torch.randn(30, 8, dim, generator=g, device=device).to(BF16)
+    k, v = (torch.randn(30, 400, 2, dim, generator=g, device=device).to(BF16) for _ in "kv")
+    got = attention.cached_attention(q, k, v, torch.full((30,), 400, dtype=torch.int32, device=device), cap=cap)
+    want = torch.cat([R.attention(q[s:s + 1], k[s], v[s], cap=cap)[0]["out"] for s in range(30)])
+    _assert_rounded_twice(got, want, "out")
