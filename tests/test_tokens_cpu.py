@@ -4,6 +4,7 @@ import ctypes
 import pytest
 import torch
 
+import token_rounding as T
 from gs_voxelizer import _lib, _tokens
 
 OK, SIZE_OVERFLOW = 0, 4
@@ -111,3 +112,23 @@ def test_the_norm_s_partial_sums_go_by_the_rows_and_scenes_there_are(longest):
                   starts=1024, x=1024, branch=1024, weight=1024, x_row=1024, branch_row=1024)
     assert _lib.load().gsv_gated_norm_bwd_workspace_bytes(ctypes.byref(a), ctypes.byref(n)) == OK
     assert n.value <= 2 * 4 * 1024 * (1024 + 7)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_the_bounds_tell_a_lost_part_of_out_and_the_rows_rests(dim, causal):
+    """The bounds of the GPU tests, on the oracle with the kernels' roundings: they hold, and fail where D
+    comes from the rounded output alone, or the rows' rests stay in the slopes' gradient."""
+    found = 0
+    for seed in range(4):
+        args, want = T.clear_winners(450, dim, seed, causal)
+        right = T.rounded_head(*args)
+        for n in ("out", "dq", "dk", "dv"):
+            T.assert_rounded_twice(right[n], want[n], n)
+        assert T.off(right["dslopes"], want["dslopes"]) <= T.SLOPES
+        wrong = T.rounded_head(*args, whole_out=False)
+        for n in ("dq", "dk"):
+            assert T.off(wrong[n], want[n]) > T.rounded_twice(want[n])
+        wrong = T.rounded_head(*args, rests=False)
+        found += T.off(wrong["dslopes"], want["dslopes"]) > T.SLOPES
+    assert found >= 3
