@@ -237,3 +237,141 @@ def test_scores_with_clear_winners(device, dim, cap, causal, lengths, heads):
     for n in ("out", "dq", "dk", "dv"):
         assert_rounded_twice(got[n], want[n], n)
     assert off(got["dslopes"], want["dslopes"]) <= SLOPES
+
+
+@TYPES
+@pytest.mark.parametrize("offset", [1e5, 1e6])
+@pytest.mark.parametrize("lengths", [[300], [300] + [1] * 200], ids=["few", "many"])
+def test_positions_far_from_the_origin(device, dtype, offset, lengths):
+    """Differences of positions come out of sums of bfloat16 products of the coordinates' parts: no less
+    exact where the coordinates are large and the differences small."""
+    c = _case(device, dtype, lengths, 2, 2, 64, offset=offset)
+    got, (val, tol) = _run(c), R.attention(**c)
+    for n in got:
+        R.assert_within(got[n], val[n], tol[n], n)
+    if dtype == BF16:
+        assert_rounded_twice(got["out"][:300], val["out"][:300], "out")
+
+
+# ---- which route a call takes, and captured training steps
+
+
+@pytest.fixture
+def taken(monkeypatch):
+    """The native functions' answers, in order: whether each took its call."""
+    assert _native.available
+    log = []
+    for name in ("rotate", "gated_norm", "scene_attention", "cached_attention"):
+        def record(*args, call=getattr(_native, name)):
+            out = call(*args)
+            log.append(bool(out))
+            return out
+        monkeypatch.setattr(_native, name, record)
+    return log
+
+
+@TYPES
+def test_plain_calls_take_the_native_nodes(device, taken, dtype):
+    g = _gen(device, 6)
+
+    def normal(*shape, t=dtype):
+        return torch.randn(shape, generator=g, device=device).to(t)
+
+    qkv = normal(50, 8, 48).requires_grad_()
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    pos = torch.rand(50, 4, generator=g, device=device)
+    starts = torch.tensor([0, 20, 50], dtype=torch.int32, device=device)
+    f = rotary.axis_frequencies((8, 8, 8), device=device)
+    for interleaved in (False, True):
+        rotary.rotate_qk(q, k, pos[:, :3], f, interleaved=interleaved)
+    with torch.no_grad():
+        rotary.rotate_qk(q, k, pos[:, :3], f)
+    slopes = torch.rand(4, device=device)
+    hits = torch.ones(50, dtype=torch.int32, device=device)
+    for more in (dict(), dict(scene_starts=starts, longest=30), dict(causal=True, cap=5.0),
+                 dict(scene_starts=starts, causal=True, prefix=starts[:2]), dict(scale=0.3),
+                 dict(positions=pos[:, :3], slopes=slopes), dict(keep=hits), dict(keep=hits.bool()),
+                 dict(positions=pos[:, :3], slopes=slopes.to(dtype), keep=hits.to(torch.uint8)),
+                 dict(scene_starts=starts, key_starts=starts, positions=pos[:, :3], key_positions=pos[:, 1:],
+                      slopes=slopes)):
+        attention.scene_attention(q, k, v, **more)
+        with torch.no_grad():
+            attention.scene_attention(q, k, v, **more)
+    with torch.no_grad():
+        n = torch.tensor([50], dtype=torch.int32, device=device)
+        attention.cached_attention(q[:1], k[None], v[None], n)
+        attention.cached_attention(q[:1], k[None], v[None], n, cap=5.0, positions=pos[:1, :3],
+                                   key_positions=pos[None, :, :3], slopes=slopes, keep=hits[None])
+    x, w = normal(50, 40, t=F32).requires_grad_(), torch.rand(40, device=device)
+    for stream, branch in ((x, normal(50, 40)), (normal(50, 40), normal(50, 40))):
+        for more in (dict(), dict(scale=w, branch_weight=w), dict(gate=normal(50, 40)), dict(gate=normal(1, 40)),
+                     dict(gate=normal(2, 40), scene_starts=starts, longest=30), dict(gate=normal(1, 40, t=F32))):
+            gated_norm.gated_residual_norm(stream, branch, w, **more)
+    assert taken == [True] * len(taken) and len(taken) == 3 + 20 + 2 + 12
+
+
+@TYPES
+def test_calls_the_native_nodes_leave(device, taken, dtype):
+    """Empty batches, rows off alignment, strided last axes: the Python classes do them, and give the values
+    of plain tensors."""
+    g = _gen(device, 7)
+    q = torch.randn(30, 2, 32, generator=g, device=device).to(dtype)
+    want = attention.scene_attention(q, q, q)
+    odd = torch.zeros(30, 2, 33, dtype=dtype, device=device)[..., 1:].copy_(q)
+    strided = q.transpose(1, 2).contiguous().transpose(1, 2)
+    for t in (odd, strided):
+        assert torch.equal(attention.scene_attention(t, q, t), want)
+    assert attention.scene_attention(q[:0], q[:0], q[:0]).shape == (0, 2, 32)
+    f, pos = torch.rand(1, 16, device=device), torch.rand(30, 1, device=device)
+    rotary.rotate_qk(q, None, pos, f)  # not asked
+    rotary.rotate_qk(strided, q, pos, f)
+    w = torch.ones(32, device=device)
+    gated_norm.gated_residual_norm(strided[:, 0], q[:, 0], w)
+    gated_norm.gated_residual_norm(q[:0, 0], q[:0, 0], w)
+    assert taken == [True] + [False] * 6
+
+
+@pytest.mark.parametrize("scenes", [[40, 33, 1], [5] * 200], ids=["few", "many"])
+def test_a_captured_training_step(device, route, scenes):
+    """A block of all three operators with their gradients in a HIP graph: each replay, after new
+    inputs and eager work, equals the eager step."""
+    g, T, H, D = _gen(device, 8), sum(scenes), 4, 32
+    C = H * D
+
+    def normal(*shape):
+        return torch.randn(shape, generator=g, device=device).to(BF16)
+
+    starts = torch.tensor([0] + scenes, device=device).cumsum(0).int()
+    pos, f = 40 * torch.rand(T, 3, generator=g, device=device), rotary.axis_frequencies((6, 5, 5), device=device)
+    w = torch.rand(C, generator=g, device=device)
+    inputs = [normal(T, 3 * H, D), normal(T, C), normal(len(scenes), C), torch.full((H,), 0.1, device=device)]
+    grads = normal(T, C), normal(T, C)
+
+    def step():
+        # (views as leaves: nothing but these operators' kernels is captured)
+        qkv, x, gate, slopes = inputs
+        leaves = [t.detach().requires_grad_() for t in (qkv[:, :H], qkv[:, H:2 * H], qkv[:, 2 * H:], x, gate, slopes)]
+        q, k = rotary.rotate_qk(*leaves[:2], pos, f)
+        o = attention.scene_attention(q, k, leaves[2], scene_starts=starts, causal=True, cap=20.0,
+                                      positions=pos, slopes=leaves[5])
+        out = gated_norm.gated_residual_norm(leaves[3], o.flatten(1), w, branch_weight=w, gate=leaves[4],
+                                             scene_starts=starts)
+        return out + torch.autograd.grad(out, leaves, grads)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for n in range(4):
+        for t in inputs[:3]:
+            t.copy_(torch.randn(t.shape, generator=g, device=device))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b), n
