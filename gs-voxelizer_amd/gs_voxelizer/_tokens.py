@@ -5,6 +5,10 @@ int32 holds each scene's first row.  The first scene begins at row 0 and the las
 with the array; entries 0 and ``scenes`` are not read.  Errors are raised as ValueError
 before anything is launched; outputs and workspaces are torch tensors, and
 every kernel is enqueued on torch's current stream of the tensors' device.
+
+Calls that the native nodes leave go through autograd functions, also where nothing asks for
+a gradient: a trace records them as one operation, whose checks run at each replay, and forward
+mode and transforms raise there.
 """
 import ctypes
 import functools
@@ -92,10 +96,10 @@ def starts(t, what, device):
 
 
 def fixed(t, what, why):
-    """Refuses a tensor that asks for a gradient that the operator does not form."""
-    check(not (torch.is_grad_enabled() and t.requires_grad),
+    """Refuses a tensor that asks for a gradient that the operator does not form (outside the
+    autograd functions, whose forward runs without gradients)."""
+    check(not (isinstance(t, torch.Tensor) and torch.is_grad_enabled() and t.requires_grad),
           f"{what} get{why} no gradient here: pass {what}.detach()")
-    return t
 
 
 def positions(t, what, shape, device):
@@ -104,7 +108,6 @@ def positions(t, what, shape, device):
           f"{what} must be a float32 tensor")
     check(t.device == device, f"{what} must be on {device}, got {t.device}")
     check(tuple(t.shape) == shape, f"{what} must have shape {shape}, got {tuple(t.shape)}")
-    fixed(t, what, "")
     return t if t.stride(-1) == 1 else t.contiguous()
 
 

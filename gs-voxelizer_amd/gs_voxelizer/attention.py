@@ -88,41 +88,11 @@ def scene_attention(q: Tensor, k: Tensor, v: Tensor, *, scene_starts: Optional[T
                                       positions, key_positions, slopes, keep)
         if out:
             return out[0]
-    H, K, D = _heads(q, k, v, 3)
-    dev, T, N = q.device, q.shape[0], k.shape[0]
-    _t.check(T <= _t.MAX_TOKENS and N <= _t.MAX_TOKENS, "too many tokens")
-    qs, scenes = _t.starts(scene_starts, "scene_starts", dev)
-    if key_starts is None:
-        _t.check(scenes == 1 or N == T, f"{N} keys for {T} queries need key_starts")
-        ks = qs
-    else:
-        ks, n = _t.starts(key_starts, "key_starts", dev)
-        _t.check(n == scenes, f"key_starts hold {n} scenes, scene_starts {scenes}")
-    a = _lib.Attention(dtype=_t.TYPES[q.dtype], q_tokens=T, k_tokens=N, heads=H, kv_heads=K, dim=D,
-                       scenes=scenes, causal=bool(causal), longest_q=int(longest or 0),
-                       longest_k=int(longest or 0))
-    slopes = _options(a, q, scale, cap, slopes)
-    held = [qs, ks, None, None, None, None]
-    if prefix is not None:
-        _t.check(causal, "prefix needs causal=True")
-        held[2] = _t.int32s(prefix, "prefix", scenes, dev)
-    if slopes is not None:
-        _t.check(positions is not None, "slopes need positions")
-        held[3] = _t.positions(positions, "positions", (T, 3), dev)
-        if key_positions is None:
-            _t.check(N == T, f"{N} keys for {T} queries need key_positions")
-            held[4] = held[3]
-        else:
-            held[4] = _t.positions(key_positions, "key_positions", (N, 3), dev)
-    else:
-        _t.check(positions is None and key_positions is None, "positions need slopes")
-    if keep is not None:
-        held[5] = _t.mask(keep, "keep", (N,), dev)
-    q, k, v = _t.rows16(q), _t.rows16(k), _t.rows16(v)
-    if not (torch.is_grad_enabled()
-            and any(t is not None and t.requires_grad for t in (q, k, v, slopes))):
-        return _forward(a, q, k, v, slopes, held, None, None)
-    return _SceneAttention.apply(q, k, v, slopes, a, *held)
+    _t.fixed(positions, "positions", "")
+    _t.fixed(key_positions, "key_positions", "")
+    return _SceneAttention.apply(q, k, v, slopes, scene_starts, key_starts, prefix, positions,
+                                 key_positions, keep, int(longest or 0), bool(causal), scale, cap,
+                                 torch.is_grad_enabled())
 
 
 def _point(a, q, k, v, slopes):
@@ -152,9 +122,49 @@ def _forward(a, q, k, v, slopes, held, low, lse):
     return out
 
 
+def _checked(q, k, v, slopes, scene_starts, key_starts, prefix, positions, key_positions, keep,
+             longest, causal, scale, cap):
+    """The call's arguments as the kernels take them."""
+    H, K, D = _heads(q, k, v, 3)
+    dev, T, N = q.device, q.shape[0], k.shape[0]
+    _t.check(T <= _t.MAX_TOKENS and N <= _t.MAX_TOKENS, "too many tokens")
+    qs, scenes = _t.starts(scene_starts, "scene_starts", dev)
+    if key_starts is None:
+        _t.check(scenes == 1 or N == T, f"{N} keys for {T} queries need key_starts")
+        ks = qs
+    else:
+        ks, n = _t.starts(key_starts, "key_starts", dev)
+        _t.check(n == scenes, f"key_starts hold {n} scenes, scene_starts {scenes}")
+    a = _lib.Attention(dtype=_t.TYPES[q.dtype], q_tokens=T, k_tokens=N, heads=H, kv_heads=K, dim=D,
+                       scenes=scenes, causal=causal, longest_q=longest, longest_k=longest)
+    slopes = _options(a, q, scale, cap, slopes)
+    held = [qs, ks, None, None, None, None]
+    if prefix is not None:
+        _t.check(causal, "prefix needs causal=True")
+        held[2] = _t.int32s(prefix, "prefix", scenes, dev)
+    if slopes is not None:
+        _t.check(positions is not None, "slopes need positions")
+        held[3] = _t.positions(positions, "positions", (T, 3), dev)
+        if key_positions is None:
+            _t.check(N == T, f"{N} keys for {T} queries need key_positions")
+            held[4] = held[3]
+        else:
+            held[4] = _t.positions(key_positions, "key_positions", (N, 3), dev)
+    else:
+        _t.check(positions is None and key_positions is None, "positions need slopes")
+    if keep is not None:
+        held[5] = _t.mask(keep, "keep", (N,), dev)
+    return a, _t.rows16(q), _t.rows16(k), _t.rows16(v), slopes, held
+
+
 class _SceneAttention(Function):
     @staticmethod
-    def forward(ctx, q, k, v, slopes, a, *held):
+    def forward(ctx, q, k, v, slopes, scene_starts, key_starts, prefix, positions, key_positions,
+                keep, longest, causal, scale, cap, grad):
+        a, q, k, v, slopes, held = _checked(q, k, v, slopes, scene_starts, key_starts, prefix, positions,
+                                            key_positions, keep, longest, causal, scale, cap)
+        if not (grad and any(ctx.needs_input_grad[:4])):
+            return _forward(a, q, k, v, slopes, held, None, None)
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
         # what rounding took from the output: the backward needs it whole
         low = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q.dtype == torch.bfloat16 else None
@@ -178,7 +188,7 @@ class _SceneAttention(Function):
             _t.call("attention_bwd", ctypes.byref(a), out.data_ptr(), _t.ptr(low),
                     lse.data_ptr(), dout.data_ptr(), dout.stride(0), dout.stride(1), dq.data_ptr(), dk.data_ptr(),
                     dv.data_ptr(), _t.ptr(ds), ws.data_ptr(), n, _t.stream(dev))
-        return (dq, dk, dv, ds, None) + (None,) * 6
+        return (dq, dk, dv, ds) + (None,) * 11
 
 
 def cached_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor, *,
@@ -203,38 +213,50 @@ def cached_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tenso
                                        float(cap or 0.0), positions, key_positions, slopes, keep)
         if out:
             return out[0]
-    H, K, D = _heads(q, k_cache, v_cache, 4)
-    dev, S, N = q.device, q.shape[0], k_cache.shape[1]
-    _t.check(k_cache.shape[0] == S, f"k_cache holds {k_cache.shape[0]} scenes, q {S}")
-    _t.check(N <= _t.MAX_TOKENS, "too many tokens")
-    for t, what in ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache")):
-        _t.fixed(t, what, "s")
-    lengths = _t.int32s(lengths, "lengths", S, dev)
-    a = _lib.Attention(dtype=_t.TYPES[q.dtype], q_tokens=S, k_tokens=N, heads=H, kv_heads=K, dim=D,
-                       scenes=S)
-    slopes = _options(a, q, scale, cap, slopes)
-    kp_scene = keep_scene = 0
-    if slopes is not None:
-        _t.fixed(slopes, "slopes", "")
-        _t.check(positions is not None and key_positions is not None,
-                 "slopes need positions and key_positions")
-        positions = _t.positions(positions, "positions", (S, 3), dev)
-        key_positions = _t.positions(key_positions, "key_positions", (S, N, 3), dev)
-        a.q_positions, a.q_pos_row = positions.data_ptr(), positions.stride(0)
-        a.k_positions, a.k_pos_row = key_positions.data_ptr(), key_positions.stride(1)
-        kp_scene = key_positions.stride(0)
-    else:
-        _t.check(positions is None and key_positions is None, "positions need slopes")
-    if keep is not None:
-        keep = _t.mask(keep, "keep", (S, N), dev)
-        a.keep, a.keep_bytes, keep_scene = keep.data_ptr(), keep.element_size(), keep.stride(0)
-    q, k_cache, v_cache = _t.rows16(q), _t.rows16(k_cache), _t.rows16(v_cache)
-    _point(a, q, k_cache, v_cache, slopes)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    with torch.cuda.device(dev):
-        n = _t.workspace_bytes("attention_cached_workspace_bytes", a)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        _t.call("attention_cached", ctypes.byref(a), lengths.data_ptr(), k_cache.stride(0),
-                v_cache.stride(0), kp_scene, keep_scene, out.data_ptr(), ws.data_ptr(), n,
-                _t.stream(dev))
-    return out
+    for t, what, why in ((q, "q", "s"), (k_cache, "k_cache", "s"), (v_cache, "v_cache", "s"),
+                         (positions, "positions", ""), (key_positions, "key_positions", ""),
+                         (slopes, "slopes", "")):
+        _t.fixed(t, what, why)
+    return _CachedAttention.apply(q, k_cache, v_cache, lengths, slopes, positions, key_positions, keep,
+                                  scale, cap)
+
+
+class _CachedAttention(Function):
+    @staticmethod
+    def forward(ctx, q, k_cache, v_cache, lengths, slopes, positions, key_positions, keep, scale, cap):
+        H, K, D = _heads(q, k_cache, v_cache, 4)
+        dev, S, N = q.device, q.shape[0], k_cache.shape[1]
+        _t.check(k_cache.shape[0] == S, f"k_cache holds {k_cache.shape[0]} scenes, q {S}")
+        _t.check(N <= _t.MAX_TOKENS, "too many tokens")
+        lengths = _t.int32s(lengths, "lengths", S, dev)
+        a = _lib.Attention(dtype=_t.TYPES[q.dtype], q_tokens=S, k_tokens=N, heads=H, kv_heads=K, dim=D,
+                           scenes=S)
+        slopes = _options(a, q, scale, cap, slopes)
+        kp_scene = keep_scene = 0
+        if slopes is not None:
+            _t.check(positions is not None and key_positions is not None,
+                     "slopes need positions and key_positions")
+            positions = _t.positions(positions, "positions", (S, 3), dev)
+            key_positions = _t.positions(key_positions, "key_positions", (S, N, 3), dev)
+            a.q_positions, a.q_pos_row = positions.data_ptr(), positions.stride(0)
+            a.k_positions, a.k_pos_row = key_positions.data_ptr(), key_positions.stride(1)
+            kp_scene = key_positions.stride(0)
+        else:
+            _t.check(positions is None and key_positions is None, "positions need slopes")
+        if keep is not None:
+            keep = _t.mask(keep, "keep", (S, N), dev)
+            a.keep, a.keep_bytes, keep_scene = keep.data_ptr(), keep.element_size(), keep.stride(0)
+        q, k_cache, v_cache = _t.rows16(q), _t.rows16(k_cache), _t.rows16(v_cache)
+        _point(a, q, k_cache, v_cache, slopes)
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        with torch.cuda.device(dev):
+            n = _t.workspace_bytes("attention_cached_workspace_bytes", a)
+            ws = torch.empty(n, dtype=torch.uint8, device=dev)
+            _t.call("attention_cached", ctypes.byref(a), lengths.data_ptr(), k_cache.stride(0),
+                    v_cache.stride(0), kp_scene, keep_scene, out.data_ptr(), ws.data_ptr(), n,
+                    _t.stream(dev))
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        raise RuntimeError("gs_voxelizer: cached_attention has no gradients")

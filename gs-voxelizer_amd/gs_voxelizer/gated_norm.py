@@ -44,6 +44,11 @@ def gated_residual_norm(x: Tensor, branch: Tensor, weight: Tensor, *,
                                  float(eps))
         if out:
             return tuple(out)
+    return _GatedNorm.apply(x, branch, weight, branch_weight, scale, gate, scene_starts, eps)
+
+
+def _checked(x, branch, weight, branch_weight, scale, gate, scene_starts, eps):
+    """The starts that matter, and what else _args takes."""
     _t.activations(x, "x", 2)
     _t.activations(branch, "branch", 2)
     dev, (T, C) = x.device, x.shape
@@ -72,11 +77,7 @@ def gated_residual_norm(x: Tensor, branch: Tensor, weight: Tensor, *,
     _t.check(eps >= 0, f"eps must not be negative, got {eps}")
     if gate is None or per_token:
         starts, scenes = None, 1  # no value depends on the scenes
-    opts = (per_token, scenes, float(eps))
-    tensors = (x, branch, weight, branch_weight, scale, gate)
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)):
-        return _forward(*tensors, starts, opts)
-    return _GatedNorm.apply(*tensors, starts, opts)
+    return starts, (per_token, scenes, float(eps))
 
 
 def _args(x, branch, weight, branch_weight, scale, gate, starts, opts):
@@ -110,11 +111,11 @@ def _forward(x, branch, weight, branch_weight, scale, gate, starts, opts):
 
 class _GatedNorm(Function):
     @staticmethod
-    def forward(ctx, x, branch, weight, branch_weight, scale, gate, starts, opts):
-        ctx.opts = opts
+    def forward(ctx, x, branch, weight, branch_weight, scale, gate, scene_starts, eps):
+        starts, ctx.opts = _checked(x, branch, weight, branch_weight, scale, gate, scene_starts, eps)
         ctx.save_for_backward(x, branch, weight, branch_weight, scale, gate, starts)
         ctx.set_materialize_grads(False)
-        return _forward(x, branch, weight, branch_weight, scale, gate, starts, opts)
+        return _forward(x, branch, weight, branch_weight, scale, gate, starts, ctx.opts)
 
     @staticmethod
     @_t.once

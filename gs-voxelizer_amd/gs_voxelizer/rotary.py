@@ -47,6 +47,13 @@ def rotate_qk(q: Tensor, k: Optional[Tensor], positions: Tensor, frequencies: Te
         out = _native.rotate(q, k, positions, frequencies, bool(interleaved))
         if out:
             return tuple(out)
+    _t.fixed(positions, "positions", "")
+    _t.fixed(frequencies, "frequencies", "")
+    return _RotateQK.apply(q, k, positions, frequencies, bool(interleaved))
+
+
+def _checked(q, k, positions, frequencies):
+    """The frequencies as the kernel takes them."""
     _t.activations(q, "q", 3)
     dev = q.device
     if k is not None:
@@ -58,7 +65,6 @@ def rotate_qk(q: Tensor, k: Optional[Tensor], positions: Tensor, frequencies: Te
         _t.check(isinstance(t, Tensor) and t.dtype == torch.float32 and t.dim() == 2,
                  f"{what} must be a 2-D float32 tensor")
         _t.check(t.device == dev, f"{what} must be on {dev}, got {t.device}")
-        _t.fixed(t, what, "")
     A, P = frequencies.shape
     _t.check(tuple(positions.shape) == (T, A),
              f"positions must have shape {(T, A)}, got {tuple(positions.shape)}")
@@ -67,10 +73,7 @@ def rotate_qk(q: Tensor, k: Optional[Tensor], positions: Tensor, frequencies: Te
     _t.check(D <= 1024, f"at most 1024 channels, got {D}")
     _t.check(q.shape[1] + (0 if k is None else k.shape[1]) <= 4096, "at most 4096 heads")
     _t.check(T <= _t.MAX_TOKENS, "too many tokens")
-    frequencies = frequencies.contiguous()
-    if not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
-        return _turn(q, k, positions, frequencies, interleaved, False)
-    return _RotateQK.apply(q, k, positions, frequencies, bool(interleaved))
+    return frequencies.contiguous()
 
 
 def _turn(q, k, positions, frequencies, interleaved, inverse):
@@ -99,6 +102,7 @@ def _turn(q, k, positions, frequencies, interleaved, inverse):
 class _RotateQK(Function):
     @staticmethod
     def forward(ctx, q, k, positions, frequencies, interleaved):
+        frequencies = _checked(q, k, positions, frequencies)
         ctx.interleaved = interleaved
         ctx.save_for_backward(positions, frequencies)
         ctx.set_materialize_grads(False)

@@ -375,3 +375,79 @@ def test_a_captured_training_step(device, route, scenes):
         got = [t.clone() for t in out]
         for a, b in zip(got, step()):
             assert torch.equal(a, b), n
+
+
+# ---- traces, modes and transforms
+
+
+@pytest.fixture(params=["rotary", "norm", "attention", "attention with grad", "cached"])
+def operator(request, device):
+    """(a call of one operator on a (6, 4, 32) tensor, that tensor)."""
+    g = _gen(device, 9)
+    pos, f = torch.rand(6, 3, generator=g, device=device), rotary.axis_frequencies((6, 5, 5), device=device)
+    w, cache = torch.rand(32, device=device), torch.randn(6, 9, 2, 32, generator=g, device=device)
+    n = torch.tensor([0, 1, 5, 9, 9, 3], dtype=torch.int32, device=device)
+    starts = torch.tensor([0, 2, 6], dtype=torch.int32, device=device)
+    slopes = torch.rand(4, generator=g, device=device)
+
+    def scene(q):
+        return attention.scene_attention(q, q[:, :2], q[:, 2:], scene_starts=starts, causal=True, cap=9.0,
+                                         positions=pos, slopes=slopes)
+
+    call = {"rotary": lambda q: rotary.rotate_qk(q, q[:, :2], pos, f)[1],
+            "norm": lambda q: gated_norm.gated_residual_norm(q[:, 0], q[:, 1], w, scale=w, gate=q[:2, 2],
+                                                             scene_starts=starts)[1],
+            "attention": scene, "attention with grad": scene,
+            "cached": lambda q: attention.cached_attention(q, cache, cache, n)}[request.param]
+    q = torch.randn(6, 4, 32, generator=g, device=device)
+    return call, q.requires_grad_(request.param == "attention with grad")
+
+
+def test_a_trace_replays_on_other_values(operator, request):
+    """A traced call is recorded with its checks: other inputs give their own results; a count of tokens that
+    the other tensors do not have is refused before anything is launched, and one that they allow (the
+    norm's starts end with the rows) is taken."""
+    call, q = operator
+    traced = torch.jit.trace(call, (q,), check_trace=False)
+    for n in range(3):
+        x = (q.detach() * (n + 2)).requires_grad_(q.requires_grad)
+        assert torch.equal(traced(x), call(x)), n
+    x = q.detach()[:5].contiguous().requires_grad_(q.requires_grad)
+    if request.node.callspec.params["operator"] == "norm":
+        assert torch.equal(traced(x), call(x))
+    else:
+        with pytest.raises(RuntimeError, match="ValueError|must|need"):
+            traced(x)
+
+
+def test_modes_and_transforms(operator):
+    """Dispatch and function modes change nothing; what has no rule here raises, and loses nothing silently."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.autograd import forward_ad
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Dispatch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    class Functions(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    call, q = operator
+    want = call(q)
+    for mode in (Dispatch, Functions):
+        with mode():
+            assert torch.equal(call(q), want), mode
+    x = q.detach()
+    with forward_ad.dual_level():
+        assert torch.equal(call(x), want)  # no tangent: nothing to lose
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            call(forward_ad.make_dual(x, x))
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.vmap(call)(torch.stack((x, x)))
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(call, (x,), (x,))
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode, pytest.raises(RuntimeError):
+        call(mode.from_tensor(x))
