@@ -213,21 +213,23 @@ template <typename F> void attention_variant(const AttnArgs &a, int dtype, F &f)
     else attention_channels<float>(a, f);
 }
 
-// Workgroups of 128 rows of one head, a mean scene's and all scenes'.
-inline int64_t attention_tiles(const AttnArgs &a, bool mean) {
-    const int64_t each = (int64_t)a.q_tokens / a.scenes / 128 * a.heads;
-    return mean ? each : ((int64_t)a.q_tokens / 128 + a.scenes) * a.heads;
+// Workgroups of 128 rows of one head, all scenes'.
+inline int64_t attention_tiles(const AttnArgs &a) {
+    return ((int64_t)a.q_tokens / 128 + a.scenes) * a.heads;
 }
-// Whether a wave takes two heads (for their distances): where a scene's workgroups fill two a CU
-// all the same.  One scene, 8 heads of 64: 16,000 tokens take 0.93 ms in pairs and 1.17 without, 6,000
-// 0.27 and 0.22; 8 scenes of 1,000, 16 heads 0.15 and 0.11.
+// Whether a wave takes two heads (for their distances): where the workgroups of one head pass a round of
+// three a CU, so that half as many, each 1.7 times as long, end sooner.  Not under a causal mask, whose
+// workgroups differ in length and fill the rounds' ends better the smaller they are, nor for short scenes, whose
+// last tiles are part empty.  8 heads of 64, forward: one scene of 12,000 tokens (752 workgroups) takes 687 us in
+// pairs and 585 without, 14,000 (880) 830 and 920, 16,000 913 and 1,059, and causal 703 and 521; 8 scenes of
+// 2,000 (1,064) 133 and 148; 32 scenes of 1,000, 16 heads 273 and 293; 200 scenes of 200 81 and 76.
 inline bool attention_pairs(const AttnArgs &a) {
-    return a.heads % 2 == 0 && attention_tiles(a, true) >= 2 * 448;
+    return a.heads % 2 == 0 && !a.causal && attention_tiles(a) > 3 * 256 && a.q_tokens / a.scenes >= 512;
 }
 // Whether rows are so few that the waves of a workgroup share them and split the keys: below three
 // workgroups of 128 rows for four CUs.  8 heads of 64, one scene: 500 tokens forward 13 us so and 22
 // otherwise, 2,000 36 and 66, 4,000 118 and 110.
-inline bool attention_few(const AttnArgs &a) { return attention_tiles(a, false) < 192; }
+inline bool attention_few(const AttnArgs &a) { return attention_tiles(a) < 192; }
 // Whether a scene's bfloat16 weights and ds enter the products in two parts (16 bits): where its rows see
 // too few keys to average their roundings.  The gradients of scenes of two tokens are 0.0017 off (2-norm:
 // the rounding of the results) so and 0.0025 in one part, of 64 tokens 0.0017 and 0.0024.  Its own keys alone

@@ -451,3 +451,39 @@ def test_modes_and_transforms(operator):
         torch.func.jvp(call, (x,), (x,))
     with FakeTensorMode(allow_non_fake_inputs=True) as mode, pytest.raises(RuntimeError):
         call(mode.from_tensor(x))
+
+
+# ---- long scenes, through the kernels of large calls, elementwise
+
+
+def _within(c, what):
+    got, (val, tol) = _run(c), R.attention(**c)
+    for n in got:
+        R.assert_within(got[n], val[n], tol[n], f"{what} {n}")
+    return got
+
+
+@TYPES
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("causal,cap,bias", [(False, 0.0, True), (True, 30.0, True), (True, 0.0, False)])
+def test_long_scenes(device, dtype, dim, causal, cap, bias):
+    c = _case(device, dtype, [2600, 900], 8, 2, dim, causal=causal, cap=cap, bias=bias)
+    if causal:
+        c["prefix"] = torch.tensor([600, 0], dtype=torch.int32, device=device)
+    c["keep"] = torch.rand(3500, generator=_gen(device, 1), device=device) >= 0.05
+    _within(c, "long")
+
+
+@pytest.mark.parametrize("kv", [8, 4, 1], ids=lambda k: f"kv{k}")
+@pytest.mark.parametrize("dim,cap", [(32, 9.0), (64, 9.0), (64, 0.0)])
+def test_pairs_of_heads_over_several_scenes(device, kv, dim, cap):
+    """Two heads of a wave share their distances, also where no scene alone would fill the chip; the results
+    of a training call and of one without gradients are the same bits."""
+    c = _case(device, BF16, [2000, 511, 2300, 1500], 24, 3 * kv, dim, cap=cap)
+    c["keep"] = torch.rand(6311, generator=_gen(device, 1), device=device) >= 0.05
+    got = _within(c, "pairs")
+    with torch.no_grad():
+        again = attention.scene_attention(
+            c["q"], c["k"], c["v"], scene_starts=c["q_starts"], cap=cap, positions=c["q_positions"],
+            slopes=c["slopes"], keep=c["keep"])
+    assert torch.equal(again, got["out"])
