@@ -145,7 +145,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
             live = next_live;
             if (more) fetch(b ^ 1, j0 + KB);
             if (j0 < mine) {
-                const bool masked = j0 + KB > all || (KB == 64 ? ~live : (uint32_t)~live) != 0;
+                // (a branch of its own for the scores of two parts costs long scenes 2 %)
+                const bool masked = fine || j0 + KB > all || (KB == 64 ? ~live : (uint32_t)~live) != 0;
 #pragma unroll 1
                 for (int kb = 0; kb < KB / 32; ++kb) {
                     f32x16 d = {}, w[HEADS] = {};
@@ -170,8 +171,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void k_att
 #pragma unroll
                             for (int r = 0; r < 16; ++r)
                                 if (!(seen & (1u << result_row(r)))) w[n][r] = -INFINITY;
+                        if (fine)
+#pragma unroll
+                            for (int n = 0; n < HEADS; ++n)
+#pragma unroll
+                                for (int r = 0; r < 16; ++r) w[n][r] *= unit;
                     }
-                    if (kExact || fine)
+                    if constexpr (kExact)
 #pragma unroll
                         for (int n = 0; n < HEADS; ++n)
 #pragma unroll

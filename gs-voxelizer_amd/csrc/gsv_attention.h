@@ -83,9 +83,12 @@ template <typename T, int DP> struct Tile {
         const int i = lane & 15, r4 = 4 * g + (i >> 2);
         col_at = r4 * kRowBytes + ((((lane >> 3) & 2) + ((i & 3) >> 1)) ^ turn(r4)) * 16 + (i & 1) * 8;
     }
-    // Lets the compiler know nothing of the columns' offset, in a loop over the parts of the weights: it
-    // would form all their addresses before the loop, and keep them in registers there are not.
-    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(col_at)); }
+    // At 128 channels, lets the compiler know nothing of the columns' offset in a loop over the parts of the
+    // weights: it would form all their addresses before the loop, and keep them in registers there are
+    // not.  (Below they fit; formed again for each block, they cost the forward 4 %.)
+    __device__ __forceinline__ void forget() {
+        if constexpr (DP == 128) asm volatile("" : "+v"(col_at));
+    }
     // An address in LDS, as a number.  A tile starts at a multiple of 1024 bytes, so a lane's part
     // `bits` from its first is (base + at) ^ bits or base + (at ^ bits).  The first form keeps one
     // register, the second one for each part and saves an instruction a read: 16,000 tokens, 64
