@@ -8,14 +8,16 @@
 // D_i is formed from o_i in two parts (out, and out_low, what its rounding took): where one key has
 // nearly all of a row's weight, do_i.v_j - D_i is a small difference, and 8 bits of o_i would leave
 // little of it.  Two kernels form the scores twice, one with the rows' sums (dq, D, dslope) and one with
-// the keys' (dk, dv): each sum stays in the registers of one wave, in a fixed order, with
-// no atomics and no partial gradients in memory.
+// the keys' (dk, dv): each sum stays in the registers of one wave, in a fixed order, with no atomics
+// (and partial gradients in memory only where few key tiles have many rows: bwd_parts).
 //
 // The rows' kernel does 6 dim operations an element in its products, the keys' 8 dim; both pay
 // the forward's vector instructions for an element's weight again and some for its gradient, and
 // two waves a SIMD (one at 128 channels, where dk and dv alone take 128 registers) overlap the two only
-// in part.  16,000 tokens, 8 heads of 64, bias, bfloat16: rows 1.36 ms (579 TFLOP/s), keys
-// 1.58 ms (665 TFLOP/s); 10,007 tokens in 4 causal scenes, 16 heads of 128 on 4, capped: 0.43 and 0.76 ms.
+// in part.  16,000 tokens, 8 heads of 64, bias, bfloat16: rows 1.44 ms (545 TFLOP/s; vector instructions issue in
+// 71 % of the cycles, the matrix units work in 30 %), keys 1.64 ms (639 TFLOP/s; 56 and 33 %).  8,001 tokens in
+// 8 scenes: 110 us each (43 and 13 %, 32 and 16 %, at 4.4 waves a CU).  10,007 tokens in 4 causal scenes, 16
+// heads of 128 on 4, capped: 414 us (54 and 23 %) and 673 us (35 and 17 %, one wave a SIMD: it waits).
 #include "gsv_attention.h"
 
 namespace gsv {
@@ -657,8 +659,9 @@ size_t delta_bytes(const AttnArgs &a) {
 // causal mask, a few of them have most of the work.  About four rounds of workgroups at one a CU
 // (128 channels), one at two a CU; eight parts at most, each with four tiles of a mean scene's
 // rows at least (sizes alone decide: the longest scene's length is a hint that changes no sum of these).
-// Partial sums then pass through memory: 10,007 tokens of 4 causal scenes, 16 heads on 4, 128
-// channels take 945 us in one part and 770 in four; 8 heads of 64, 8,001 tokens gain nothing.
+// Partial sums then pass through memory.  Training, against one part: 10,007 tokens of 4 causal scenes, 16
+// heads on 4, 128 channels 1,318 and 1,673 us, 3 scenes of 3,000, 8 heads of 64 on 1 602 and 1,359; 8 heads of 64
+// on 8, 8 scenes of 1,000, gain nothing (189 and 190).
 int bwd_parts(const AttnArgs &a, int elem) {
     const int64_t tiles = ((int64_t)a.k_tokens / kRows + a.scenes) * a.kv_heads;
     const int64_t want = (a.dim > 64 ? 1024 : 512) / tiles + (a.dim > 64);

@@ -11,9 +11,9 @@
 //   dbranch_weight = sum_s gate scale A, dweight = B
 // first over each workgroup's rows of one scene, then over workgroups, in a fixed order.
 //
-// 20,000 rows of 1024, bfloat16 with a float32 residual (246 MB forward, 369 backward): 48 us (5.1 TB/s) and
-// 97 (3.8 TB/s) + 16 for the sums.  200,000 rows of 500, bfloat16 (0.8 and 1.2 GB): 216 us (3.7 TB/s)
-// and 357 (3.4 TB/s) + 18.
+// 20,000 rows of 1024, bfloat16 with a float32 residual (246 MB forward, 369 backward): 49 us (5.0 TB/s) and
+// 75 (4.9 TB/s) + 13 for the sums.  200,000 rows of 500, bfloat16 (0.8 and 1.2 GB): 197 us (4.1 TB/s)
+// and 339 (3.5 TB/s) + 21.
 #include "gsv_device.h"
 
 namespace gsv {
@@ -382,8 +382,8 @@ void launch_bwd(const NormArgs &a, hipStream_t s) {
     else hipLaunchKernelGGL((k_norm_bwd<TX, TF, VEC, E, WAVES, false>), grid, dim3(256), 0, s, a);
 }
 // Channels of a lane and waves of a row.  The backward keeps eight vectors of them, so 8 channels a
-// lane (112 registers, four waves a SIMD) and more waves a row: 20,000 rows of 1024 take 97 us, with 16
-// channels a lane and one wave (190 registers) 140.
+// lane (105 registers, four waves a SIMD) and more waves a row: 20,000 rows of 1024 train in 127 us, with 16
+// channels a lane and one wave (190 registers) in 143; of 768 in 97 and 111.
 template <typename TX, typename TF, int VEC>
 void launch_width(const NormArgs &a, bool backward, hipStream_t s) {
     if (!backward) {

@@ -91,9 +91,9 @@ template <typename T, int DP> struct Tile {
     }
     // An address in LDS, as a number.  A tile starts at a multiple of 1024 bytes, so a lane's part
     // `bits` from its first is (base + at) ^ bits or base + (at ^ bits).  The first form keeps one
-    // register, the second one for each part and saves an instruction a read: 16,000 tokens, 64
-    // channels train in 3.8 against 4.0 ms; at 128 channels its registers do not fit (the rows'
-    // kernel of the backward takes 590 instead of 440 us for 10,007 tokens).
+    // register, the second one for each part and saves an instruction a read (5 % of the training time
+    // of 16,000 tokens, 64 channels, when it was chosen); at 128 channels its registers do not fit (the
+    // rows' kernel of the backward took 590 instead of 440 us for 10,007 tokens).
     static __device__ __forceinline__ uint32_t part(uint32_t base, uint32_t at, uint32_t bits) {
         return DP == 128 ? (base + at) ^ bits : base + (at ^ bits);
     }
@@ -230,8 +230,8 @@ inline bool attention_pairs(const AttnArgs &a) {
     return a.heads % 2 == 0 && !a.causal && attention_tiles(a) > 3 * 256 && a.q_tokens / a.scenes >= 512;
 }
 // Whether rows are so few that the waves of a workgroup share them and split the keys: below three
-// workgroups of 128 rows for four CUs.  8 heads of 64, one scene: 500 tokens forward 13 us so and 22
-// otherwise, 2,000 36 and 66, 4,000 118 and 110.
+// workgroups of 128 rows for four CUs.  8 heads of 64, one scene: 500 tokens forward 10 us so and 21
+// otherwise, 2,000 35 and 68, 2,900 68 and 94, 4,000 111 and 112, where training takes 455 and 381.
 inline bool attention_few(const AttnArgs &a) { return attention_tiles(a) < 192; }
 // Whether a scene's bfloat16 weights and ds enter the products in two parts (16 bits): where its rows see
 // too few keys to average their roundings.  The gradients of scenes of two tokens are 0.0017 off (2-norm:

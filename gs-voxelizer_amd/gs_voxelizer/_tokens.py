@@ -2,7 +2,7 @@
 
 A batch packs the tokens of several scenes in one array; ``scene_starts`` (scenes + 1,)
 int32 holds each scene's first row.  The first scene begins at row 0 and the last ends
-with the array; entries 0 and ``scenes`` are not read.  Errors are raised as ValueError
+with the array; entries 0 and ``scenes`` are not read, and the others ascend.  Errors are raised as ValueError
 before anything is launched; outputs and workspaces are torch tensors, and
 every kernel is enqueued on torch's current stream of the tensors' device.
 

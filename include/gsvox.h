@@ -366,8 +366,9 @@ int gsv_wave_timeline(int32_t kernel, uint64_t *records, int32_t capacity);
  * where its keys end).  A row that sees no key gives 0.
  * q_starts, k_starts: (scenes + 1) first rows of the scenes, ascending; the first scene
  * begins at row 0 and the last one ends with the arrays (entries 0 and `scenes` are not
- * read).  NULL only for one scene.  longest_q, longest_k: rows of the longest scene, 0 if
- * unknown; they only size the launch.  positions: rows of float x, y, z.
+ * read).  Entries that do not ascend can leave rows of the outputs unwritten; no access leaves
+ * the arrays for it.  NULL only for one scene.  longest_q, longest_k: rows of the longest scene,
+ * 0 if unknown: scenes of one length then take fewer workgroups.  positions: rows of float x, y, z.
  */
 typedef struct gsv_attention {
     const void *q, *k, *v;
