@@ -91,8 +91,7 @@ def scene_attention(q: Tensor, k: Tensor, v: Tensor, *, scene_starts: Optional[T
     _t.fixed(positions, "positions", "")
     _t.fixed(key_positions, "key_positions", "")
     return _SceneAttention.apply(q, k, v, slopes, scene_starts, key_starts, prefix, positions,
-                                 key_positions, keep, int(longest or 0), bool(causal), scale, cap,
-                                 torch.is_grad_enabled())
+                                 key_positions, keep, int(longest or 0), bool(causal), scale, cap)
 
 
 def _point(a, q, k, v, slopes):
@@ -160,10 +159,10 @@ def _checked(q, k, v, slopes, scene_starts, key_starts, prefix, positions, key_p
 class _SceneAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, scene_starts, key_starts, prefix, positions, key_positions,
-                keep, longest, causal, scale, cap, grad):
+                keep, longest, causal, scale, cap):
         a, q, k, v, slopes, held = _checked(q, k, v, slopes, scene_starts, key_starts, prefix, positions,
                                             key_positions, keep, longest, causal, scale, cap)
-        if not (grad and any(ctx.needs_input_grad[:4])):
+        if not any(ctx.needs_input_grad[:4]):
             return _forward(a, q, k, v, slopes, held, None, None)
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
         # what rounding took from the output: the backward needs it whole
@@ -188,7 +187,7 @@ class _SceneAttention(Function):
             _t.call("attention_bwd", ctypes.byref(a), out.data_ptr(), _t.ptr(low),
                     lse.data_ptr(), dout.data_ptr(), dout.stride(0), dout.stride(1), dq.data_ptr(), dk.data_ptr(),
                     dv.data_ptr(), _t.ptr(ds), ws.data_ptr(), n, _t.stream(dev))
-        return (dq, dk, dv, ds) + (None,) * 11
+        return (dq, dk, dv, ds) + (None,) * 10
 
 
 def cached_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor, *,

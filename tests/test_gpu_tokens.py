@@ -408,7 +408,7 @@ def test_a_trace_replays_on_other_values(operator, request):
     the other tensors do not have is refused before anything is launched, and one that they allow (the
     norm's starts end with the rows) is taken."""
     call, q = operator
-    traced = torch.jit.trace(call, (q,), check_trace=False)
+    traced = torch.jit.trace(call, (q,))
     for n in range(3):
         x = (q.detach() * (n + 2)).requires_grad_(q.requires_grad)
         assert torch.equal(traced(x), call(x)), n
