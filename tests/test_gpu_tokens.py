@@ -487,3 +487,35 @@ def test_pairs_of_heads_over_several_scenes(device, kv, dim, cap):
             c["q"], c["k"], c["v"], scene_starts=c["q_starts"], cap=cap, positions=c["q_positions"],
             slopes=c["slopes"], keep=c["keep"])
     assert torch.equal(again, got["out"])
+
+
+# ---- launches past a grid's x axis
+
+
+@pytest.mark.parametrize("longest", [None, 1], ids=["by tiles", "by slots"])
+@pytest.mark.parametrize("first", [1, 5000], ids=["even", "long first"])
+def test_hundreds_of_thousands_of_scenes(device, first, longest):
+    """More workgroups than the grid's x axis takes (four million), scenes looked for over three levels: a
+    token alone in its scene has its own value, and its gradient goes there."""
+    n, H, D = 300_000, 16, 8
+    starts = torch.cat((torch.zeros(1, device=device), first + torch.arange(n, device=device))).int()
+    T, g = n + first - 1, _gen(device, 10)
+    q, k, v, dout = (torch.randn(T, H, D, generator=g, device=device).to(BF16) for _ in range(4))
+    slopes = torch.full((H,), 0.1, device=device)
+    pos = torch.rand(T, 3, generator=g, device=device)
+    leaves = [t.requires_grad_() for t in (q, k, v, slopes)]
+    out = attention.scene_attention(*leaves[:3], scene_starts=starts, longest=longest, positions=pos,
+                                    slopes=leaves[3])
+    got = torch.autograd.grad(out, leaves, dout)
+    alone = slice(first if first > 1 else 0, None)
+    assert torch.equal(out[alone], v[alone]) and torch.equal(got[2][alone], dout[alone])
+    assert not got[0][alone].any() and not got[1][alone].any()
+    if first > 1:
+        one = attention.scene_attention(q[:first], k[:first], v[:first], positions=pos[:first], slopes=leaves[3])
+        assert off(out[:first], one.detach().double()) <= 2.0 ** -8
+    else:
+        assert not got[3].any()
+
+
+def test_norm_of_more_scenes_than_a_grid_s_axis(device):
+    norms._check(norms._case(device, 66_000, 8, [1] * 66_000, (F32, BF16)))
