@@ -195,6 +195,28 @@ def test_norm_packings(device, types, lengths):
             assert torch.equal(again[n], got[n]), (longest, n)
 
 
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (50.0, True)])
+def test_long_caches(device, dim, cap, bias):
+    """Over long caches too the results are as exact as their type."""
+    g, lengths, N = _gen(device, 5), [128, 129, 1000, 20_000], 20_000
+    H, K = 32, 4
+    q = torch.randn(4, H, dim, generator=g, device=device).to(BF16)
+    k, v = (torch.randn(4, N, K, dim, generator=g, device=device).to(BF16) for _ in "kv")
+    more = {}
+    if bias:
+        more = dict(positions=40 * torch.rand(4, 3, generator=g, device=device),
+                    key_positions=40 * torch.rand(4, N, 3, generator=g, device=device),
+                    slopes=torch.full((H,), 0.1, device=device).to(BF16))
+    got = attention.cached_attention(q, k, v, torch.tensor(lengths, dtype=torch.int32, device=device),
+                                     cap=cap, **more)
+    for s, n in enumerate(lengths):
+        ref = dict(q_positions=more["positions"][s:s + 1], k_positions=more["key_positions"][s, :n],
+                   slopes=more["slopes"]) if bias else {}
+        want = R.attention(q[s:s + 1], k[s, :n], v[s, :n], cap=cap, **ref)[0]["out"]
+        assert_rounded_once(got[s:s + 1], want, n)
+
+
 # ---- caps far above the scores
 
 
