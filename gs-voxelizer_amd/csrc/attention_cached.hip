@@ -6,8 +6,8 @@
 // have an order of magnitude to spare here).  A cache is split over workgroups, a split over
 // four waves that never wait for each other; a second kernel joins the splits.
 //
-// Two caches of 200,003 rows, 4 heads of 128, bfloat16 (316 MB of live rows): 62 us, 5.1 TB/s, and 5 us
-// for the join.  16 caches of 4,096, 2 heads of 64 (23 MB): 9.9 us and 3.9; there the time from
+// Two caches of 200,003 rows, 4 heads of 128, bfloat16 (316 MB of live rows): 65 us, 4.9 TB/s, and 5 us
+// for the join.  16 caches of 4,096, 2 heads of 64 (23 MB): 10.8 us and 3.9; there the time from
 // launch to the first bytes and a wave's few steps one after the other bound it.
 #include "gsv_attention.h"
 
