@@ -21,7 +21,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "gs_voxelizer", "libgsvox.so")
 AUTOGRAD = os.path.join(HERE, "gs_voxelizer", "_autograd.so")
 SOURCES = ["scan.hip", "project.hip", "binning.hip", "voxelize.hip", "rotary.hip",
-           "gated_norm.hip", "attention_fwd.hip", "attention_bwd.hip", "attention_cached.hip"]
+           "gated_norm.hip", "attention_fwd.hip", "attention_bwd.hip", "attention_cached.hip",
+           "attention_paged.hip", "paged_append.hip", "adamw.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

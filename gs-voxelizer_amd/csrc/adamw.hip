@@ -1,0 +1,355 @@
+// adamw.hip — one AdamW step over many tensors.
+//
+//   g' = g min(1, max_norm / (|all g| + 1e-6))
+//   m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
+//   w = w (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Bytes bound it: 28 an element in float32, or in bfloat16 with 32-bit masters.  The tensors' addresses and sizes
+// are a table in the kernel's own arguments, so a launch takes as many as fit there (kTensors) and copies
+// nothing to the device first; a workgroup finds its tensor from its number.  The norm needs all gradients before
+// the first update: a pass of its own, whose sums one workgroup adds up, and which the
+// update then reads again, from the caches where they hold it.
+#include "gsv_device.h"
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+
+namespace gsv {
+namespace {
+
+typedef __bf16 bf16;
+
+struct Entry {
+    void *p;
+    const void *g;
+    float *m, *v, *w;  // w: the 32-bit master, or unused
+    const float *lr_device;
+    int64_t n;
+    double lr;  // lr decay is formed in binary64: 1 less it is near 1
+    float decay, by_m, by_v;  // by_m = 1 / (1 - b1^t), by_v = 1 / sqrt(1 - b2^t)
+    int first;                // the tensor's first workgroup
+};
+constexpr int kTensors = 45;  // 80 bytes each: the arguments of a kernel end at 4 KB
+struct Table {
+    int count;
+    Entry t[kTensors];
+};
+struct Rates {
+    float b1, c1, b2, c2, eps;  // c = 1 - b
+    const float *shared;        // by_m, by_v, the gradients' factor; NULL: the entries', and 1
+    int counted;                // by_m and by_v are those of `shared`
+};
+
+// Elements of a thread's step: 16 bytes of the 32-bit arrays.
+constexpr int kVec = 4;
+template <typename T> struct __align__(sizeof(T) * kVec) Four {
+    T v[kVec];
+};
+
+__device__ __forceinline__ const Entry &entry_of(const Table &t, int block) {
+    int lo = 0, n = t.count;
+    while (n > 1) {
+        const int half = n / 2;
+        if (t.t[lo + half].first <= block) lo += half, n -= half;
+        else n = half;
+    }
+    return t.t[lo];
+}
+
+struct Step {
+    float b1, c1, b2, c2, eps, factor, keep, rate, by_v;
+};
+
+__device__ __forceinline__ void update(float g, float &m, float &v, float &w, const Step &s) {
+    g *= s.factor;
+    m = fmaf(s.b1, m, s.c1 * g);
+    v = fmaf(s.b2, v, s.c2 * (g * g));
+    w = fmaf(-s.rate, m / fmaf(sqrtf(v), s.by_v, s.eps), w * s.keep);
+}
+
+// STEPS: steps of a thread.  P, G: types of the param and its gradient; MASTER: a bfloat16 param's 32-bit copy.
+template <typename P, typename G, bool MASTER, int STEPS>
+__global__ __launch_bounds__(256) void k_adamw(const Table table, const Rates r) {
+    const Entry &e = entry_of(table, blockIdx.x);
+    const double lr = e.lr_device ? (double)*e.lr_device : e.lr;
+    Step s{r.b1, r.c1, r.b2, r.c2, r.eps, 1.f, (float)(1.0 - lr * (double)e.decay), 0.f, e.by_v};
+    float by_m = e.by_m;
+    if (r.shared) {
+        s.factor = r.shared[2];
+        if (r.counted) by_m = r.shared[0], s.by_v = r.shared[1];
+    }
+    s.rate = (float)(lr * (double)by_m);
+    P *const p = static_cast<P *>(e.p);
+    const G *const g = static_cast<const G *>(e.g);
+    float *const m = e.m, *const v = e.v, *const w = e.w;
+    const int64_t n = e.n, base = (int64_t)(blockIdx.x - e.first) * (256 * kVec * STEPS);
+    // An array off alignment, or the tensor's last elements: by single elements, 256 apart for a thread.
+    const bool wide = (reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v) |
+                       (MASTER ? reinterpret_cast<uintptr_t>(w) : 0)) % 16 == 0 &&
+                      reinterpret_cast<uintptr_t>(p) % sizeof(Four<P>) == 0 &&
+                      reinterpret_cast<uintptr_t>(g) % sizeof(Four<G>) == 0 && base + 256 * kVec * STEPS <= n;
+    Four<float> mm[STEPS], vv[STEPS], ww[STEPS];
+    Four<G> gg[STEPS];
+    Four<P> pp[STEPS];
+    if (wide) {
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+            const int64_t i = base + (k * 256 + threadIdx.x) * kVec;
+            gg[k] = *reinterpret_cast<const Four<G> *>(g + i);
+            mm[k] = *reinterpret_cast<const Four<float> *>(m + i);
+            vv[k] = *reinterpret_cast<const Four<float> *>(v + i);
+            if constexpr (MASTER) ww[k] = *reinterpret_cast<const Four<float> *>(w + i);
+            else pp[k] = *reinterpret_cast<const Four<P> *>(p + i);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+                const int64_t i = base + (k * kVec + j) * 256 + threadIdx.x;
+                if (i >= n) continue;
+                gg[k].v[j] = g[i], mm[k].v[j] = m[i], vv[k].v[j] = v[i];
+                if constexpr (MASTER) ww[k].v[j] = w[i];
+                else pp[k].v[j] = p[i];
+            }
+    }
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+            float wi = MASTER ? ww[k].v[j] : (float)pp[k].v[j];
+            update((float)gg[k].v[j], mm[k].v[j], vv[k].v[j], wi, s);
+            ww[k].v[j] = wi, pp[k].v[j] = (P)wi;
+        }
+        if (wide) {
+            const int64_t i = base + (k * 256 + threadIdx.x) * kVec;
+            *reinterpret_cast<Four<float> *>(m + i) = mm[k];
+            *reinterpret_cast<Four<float> *>(v + i) = vv[k];
+            *reinterpret_cast<Four<P> *>(p + i) = pp[k];
+            if constexpr (MASTER) *reinterpret_cast<Four<float> *>(w + i) = ww[k];
+        } else {
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+                const int64_t i = base + (k * kVec + j) * 256 + threadIdx.x;
+                if (i >= n) continue;
+                m[i] = mm[k].v[j], v[i] = vv[k].v[j], p[i] = pp[k].v[j];
+                if constexpr (MASTER) w[i] = ww[k].v[j];
+            }
+        }
+    }
+}
+
+// The sum over a workgroup of 256, in its first thread.
+__device__ __forceinline__ double block_sum(double x) {
+    __shared__ double part[4];
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) x += __shfl_xor(x, k);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// Sums of squares in binary64: no overflow, and no length at which the small terms are lost.
+constexpr int kNormSteps = 8;
+template <typename G> __global__ __launch_bounds__(256) void k_adamw_squares(const Table table, double *sums) {
+    const Entry &e = entry_of(table, blockIdx.x);
+    const G *const g = static_cast<const G *>(e.g);
+    constexpr int64_t kAll = 256 * kVec * kNormSteps;
+    const int64_t base = (int64_t)(blockIdx.x - e.first) * kAll;
+    double sum = 0.0;
+    if (reinterpret_cast<uintptr_t>(g) % sizeof(Four<G>) || base + kAll > e.n) {
+        const int64_t end = imin64(e.n, base + kAll);
+        for (int64_t i = base + threadIdx.x; i < end; i += 256) sum = fma((double)(float)g[i], (double)(float)g[i], sum);
+    } else {
+        Four<G> x[kNormSteps];
+#pragma unroll
+        for (int k = 0; k < kNormSteps; ++k)
+            x[k] = *reinterpret_cast<const Four<G> *>(g + base + (k * 256 + threadIdx.x) * kVec);
+#pragma unroll
+        for (int k = 0; k < kNormSteps; ++k)
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) sum = fma((double)(float)x[k].v[j], (double)(float)x[k].v[j], sum);
+    }
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) sums[blockIdx.x] = sum;
+}
+
+// What all tensors share, by one workgroup: the norm from the squares' sums, and the step that `counter` counts.
+__global__ __launch_bounds__(256) void k_adamw_shared(const double *sums, int count, double max_norm, double b1,
+                                                      double b2, int *counter, float *norm, float *shared) {
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < count; i += 256) sum += sums[i];
+    sum = block_sum(sum);
+    if (threadIdx.x) return;
+    if (max_norm > 0.0) {
+        const double all = sqrt(sum), by = max_norm / (all + 1e-6);
+        if (norm) *norm = (float)all;
+        shared[2] = by < 1.0 || by != by ? (float)by : 1.f;
+    } else {
+        shared[2] = 1.f;
+    }
+    if (counter) {
+        const int t = *counter + 1;
+        *counter = t;
+        shared[0] = (float)(1.0 / (1.0 - pow(b1, (double)t)));
+        shared[1] = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
+    }
+}
+
+struct Sizes {
+    int64_t elements, squares;  // workgroups of the norm's pass
+};
+
+constexpr int64_t kMostElements = (int64_t)1 << 34;  // (all workgroups of a launch then fit its grid)
+
+int adamw_check(const gsv_adamw_args *a, Sizes *out) {
+    if (!a || a->count < 0 || (a->count && !a->tensors) || !(a->beta1 >= 0 && a->beta1 < 1) ||
+        !(a->beta2 >= 0 && a->beta2 < 1) || !(a->eps >= 0) || !(a->max_norm >= 0))
+        return GSV_ERR_INVALID_ARGUMENT;
+    *out = Sizes{};
+    for (int64_t i = 0; i < a->count; ++i) {
+        const gsv_adamw_tensor &t = a->tensors[i];
+        if (t.numel < 0 || (!a->counter && t.step < 1) || (t.dtype != GSV_F32 && t.dtype != GSV_BF16) ||
+            (t.grad_dtype != GSV_F32 && t.grad_dtype != GSV_BF16) || (t.master && t.dtype != GSV_BF16))
+            return GSV_ERR_INVALID_ARGUMENT;
+        if (t.numel > kMostElements || out->elements > kMostElements) return GSV_ERR_SIZE_OVERFLOW;
+        if (t.numel == 0) continue;
+        const uintptr_t words = reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq) |
+                                reinterpret_cast<uintptr_t>(t.master) | reinterpret_cast<uintptr_t>(t.lr_device);
+        if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || words % 4 ||
+            reinterpret_cast<uintptr_t>(t.param) % (t.dtype == GSV_BF16 ? 2 : 4) ||
+            reinterpret_cast<uintptr_t>(t.grad) % (t.grad_dtype == GSV_BF16 ? 2 : 4))
+            return GSV_ERR_INVALID_ARGUMENT;
+        out->elements += t.numel;
+        out->squares += (t.numel + 256 * kVec * kNormSteps - 1) / (256 * kVec * kNormSteps);
+    }
+    if (out->elements > kMostElements) return GSV_ERR_SIZE_OVERFLOW;
+    return GSV_OK;
+}
+
+// Tables of the tensors that `takes`, each handed to `launch` with its workgroups when it is full.
+template <typename Takes, typename Launch>
+void tables(const gsv_adamw_args *a, int64_t per_block, const Takes &takes, const Launch &launch) {
+    Table t;
+    t.count = 0;
+    int64_t blocks = 0;
+    for (int64_t i = 0; i < a->count; ++i) {
+        const gsv_adamw_tensor &x = a->tensors[i];
+        if (!x.numel || !takes(x)) continue;
+        const int64_t own = (x.numel + per_block - 1) / per_block;
+        if (t.count == kTensors || (t.count && blocks + own > (1 << 23))) {
+            launch(t, blocks);
+            t.count = 0, blocks = 0;
+        }
+        float by_m = 1.f, by_v = 1.f;
+        if (!a->counter) {
+            by_m = (float)(1.0 / (1.0 - std::pow(a->beta1, (double)x.step)));
+            by_v = (float)(1.0 / std::sqrt(1.0 - std::pow(a->beta2, (double)x.step)));
+        }
+        t.t[t.count++] = Entry{x.param, x.grad, x.exp_avg, x.exp_avg_sq, x.master, x.lr_device, x.numel, x.lr,
+                               (float)x.weight_decay, by_m, by_v, (int)blocks};
+        blocks += own;
+    }
+    if (t.count) launch(t, blocks);
+}
+
+template <typename P, typename G, bool MASTER>
+void update_all(const gsv_adamw_args *a, const Rates &r, int steps, hipStream_t st) {
+    constexpr int p = sizeof(P) == 2 ? GSV_BF16 : GSV_F32, g = sizeof(G) == 2 ? GSV_BF16 : GSV_F32;
+    const auto takes = [](const gsv_adamw_tensor &t) {
+        return t.dtype == p && t.grad_dtype == g && (t.master != nullptr) == MASTER;
+    };
+    tables(a, 256 * kVec * steps, takes, [&](const Table &t, int64_t blocks) {
+        const dim3 grid((unsigned)blocks), block(256);
+        if (steps == 4) hipLaunchKernelGGL((k_adamw<P, G, MASTER, 4>), grid, block, 0, st, t, r);
+        else hipLaunchKernelGGL((k_adamw<P, G, MASTER, 1>), grid, block, 0, st, t, r);
+    });
+}
+
+template <typename G> void squares_all(const gsv_adamw_args *a, double *sums, int64_t *at, hipStream_t st) {
+    constexpr int g = sizeof(G) == 2 ? GSV_BF16 : GSV_F32;
+    tables(a, 256 * kVec * kNormSteps, [](const gsv_adamw_tensor &t) { return t.grad_dtype == g; },
+           [&](const Table &t, int64_t blocks) {
+               hipLaunchKernelGGL(k_adamw_squares<G>, dim3((unsigned)blocks), dim3(256), 0, st, t, sums + *at);
+               *at += blocks;
+           });
+}
+
+// Whether two tensors that the step writes share memory.
+bool written_twice(const gsv_adamw_args *a) {
+    struct Span {
+        uintptr_t first, end;
+    };
+    Span *spans = new (std::nothrow) Span[4 * a->count];
+    if (!spans) return true;
+    int64_t n = 0;
+    for (int64_t i = 0; i < a->count; ++i) {
+        const gsv_adamw_tensor &t = a->tensors[i];
+        if (!t.numel) continue;
+        const auto add = [&](const void *p, int64_t size) {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+            spans[n++] = Span{at, at + (uintptr_t)(t.numel * size)};
+        };
+        add(t.param, t.dtype == GSV_BF16 ? 2 : 4);
+        add(t.exp_avg, 4);
+        add(t.exp_avg_sq, 4);
+        if (t.master) add(t.master, 4);
+    }
+    std::sort(spans, spans + n, [](const Span &x, const Span &y) { return x.first < y.first; });
+    bool twice = false;
+    for (int64_t i = 1; i < n; ++i) twice |= spans[i].first < spans[i - 1].end;
+    delete[] spans;
+    return twice;
+}
+
+size_t squares_bytes(const Sizes &s) { return sizeof(double) * (size_t)s.squares; }
+
+}  // namespace
+}  // namespace gsv
+
+using namespace gsv;
+
+extern "C" int gsv_adamw_workspace_bytes(const gsv_adamw_args *args, size_t *bytes) {
+    Sizes s;
+    if (!bytes) return GSV_ERR_INVALID_ARGUMENT;
+    const int st = adamw_check(args, &s);
+    if (st != GSV_OK) return st;
+    *bytes = args->max_norm > 0 || args->counter ? (args->max_norm > 0 ? squares_bytes(s) : 0) + 4 * sizeof(float) : 0;
+    return GSV_OK;
+}
+
+extern "C" int gsv_adamw(const gsv_adamw_args *args, void *workspace, size_t workspace_bytes, void *stream) {
+    Sizes s;
+    size_t need;
+    int st = adamw_check(args, &s);
+    if (st != GSV_OK) return st;
+    if ((st = gsv_adamw_workspace_bytes(args, &need)) != GSV_OK) return st;
+    if (need > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
+    if ((need && !workspace) || reinterpret_cast<uintptr_t>(workspace) % 16 || written_twice(args))
+        return GSV_ERR_INVALID_ARGUMENT;
+    hipStream_t stm = as_stream(stream);
+    float *shared = nullptr;
+    if (need) {
+        double *sums = static_cast<double *>(workspace);
+        int64_t count = 0;
+        if (args->max_norm > 0) {
+            squares_all<float>(args, sums, &count, stm);
+            squares_all<bf16>(args, sums, &count, stm);
+        }
+        shared = reinterpret_cast<float *>(static_cast<char *>(workspace) + need - 4 * sizeof(float));
+        hipLaunchKernelGGL(k_adamw_shared, dim3(1), dim3(256), 0, stm, sums, (int)count, args->max_norm, args->beta1,
+                           args->beta2, args->counter, args->norm, shared);
+    }
+    const Rates r{(float)args->beta1, (float)(1.0 - args->beta1), (float)args->beta2, (float)(1.0 - args->beta2),
+                  (float)args->eps, shared, args->counter != nullptr};
+    // Elements of a workgroup: 1,024, and 4,096 (more loads at once) where that leaves workgroups enough.
+    const int steps = s.elements >= (int64_t)4096 * 2048 ? 4 : 1;
+    update_all<float, float, false>(args, r, steps, stm);
+    update_all<float, bf16, false>(args, r, steps, stm);
+    update_all<bf16, float, false>(args, r, steps, stm);
+    update_all<bf16, bf16, false>(args, r, steps, stm);
+    update_all<bf16, float, true>(args, r, steps, stm);
+    update_all<bf16, bf16, true>(args, r, steps, stm);
+    return check_launch();
+}

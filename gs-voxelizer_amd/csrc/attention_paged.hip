@@ -1,0 +1,127 @@
+// attention_paged.hip — one query token a scene against a cache whose rows lie in pages.
+//
+// The kernel is gsv_cached.h's: a page holds a multiple of 16 rows, so 16 rows of a step have one page, whose
+// first row is the base of their copy.  A table names the pages of a scene; a wave reads the entries of 32 of its
+// steps by one load, 32 steps ahead.  Scenes of a batch differ in length, and their lengths are known on
+// the device alone: every workgroup forms the pieces that the batch's rows are cut into, all of one
+// size, and takes its own (paged_piece).
+#include "gsv_cached.h"
+
+// (a product and a difference stay two roundings where they are written as two)
+#pragma clang fp contract(off)
+
+namespace gsv {
+namespace {
+
+// One workgroup a scene and head; scenes of one piece have their row already.
+template <typename T>
+__global__ __launch_bounds__(256) void k_paged_join(const AttnArgs a, const CacheArgs c, T *__restrict__ out) {
+    const int64_t row = blockIdx.x;
+    const int s = row / a.heads, h = row % a.heads;
+    const int2 p = scene_pieces(a, c, s);
+    if (p.y == 1) return;
+    join_row<T>(c.part_o, c.part_ms, (int64_t)p.x * a.heads + h, a.heads, p.y, a.dim, out + row * a.dim);
+}
+
+// Pieces that the batch's rows are cut into (and one more a scene at most, for the remainders), or 0 where scenes
+// stay whole: one round of workgroups, as many as the CUs hold at once, each with a step at
+// least for all its waves.
+int paged_pieces(const AttnArgs &a, int head_tiles, int dtype) {
+    const int64_t size = dtype == GSV_BF16 ? 2 : 4, dp = a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : 128;
+    const int64_t waves = dp * size > 256 ? 2 : 4;
+    if (a.k_tokens <= waves * kKeys) return 0;
+    const int64_t lds = waves * (4 * kKeys * dp * size + (a.slopes ? 6 * kKeys * (size == 2 ? 16 : 4) : 0)) + 2048;
+    const int64_t round = 256 * imin64(163840 / lds, 4);
+    const int64_t most = ((int64_t)a.k_tokens + waves * kKeys - 1) / (waves * kKeys) * a.scenes;
+    return (int)imax64(1, imin64(round / ((int64_t)a.kv_heads * head_tiles), most));
+}
+
+struct Paged {
+    const AttnArgs &a;
+    const CacheArgs &c;
+    void *out;
+    hipStream_t st;
+    template <typename T, int DP, bool FAR, int CAP> void run() const {
+        T *o = static_cast<T *>(out);
+        const int64_t pieces = (int64_t)a.scenes + c.even;
+        hipLaunchKernelGGL((k_attention_cached<T, DP, FAR, CAP, true>),
+                           dim3((unsigned)(pieces * a.kv_heads * c.head_tiles)), dim3(64 * kWaves<T, DP>), 0,
+                           st, a, c, o);
+        if (c.even)
+            hipLaunchKernelGGL(k_paged_join<T>, dim3((unsigned)(a.scenes * a.heads)), dim3(256), 0, st, a, c, o);
+    }
+};
+
+int paged_plan(const gsv_attention *args, const gsv_pages *p, AttnArgs *a, CacheArgs *c) {
+    if (!args || !p || args->causal || args->prefix || args->q_starts || args->k_starts ||
+        args->scenes < 0 || args->scenes != args->q_tokens || p->pages < 1 || p->page_rows < kPageUnit ||
+        p->page_rows % kPageUnit || p->table_pages < 0 || p->table_row < 0)
+        return GSV_ERR_INVALID_ARGUMENT;
+    const int64_t rows = (int64_t)p->page_rows * p->table_pages;
+    if (rows > GSV_MAX_TOKENS) return GSV_ERR_SIZE_OVERFLOW;
+    gsv_attention one = *args;
+    one.scenes = 1;  // rows are addressed by scene and page here, not packed
+    one.k = p->k, one.v = p->v, one.k_positions = p->positions, one.k_pos_row = p->pos_row;
+    one.k_row = p->k_row, one.v_row = p->v_row, one.k_head = p->k_head, one.v_head = p->v_head;
+    one.keep = p->keep, one.keep_bytes = p->keep_bytes;
+    one.k_tokens = (int)rows;
+    const int st = attention_args(&one, a);
+    if (st != GSV_OK) return st;
+    a->scenes = args->scenes;
+    const int64_t tiles = (a->heads / a->kv_heads + kHeads - 1) / kHeads;
+    if ((int64_t)a->scenes * a->kv_heads * tiles > (1 << 22) || (int64_t)a->scenes * a->heads >= (1 << 24))
+        return GSV_ERR_SIZE_OVERFLOW;
+    *c = CacheArgs{};
+    c->head_tiles = (int)tiles;
+    c->even = a->scenes ? paged_pieces(*a, (int)tiles, args->dtype) : 0;
+    c->splits = c->even ? 2 : 1;
+    return GSV_OK;
+}
+
+size_t part_rows(const AttnArgs &a, const CacheArgs &c) {
+    return c.even ? ((size_t)a.scenes + c.even) * a.heads : 0;
+}
+
+}  // namespace
+}  // namespace gsv
+
+using namespace gsv;
+
+extern "C" int gsv_attention_paged_workspace_bytes(const gsv_attention *args, const gsv_pages *pages,
+                                                   size_t *bytes) {
+    AttnArgs a;
+    CacheArgs c;
+    if (!bytes) return GSV_ERR_INVALID_ARGUMENT;
+    const int st = paged_plan(args, pages, &a, &c);
+    if (st != GSV_OK) return st;
+    *bytes = part_rows(a, c) * (sizeof(float) * a.dim + sizeof(float2));
+    return GSV_OK;
+}
+
+extern "C" int gsv_attention_paged(const gsv_attention *args, const gsv_pages *pages, const int32_t *lengths,
+                                   void *out, void *workspace, size_t workspace_bytes, void *stream) {
+    AttnArgs a;
+    CacheArgs c;
+    int st = paged_plan(args, pages, &a, &c);
+    if (st != GSV_OK) return st;
+    if (a.scenes == 0) return GSV_OK;
+    const size_t rows = part_rows(a, c), need = rows * (sizeof(float) * a.dim + sizeof(float2));
+    if (need > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
+    const int64_t chunk = args->dtype == GSV_BF16 ? 8 : 4;
+    c.k_scene = used_stride(pages->k_page, pages->pages);
+    c.v_scene = used_stride(pages->v_page, pages->pages);
+    if (!lengths || (pages->table_pages && !pages->table) || !out || (need && !workspace) ||
+        c.k_scene % chunk || c.v_scene % chunk || reinterpret_cast<uintptr_t>(out) % 16 ||
+        reinterpret_cast<uintptr_t>(workspace) % 16)
+        return GSV_ERR_INVALID_ARGUMENT;
+    c.lengths = lengths;
+    c.k_pos_scene = pages->pos_page, c.keep_scene = pages->keep_page;
+    c.part_o = static_cast<float *>(workspace);  // a multiple of 32 bytes
+    c.part_ms = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + sizeof(float) * rows * a.dim);
+    c.table = pages->table, c.table_row = pages->table_row;
+    c.pages = pages->pages, c.page_rows = pages->page_rows;
+    c.by_rows = make_fastdiv(pages->page_rows);
+    Paged f{a, c, out, as_stream(stream)};
+    attention_variant(a, args->dtype, f);
+    return check_launch();
+}

@@ -39,7 +39,9 @@ using torch::autograd::variable_list;
     X(gsv_voxelize_bwd_workspace_bytes) X(gsv_voxelize_bwd) X(gsv_voxelize_bwd_l1)                 \
     X(gsv_rotary) X(gsv_gated_norm_fwd) X(gsv_gated_norm_bwd_workspace_bytes)                      \
     X(gsv_gated_norm_bwd) X(gsv_attention_fwd) X(gsv_attention_bwd_workspace_bytes)                \
-    X(gsv_attention_bwd) X(gsv_attention_cached_workspace_bytes) X(gsv_attention_cached)
+    X(gsv_attention_bwd) X(gsv_attention_cached_workspace_bytes) X(gsv_attention_cached)       \
+    X(gsv_attention_paged_workspace_bytes) X(gsv_attention_paged) X(gsv_paged_append)              \
+    X(gsv_adamw_workspace_bytes) X(gsv_adamw)
 struct Library {
 #define GSV_FIELD(name) decltype(&::name) name = nullptr;
     GSV_ENTRIES(GSV_FIELD)
@@ -474,6 +476,8 @@ std::tuple<int64_t, std::vector<Tensor>> voxelize(
 }  // namespace
 
 #include "autograd_tokens.h"
+#include "autograd_paged.h"
+#include "autograd_adamw.h"
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.attr("torch_version") = GSV_TORCH_VERSION;  // the torch it was compiled against
@@ -484,4 +488,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("gated_norm", &gated_norm, py::call_guard<py::gil_scoped_release>());
     m.def("scene_attention", &scene_attention, py::call_guard<py::gil_scoped_release>());
     m.def("cached_attention", &cached_attention, py::call_guard<py::gil_scoped_release>());
+    m.def("append_tokens", &append_tokens, py::call_guard<py::gil_scoped_release>());
+    m.def("paged_attention", &paged_attention, py::call_guard<py::gil_scoped_release>());
+    m.def("adamw_step", &adamw_step, py::call_guard<py::gil_scoped_release>());
 }

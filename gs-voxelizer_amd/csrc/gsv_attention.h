@@ -380,11 +380,14 @@ template <typename T, int DP, int ROWS, int WAVES> struct Copy {
             at[i] = col < dim ? (uint32_t)(row * (int)stride + col) * (uint32_t)sizeof(T) : kNowhere;
         }
     }
-    // rows: live rows from base on, 1 at least; with `some`, those whose bit is set in `live`
+    // rows: live rows from base on, 1 at least (with NONE, none where it is 0 or less); with `some`, those whose
+    // bit is set in `live`
+    template <bool NONE = false>
     __device__ __forceinline__ void start(T *tile, const T *base, int64_t stride, int dim, int rows,
                                           bool some, uint64_t live, int wave, int lane) const {
         // (the same in all lanes, but loaded in a loop: said so, it lies in scalar registers)
-        const int bytes = __builtin_amdgcn_readfirstlane(((min(rows, ROWS) - 1) * (int)stride + dim) * (int)sizeof(T));
+        int bytes = __builtin_amdgcn_readfirstlane(((min(rows, ROWS) - 1) * (int)stride + dim) * (int)sizeof(T));
+        if (NONE && rows <= 0) bytes = 0;
         const uint64_t p = reinterpret_cast<uintptr_t>(base);
         const uint64_t first_byte = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
                                     (uint32_t)__builtin_amdgcn_readfirstlane((int)p);

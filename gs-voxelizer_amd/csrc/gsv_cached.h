@@ -1,0 +1,390 @@
+// gsv_cached.h — the kernel of one query token a scene against a cache of keys and values, whose rows
+// lie together (attention_cached.hip) or in pages that a table names (attention_paged.hip).
+//
+// Same scores as attention_fwd.hip.  The bytes of the cache are the floor: each is read
+// once, by coalesced 16-byte loads, and serves all query heads of its key head, which
+// are the columns of a matrix product (32, those past the group idle: the matrix units
+// have an order of magnitude to spare here).  A cache is split over workgroups, a split over
+// four waves that never wait for each other; a second kernel joins the splits.
+#pragma once
+
+#include "gsv_attention.h"
+
+// (a product and a difference stay two roundings where they are written as two)
+#pragma clang fp contract(off)
+
+namespace gsv {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kKeys = 32;   // keys of a wave's step
+constexpr int kHeads = 32;  // query heads of a workgroup
+constexpr float kSlack = 8.f;
+constexpr int kPageUnit = 16;  // a page holds a multiple of so many rows: a copy never leaves one
+
+struct CacheArgs {
+    const int *lengths;
+    // strides from scene to scene, or from page to page
+    int64_t k_scene, v_scene, k_pos_scene, keep_scene;
+    int splits, head_tiles;  // splits: of each scene; of paged scenes, 1 where none is split
+    float *part_o;   // (scenes, heads, splits, dim) or (pieces, heads, dim): sums of weights times values
+    float2 *part_ms; // the same but the channels: maximum (log2) and sum of weights
+    // paged: scene s's row j is row j % page_rows of page table[s table_row + j / page_rows]
+    const int *table;
+    int64_t table_row;
+    int pages, page_rows;
+    FastDiv by_rows;
+    int even;  // pieces of a batch without remainders (paged_piece)
+};
+
+// A paged scene's keys, begin .. end - 1 of one of its `count` pieces; s < 0: no scene's.
+struct Piece {
+    int s, begin, end, count;
+};
+__device__ __forceinline__ int live_rows(const AttnArgs &a, const CacheArgs &c, int s) {
+    return s < a.scenes ? min(max(c.lengths[s], 0), a.k_tokens) : 0;
+}
+// Keys of a piece: the batch's rows over `even`, a multiple of a wave's step, so that a batch has at most
+// even + scenes pieces (a scene of len rows has less than len / per + 1, and one at least).  A lane
+// adds its scenes' rows as integers; the wave's sum of 64 floats is raised by more than its roundings.
+__device__ __forceinline__ int paged_rows(const AttnArgs &a, const CacheArgs &c, int each, int lane) {
+    int64_t mine = 0;
+    for (int i = 0; i < each; ++i) mine += live_rows(a, c, lane * each + i);
+    const float rows = wave_sum((float)mine) * 1.000002f;
+    return (int)imin64((int64_t)(rows / (float)c.even * 1.000002f) / kKeys * kKeys + kKeys, INT32_MAX);
+}
+// (an empty scene has a piece, which writes its zeros)
+__device__ __forceinline__ int pieces_of(int len, int per) { return len > 0 ? (len - 1) / per + 1 : 1; }
+// Piece n of the batch: of the scenes one after the other.  A lane counts those of a run of scenes, so that
+// up to 64 scenes take one load and a scan over the lanes.
+__device__ __forceinline__ Piece paged_piece(const AttnArgs &a, const CacheArgs &c, int n) {
+    if (c.splits == 1) return {n, 0, __builtin_amdgcn_readfirstlane(live_rows(a, c, n)), 1};
+    const int lane = threadIdx.x & 63, each = (a.scenes + 63) / 64;
+    const int per = __builtin_amdgcn_readfirstlane(paged_rows(a, c, each, lane));
+    int mine = 0;
+    for (int i = 0; i < each; ++i)
+        if (lane * each + i < a.scenes) mine += pieces_of(live_rows(a, c, lane * each + i), per);
+    int last = mine;  // pieces up to this lane's scenes
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+        const int x = __shfl_up(last, k);
+        if (lane >= k) last += x;
+    }
+    const uint64_t past = __ballot(last > n);
+    if (!past) return {-1, 0, 0, 0};
+    const int holder = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(past));
+    n -= __builtin_amdgcn_readlane(last - mine, holder);
+    for (int s = holder * each;; ++s) {
+        const int len = __builtin_amdgcn_readfirstlane(live_rows(a, c, s)), count = pieces_of(len, per);
+        // (the holder's pieces are more than n; the bound only makes the loop's end plain)
+        if (n < count || s + 1 >= a.scenes) return {s, n * per, len - n * per > per ? n * per + per : len, count};
+        n -= count;
+    }
+}
+// The first piece of scene s, and how many it has.
+__device__ __forceinline__ int2 scene_pieces(const AttnArgs &a, const CacheArgs &c, int s) {
+    const int lane = threadIdx.x & 63, each = (a.scenes + 63) / 64;
+    const int per = __builtin_amdgcn_readfirstlane(paged_rows(a, c, each, lane));
+    int before = 0;
+    for (int i = 0; i < each; ++i)
+        if (lane * each + i < s) before += pieces_of(live_rows(a, c, lane * each + i), per);
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) before += __shfl_xor(before, k);
+    return make_int2(before, pieces_of(live_rows(a, c, s), per));
+}
+
+// Waves of a workgroup: four, two where their tiles would pass the LDS of a CU.
+template <typename T, int DP> constexpr int kWaves = DP * sizeof(T) > 256 ? 2 : 4;
+
+// bfloat16 weights enter the product with the values in two parts: the results are as exact as their type
+// (0.0017 in the 2-norm, in one part 0.0018 to 0.0020), for 0 to 4 % of the time beside the cache's bytes.
+template <typename T> constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
+
+template <typename T, int DP, bool FAR, int CAP, bool PAGED>
+__global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const AttnArgs a, const CacheArgs c,
+                                                          T *__restrict__ out) {
+    typedef typename Elem<T>::frag frag;
+    constexpr int W = kWaves<T, DP>;
+    static_assert(4 * kKeys * DP * sizeof(T) >= kHeads * DP * sizeof(float), "sums reuse the tiles");
+    __shared__ __align__(1024) T tiles[W][4 * kKeys * DP];  // a wave's keys and values, two buffers
+    __shared__ __align__(16) typename Places<T>::Row spos[W][2][3 * kKeys];
+    __shared__ float sm[W][kHeads], ss[W][kHeads];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = a.heads / a.kv_heads;
+    int n = blockIdx.x;
+    const int hk = n % a.kv_heads;
+    n /= a.kv_heads;
+    const int ht = n % c.head_tiles;
+    n /= c.head_tiles;
+    int s, j_begin, j_end;
+    bool whole;    // all of the scene's keys: the result goes to out
+    int64_t part;  // else to this row, plus the head
+    if constexpr (PAGED) {
+        const Piece p = paged_piece(a, c, n);
+        if (p.s < 0) return;
+        s = p.s, j_begin = p.begin, j_end = p.end, whole = p.count == 1;
+        part = (int64_t)n * a.heads;
+    } else {
+        const int split = n % c.splits;
+        s = n / c.splits;
+        const int len = min(max(c.lengths[s], 0), a.k_tokens);
+        const int per = ((len + c.splits - 1) / c.splits + kKeys - 1) / kKeys * kKeys;
+        j_begin = min((int64_t)split * per, (int64_t)len), j_end = min(j_begin + per, len);
+        whole = c.splits == 1;
+        part = (int64_t)s * a.heads * c.splits + split;
+    }
+    const int col = ht * kHeads + (lane & 31);  // query head within the group
+    const bool head = col < group;
+    const int h = hk * group + (head ? col : 0);
+
+    constexpr bool far = FAR, capped = CAP != kNoCap;
+    const float slope = slope_of(a, h);
+    const float unit = capped ? kLog2e : a.scale * kLog2e;
+    const float far_unit = capped ? slope : slope / a.scale;
+    const float in_cap = capped ? a.scale / a.cap : 0.f;
+    frag q[DP / 16];
+    load_column<T, DP>(q, static_cast<const T *>(a.q) + s * a.q_row + h * a.q_head, a.dim, head, lane);
+    float x = 0.f, y = 0.f, z = 0.f;
+    if (far) {
+        const float *p = a.q_pos + s * a.q_pos_row;
+        x = p[0], y = p[1], z = p[2];
+    }
+    Places<T> place;
+        place.set(x, y, z, lane);
+    const T *kbase = static_cast<const T *>(a.k) + (PAGED ? 0 : s * c.k_scene) + hk * a.k_head;
+    const T *vbase = static_cast<const T *>(a.v) + (PAGED ? 0 : s * c.v_scene) + hk * a.v_head;
+    T *const sk = tiles[wave], *const sv = sk + 2 * kKeys * DP;
+    Tile<T, DP> at;
+    at.plan(lane);
+    // what one copy fills: a step's keys, or those of it in one page
+    constexpr int kGroup = PAGED ? kPageUnit : kKeys, kGroups = kKeys / kGroup;
+    Copy<T, DP, kGroup, 1> ck, cv;
+    ck.plan(a.k_row, a.dim, 0, lane);
+    cv.plan(a.v_row, a.dim, 0, lane);
+    f32x16 o[DP / 32] = {};
+    float m = -INFINITY, sum = 0.f;
+    float gp[2] = {};
+    int raw = 0;
+    uint32_t live = ~0u, next_live = ~0u;
+    const int step = W * kKeys;
+    // paged: the pages of 32 of this wave's steps (two groups each), a lane each, and of the next 32;
+    // of the step that is fetched next, each group's page (below 0: none) and its first row in it
+    int ids = 0, next_ids = 0, page[kGroups], at_row[kGroups];
+    auto entries = [&](int j0) {
+        const int row = min(j0 + (lane >> 1) * step + (lane & 1) * kPageUnit, j_end - 1);
+        return c.table[s * c.table_row + fastdiv(row, c.by_rows)];
+    };
+    auto look = [&](int j0) {
+        if constexpr (PAGED) {
+            const int first = j_begin + wave * kKeys, n = (j0 - first) / step;
+            if ((n & 15) == 0) {
+                const bool ahead = n & 16;
+                const int e = n == 0 || ahead ? entries(ahead ? j0 + 16 * step : j0) : next_ids;
+                ids = ahead ? ids : e, next_ids = ahead ? e : next_ids;
+            }
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                const int row = j0 + g * kPageUnit;
+                page[g] = __builtin_amdgcn_readlane(ids, (n & 31) * 2 + g);
+                if (page[g] >= c.pages || row >= j_end) page[g] = -1;
+                at_row[g] = row - fastdiv(min(row, j_end - 1), c.by_rows) * c.page_rows;
+            }
+        }
+        if (a.keep && j0 < j_end) {
+            if constexpr (PAGED) {
+                const int r = min(lane & 31, j_end - 1 - j0), g = r / kPageUnit;
+                const int p = g ? page[1 % kGroups] : page[0], first = g ? at_row[1 % kGroups] : at_row[0];
+                raw = p < 0 ? 0 : keep_raw(a, p * c.keep_scene + first + r % kPageUnit);
+            } else {
+                raw = keep_raw(a, s * c.keep_scene + min(j0 + (lane & 31), j_end - 1));
+            }
+        }
+    };
+    auto fetch = [&](int b, int j0) {
+        if (a.keep) next_live = (uint32_t)__ballot(raw != 0);
+        if constexpr (PAGED) {
+            const int left = j_end - j0;
+            if (!a.keep) next_live = ~0u;
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                // rows of a page that is none are not there
+                const int rows = page[g] < 0 ? 0 : left - g * kPageUnit;
+                if (page[g] < 0) next_live &= ~(0xffffu << (g * kPageUnit));
+                const int64_t p = max(page[g], 0);
+                ck.template start<true>(sk + (b * kKeys + g * kPageUnit) * DP, kbase + p * c.k_scene + at_row[g] * a.k_row, a.k_row,
+                         a.dim, rows, a.keep, next_live >> (g * kPageUnit), 0, lane);
+                cv.template start<true>(sv + (b * kKeys + g * kPageUnit) * DP, vbase + p * c.v_scene + at_row[g] * a.v_row, a.v_row,
+                         a.dim, rows, a.keep, next_live >> (g * kPageUnit), 0, lane);
+            }
+            if (far)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = min((i * 64 + lane) % kKeys, left - 1), ax = min((i * 64 + lane) / kKeys, 2);
+                    const int g = r / kPageUnit, p = g ? page[1 % kGroups] : page[0];
+                    const int first = g ? at_row[1 % kGroups] : at_row[0];
+                    gp[i] = p < 0 ? 0.f : a.k_pos[p * c.k_pos_scene + (first + r % kPageUnit) * a.k_pos_row + ax];
+                }
+            look(j0 + step);
+        } else {
+            look(j0 + step);
+            const int left = j_end - j0;
+            ck.start(sk + b * kKeys * DP, kbase + (int64_t)j0 * a.k_row, a.k_row, a.dim, left, a.keep,
+                     next_live, 0, lane);
+            cv.start(sv + b * kKeys * DP, vbase + (int64_t)j0 * a.v_row, a.v_row, a.dim, left, a.keep,
+                     next_live, 0, lane);
+            if (far)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = min((i * 64 + lane) % kKeys, left - 1), ax = min((i * 64 + lane) / kKeys, 2);
+                    gp[i] = a.k_pos[s * c.k_pos_scene + (int64_t)(j0 + r) * a.k_pos_row + ax];
+                }
+        }
+    };
+    // the tiles are this wave's own: its copies and LDS accesses need no barrier, only waits
+    auto put = [&](int b) {
+        if (far) {
+            spos[wave][b][lane] = Places<T>::row(gp[0]);
+            if (lane < kKeys) spos[wave][b][64 + lane] = Places<T>::row(gp[1]);
+        }
+        tile_wait();
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    int b = 0;
+    if (j_begin + wave * kKeys < j_end) {
+        look(j_begin + wave * kKeys);
+        fetch(0, j_begin + wave * kKeys);
+        put(0);
+    }
+    for (int j0 = j_begin + wave * kKeys; j0 < j_end; j0 += step, b ^= 1) {
+        const bool more = j0 + step < j_end;
+        live = next_live;
+        if (j_end - j0 < kKeys) live &= (1u << (j_end - j0)) - 1;
+        if (more) fetch(b ^ 1, j0 + step);
+        const T *kt = sk + b * kKeys * DP, *vt = sv + b * kKeys * DP;
+        f32x16 d = {}, w = {};
+        if (far) d = distances<T>(place, spos[wave][b], kKeys, 0, lane);
+        if (far && !capped)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) w[r] = -far_unit * d[r];
+#pragma unroll
+        for (int st = 0; st < DP / 16; ++st) w = mma(at.rows(kt, st), q[st], w);
+        if (capped)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                w[r] = a.cap * tanh_of<T, CAP>(w[r] * in_cap);
+                if (far) w[r] = fmaf(-far_unit, d[r], w[r]);
+            }
+        if (live != 0xffffffffu) {
+            const uint32_t seen = live >> (4 * (lane >> 5));
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (!(seen & (1u << result_row(r)))) w[r] = -INFINITY;
+        }
+        // rounded here, so that the largest weight is a power of two exactly
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[r] *= unit;
+        float top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, w[r]);
+        if (__any(top > m + kSlack)) {
+            const float next = fmaxf(m, fmaxf(top, other_half(top)));
+            const float by = next == -INFINITY ? 1.f : fast_exp2(m - next);
+            m = next;
+            sum *= by;
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b) o[b] *= by;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            w[r] = fast_exp2(w[r] - ref);
+        }
+#pragma unroll
+        for (int part = 0; part < kParts<T>; ++part) {
+            if (part) w = remainders<T>(w);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const frag p = to_frag<T>(w, half);
+                sum = add_weights(p, sum);
+#pragma unroll
+                for (int e = 0; e < DP / 32; ++e)
+                    o[e] = mma(at.columns(vt + half * 16 * DP, e, lane), p, o[e]);
+            }
+        }
+        if (more) put(b ^ 1);
+    }
+    sum += other_half(sum);
+    // the waves' sums, joined
+    if (lane < 32) sm[wave][lane] = m, ss[wave][lane] = sum;
+    float *so = reinterpret_cast<float *>(tiles[wave]);
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                so[(lane & 31) * DP + b * 32 + 8 * g + 4 * (lane >> 5) + e] = o[b][4 * g + e];
+    __syncthreads();
+    const int heads = min(group - ht * kHeads, kHeads);
+    for (int i = threadIdx.x; i < heads * DP; i += 64 * W) {
+        const int r = i / DP, dd = i % DP;
+        float top = -INFINITY, total = 0.f, val = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = fmaxf(top, sm[w][r]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            // a wave without keys has the maximum -inf and the sum 0; NaN sums pass
+            const float by = sm[w][r] == -INFINITY ? 1.f : fast_exp2(sm[w][r] - top);
+            total = fmaf(by, ss[w][r], total);
+            val = fmaf(by, reinterpret_cast<const float *>(tiles[w])[i], val);
+        }
+        if (dd >= a.dim) continue;
+        const int hh = hk * group + ht * kHeads + r;
+        if (whole) {
+            out[((int64_t)s * a.heads + hh) * a.dim + dd] = (T)(total == 0.f ? 0.f : val / total);
+        } else {
+            const int64_t at = part + (int64_t)hh * (PAGED ? 1 : c.splits);
+            c.part_o[at * a.dim + dd] = val;
+            if (dd == 0) c.part_ms[at] = make_float2(top, total);
+        }
+    }
+}
+
+// The row of one scene and head from its `splits` parts, rows first, first + step .. of the workspace: four
+// waves take them in turn, then their sums are joined, always in the same order.
+template <typename T>
+__device__ __forceinline__ void join_row(const float *__restrict__ part_o, const float2 *__restrict__ part_ms,
+                                         int64_t first, int64_t step, int splits, int dim, T *__restrict__ out) {
+    __shared__ float so[4][128], ss[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float2 *ms = part_ms + first;
+    float top = -INFINITY;
+    for (int p = lane; p < splits; p += 64) top = fmaxf(top, ms[p * step].x);
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+    float total = 0.f, v0 = 0.f, v1 = 0.f;
+    const int d0 = min(lane, dim - 1), d1 = min(lane + 64, dim - 1);
+#pragma unroll 4
+    for (int p = wave; p < splits; p += 4) {
+        const float2 e = ms[p * step];
+        const float by = e.x == -INFINITY ? 1.f : fast_exp2(e.x - top);
+        total = fmaf(by, e.y, total);
+        const float *o = part_o + (first + p * step) * dim;
+        v0 = fmaf(by, o[d0], v0);
+        v1 = fmaf(by, o[d1], v1);
+    }
+    so[wave][lane] = v0, so[wave][64 + lane] = v1;
+    if (lane == 0) ss[wave] = total;
+    __syncthreads();
+    if (threadIdx.x >= (unsigned)dim) return;
+    const int d = threadIdx.x;
+    total = ss[0] + ss[1] + ss[2] + ss[3];
+    const float v = so[0][d] + so[1][d] + so[2][d] + so[3][d];
+    out[d] = (T)(total == 0.f ? 0.f : v / total);
+}
+
+}  // namespace
+}  // namespace gsv

@@ -1,0 +1,222 @@
+// paged_append.hip — new tokens' keys and values into a cache in pages, the keys turned on the way.
+//
+// Token i of scene s's n new ones becomes row r = lengths[s] - n + i of the scene, row r % page_rows of the page
+// that its table names; keys (and the queries, which go to an output of their own) are turned as by rotary.hip.
+// Bytes bound it: each head is read and written once, in one launch.  A workgroup takes a few tokens: one wave
+// finds their rows, a lane each, while the others form the angles; both serve all heads from LDS.
+#include "gsv_rotary.h"
+
+namespace gsv {
+namespace {
+
+struct AppendArgs {
+    const void *q, *k, *v;
+    void *q_out, *k_pool, *v_pool;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    int64_t kp_page, kp_row, kp_head, vp_page, vp_row, vp_head;
+    int tokens, heads, kv_heads, dim, pairs, axes;
+    const float *positions, *frequencies;
+    int64_t pos_row, pos_axis;
+    float *pos_pool;
+    int64_t pp_page, pp_row;
+    const void *keep;
+    void *keep_pool;
+    int64_t keep_page;
+    int keep_bytes, keep_pool_bytes;
+    const int *lengths, *starts, *table;
+    int64_t table_row;
+    int scenes, pages, page_rows, capacity;
+    int block_tokens;
+    FastDiv by_rows, by_pairs, by_items, by_heads, by_kv_heads;
+};
+
+// The row of a token's own in the pools: page, and row in it; page < 0: none.
+struct Target {
+    int page, row;
+};
+
+__device__ __forceinline__ int start_of(const AppendArgs &a, int s) {
+    if (s <= 0) return 0;
+    if (s >= a.scenes) return a.tokens;
+    return min(max(a.starts[s], 0), a.tokens);
+}
+
+// Token t's scene is s0 or a later one: looked for in steps that double, then halve.
+__device__ __forceinline__ Target target_of(const AppendArgs &a, int t, int s0) {
+    int s = a.starts ? s0 : t, ahead = 1;
+    if (a.starts) {
+        int step = 1;
+        while (s + step < a.scenes && start_of(a, s + step) <= t) s += step, step *= 2;
+        for (; step > 1;) {
+            step /= 2;
+            if (s + step < a.scenes && start_of(a, s + step) <= t) s += step;
+        }
+        ahead = start_of(a, s + 1) - t;  // of the scene's tokens, this one and those behind it
+    }
+    const int64_t row = (int64_t)a.lengths[s] - ahead;
+    if (ahead < 1 || row < 0 || row >= a.capacity) return {-1, 0};
+    const int entry = fastdiv((uint32_t)row, a.by_rows);
+    const int page = a.table[s * a.table_row + entry];
+    if (page < 0 || page >= a.pages) return {-1, 0};
+    return {page, (int)row - entry * a.page_rows};
+}
+
+template <typename T, int VEC, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void k_paged_append(const AppendArgs a) {
+    extern __shared__ float2 turns[];  // cos, sin of block_tokens x pairs
+    __shared__ Target target[64];
+    const int t0 = blockIdx.x * a.block_tokens, nt = min(a.block_tokens, a.tokens - t0);
+    if (threadIdx.x >= 192) {  // the last wave: it has the fewest angles
+        const int lane = threadIdx.x & 63;
+        int s0 = 0;
+        if (a.starts) s0 = last_at_most(a.scenes, t0, [&](int s) { return start_of(a, s); });
+        if (lane < nt) target[lane] = target_of(a, t0 + lane, s0);
+    }
+    for (int i = threadIdx.x; i < nt * a.pairs; i += 256) {
+        const int t = fastdiv(i, a.by_pairs), p = i - t * a.pairs;
+        turns[i] = turn_of(a.positions + (t0 + t) * a.pos_row, a.pos_axis, a.frequencies + p, a.pairs, a.axes);
+    }
+    __syncthreads();
+    const int all = a.heads + a.kv_heads, turning = a.pairs / VEC;
+    const int items = turning + (a.dim - 2 * a.pairs) / kPassed<VEC, INTERLEAVED>;
+    for (int i = threadIdx.x; i < nt * all * items; i += 256) {
+        const int row = fastdiv(i, a.by_items), item = i - row * items;
+        const int t = fastdiv(row, a.by_heads), h = row - t * all;
+        const int64_t token = t0 + t;
+        const T *in;
+        T *out;
+        if (h < a.heads) {
+            in = static_cast<const T *>(a.q) + token * a.q_row + h * a.q_head;
+            out = static_cast<T *>(a.q_out) + (token * a.heads + h) * a.dim;
+        } else {
+            const Target to = target[t];
+            if (to.page < 0) continue;
+            in = static_cast<const T *>(a.k) + token * a.k_row + (h - a.heads) * a.k_head;
+            out = static_cast<T *>(a.k_pool) + to.page * a.kp_page + to.row * a.kp_row + (h - a.heads) * a.kp_head;
+        }
+        turn_item<T, VEC, INTERLEAVED>(in, out, item, turning, a.pairs, turns + t * a.pairs);
+    }
+    // the values, 16 bytes at a time (a row holds at most 32 of them)
+    constexpr int kChunk = 16 / sizeof(T);
+    typedef Pack<T, kChunk> P;
+    const int chunks = a.dim / kChunk;
+    for (int i = threadIdx.x; i < nt * a.kv_heads * 32; i += 256) {
+        const int row = i >> 5, chunk = i & 31;
+        const int t = fastdiv(row, a.by_kv_heads), h = row - t * a.kv_heads;
+        const Target to = target[t];
+        if (chunk >= chunks || to.page < 0) continue;
+        const int64_t token = t0 + t;
+        *reinterpret_cast<P *>(static_cast<T *>(a.v_pool) + to.page * a.vp_page + to.row * a.vp_row + h * a.vp_head +
+                               chunk * kChunk) =
+            *reinterpret_cast<const P *>(static_cast<const T *>(a.v) + token * a.v_row + h * a.v_head + chunk * kChunk);
+    }
+    if (a.pos_pool && threadIdx.x < nt * 3) {
+        const int t = threadIdx.x / 3, ax = threadIdx.x % 3;
+        const Target to = target[t];
+        if (to.page >= 0)
+            a.pos_pool[to.page * a.pp_page + to.row * a.pp_row + ax] =
+                a.positions[(t0 + t) * a.pos_row + ax * a.pos_axis];
+    }
+    if (a.keep_pool && threadIdx.x < nt) {
+        const Target to = target[threadIdx.x];
+        const int64_t t = t0 + threadIdx.x;
+        const int on = a.keep_bytes == 1 ? static_cast<const uint8_t *>(a.keep)[t] != 0
+                                         : static_cast<const int *>(a.keep)[t] != 0;
+        if (to.page >= 0) {
+            const int64_t at = to.page * a.keep_page + to.row;
+            if (a.keep_pool_bytes == 1) static_cast<uint8_t *>(a.keep_pool)[at] = (uint8_t)on;
+            else static_cast<int *>(a.keep_pool)[at] = on;
+        }
+    }
+}
+
+template <typename T, bool INTERLEAVED> void launch_append(const AppendArgs &a, int vec, hipStream_t s) {
+    const dim3 grid((a.tokens + a.block_tokens - 1) / a.block_tokens), block(256);
+    const size_t lds = sizeof(float2) * a.block_tokens * a.pairs;
+    switch (vec) {
+        case 8:
+            if constexpr (!INTERLEAVED && sizeof(T) == 2) {
+                hipLaunchKernelGGL((k_paged_append<T, 8, INTERLEAVED>), grid, block, lds, s, a);
+                break;
+            }
+            [[fallthrough]];
+        case 4:
+            if constexpr (!(INTERLEAVED && sizeof(T) == 4)) {
+                hipLaunchKernelGGL((k_paged_append<T, 4, INTERLEAVED>), grid, block, lds, s, a);
+                break;
+            }
+            [[fallthrough]];
+        case 2: hipLaunchKernelGGL((k_paged_append<T, 2, INTERLEAVED>), grid, block, lds, s, a); break;
+        default: hipLaunchKernelGGL((k_paged_append<T, 1, INTERLEAVED>), grid, block, lds, s, a);
+    }
+}
+
+// The stride of an axis of one entry is never used, whatever a caller's view holds there.
+int64_t used(int64_t stride, int64_t entries) { return entries > 1 ? stride : 0; }
+
+}  // namespace
+}  // namespace gsv
+
+using namespace gsv;
+
+extern "C" int gsv_paged_append(const gsv_rotary_args *r, const void *v, int64_t v_row, int64_t v_head,
+                                const gsv_pages *p, const int32_t *lengths, const int32_t *starts, int32_t scenes,
+                                const void *keep, int32_t keep_bytes, void *q_out, void *stream) {
+    if (!r || !p || (r->dtype != GSV_F32 && r->dtype != GSV_BF16) || r->tokens < 0 || r->heads < 0 ||
+        r->kv_heads < 1 || r->dim < 8 || r->dim > 128 || r->dim % 8 || r->pairs < 0 || 2 * r->pairs > r->dim ||
+        (r->pairs && (r->axes < 1 || r->axes > 8)) || (r->heads && !r->pairs) || scenes < 0 ||
+        (!starts && scenes != r->tokens) || p->pages < 1 || p->page_rows < 16 || p->page_rows % 16 ||
+        p->table_pages < 0 || p->table_row < 0)
+        return GSV_ERR_INVALID_ARGUMENT;
+    const int64_t rows = (int64_t)p->page_rows * p->table_pages;
+    if (r->tokens > GSV_MAX_TOKENS || scenes > GSV_MAX_TOKENS || rows > GSV_MAX_TOKENS) return GSV_ERR_SIZE_OVERFLOW;
+    if ((int64_t)r->heads + r->kv_heads > 4096 || (r->tokens && scenes < 1)) return GSV_ERR_INVALID_ARGUMENT;
+    if (r->tokens == 0) return GSV_OK;
+    if (!r->k || !v || (r->heads && (!r->q || !q_out)) || !p->k || !p->v || !lengths || (rows && !p->table) ||
+        ((r->pairs || p->positions) && !r->positions) || (r->pairs && !r->frequencies) ||
+        (p->positions && r->axes != 3) || (p->keep != nullptr) != (keep != nullptr) ||
+        (keep && ((keep_bytes != 1 && keep_bytes != 4) || (p->keep_bytes != 1 && p->keep_bytes != 4))))
+        return GSV_ERR_INVALID_ARGUMENT;
+    const int64_t size = r->dtype == GSV_BF16 ? 2 : 4, K = r->kv_heads, T = r->tokens;
+    uintptr_t all = reinterpret_cast<uintptr_t>(r->k) | reinterpret_cast<uintptr_t>(v) |
+                    reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v);
+    if (r->heads)
+        all |= reinterpret_cast<uintptr_t>(r->q) | reinterpret_cast<uintptr_t>(q_out) |
+               (uintptr_t)(used(r->q_row, T) * size) | (uintptr_t)(used(r->q_head, r->heads) * size);
+    for (int64_t x : {used(r->k_row, T), used(r->k_head, K), used(v_row, T), used(v_head, K),
+                      used(p->k_page, p->pages), p->k_row, used(p->k_head, K), used(p->v_page, p->pages), p->v_row,
+                      used(p->v_head, K)})
+        all |= (uintptr_t)(x * size);
+    if (all % 16) return GSV_ERR_INVALID_ARGUMENT;
+    // the widest access that both halves of a row's pairs and what follows them are aligned for
+    uint64_t low = 16 | (uint64_t)(r->dim * size) | (uint64_t)((r->dim - 2 * r->pairs) * size) |
+                   (uint64_t)(r->pairs * size * (r->interleaved ? 2 : 1));
+    const int bytes = (int)(low & (0 - low));
+    const int vec = r->interleaved && bytes > size ? bytes / size / 2 : bytes / size;
+    const int passed = r->interleaved && vec > 1 ? 2 * vec : vec;
+    // Tokens of a workgroup: enough for four items a thread, fewer where the launch would leave CUs idle; their
+    // angles within 16 KB of LDS, a lane for each.
+    const int items = r->pairs / vec + (r->dim - 2 * r->pairs) / passed;
+    int64_t bt = imax64(1, 1024 / ((int64_t)(r->heads + 2 * K) * items));
+    bt = imin64(bt, imax64(1, T / 1024));
+    bt = imin64(bt, r->pairs ? imax64(1, 2048 / r->pairs) : 64);
+    bt = imin64(bt, 64);
+    if ((T + bt - 1) / bt >= (1 << 24)) return GSV_ERR_SIZE_OVERFLOW;
+    const AppendArgs a{r->q, r->k, v, q_out, p->k, p->v,
+                       used(r->q_row, T), used(r->q_head, r->heads), used(r->k_row, T), used(r->k_head, K),
+                       used(v_row, T), used(v_head, K),
+                       used(p->k_page, p->pages), p->k_row, used(p->k_head, K),
+                       used(p->v_page, p->pages), p->v_row, used(p->v_head, K),
+                       r->tokens, r->heads, r->kv_heads, r->dim, r->pairs, r->axes, r->positions, r->frequencies,
+                       r->pos_row, r->pos_axis, p->positions, p->pos_page, p->pos_row, keep, p->keep, p->keep_page,
+                       keep_bytes, p->keep_bytes, lengths, starts, p->table, p->table_row, scenes, p->pages,
+                       p->page_rows, (int)rows, (int)bt, make_fastdiv(p->page_rows),
+                       make_fastdiv(r->pairs ? r->pairs : 1), make_fastdiv(items),
+                       make_fastdiv(r->heads + r->kv_heads), make_fastdiv(r->kv_heads)};
+    hipStream_t s = as_stream(stream);
+    if (r->dtype == GSV_BF16)
+        r->interleaved ? launch_append<bf16, true>(a, vec, s) : launch_append<bf16, false>(a, vec, s);
+    else
+        r->interleaved ? launch_append<float, true>(a, vec, s) : launch_append<float, false>(a, vec, s);
+    return check_launch();
+}

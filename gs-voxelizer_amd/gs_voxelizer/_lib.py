@@ -35,7 +35,16 @@ Norm = _struct("Norm", (
     (_P, "x branch gate weight branch_weight scale starts"), (_c_i64, "x_row branch_row gate_row"),
     (_c_int, "dtype branch_dtype gate_dtype gate_per_token tokens channels scenes longest"),
     (_c_float, "eps")))
-_ATT, _ROT, _NORM = (ctypes.POINTER(t) for t in (Attention, Rotary, Norm))
+Pages = _struct("Pages", (
+    (_P, "k v"), (_c_i64, "k_page k_row k_head v_page v_row v_head"), (_P, "positions"),
+    (_c_i64, "pos_page pos_row"), (_P, "keep"), (_c_i64, "keep_page"), (_P, "table"),
+    (_c_i64, "table_row"), (_c_int, "pages page_rows table_pages keep_bytes")))
+AdamwTensor = _struct("AdamwTensor", (
+    (_P, "param grad exp_avg exp_avg_sq master lr_device"), (_c_i64, "numel step"),
+    (ctypes.c_double, "lr weight_decay"), (_c_int, "dtype grad_dtype")))
+Adamw = _struct("Adamw", (
+    (_P, "tensors"), (_c_i64, "count"), (ctypes.c_double, "beta1 beta2 eps max_norm"), (_P, "counter norm")))
+_ATT, _ROT, _NORM, _PAGES, _ADAMW = (ctypes.POINTER(t) for t in (Attention, Rotary, Norm, Pages, Adamw))
 _BYTES = ctypes.POINTER(_c_size_t)
 
 # name -> argument types, in the order of include/gsvox.h
@@ -85,6 +94,11 @@ SIGNATURES = {
     "gsv_attention_bwd": [_ATT, _P, _P, _P, _P, _c_i64, _c_i64, _P, _P, _P, _P, _P, _c_size_t, _P],
     "gsv_attention_cached_workspace_bytes": [_ATT, _BYTES],
     "gsv_attention_cached": [_ATT, _P, _c_i64, _c_i64, _c_i64, _c_i64, _P, _P, _c_size_t, _P],
+    "gsv_attention_paged_workspace_bytes": [_ATT, _PAGES, _BYTES],
+    "gsv_attention_paged": [_ATT, _PAGES, _P, _P, _P, _c_size_t, _P],
+    "gsv_paged_append": [_ROT, _P, _c_i64, _c_i64, _PAGES, _P, _P, _c_int, _P, _c_int, _P, _P],
+    "gsv_adamw_workspace_bytes": [_ADAMW, _BYTES],
+    "gsv_adamw": [_ADAMW, _P, _c_size_t, _P],
     "gsv_kernel_timing_enable": [_c_int],
     "gsv_kernel_timing_collect": [_c_int, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_c_int)],
     "gsv_wave_timeline": [_c_int, _P, _c_int],

@@ -2,9 +2,10 @@
 
 Plain calls of ``optim_to_render`` and ``voxelize_gaussians`` (ordinary tensors,
 no transform or mode active) go to ``project`` and ``voxelize``, those of the operators on
-packed tokens to ``rotate``, ``gated_norm``, ``scene_attention`` and ``cached_attention``; all return
-nothing for a call they do not take; the Python autograd classes then do it, and
-raise its errors.  Without a module built for this torch, or in a torch that no
+packed tokens to ``rotate``, ``gated_norm``, ``scene_attention`` and ``cached_attention``, those of a cache in
+pages to ``append_tokens`` and ``paged_attention``, an optimiser's to ``adamw_step``; all return
+nothing for a call they do not take; the Python code then does it, and
+raises its errors.  Without a module built for this torch, or in a torch that no
 longer has one of the private names that `plain` asks, the classes do all calls
 (same kernels and results, more host time), after a warning.
 """
@@ -22,7 +23,9 @@ _ENTRIES = ("gsv_status_string", "gsv_last_hip_error", "gsv_project_fwd", "gsv_p
             "gsv_voxelize_bwd_workspace_bytes", "gsv_voxelize_bwd", "gsv_voxelize_bwd_l1",
             "gsv_rotary", "gsv_gated_norm_fwd", "gsv_gated_norm_bwd_workspace_bytes",
             "gsv_gated_norm_bwd", "gsv_attention_fwd", "gsv_attention_bwd_workspace_bytes",
-            "gsv_attention_bwd", "gsv_attention_cached_workspace_bytes", "gsv_attention_cached")
+            "gsv_attention_bwd", "gsv_attention_cached_workspace_bytes", "gsv_attention_cached",
+            "gsv_attention_paged_workspace_bytes", "gsv_attention_paged", "gsv_paged_append",
+            "gsv_adamw_workspace_bytes", "gsv_adamw")
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
@@ -56,6 +59,8 @@ if available:
     project, voxelize = _module.project, _module.voxelize
     rotate, gated_norm = _module.rotate, _module.gated_norm
     scene_attention, cached_attention = _module.scene_attention, _module.cached_attention
+    append_tokens, paged_attention = _module.append_tokens, _module.paged_attention
+    adamw_step = _module.adamw_step
 else:
     warnings.warn(f"gs_voxelizer: no native autograd nodes ({_why}); every call takes the Python "
                   "classes. Build them with `python gs-voxelizer_amd/build.py`.", RuntimeWarning)

@@ -14,6 +14,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .cuda import _status_error
@@ -146,3 +147,16 @@ def present(*tensors):
 
 def ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def eager(what):
+    """Refuses a call that writes in place where it would be traced or transformed: a trace would hold
+    its result and not the call."""
+    if (torch._C._get_tracing_state() is not None or torch._C._are_functorch_transforms_active()
+            or forward_ad._current_level >= 0):
+        raise RuntimeError(f"gs_voxelizer: {what} writes in place and cannot be traced or transformed")
+
+
+def written(*tensors):
+    """Tells autograd that a kernel has written into these tensors."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None and not t.is_inference()])

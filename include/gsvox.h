@@ -411,6 +411,36 @@ int gsv_attention_cached(const gsv_attention *args, const int32_t *lengths, int6
                          void *workspace, size_t workspace_bytes, void *stream);
 
 /*
+ * A cache of several scenes in pages: pools k and v (pages, page_rows, kv_heads, dim), with the given
+ * strides (multiples of 16 bytes, pointers too), page_rows a multiple of 16.  Row j of scene s is
+ * row j % page_rows of page table[s * table_row + j / page_rows], for j below page_rows *
+ * table_pages (at most GSV_MAX_TOKENS); an entry outside 0 .. pages - 1 is no page: its rows are not read (their
+ * keys are not seen) and not written.  positions (pages, page_rows) rows of float x, y, z, and
+ * keep (pages, page_rows) with rows together: NULL where they are not used.  Scenes may share
+ * pages that are only read.
+ */
+typedef struct gsv_pages {
+    void *k, *v;
+    int64_t k_page, k_row, k_head, v_page, v_row, v_head;
+    float *positions;
+    int64_t pos_page, pos_row;
+    void *keep;
+    int64_t keep_page;
+    const int32_t *table;
+    int64_t table_row;
+    int32_t pages, page_rows, table_pages, keep_bytes;
+} gsv_pages;
+
+/*
+ * gsv_attention_cached over such a cache: of args, the keys' members (k, v, k_positions, keep, their strides and
+ * k_tokens) are not read.  lengths[s] rows of scene s are live (clamped to 0 .. page_rows * table_pages).  Where a
+ * batch's rows are split goes by the lengths, on the device.
+ */
+int gsv_attention_paged_workspace_bytes(const gsv_attention *args, const gsv_pages *pages, size_t *bytes);
+int gsv_attention_paged(const gsv_attention *args, const gsv_pages *pages, const int32_t *lengths, void *out,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * Rotary positions: theta[t, p] = sum_a positions[t, a] frequencies[a, p] for `pairs`
  * channel pairs of every head of q (tokens, heads, dim) and k (tokens, kv_heads, dim);
  * pair p is channels (p, pairs + p), or (2 p, 2 p + 1) where interleaved; channels from
@@ -425,6 +455,19 @@ typedef struct gsv_rotary_args {
     int32_t dtype, tokens, heads, kv_heads, dim, pairs, axes, interleaved;
 } gsv_rotary_args;
 int gsv_rotary(const gsv_rotary_args *args, void *q_out, void *k_out, int32_t inverse, void *stream);
+
+/*
+ * Appends new tokens to a cache in pages: token i of scene s's n new ones becomes row lengths[s] - n + i (lengths
+ * count them in); one whose row is below 0, past the table or in no page is not written.  args->k (turned as by
+ * gsv_rotary; pairs 0: as it is) and v (tokens, kv_heads, dim; strides v_row, v_head) go to the
+ * pools; q, turned, to q_out (heads may be 0).  dim a multiple of 8, 8 .. 128; k, v and q with pointers and
+ * strides of 16 bytes.  With pages->positions the tokens' positions (axes 3) go there, with pages->keep
+ * keep[t] != 0 of keep (keep_bytes 1 or 4), as 0 or 1.  starts (scenes + 1) as for gsv_attention, NULL: one token
+ * a scene.  Which one stays where two tokens have the same row is not said.
+ */
+int gsv_paged_append(const gsv_rotary_args *args, const void *v, int64_t v_row, int64_t v_head,
+                     const gsv_pages *pages, const int32_t *lengths, const int32_t *starts, int32_t scenes,
+                     const void *keep, int32_t keep_bytes, void *q_out, void *stream);
 
 /*
  * The norms around a block with its gate and residual scale, rows of `channels` (1 .. 8192):
@@ -454,6 +497,37 @@ int gsv_gated_norm_bwd(const gsv_norm *args, const void *dy, int64_t dy_row, con
                        int64_t dh_row, void *dx, void *dbranch, float *dweight,
                        float *dbranch_weight, float *dscale, void *dgate, void *workspace,
                        size_t workspace_bytes, void *stream);
+
+/*
+ * One AdamW step over many tensors:
+ *   g' = grad min(1, max_norm / (|all grads| + 1e-6))   (max_norm 0: g' = grad)
+ *   exp_avg = beta1 exp_avg + (1 - beta1) g',  exp_avg_sq = beta2 exp_avg_sq + (1 - beta2) g'^2
+ *   w = w (1 - lr weight_decay) - lr / (1 - beta1^t) exp_avg / (sqrt(exp_avg_sq / (1 - beta2^t)) + eps)
+ * with w the master where there is one (param then receives it, rounded), else the param.  param and grad are
+ * GSV_F32 or GSV_BF16 (a master needs a GSV_BF16 param), the rest float32; all of numel
+ * values in the same order, aligned to their own size.  t is the tensor's step, 1 or more; with `counter` (one
+ * int32 on the device, steps made so far) t = *counter + 1 for all, and the call advances it.  lr_device: NULL, or the
+ * rate, one float on the device.  norm (NULL, or one float on the device) receives |all grads| where max_norm > 0.
+ * Tensors that share memory are refused (GSV_ERR_INVALID_ARGUMENT).  The norm is summed in binary64 in a fixed order.
+ */
+typedef struct gsv_adamw_tensor {
+    void *param;
+    const void *grad;
+    float *exp_avg, *exp_avg_sq, *master;
+    const float *lr_device;
+    int64_t numel, step;
+    double lr, weight_decay;
+    int32_t dtype, grad_dtype;
+} gsv_adamw_tensor;
+typedef struct gsv_adamw_args {
+    const gsv_adamw_tensor *tensors;
+    int64_t count;
+    double beta1, beta2, eps, max_norm;
+    int32_t *counter;
+    float *norm;
+} gsv_adamw_args;
+int gsv_adamw_workspace_bytes(const gsv_adamw_args *args, size_t *bytes);
+int gsv_adamw(const gsv_adamw_args *args, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
