@@ -19,7 +19,7 @@ __global__ __launch_bounds__(256) void k_cached_join(const float *__restrict__ p
                                                      const float2 *__restrict__ part_ms, int splits,
                                                      int dim, T *__restrict__ out) {
     const int64_t row = blockIdx.x;
-    join_row<T>(part_o, part_ms, row * splits, 1, splits, dim, out + row * dim);
+    join_row<T, 4>(part_o, part_ms, row * splits, 1, splits, dim, out + row * dim);
 }
 
 // Splits of a cache: one round of workgroups, as many as the CUs hold at once (their tiles fill the
@@ -45,7 +45,7 @@ struct Cached {
         T *o = static_cast<T *>(out);
         hipLaunchKernelGGL((k_attention_cached<T, DP, FAR, CAP, false>),
                            dim3((unsigned)(a.scenes * a.kv_heads * c.head_tiles * c.splits)),
-                           dim3(64 * kWaves<T, DP>), 0, st, a, c, o);
+                           dim3(64 * kWaves<T, DP, false>), 0, st, a, c, o);
         if (c.splits > 1)
             hipLaunchKernelGGL(k_cached_join<T>, dim3((unsigned)(a.scenes * a.heads)), dim3(256), 0,
                                st, c.part_o, c.part_ms, c.splits, a.dim, o);

@@ -13,27 +13,38 @@
 namespace gsv {
 namespace {
 
+constexpr int kRounds = 2;
+
 // One workgroup a scene and head; scenes of one piece have their row already.
+constexpr int kJoinWaves = 8;
 template <typename T>
-__global__ __launch_bounds__(256) void k_paged_join(const AttnArgs a, const CacheArgs c, T *__restrict__ out) {
-    const int64_t row = blockIdx.x;
-    const int s = row / a.heads, h = row % a.heads;
-    const int2 p = scene_pieces(a, c, s);
+__global__ __launch_bounds__((64 * kJoinWaves)) void k_paged_join(const float *__restrict__ part_o,
+                                                                  const float2 *__restrict__ part_ms,
+                                                                  const int2 *__restrict__ pieces, FastDiv by_heads,
+                                                                  int heads, int dim, T *__restrict__ out) {
+    const int row = blockIdx.x, s = fastdiv(row, by_heads), h = row - s * heads;
+    const int2 p = pieces[s];
     if (p.y == 1) return;
-    join_row<T>(c.part_o, c.part_ms, (int64_t)p.x * a.heads + h, a.heads, p.y, a.dim, out + row * a.dim);
+    join_row<T, kJoinWaves>(part_o, part_ms, (int64_t)p.x * heads + h, heads, p.y, dim, out + (int64_t)row * dim);
 }
 
-// Pieces that the batch's rows are cut into (and one more a scene at most, for the remainders), or 0 where scenes
-// stay whole: one round of workgroups, as many as the CUs hold at once, each with a step at
-// least for all its waves.
-int paged_pieces(const AttnArgs &a, int head_tiles, int dtype) {
+// Sets the pieces that one round of workgroups holds, as many as the CUs have room for at once, each with a step
+// at least for all its waves; 0 where scenes stay whole.
+void paged_pieces(const AttnArgs &a, int dtype, CacheArgs *c) {
     const int64_t size = dtype == GSV_BF16 ? 2 : 4, dp = a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : 128;
-    const int64_t waves = dp * size > 256 ? 2 : 4;
-    if (a.k_tokens <= waves * kKeys) return 0;
+    const int64_t waves = 512 / imax64(128, dp * size);
+    c->splits = 1, c->even = 0, c->rounds = 0;
+    if (!a.scenes || a.k_tokens <= waves * kKeys) return;
     const int64_t lds = waves * (4 * kKeys * dp * size + (a.slopes ? 6 * kKeys * (size == 2 ? 16 : 4) : 0)) + 2048;
-    const int64_t round = 256 * imin64(163840 / lds, 4);
+    const int64_t round = 256 * imin64(163840 / lds, 12 / waves);
     const int64_t most = ((int64_t)a.k_tokens + waves * kKeys - 1) / (waves * kKeys) * a.scenes;
-    return (int)imax64(1, imin64(round / ((int64_t)a.kv_heads * head_tiles), most));
+    c->splits = 2;
+    c->even = (int)imax64(1, imin64(round / ((int64_t)a.kv_heads * c->head_tiles), most + a.scenes));
+    if (a.scenes * 2 >= c->even) c->rounds = kRounds;
+}
+// The pieces of a launch.
+int64_t paged_places(const AttnArgs &a, const CacheArgs &c) {
+    return c.splits == 1 ? a.scenes : c.rounds == 0 ? c.even : (int64_t)c.even * c.rounds + a.scenes;
 }
 
 struct Paged {
@@ -43,12 +54,12 @@ struct Paged {
     hipStream_t st;
     template <typename T, int DP, bool FAR, int CAP> void run() const {
         T *o = static_cast<T *>(out);
-        const int64_t pieces = (int64_t)a.scenes + c.even;
         hipLaunchKernelGGL((k_attention_cached<T, DP, FAR, CAP, true>),
-                           dim3((unsigned)(pieces * a.kv_heads * c.head_tiles)), dim3(64 * kWaves<T, DP>), 0,
+                           dim3((unsigned)(paged_places(a, c) * a.kv_heads * c.head_tiles)), dim3(64 * kWaves<T, DP, true>), 0,
                            st, a, c, o);
-        if (c.even)
-            hipLaunchKernelGGL(k_paged_join<T>, dim3((unsigned)(a.scenes * a.heads)), dim3(256), 0, st, a, c, o);
+        if (c.splits > 1)
+            hipLaunchKernelGGL(k_paged_join<T>, dim3((unsigned)(a.scenes * a.heads)), dim3(64 * kJoinWaves), 0, st,
+                               c.part_o, c.part_ms, c.pieces, make_fastdiv(a.heads), a.heads, a.dim, o);
     }
 };
 
@@ -73,13 +84,22 @@ int paged_plan(const gsv_attention *args, const gsv_pages *p, AttnArgs *a, Cache
         return GSV_ERR_SIZE_OVERFLOW;
     *c = CacheArgs{};
     c->head_tiles = (int)tiles;
-    c->even = a->scenes ? paged_pieces(*a, (int)tiles, args->dtype) : 0;
-    c->splits = c->even ? 2 : 1;
+    paged_pieces(*a, args->dtype, c);
     return GSV_OK;
 }
 
-size_t part_rows(const AttnArgs &a, const CacheArgs &c) {
-    return c.even ? ((size_t)a.scenes + c.even) * a.heads : 0;
+// The workspace: parts of the sums, their maxima and sums of weights, and the scenes' pieces.
+struct Workspace {
+    size_t rows, ms, pieces, bytes;
+};
+Workspace paged_workspace(const AttnArgs &a, const CacheArgs &c) {
+    if (c.splits == 1) return {};
+    Workspace w;
+    w.rows = (size_t)paged_places(a, c) * a.heads;
+    w.ms = w.rows * a.dim * sizeof(float);  // a multiple of 32 bytes
+    w.pieces = w.ms + w.rows * sizeof(float2);
+    w.bytes = w.pieces + a.scenes * sizeof(int2);
+    return w;
 }
 
 }  // namespace
@@ -94,7 +114,7 @@ extern "C" int gsv_attention_paged_workspace_bytes(const gsv_attention *args, co
     if (!bytes) return GSV_ERR_INVALID_ARGUMENT;
     const int st = paged_plan(args, pages, &a, &c);
     if (st != GSV_OK) return st;
-    *bytes = part_rows(a, c) * (sizeof(float) * a.dim + sizeof(float2));
+    *bytes = paged_workspace(a, c).bytes;
     return GSV_OK;
 }
 
@@ -105,19 +125,20 @@ extern "C" int gsv_attention_paged(const gsv_attention *args, const gsv_pages *p
     int st = paged_plan(args, pages, &a, &c);
     if (st != GSV_OK) return st;
     if (a.scenes == 0) return GSV_OK;
-    const size_t rows = part_rows(a, c), need = rows * (sizeof(float) * a.dim + sizeof(float2));
-    if (need > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
+    const Workspace ws = paged_workspace(a, c);
+    if (ws.bytes > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
     const int64_t chunk = args->dtype == GSV_BF16 ? 8 : 4;
     c.k_scene = used_stride(pages->k_page, pages->pages);
     c.v_scene = used_stride(pages->v_page, pages->pages);
-    if (!lengths || (pages->table_pages && !pages->table) || !out || (need && !workspace) ||
+    if (!lengths || (pages->table_pages && !pages->table) || !out || (ws.bytes && !workspace) ||
         c.k_scene % chunk || c.v_scene % chunk || reinterpret_cast<uintptr_t>(out) % 16 ||
         reinterpret_cast<uintptr_t>(workspace) % 16)
         return GSV_ERR_INVALID_ARGUMENT;
     c.lengths = lengths;
     c.k_pos_scene = pages->pos_page, c.keep_scene = pages->keep_page;
-    c.part_o = static_cast<float *>(workspace);  // a multiple of 32 bytes
-    c.part_ms = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + sizeof(float) * rows * a.dim);
+    c.part_o = static_cast<float *>(workspace);
+    c.part_ms = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + ws.ms);
+    c.pieces = reinterpret_cast<int2 *>(static_cast<char *>(workspace) + ws.pieces);
     c.table = pages->table, c.table_row = pages->table_row;
     c.pages = pages->pages, c.page_rows = pages->page_rows;
     c.by_rows = make_fastdiv(pages->page_rows);

@@ -490,5 +490,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("cached_attention", &cached_attention, py::call_guard<py::gil_scoped_release>());
     m.def("append_tokens", &append_tokens, py::call_guard<py::gil_scoped_release>());
     m.def("paged_attention", &paged_attention, py::call_guard<py::gil_scoped_release>());
-    m.def("adamw_step", &adamw_step, py::call_guard<py::gil_scoped_release>());
+    m.def("adamw_step", &adamw_step);
 }

@@ -34,7 +34,8 @@ struct CacheArgs {
     int64_t table_row;
     int pages, page_rows;
     FastDiv by_rows;
-    int even;  // pieces of a batch without remainders (paged_piece)
+    int2 *pieces;  // of each scene: its first piece, and how many it has
+    int even, rounds;  // pieces that one round of workgroups holds; see paged_rows
 };
 
 // A paged scene's keys, begin .. end - 1 of one of its `count` pieces; s < 0: no scene's.
@@ -44,17 +45,34 @@ struct Piece {
 __device__ __forceinline__ int live_rows(const AttnArgs &a, const CacheArgs &c, int s) {
     return s < a.scenes ? min(max(c.lengths[s], 0), a.k_tokens) : 0;
 }
-// Keys of a piece: the batch's rows over `even`, a multiple of a wave's step, so that a batch has at most
-// even + scenes pieces (a scene of len rows has less than len / per + 1, and one at least).  A lane
-// adds its scenes' rows as integers; the wave's sum of 64 floats is raised by more than its roundings.
+// (an empty scene has a piece, which writes its zeros)
+__device__ __forceinline__ int pieces_of(int len, int per) { return len > 0 ? (len - 1) / per + 1 : 1; }
+// Keys of a piece, a multiple of a wave's step.  Scenes have at most rows / per + scenes pieces (one of len rows
+// has less than len / per + 1, and one at least).  With `rounds` 1, scenes are few against the pieces that one
+// round of workgroups has room for (`even`), and this is the least that fits in, from rows / even on;
+// rows / (even - scenes) always does.  Else the launch holds rounds * even + scenes of them, rows / (rounds * even)
+// each.  A lane adds its scenes' rows as integers; the wave's sum of 64 floats is raised by more
+// than its roundings.
 __device__ __forceinline__ int paged_rows(const AttnArgs &a, const CacheArgs &c, int each, int lane) {
     int64_t mine = 0;
     for (int i = 0; i < each; ++i) mine += live_rows(a, c, lane * each + i);
     const float rows = wave_sum((float)mine) * 1.000002f;
-    return (int)imin64((int64_t)(rows / (float)c.even * 1.000002f) / kKeys * kKeys + kKeys, INT32_MAX);
+    const auto over = [&](float pieces) { return (int64_t)(rows / pieces * 1.000002f) / kKeys + 1; };
+    int64_t low = over((float)c.even * (c.rounds ? c.rounds : 1));
+    if (c.rounds == 0) {
+        int64_t high = over((float)(c.even - a.scenes));
+        while (low < high) {
+            const int64_t mid = (low + high) / 2;
+            int count = 0;
+            for (int i = 0; i < each; ++i)
+                if (lane * each + i < a.scenes) count += pieces_of(live_rows(a, c, lane * each + i), (int)imin64(mid * kKeys, INT32_MAX));
+            // (at most a few thousand: exact)
+            if (wave_sum((float)count) <= (float)c.even) high = mid;
+            else low = mid + 1;
+        }
+    }
+    return (int)imin64(low * kKeys, INT32_MAX);
 }
-// (an empty scene has a piece, which writes its zeros)
-__device__ __forceinline__ int pieces_of(int len, int per) { return len > 0 ? (len - 1) / per + 1 : 1; }
 // Piece n of the batch: of the scenes one after the other.  A lane counts those of a run of scenes, so that
 // up to 64 scenes take one load and a scan over the lanes.
 __device__ __forceinline__ Piece paged_piece(const AttnArgs &a, const CacheArgs &c, int n) {
@@ -81,30 +99,19 @@ __device__ __forceinline__ Piece paged_piece(const AttnArgs &a, const CacheArgs 
         n -= count;
     }
 }
-// The first piece of scene s, and how many it has.
-__device__ __forceinline__ int2 scene_pieces(const AttnArgs &a, const CacheArgs &c, int s) {
-    const int lane = threadIdx.x & 63, each = (a.scenes + 63) / 64;
-    const int per = __builtin_amdgcn_readfirstlane(paged_rows(a, c, each, lane));
-    int before = 0;
-    for (int i = 0; i < each; ++i)
-        if (lane * each + i < s) before += pieces_of(live_rows(a, c, lane * each + i), per);
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) before += __shfl_xor(before, k);
-    return make_int2(before, pieces_of(live_rows(a, c, s), per));
-}
-
 // Waves of a workgroup: four, two where their tiles would pass the LDS of a CU.
-template <typename T, int DP> constexpr int kWaves = DP * sizeof(T) > 256 ? 2 : 4;
+template <typename T, int DP, bool PAGED>
+constexpr int kWaves = PAGED ? 512 / (DP * sizeof(T) < 128 ? 128 : DP * sizeof(T)) : DP * sizeof(T) > 256 ? 2 : 4;
 
 // bfloat16 weights enter the product with the values in two parts: the results are as exact as their type
 // (0.0017 in the 2-norm, in one part 0.0018 to 0.0020), for 0 to 4 % of the time beside the cache's bytes.
 template <typename T> constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
 
 template <typename T, int DP, bool FAR, int CAP, bool PAGED>
-__global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const AttnArgs a, const CacheArgs c,
+__global__ __launch_bounds__((64 * kWaves<T, DP, PAGED>)) void k_attention_cached(const AttnArgs a, const CacheArgs c,
                                                           T *__restrict__ out) {
     typedef typename Elem<T>::frag frag;
-    constexpr int W = kWaves<T, DP>;
+    constexpr int W = kWaves<T, DP, PAGED>;
     static_assert(4 * kKeys * DP * sizeof(T) >= kHeads * DP * sizeof(float), "sums reuse the tiles");
     __shared__ __align__(1024) T tiles[W][4 * kKeys * DP];  // a wave's keys and values, two buffers
     __shared__ __align__(16) typename Places<T>::Row spos[W][2][3 * kKeys];
@@ -124,6 +131,7 @@ __global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const
         const Piece p = paged_piece(a, c, n);
         if (p.s < 0) return;
         s = p.s, j_begin = p.begin, j_end = p.end, whole = p.count == 1;
+        if (j_begin == 0 && hk == 0 && ht == 0 && threadIdx.x == 0 && c.splits > 1) c.pieces[s] = make_int2(n, p.count);
         part = (int64_t)n * a.heads;
     } else {
         const int split = n % c.splits;
@@ -178,11 +186,8 @@ __global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const
     auto look = [&](int j0) {
         if constexpr (PAGED) {
             const int first = j_begin + wave * kKeys, n = (j0 - first) / step;
-            if ((n & 15) == 0) {
-                const bool ahead = n & 16;
-                const int e = n == 0 || ahead ? entries(ahead ? j0 + 16 * step : j0) : next_ids;
-                ids = ahead ? ids : e, next_ids = ahead ? e : next_ids;
-            }
+            if ((n & 31) == 0 && n) ids = next_ids;
+            if ((n & 31) == 16) next_ids = entries(j0 + 16 * step);
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) {
                 const int row = j0 + g * kPageUnit;
@@ -254,6 +259,7 @@ __global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const
     };
     int b = 0;
     if (j_begin + wave * kKeys < j_end) {
+        if constexpr (PAGED) ids = entries(j_begin + wave * kKeys);
         look(j_begin + wave * kKeys);
         fetch(0, j_begin + wave * kKeys);
         put(0);
@@ -353,12 +359,12 @@ __global__ __launch_bounds__((64 * kWaves<T, DP>)) void k_attention_cached(const
     }
 }
 
-// The row of one scene and head from its `splits` parts, rows first, first + step .. of the workspace: four
-// waves take them in turn, then their sums are joined, always in the same order.
-template <typename T>
+// The row of one scene and head from its `splits` parts, rows first, first + step .. of the workspace: the
+// W waves take them in turn, then their sums are joined, always in the same order.
+template <typename T, int W>
 __device__ __forceinline__ void join_row(const float *__restrict__ part_o, const float2 *__restrict__ part_ms,
                                          int64_t first, int64_t step, int splits, int dim, T *__restrict__ out) {
-    __shared__ float so[4][128], ss[4];
+    __shared__ float so[W][128], ss[W];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float2 *ms = part_ms + first;
     float top = -INFINITY;
@@ -368,7 +374,7 @@ __device__ __forceinline__ void join_row(const float *__restrict__ part_o, const
     float total = 0.f, v0 = 0.f, v1 = 0.f;
     const int d0 = min(lane, dim - 1), d1 = min(lane + 64, dim - 1);
 #pragma unroll 4
-    for (int p = wave; p < splits; p += 4) {
+    for (int p = wave; p < splits; p += W) {
         const float2 e = ms[p * step];
         const float by = e.x == -INFINITY ? 1.f : fast_exp2(e.x - top);
         total = fmaf(by, e.y, total);
@@ -381,8 +387,10 @@ __device__ __forceinline__ void join_row(const float *__restrict__ part_o, const
     __syncthreads();
     if (threadIdx.x >= (unsigned)dim) return;
     const int d = threadIdx.x;
-    total = ss[0] + ss[1] + ss[2] + ss[3];
-    const float v = so[0][d] + so[1][d] + so[2][d] + so[3][d];
+    total = ss[0];
+    float v = so[0][d];
+#pragma unroll
+    for (int w = 1; w < W; ++w) total += ss[w], v += so[w][d];
     out[d] = (T)(total == 0.f ? 0.f : v / total);
 }
 

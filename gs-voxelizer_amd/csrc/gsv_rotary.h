@@ -33,43 +33,55 @@ __device__ __forceinline__ float2 turn_of(const float *position, int64_t axis, c
 // A row's items: its pairs, VEC at a time, then the channels past them, kPassed at a time.
 template <int VEC, bool INTERLEAVED> constexpr int kPassed = INTERLEAVED && VEC > 1 ? 2 * VEC : VEC;
 
-// One item of a head's row: pairs turned by `turns` (a token's cos and sin of each pair), or channels that pass
-// through.  VEC pairs an item are two runs of VEC channels, or one of 2 VEC where pairs are interleaved.
-template <typename T, int VEC, bool INTERLEAVED>
-__device__ __forceinline__ void turn_item(const T *in, T *out, int item, int turning, int pairs, const float2 *turns) {
-    if (item >= turning) {
-        constexpr int W = kPassed<VEC, INTERLEAVED>;
-        typedef Pack<T, W> P;
-        const int d = 2 * pairs + (item - turning) * W;
-        *reinterpret_cast<P *>(out + d) = *reinterpret_cast<const P *>(in + d);
-        return;
-    }
-    const int p = item * VEC;
-    const float2 *tp = turns + p;
-    if constexpr (INTERLEAVED && VEC == 1) {
-        const float2 z = turned((float)in[2 * p], (float)in[2 * p + 1], *tp);
-        out[2 * p] = (T)z.x, out[2 * p + 1] = (T)z.y;
-    } else if constexpr (INTERLEAVED) {
-        typedef Pack<T, 2 * VEC> P;
-        P x = *reinterpret_cast<const P *>(in + 2 * p);
+// One item of a head's row, loaded and then turned by `turns` (a token's cos and sin of each pair), or channels
+// that pass through.  VEC pairs an item are two runs of VEC channels, or one of 2 VEC where pairs are interleaved.
+template <typename T, int VEC, bool INTERLEAVED> struct TurnItem {
+    static constexpr int kRun = INTERLEAVED ? 2 * VEC : VEC, W = kPassed<VEC, INTERLEAVED>;
+    typedef Pack<T, kRun> Run;
+    typedef Pack<T, W> Passed;
+    Run x, z;
+    // pairs: of the row; `turning` items of it are turned
+    __device__ __forceinline__ void load(const T *in, int item, int turning, int pairs) {
+        if (item >= turning) {
+            const Passed p = *reinterpret_cast<const Passed *>(in + 2 * pairs + (item - turning) * W);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float2 z = turned((float)x.v[2 * e], (float)x.v[2 * e + 1], tp[e]);
-            x.v[2 * e] = (T)z.x, x.v[2 * e + 1] = (T)z.y;
+            for (int e = 0; e < W; ++e) x.v[e] = p.v[e];
+        } else if constexpr (INTERLEAVED && VEC == 1) {  // (a pair may lie off its own alignment)
+            x.v[0] = in[2 * item], x.v[1] = in[2 * item + 1];
+        } else if constexpr (INTERLEAVED) {
+            x = *reinterpret_cast<const Run *>(in + 2 * item * VEC);
+        } else {
+            x = *reinterpret_cast<const Run *>(in + item * VEC);
+            z = *reinterpret_cast<const Run *>(in + pairs + item * VEC);
         }
-        *reinterpret_cast<P *>(out + 2 * p) = x;
-    } else {
-        typedef Pack<T, VEC> P;
-        P x = *reinterpret_cast<const P *>(in + p);
-        P z = *reinterpret_cast<const P *>(in + pairs + p);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float2 y = turned((float)x.v[e], (float)z.v[e], tp[e]);
-            x.v[e] = (T)y.x, z.v[e] = (T)y.y;
-        }
-        *reinterpret_cast<P *>(out + p) = x;
-        *reinterpret_cast<P *>(out + pairs + p) = z;
     }
-}
+    __device__ __forceinline__ void store(T *out, int item, int turning, int pairs, const float2 *turns) {
+        if (item >= turning) {
+            Passed p;
+#pragma unroll
+            for (int e = 0; e < W; ++e) p.v[e] = x.v[e];
+            *reinterpret_cast<Passed *>(out + 2 * pairs + (item - turning) * W) = p;
+            return;
+        }
+        const float2 *tp = turns + item * VEC;
+        if constexpr (INTERLEAVED) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float2 y = turned((float)x.v[2 * e], (float)x.v[2 * e + 1], tp[e]);
+                x.v[2 * e] = (T)y.x, x.v[2 * e + 1] = (T)y.y;
+            }
+            if constexpr (VEC == 1) out[2 * item] = x.v[0], out[2 * item + 1] = x.v[1];
+            else *reinterpret_cast<Run *>(out + 2 * item * VEC) = x;
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float2 y = turned((float)x.v[e], (float)z.v[e], tp[e]);
+                x.v[e] = (T)y.x, z.v[e] = (T)y.y;
+            }
+            *reinterpret_cast<Run *>(out + item * VEC) = x;
+            *reinterpret_cast<Run *>(out + pairs + item * VEC) = z;
+        }
+    }
+};
 
 }  // namespace gsv

@@ -27,7 +27,8 @@ struct AppendArgs {
     int64_t table_row;
     int scenes, pages, page_rows, capacity;
     int block_tokens;
-    FastDiv by_rows, by_pairs, by_items, by_heads, by_kv_heads;
+    int token_items;  // of a token
+    FastDiv by_rows, by_pairs, by_token, by_items, by_value;
 };
 
 // The row of a token's own in the pools: page, and row in it; page < 0: none.
@@ -61,54 +62,90 @@ __device__ __forceinline__ Target target_of(const AppendArgs &a, int t, int s0) 
     return {page, (int)row - entry * a.page_rows};
 }
 
+// A thread's part of each token: some channels of one head.  It is found once, and then the same for all of the
+// workgroup's tokens: found anew for each, its divisions took more time than the bytes.
+template <typename T, int VEC, bool INTERLEAVED> struct Part {
+    const T *in;   // of token 0 of the array
+    T *out;        // of token 0 of q_out, or of page 0's first row
+    int64_t in_row, out_page, out_row;
+    int item, turning, pairs;
+    bool q;
+    __device__ __forceinline__ Part(const AppendArgs &a, int j) {
+        constexpr int W = kPassed<VEC, INTERLEAVED>;
+        const int items = a.pairs / VEC + (a.dim - 2 * a.pairs) / W, all = (a.heads + a.kv_heads) * items;
+        q = false, turning = a.pairs / VEC, pairs = a.pairs;
+        if (j >= all) {
+            const int h = fastdiv(j - all, a.by_value);
+            item = j - all - h * (a.dim / W), turning = pairs = 0;
+            in = static_cast<const T *>(a.v) + h * a.v_head, in_row = a.v_row;
+            out = static_cast<T *>(a.v_pool) + h * a.vp_head, out_page = a.vp_page, out_row = a.vp_row;
+            return;
+        }
+        int h = fastdiv(j, a.by_items);
+        item = j - h * items;
+        if (h < a.heads) {
+            q = true;
+            in = static_cast<const T *>(a.q) + h * a.q_head, in_row = a.q_row;
+            out = static_cast<T *>(a.q_out) + (int64_t)h * a.dim, out_page = 0, out_row = (int64_t)a.heads * a.dim;
+        } else {
+            h -= a.heads;
+            in = static_cast<const T *>(a.k) + h * a.k_head, in_row = a.k_row;
+            out = static_cast<T *>(a.k_pool) + h * a.kp_head, out_page = a.kp_page, out_row = a.kp_row;
+        }
+    }
+};
+
+// Tokens of a thread that are loaded at once (the first ones before their rows and angles are known), and all that it
+// takes, over which the chains of loads at a workgroup's start spread.  20,000 tokens (below) take 28.9 us with 8 of
+// them, 30.9 with 16 and 30.0 with 4 at once and no more; 65,537 104, 105 and 116.
+constexpr int kDeep = 2, kTokens = 8;
+
 template <typename T, int VEC, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void k_paged_append(const AppendArgs a) {
     extern __shared__ float2 turns[];  // cos, sin of block_tokens x pairs
     __shared__ Target target[64];
     const int t0 = blockIdx.x * a.block_tokens, nt = min(a.block_tokens, a.tokens - t0);
-    if (threadIdx.x >= 192) {  // the last wave: it has the fewest angles
-        const int lane = threadIdx.x & 63;
-        int s0 = 0;
-        if (a.starts) s0 = last_at_most(a.scenes, t0, [&](int s) { return start_of(a, s); });
-        if (lane < nt) target[lane] = target_of(a, t0 + lane, s0);
-    }
-    for (int i = threadIdx.x; i < nt * a.pairs; i += 256) {
-        const int t = fastdiv(i, a.by_pairs), p = i - t * a.pairs;
-        turns[i] = turn_of(a.positions + (t0 + t) * a.pos_row, a.pos_axis, a.frequencies + p, a.pairs, a.axes);
-    }
-    __syncthreads();
-    const int all = a.heads + a.kv_heads, turning = a.pairs / VEC;
-    const int items = turning + (a.dim - 2 * a.pairs) / kPassed<VEC, INTERLEAVED>;
-    for (int i = threadIdx.x; i < nt * all * items; i += 256) {
-        const int row = fastdiv(i, a.by_items), item = i - row * items;
-        const int t = fastdiv(row, a.by_heads), h = row - t * all;
-        const int64_t token = t0 + t;
-        const T *in;
-        T *out;
-        if (h < a.heads) {
-            in = static_cast<const T *>(a.q) + token * a.q_row + h * a.q_head;
-            out = static_cast<T *>(a.q_out) + (token * a.heads + h) * a.dim;
-        } else {
-            const Target to = target[t];
-            if (to.page < 0) continue;
-            in = static_cast<const T *>(a.k) + token * a.k_row + (h - a.heads) * a.k_head;
-            out = static_cast<T *>(a.k_pool) + to.page * a.kp_page + to.row * a.kp_row + (h - a.heads) * a.kp_head;
+    // a thread's first part and token: as many tokens side by side as have room
+    const int side = max(256 / a.token_items, 1);
+    const int first_t = side > 1 ? fastdiv(threadIdx.x, a.by_token) : 0, first_j = threadIdx.x - first_t * a.token_items;
+    const bool mine = first_t < side;
+    bool begun = false;
+    for (int j = first_j; j - first_j < a.token_items; j += 256) {
+        const bool has = mine && j < a.token_items;
+        const Part<T, VEC, INTERLEAVED> p(a, has ? j : 0);
+        for (int tb = 0; tb < nt; tb += side * kDeep) {
+            TurnItem<T, VEC, INTERLEAVED> x[kDeep];
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k) {
+                const int t = tb + k * side + first_t;
+                if (has && t < nt) x[k].load(p.in + (t0 + t) * p.in_row, p.item, p.turning, p.pairs);
+            }
+            if (!begun) {
+                begun = true;
+                if (threadIdx.x >= 192) {  // the last wave: it has the fewest angles
+                    const int lane = threadIdx.x & 63;
+                    int s0 = 0;
+                    if (a.starts) s0 = last_at_most(a.scenes, t0, [&](int s) { return start_of(a, s); });
+                    if (lane < nt) target[lane] = target_of(a, t0 + lane, s0);
+                }
+                for (int i = threadIdx.x; i < nt * a.pairs; i += 256) {
+                    const int t = fastdiv(i, a.by_pairs), r = i - t * a.pairs;
+                    turns[i] = turn_of(a.positions + (t0 + t) * a.pos_row, a.pos_axis, a.frequencies + r, a.pairs,
+                                       a.axes);
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k) {
+                const int t = tb + k * side + first_t;
+                if (!has || t >= nt) continue;
+                Target to = target[t];
+                if (p.q) to = {0, t0 + t};
+                if (to.page < 0) continue;
+                x[k].store(p.out + to.page * p.out_page + to.row * p.out_row, p.item, p.turning, p.pairs,
+                           turns + t * a.pairs);
+            }
         }
-        turn_item<T, VEC, INTERLEAVED>(in, out, item, turning, a.pairs, turns + t * a.pairs);
-    }
-    // the values, 16 bytes at a time (a row holds at most 32 of them)
-    constexpr int kChunk = 16 / sizeof(T);
-    typedef Pack<T, kChunk> P;
-    const int chunks = a.dim / kChunk;
-    for (int i = threadIdx.x; i < nt * a.kv_heads * 32; i += 256) {
-        const int row = i >> 5, chunk = i & 31;
-        const int t = fastdiv(row, a.by_kv_heads), h = row - t * a.kv_heads;
-        const Target to = target[t];
-        if (chunk >= chunks || to.page < 0) continue;
-        const int64_t token = t0 + t;
-        *reinterpret_cast<P *>(static_cast<T *>(a.v_pool) + to.page * a.vp_page + to.row * a.vp_row + h * a.vp_head +
-                               chunk * kChunk) =
-            *reinterpret_cast<const P *>(static_cast<const T *>(a.v) + token * a.v_row + h * a.v_head + chunk * kChunk);
     }
     if (a.pos_pool && threadIdx.x < nt * 3) {
         const int t = threadIdx.x / 3, ax = threadIdx.x % 3;
@@ -194,10 +231,11 @@ extern "C" int gsv_paged_append(const gsv_rotary_args *r, const void *v, int64_t
     const int bytes = (int)(low & (0 - low));
     const int vec = r->interleaved && bytes > size ? bytes / size / 2 : bytes / size;
     const int passed = r->interleaved && vec > 1 ? 2 * vec : vec;
-    // Tokens of a workgroup: enough for four items a thread, fewer where the launch would leave CUs idle; their
+    // Tokens of a workgroup: as many as its threads hold at once, fewer where the launch would leave CUs idle; their
     // angles within 16 KB of LDS, a lane for each.
-    const int items = r->pairs / vec + (r->dim - 2 * r->pairs) / passed;
-    int64_t bt = imax64(1, 1024 / ((int64_t)(r->heads + 2 * K) * items));
+    const int items = r->pairs / vec + (r->dim - 2 * r->pairs) / passed, values = r->dim / passed;
+    const int64_t each = (r->heads + K) * items + K * values;
+    int64_t bt = kTokens * imax64(1, 256 / each);
     bt = imin64(bt, imax64(1, T / 1024));
     bt = imin64(bt, r->pairs ? imax64(1, 2048 / r->pairs) : 64);
     bt = imin64(bt, 64);
@@ -210,9 +248,9 @@ extern "C" int gsv_paged_append(const gsv_rotary_args *r, const void *v, int64_t
                        r->tokens, r->heads, r->kv_heads, r->dim, r->pairs, r->axes, r->positions, r->frequencies,
                        r->pos_row, r->pos_axis, p->positions, p->pos_page, p->pos_row, keep, p->keep, p->keep_page,
                        keep_bytes, p->keep_bytes, lengths, starts, p->table, p->table_row, scenes, p->pages,
-                       p->page_rows, (int)rows, (int)bt, make_fastdiv(p->page_rows),
-                       make_fastdiv(r->pairs ? r->pairs : 1), make_fastdiv(items),
-                       make_fastdiv(r->heads + r->kv_heads), make_fastdiv(r->kv_heads)};
+                       p->page_rows, (int)rows, (int)bt, (int)each, make_fastdiv(p->page_rows),
+                       make_fastdiv(r->pairs ? r->pairs : 1), make_fastdiv(each), make_fastdiv(items),
+                       make_fastdiv(values)};
     hipStream_t s = as_stream(stream);
     if (r->dtype == GSV_BF16)
         r->interleaved ? launch_append<bf16, true>(a, vec, s) : launch_append<bf16, false>(a, vec, s);

@@ -49,7 +49,9 @@ __global__ __launch_bounds__(256) void k_rotary(const RotaryArgs a) {
                            : static_cast<const T *>(a.k) + token * a.k_row + (h - a.heads) * a.k_head;
         T *out = is_q ? static_cast<T *>(a.q_out) + (token * a.heads + h) * a.dim
                       : static_cast<T *>(a.k_out) + (token * a.kv_heads + h - a.heads) * a.dim;
-        turn_item<T, VEC, INTERLEAVED>(in, out, item, turning, a.pairs, turns + t * a.pairs);
+        TurnItem<T, VEC, INTERLEAVED> x;
+        x.load(in, item, turning, a.pairs);
+        x.store(out, item, turning, a.pairs, turns + t * a.pairs);
     }
 }
 

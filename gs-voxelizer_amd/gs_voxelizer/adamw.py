@@ -55,6 +55,11 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     Returns:
         with max_norm the norm of all gradients before that, a float32 tensor; else None.
     """
+    if _native.plain():
+        done, norm = _native.adamw_step(params, grads, exp_avgs, exp_avg_sqs, masters, step, lr, weight_decay, betas,
+                                        eps, max_norm)
+        if done:
+            return norm
     counter = step if isinstance(step, Tensor) else None
     n = len(params)
     steps = [] if counter is not None else _each(step, n, "step")
@@ -67,11 +72,6 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     for x in steps:
         if not isinstance(x, int) or x < 1:
             raise ValueError(f"step must be whole numbers from 1, got {x!r}")
-    if not any(isinstance(x, Tensor) for x in rates) and _native.plain(*_t.present(counter)):
-        done, norm = _native.adamw_step(params, grads, exp_avgs, exp_avg_sqs, masters or [], steps, counter, rates,
-                                        decays, betas[0], betas[1], eps, max_norm or 0.0)
-        if done:
-            return norm
     return _step(params, grads, exp_avgs, exp_avg_sqs, masters, steps, counter, rates, decays, betas, eps, max_norm)
 
 
