@@ -43,9 +43,9 @@ struct Cached {
     hipStream_t st;
     template <typename T, int DP, bool FAR, int CAP> void run() const {
         T *o = static_cast<T *>(out);
-        hipLaunchKernelGGL((k_attention_cached<T, DP, FAR, CAP, false>),
+        hipLaunchKernelGGL((k_attention_cached<T, DP, FAR, CAP, kTogether>),
                            dim3((unsigned)(a.scenes * a.kv_heads * c.head_tiles * c.splits)),
-                           dim3(64 * kWaves<T, DP, false>), 0, st, a, c, o);
+                           dim3(64 * kWaves<T, DP, kTogether>), 0, st, a, c, o);
         if (c.splits > 1)
             hipLaunchKernelGGL(k_cached_join<T>, dim3((unsigned)(a.scenes * a.heads)), dim3(256), 0,
                                st, c.part_o, c.part_ms, c.splits, a.dim, o);

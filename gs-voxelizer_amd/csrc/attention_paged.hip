@@ -13,38 +13,31 @@
 namespace gsv {
 namespace {
 
-constexpr int kRounds = 2;
-
-// One workgroup a scene and head; scenes of one piece have their row already.
+// One workgroup a scene and head; scenes of one part have their row already.
 constexpr int kJoinWaves = 8;
 template <typename T>
 __global__ __launch_bounds__((64 * kJoinWaves)) void k_paged_join(const float *__restrict__ part_o,
                                                                   const float2 *__restrict__ part_ms,
-                                                                  const int2 *__restrict__ pieces, FastDiv by_heads,
+                                                                  const int2 *__restrict__ parts, FastDiv by_heads,
                                                                   int heads, int dim, T *__restrict__ out) {
     const int row = blockIdx.x, s = fastdiv(row, by_heads), h = row - s * heads;
-    const int2 p = pieces[s];
+    const int2 p = parts[s];
     if (p.y == 1) return;
     join_row<T, kJoinWaves>(part_o, part_ms, (int64_t)p.x * heads + h, heads, p.y, dim, out + (int64_t)row * dim);
 }
 
-// Sets the pieces that one round of workgroups holds, as many as the CUs have room for at once, each with a step
-// at least for all its waves; 0 where scenes stay whole.
-void paged_pieces(const AttnArgs &a, int dtype, CacheArgs *c) {
+// Sets the workgroups of a key head that share a batch's steps: one round of them, as many as the CUs have room for
+// at once.  Scenes of at most a step for each wave stay whole.
+void paged_shares(const AttnArgs &a, int dtype, CacheArgs *c) {
     const int64_t size = dtype == GSV_BF16 ? 2 : 4, dp = a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : 128;
     const int64_t waves = 512 / imax64(128, dp * size);
-    c->splits = 1, c->even = 0, c->rounds = 0;
+    c->splits = 1, c->shares = a.scenes;
     if (!a.scenes || a.k_tokens <= waves * kKeys) return;
     const int64_t lds = waves * (4 * kKeys * dp * size + (a.slopes ? 6 * kKeys * (size == 2 ? 16 : 4) : 0)) + 2048;
     const int64_t round = 256 * imin64(163840 / lds, 12 / waves);
     const int64_t most = ((int64_t)a.k_tokens + waves * kKeys - 1) / (waves * kKeys) * a.scenes;
     c->splits = 2;
-    c->even = (int)imax64(1, imin64(round / ((int64_t)a.kv_heads * c->head_tiles), most + a.scenes));
-    if (a.scenes * 2 >= c->even) c->rounds = kRounds;
-}
-// The pieces of a launch.
-int64_t paged_places(const AttnArgs &a, const CacheArgs &c) {
-    return c.splits == 1 ? a.scenes : c.rounds == 0 ? c.even : (int64_t)c.even * c.rounds + a.scenes;
+    c->shares = (int)imax64(1, imin64(round / ((int64_t)a.kv_heads * c->head_tiles), most + a.scenes));
 }
 
 struct Paged {
@@ -54,12 +47,12 @@ struct Paged {
     hipStream_t st;
     template <typename T, int DP, bool FAR, int CAP> void run() const {
         T *o = static_cast<T *>(out);
-        hipLaunchKernelGGL((k_attention_cached<T, DP, FAR, CAP, true>),
-                           dim3((unsigned)(paged_places(a, c) * a.kv_heads * c.head_tiles)), dim3(64 * kWaves<T, DP, true>), 0,
-                           st, a, c, o);
+        const dim3 grid((unsigned)((int64_t)c.shares * a.kv_heads * c.head_tiles)), block(64 * kWaves<T, DP, kPieces>);
+        if (a.scenes * 2 < c.shares) hipLaunchKernelGGL((k_attention_cached<T, DP, FAR, CAP, kPieces>), grid, block, 0, st, a, c, o);
+        else hipLaunchKernelGGL((k_attention_cached<T, DP, FAR, CAP, kShares>), grid, block, 0, st, a, c, o);
         if (c.splits > 1)
             hipLaunchKernelGGL(k_paged_join<T>, dim3((unsigned)(a.scenes * a.heads)), dim3(64 * kJoinWaves), 0, st,
-                               c.part_o, c.part_ms, c.pieces, make_fastdiv(a.heads), a.heads, a.dim, o);
+                               c.part_o, c.part_ms, c.parts, make_fastdiv(a.heads), a.heads, a.dim, o);
     }
 };
 
@@ -84,21 +77,21 @@ int paged_plan(const gsv_attention *args, const gsv_pages *p, AttnArgs *a, Cache
         return GSV_ERR_SIZE_OVERFLOW;
     *c = CacheArgs{};
     c->head_tiles = (int)tiles;
-    paged_pieces(*a, args->dtype, c);
+    paged_shares(*a, args->dtype, c);
     return GSV_OK;
 }
 
-// The workspace: parts of the sums, their maxima and sums of weights, and the scenes' pieces.
+// The workspace: parts of the sums, their maxima and sums of weights, and which are a scene's.
 struct Workspace {
-    size_t rows, ms, pieces, bytes;
+    size_t rows, ms, parts, bytes;
 };
 Workspace paged_workspace(const AttnArgs &a, const CacheArgs &c) {
     if (c.splits == 1) return {};
     Workspace w;
-    w.rows = (size_t)paged_places(a, c) * a.heads;
+    w.rows = ((size_t)c.shares + a.scenes) * a.heads;
     w.ms = w.rows * a.dim * sizeof(float);  // a multiple of 32 bytes
-    w.pieces = w.ms + w.rows * sizeof(float2);
-    w.bytes = w.pieces + a.scenes * sizeof(int2);
+    w.parts = w.ms + w.rows * sizeof(float2);
+    w.bytes = w.parts + a.scenes * sizeof(int2);
     return w;
 }
 
@@ -138,7 +131,7 @@ extern "C" int gsv_attention_paged(const gsv_attention *args, const gsv_pages *p
     c.k_pos_scene = pages->pos_page, c.keep_scene = pages->keep_page;
     c.part_o = static_cast<float *>(workspace);
     c.part_ms = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + ws.ms);
-    c.pieces = reinterpret_cast<int2 *>(static_cast<char *>(workspace) + ws.pieces);
+    c.parts = reinterpret_cast<int2 *>(static_cast<char *>(workspace) + ws.parts);
     c.table = pages->table, c.table_row = pages->table_row;
     c.pages = pages->pages, c.page_rows = pages->page_rows;
     c.by_rows = make_fastdiv(pages->page_rows);

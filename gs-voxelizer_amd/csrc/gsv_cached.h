@@ -27,91 +27,109 @@ struct CacheArgs {
     // strides from scene to scene, or from page to page
     int64_t k_scene, v_scene, k_pos_scene, keep_scene;
     int splits, head_tiles;  // splits: of each scene; of paged scenes, 1 where none is split
-    float *part_o;   // (scenes, heads, splits, dim) or (pieces, heads, dim): sums of weights times values
+    float *part_o;   // (scenes, heads, splits, dim) or (parts, heads, dim): sums of weights times values
     float2 *part_ms; // the same but the channels: maximum (log2) and sum of weights
     // paged: scene s's row j is row j % page_rows of page table[s table_row + j / page_rows]
     const int *table;
     int64_t table_row;
     int pages, page_rows;
     FastDiv by_rows;
-    int2 *pieces;  // of each scene: its first piece, and how many it has
-    int even, rounds;  // pieces that one round of workgroups holds; see paged_rows
+    int2 *parts;  // of each scene: its first part, and how many it has
+    int shares;   // workgroups of a key head
 };
 
-// A paged scene's keys, begin .. end - 1 of one of its `count` pieces; s < 0: no scene's.
-struct Piece {
-    int s, begin, end, count;
+// How rows lie, and what a workgroup takes of them: a cache's rows together, an equal split of one; rows in
+// pages, a piece of one scene, or an equal share of all scenes' steps.
+enum Rows { kTogether, kPieces, kShares };
+
+// What a workgroup takes of the paged scenes: `steps` from step `begin` of scene s on; s < 0: nothing.
+struct Share {
+    int s, begin, steps, most;  // most: of any workgroup
 };
 __device__ __forceinline__ int live_rows(const AttnArgs &a, const CacheArgs &c, int s) {
     return s < a.scenes ? min(max(c.lengths[s], 0), a.k_tokens) : 0;
 }
-// (an empty scene has a piece, which writes its zeros)
-__device__ __forceinline__ int pieces_of(int len, int per) { return len > 0 ? (len - 1) / per + 1 : 1; }
-// Keys of a piece, a multiple of a wave's step.  Scenes have at most rows / per + scenes pieces (one of len rows
-// has less than len / per + 1, and one at least).  With `rounds` 1, scenes are few against the pieces that one
-// round of workgroups has room for (`even`), and this is the least that fits in, from rows / even on;
-// rows / (even - scenes) always does.  Else the launch holds rounds * even + scenes of them, rows / (rounds * even)
-// each.  A lane adds its scenes' rows as integers; the wave's sum of 64 floats is raised by more
-// than its roundings.
-__device__ __forceinline__ int paged_rows(const AttnArgs &a, const CacheArgs &c, int each, int lane) {
-    int64_t mine = 0;
-    for (int i = 0; i < each; ++i) mine += live_rows(a, c, lane * each + i);
-    const float rows = wave_sum((float)mine) * 1.000002f;
-    const auto over = [&](float pieces) { return (int64_t)(rows / pieces * 1.000002f) / kKeys + 1; };
-    int64_t low = over((float)c.even * (c.rounds ? c.rounds : 1));
-    if (c.rounds == 0) {
-        int64_t high = over((float)(c.even - a.scenes));
-        while (low < high) {
-            const int64_t mid = (low + high) / 2;
-            int count = 0;
-            for (int i = 0; i < each; ++i)
-                if (lane * each + i < a.scenes) count += pieces_of(live_rows(a, c, lane * each + i), (int)imin64(mid * kKeys, INT32_MAX));
-            // (at most a few thousand: exact)
-            if (wave_sum((float)count) <= (float)c.even) high = mid;
-            else low = mid + 1;
-        }
+// (an empty scene has a step, which writes its zeros)
+__device__ __forceinline__ int steps_of(int len) { return len > 0 ? (len - 1) / kKeys + 1 : 1; }
+
+// The scenes' lengths are known on the device alone, so each workgroup cuts the batch for itself.  A lane takes a
+// run of scenes: up to 64 take one load and a scan over the lanes.
+//   kPieces (few scenes): pieces of one scene each, of the least size with which all of them fit one round of
+//     workgroups; `shares` of them do with steps / (shares - scenes) each.  Scene s's parts are its pieces.
+//   kShares: one scene after the other, cut in equal shares, which go on from a scene into the next.  However
+//     the lengths differ all workgroups end together, but one that has two scenes' keys starts twice.
+//     The part of scene s that workgroup n has is number n + s: a scene's parts are neighbours, and
+//     no two have one number.
+// 16 caches of 4,096, 2 key heads of 64 (step of 16 scenes): 16.6 us in pieces, 20.7 in shares; 20 of 8,000, 4 of 128
+// 53.5 and 57.4; 90 of 2,000 68.4 and 59.6; 100 of 3,000, 8 of 64 92.4 and 83.3.
+template <int W, int ROWS> __device__ __forceinline__ Share share_of(const AttnArgs &a, const CacheArgs &c, int n) {
+    if (c.splits == 1) {
+        const int all = __builtin_amdgcn_readfirstlane(steps_of(live_rows(a, c, n)));
+        return {n, 0, all, all};
     }
-    return (int)imin64(low * kKeys, INT32_MAX);
-}
-// Piece n of the batch: of the scenes one after the other.  A lane counts those of a run of scenes, so that
-// up to 64 scenes take one load and a scan over the lanes.
-__device__ __forceinline__ Piece paged_piece(const AttnArgs &a, const CacheArgs &c, int n) {
-    if (c.splits == 1) return {n, 0, __builtin_amdgcn_readfirstlane(live_rows(a, c, n)), 1};
     const int lane = threadIdx.x & 63, each = (a.scenes + 63) / 64;
-    const int per = __builtin_amdgcn_readfirstlane(paged_rows(a, c, each, lane));
-    int mine = 0;
-    for (int i = 0; i < each; ++i)
-        if (lane * each + i < a.scenes) mine += pieces_of(live_rows(a, c, lane * each + i), per);
-    int last = mine;  // pieces up to this lane's scenes
+    const auto sum = [&](const auto &of) {  // of a lane's scenes
+        int64_t x = 0;
+        for (int i = 0; i < each; ++i)
+            if (lane * each + i < a.scenes) x += of(steps_of(live_rows(a, c, lane * each + i)));
+        return x;
+    };
+    const auto scan = [&](int64_t x) {  // over the lanes
 #pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-        const int x = __shfl_up(last, k);
-        if (lane >= k) last += x;
+        for (int k = 1; k < 64; k <<= 1) {
+            const int64_t y = __shfl_up(x, k);
+            if (lane >= k) x += y;
+        }
+        return x;
+    };
+    int64_t mine = sum([](int steps) { return steps; }), last = scan(mine);
+    const int64_t all = __shfl(last, 63);
+    // (a scene has less than 2^26 steps)
+    int most = (int)imin64(imax64((all + c.shares - 1) / c.shares, W), INT32_MAX);
+    int64_t from = (int64_t)n * most;
+    if constexpr (ROWS == kPieces) {
+        int high = (int)imin64(imax64(all / (c.shares - a.scenes) + 1, most), INT32_MAX);
+        while (most < high) {
+            const int mid = most + (high - most) / 2;
+            const float count = wave_sum((float)sum([&](int steps) { return (steps - 1) / mid + 1; }));
+            if (count <= (float)c.shares) high = mid;  // (less than 2^11: exact)
+            else most = mid + 1;
+        }
+        most = __builtin_amdgcn_readfirstlane(most);
+        mine = sum([&](int steps) { return (steps - 1) / most + 1; }), last = scan(mine);
+        from = n;
     }
-    const uint64_t past = __ballot(last > n);
+    const uint64_t past = __ballot(last > from);
     if (!past) return {-1, 0, 0, 0};
     const int holder = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(past));
-    n -= __builtin_amdgcn_readlane(last - mine, holder);
-    for (int s = holder * each;; ++s) {
-        const int len = __builtin_amdgcn_readfirstlane(live_rows(a, c, s)), count = pieces_of(len, per);
-        // (the holder's pieces are more than n; the bound only makes the loop's end plain)
-        if (n < count || s + 1 >= a.scenes) return {s, n * per, len - n * per > per ? n * per + per : len, count};
-        n -= count;
+    int steps = (int)imin64(most, all - from);
+    from -= __shfl(last - mine, holder);
+    int s = holder * each, own = 0;
+    for (int i = 0; i < each; ++i, ++s) {  // among the holder's scenes
+        own = steps_of(live_rows(a, c, s));
+        const int has = ROWS == kPieces ? (own - 1) / most + 1 : own;
+        if (from < has || i + 1 == each) break;
+        from -= has;
     }
+    if (ROWS == kPieces) from *= most, steps = min(most, own - (int)from);
+    return {__builtin_amdgcn_readfirstlane(s), __builtin_amdgcn_readfirstlane((int)from),
+            __builtin_amdgcn_readfirstlane(steps), __builtin_amdgcn_readfirstlane(most)};
 }
+
 // Waves of a workgroup: four, two where their tiles would pass the LDS of a CU.
-template <typename T, int DP, bool PAGED>
-constexpr int kWaves = PAGED ? 512 / (DP * sizeof(T) < 128 ? 128 : DP * sizeof(T)) : DP * sizeof(T) > 256 ? 2 : 4;
+template <typename T, int DP, int ROWS>
+constexpr int kWaves = ROWS ? 512 / (DP * sizeof(T) < 128 ? 128 : DP * sizeof(T)) : DP * sizeof(T) > 256 ? 2 : 4;
 
 // bfloat16 weights enter the product with the values in two parts: the results are as exact as their type
 // (0.0017 in the 2-norm, in one part 0.0018 to 0.0020), for 0 to 4 % of the time beside the cache's bytes.
 template <typename T> constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
 
-template <typename T, int DP, bool FAR, int CAP, bool PAGED>
-__global__ __launch_bounds__((64 * kWaves<T, DP, PAGED>)) void k_attention_cached(const AttnArgs a, const CacheArgs c,
+template <typename T, int DP, bool FAR, int CAP, int ROWS>
+__global__ __launch_bounds__((64 * kWaves<T, DP, ROWS>)) void k_attention_cached(const AttnArgs a, const CacheArgs c,
                                                           T *__restrict__ out) {
     typedef typename Elem<T>::frag frag;
-    constexpr int W = kWaves<T, DP, PAGED>;
+    constexpr int W = kWaves<T, DP, ROWS>;
+    constexpr bool PAGED = ROWS != kTogether;
     static_assert(4 * kKeys * DP * sizeof(T) >= kHeads * DP * sizeof(float), "sums reuse the tiles");
     __shared__ __align__(1024) T tiles[W][4 * kKeys * DP];  // a wave's keys and values, two buffers
     __shared__ __align__(16) typename Places<T>::Row spos[W][2][3 * kKeys];
@@ -127,12 +145,23 @@ __global__ __launch_bounds__((64 * kWaves<T, DP, PAGED>)) void k_attention_cache
     int s, j_begin, j_end;
     bool whole;    // all of the scene's keys: the result goes to out
     int64_t part;  // else to this row, plus the head
+    Share share;
     if constexpr (PAGED) {
-        const Piece p = paged_piece(a, c, n);
-        if (p.s < 0) return;
-        s = p.s, j_begin = p.begin, j_end = p.end, whole = p.count == 1;
-        if (j_begin == 0 && hk == 0 && ht == 0 && threadIdx.x == 0 && c.splits > 1) c.pieces[s] = make_int2(n, p.count);
-        part = (int64_t)n * a.heads;
+        share = share_of<W, ROWS>(a, c, n);
+        if (share.s < 0) return;
+    }
+    while (true) {
+    if constexpr (PAGED) {
+        s = share.s;
+        const int len = __builtin_amdgcn_readfirstlane(live_rows(a, c, s));
+        const int all = steps_of(len), take = min(all - share.begin, share.steps);
+        j_begin = share.begin * kKeys, j_end = take < all - share.begin ? j_begin + take * kKeys : len;
+        whole = share.begin == 0 && take == all;
+        const int64_t number = (int64_t)n + (ROWS == kShares ? s : 0);
+        part = number * a.heads;
+        if (c.splits > 1 && share.begin == 0 && hk == 0 && ht == 0 && threadIdx.x == 0)
+            c.parts[s] = make_int2((int)number, 1 + (all - take + share.most - 1) / share.most);
+        share.steps -= take, share.begin = 0, ++share.s;
     } else {
         const int split = n % c.splits;
         s = n / c.splits;
@@ -356,6 +385,9 @@ __global__ __launch_bounds__((64 * kWaves<T, DP, PAGED>)) void k_attention_cache
             c.part_o[at * a.dim + dd] = val;
             if (dd == 0) c.part_ms[at] = make_float2(top, total);
         }
+    }
+    if (ROWS != kShares || share.steps <= 0 || share.s >= a.scenes) return;
+    __syncthreads();  // the next scene's copies go where the sums lay
     }
 }
 
