@@ -54,17 +54,16 @@ def test_rows_and_scenes_that_are_too_many():
 @pytest.mark.parametrize("scenes", [1, 2, 16, 65, 300, 5000])
 @pytest.mark.parametrize("table_pages", [0, 1, 8, 9, 200, 20_000])
 @pytest.mark.parametrize("dtype,dim", [(0, 32), (0, 128), (1, 40), (1, 64), (1, 128)])
-def test_the_workspace_holds_a_row_for_each_piece(scenes, table_pages, dtype, dim):
-    """Pieces are one for each scene and at most a round of workgroups more; none where a scene is one step."""
+def test_the_workspace_holds_a_row_for_each_part(scenes, table_pages, dtype, dim):
+    """Parts are one for each scene and at most a round of workgroups more; none where a scene is a step or two."""
     st, n = _plan(_query(scenes=scenes, q_tokens=scenes, dtype=dtype, dim=dim), _pages(table_pages=table_pages))
     assert st == OK
-    rows, rest = divmod(n, 4 * dim + 8)
-    assert rest == 0 and rows % 4 == 0
-    pieces = rows // 4
     if table_pages * 16 <= 64:
-        assert pieces == 0
-    elif pieces:
-        assert scenes < pieces <= scenes + 1024
+        assert n == 0
+    elif n:
+        rows, rest = divmod(n - 8 * scenes, 4 * dim + 8)
+        assert rest == 0 and rows % 4 == 0
+        assert scenes < rows // 4 <= scenes + 1024
 
 
 def test_a_workspace_that_is_too_small_is_refused():
