@@ -4,6 +4,10 @@
 // that its table names; keys (and the queries, which go to an output of their own) are turned as by rotary.hip.
 // Bytes bound it: each head is read and written once, in one launch.  A workgroup takes a few tokens: one wave
 // finds their rows, a lane each, while the others form the angles; both serve all heads from LDS.
+//
+// 20,000 tokens in 7 scenes, 8 + 8 + 8 heads of 64, bfloat16 (123 MB): 29.6 us, 4.2 TB/s; 65,537 in 190, 12 + 4 + 4 heads
+// of 40, 18 pairs, interleaved, float32 (421 MB): 87.0 us, 4.8 TB/s, what a large copy reaches.  One token for each
+// of 16 scenes: 7.8 us a call, the host's; the kernel takes 5, its chain of loads (lengths, table, tokens).
 #include "gsv_rotary.h"
 
 namespace gsv {
@@ -27,7 +31,7 @@ struct AppendArgs {
     int64_t table_row;
     int scenes, pages, page_rows, capacity;
     int block_tokens;
-    int token_items;  // of a token
+    int token_items, head_items, value_items;  // parts of a token, of one of its turned heads, of one of its values
     FastDiv by_rows, by_pairs, by_token, by_items, by_value;
 };
 
@@ -62,63 +66,101 @@ __device__ __forceinline__ Target target_of(const AppendArgs &a, int t, int s0) 
     return {page, (int)row - entry * a.page_rows};
 }
 
-// A thread's part of each token: some channels of one head.  It is found once, and then the same for all of the
-// workgroup's tokens: found anew for each, its divisions took more time than the bytes.
-template <typename T, int VEC, bool INTERLEAVED> struct Part {
-    const T *in;   // of token 0 of the array
-    T *out;        // of token 0 of q_out, or of page 0's first row
+// cos and sin of a token's angle for one pair, by the steps of rotary.hip: both give the same bits.  The angle
+// in binary64, brought into -pi .. pi there: a binary32 product would lose 2^-24 of an angle of some hundred
+// radians.
+__device__ __forceinline__ float2 turn_of(const float *position, int64_t axis, const float *frequencies, int pairs,
+                                          int axes) {
+    double th = 0.0;
+    for (int ax = 0; ax < axes; ++ax)
+        th = fma((double)position[ax * axis], (double)frequencies[ax * pairs], th);
+    const double turn = th * 0.15915494309189533577;
+    const float r = (float)((turn - rint(turn)) * 6.283185307179586477);
+    float sn, cs;
+    sincosf(r, &sn, &cs);
+    return make_float2(cs, sn);
+}
+
+// A thread's part of each token: two runs of one head's channels, both turned or both passed through.  It is
+// found once, and then the same for all of the workgroup's tokens: found anew for each, its divisions took more
+// time than the bytes.  Two runs always (the second may be the first again, where a row's runs are odd in number),
+// so that no load stands behind a branch: there the compiler waits for those before it.
+//   not interleaved: RUN pairs, channels first .. and second = first + pairs ..; interleaved: RUN / 2 pairs each.
+template <typename T, int RUN> struct Part {
+    const T *in;  // of token 0 of the array
+    T *out;       // of token 0 of q_out, or of page 0's first row
     int64_t in_row, out_page, out_row;
-    int item, turning, pairs;
-    bool q;
-    __device__ __forceinline__ Part(const AppendArgs &a, int j) {
-        constexpr int W = kPassed<VEC, INTERLEAVED>;
-        const int items = a.pairs / VEC + (a.dim - 2 * a.pairs) / W, all = (a.heads + a.kv_heads) * items;
-        q = false, turning = a.pairs / VEC, pairs = a.pairs;
-        if (j >= all) {
-            const int h = fastdiv(j - all, a.by_value);
-            item = j - all - h * (a.dim / W), turning = pairs = 0;
-            in = static_cast<const T *>(a.v) + h * a.v_head, in_row = a.v_row;
-            out = static_cast<T *>(a.v_pool) + h * a.vp_head, out_page = a.vp_page, out_row = a.vp_row;
-            return;
-        }
-        int h = fastdiv(j, a.by_items);
-        item = j - h * items;
-        if (h < a.heads) {
-            q = true;
-            in = static_cast<const T *>(a.q) + h * a.q_head, in_row = a.q_row;
-            out = static_cast<T *>(a.q_out) + (int64_t)h * a.dim, out_page = 0, out_row = (int64_t)a.heads * a.dim;
+    int first, second;
+    bool q, turns;
+};
+template <typename T, int RUN, bool INTERLEAVED> __device__ __forceinline__ Part<T, RUN> part_of(const AppendArgs &a, int j) {
+    Part<T, RUN> p;
+    const int all = (a.heads + a.kv_heads) * a.head_items;
+    int runs = a.dim / RUN, from = 0, i, h;  // the runs that are taken two by two, from a channel on
+    if (j >= all) {
+        h = fastdiv(j - all, a.by_value), i = j - all - h * a.value_items;
+        p.in = static_cast<const T *>(a.v) + h * a.v_head, p.in_row = a.v_row;
+        p.out = static_cast<T *>(a.v_pool) + h * a.vp_head, p.out_page = a.vp_page, p.out_row = a.vp_row;
+        p.q = p.turns = false;
+    } else {
+        h = fastdiv(j, a.by_items), i = j - h * a.head_items;
+        p.q = h < a.heads;
+        if (p.q) {
+            p.in = static_cast<const T *>(a.q) + h * a.q_head, p.in_row = a.q_row;
+            p.out = static_cast<T *>(a.q_out) + (int64_t)h * a.dim, p.out_page = 0, p.out_row = (int64_t)a.heads * a.dim;
         } else {
             h -= a.heads;
-            in = static_cast<const T *>(a.k) + h * a.k_head, in_row = a.k_row;
-            out = static_cast<T *>(a.k_pool) + h * a.kp_head, out_page = a.kp_page, out_row = a.kp_row;
+            p.in = static_cast<const T *>(a.k) + h * a.k_head, p.in_row = a.k_row;
+            p.out = static_cast<T *>(a.k_pool) + h * a.kp_head, p.out_page = a.kp_page, p.out_row = a.kp_row;
         }
+        const int turning = INTERLEAVED ? (2 * a.pairs / RUN + 1) / 2 : a.pairs / RUN;
+        p.turns = i < turning;
+        if (p.turns && !INTERLEAVED) {
+            p.first = i * RUN, p.second = a.pairs + i * RUN;
+            return p;
+        }
+        if (p.turns) runs = 2 * a.pairs / RUN;
+        else i -= turning, from = 2 * a.pairs, runs -= from / RUN;
     }
-};
+    const int half = (runs + 1) / 2;
+    p.first = from + i * RUN, p.second = i + half < runs ? p.first + half * RUN : p.first;
+    return p;
+}
 
 // Tokens of a thread that are loaded at once (the first ones before their rows and angles are known), and all that it
-// takes, over which the chains of loads at a workgroup's start spread.  20,000 tokens (below) take 28.9 us with 8 of
-// them, 30.9 with 16 and 30.0 with 4 at once and no more; 65,537 104, 105 and 116.
-constexpr int kDeep = 2, kTokens = 8;
+// takes, over which the chains of loads at a workgroup's start spread.  The cases above: 29.6 and 87.0 us; with 8 tokens
+// 29.7 and 92.0, with 4 at once 31.4 and 87.6, one at a time 32.0 and 90.7.
+constexpr int kDeep = 2, kTokens = 4;
 
-template <typename T, int VEC, bool INTERLEAVED>
+// A run as it lies in memory: words, which are loaded and stored in one piece (of a struct of bfloat16 the compiler
+// makes loads of two and four bytes).
+template <int BYTES> struct Words {
+    typedef uint32_t type __attribute__((ext_vector_type(BYTES / 4)));
+};
+template <> struct Words<4> { typedef uint32_t type; };
+template <> struct Words<2> { typedef uint16_t type; };
+
+template <typename T, int RUN, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void k_paged_append(const AppendArgs a) {
+    typedef typename Words<RUN * sizeof(T)>::type Run;
+    typedef Pack<T, RUN> Values;
     extern __shared__ float2 turns[];  // cos, sin of block_tokens x pairs
     __shared__ Target target[64];
     const int t0 = blockIdx.x * a.block_tokens, nt = min(a.block_tokens, a.tokens - t0);
     // a thread's first part and token: as many tokens side by side as have room
     const int side = max(256 / a.token_items, 1);
     const int first_t = side > 1 ? fastdiv(threadIdx.x, a.by_token) : 0, first_j = threadIdx.x - first_t * a.token_items;
-    const bool mine = first_t < side;
     bool begun = false;
     for (int j = first_j; j - first_j < a.token_items; j += 256) {
-        const bool has = mine && j < a.token_items;
-        const Part<T, VEC, INTERLEAVED> p(a, has ? j : 0);
+        const bool has = first_t < side && j < a.token_items;
+        const Part<T, RUN> p = part_of<T, RUN, INTERLEAVED>(a, has ? j : 0);
         for (int tb = 0; tb < nt; tb += side * kDeep) {
-            TurnItem<T, VEC, INTERLEAVED> x[kDeep];
+            Run x[kDeep], z[kDeep];
 #pragma unroll
             for (int k = 0; k < kDeep; ++k) {
-                const int t = tb + k * side + first_t;
-                if (has && t < nt) x[k].load(p.in + (t0 + t) * p.in_row, p.item, p.turning, p.pairs);
+                const T *in = p.in + (t0 + min(tb + k * side + first_t, nt - 1)) * p.in_row;
+                x[k] = *reinterpret_cast<const Run *>(in + p.first);
+                z[k] = *reinterpret_cast<const Run *>(in + p.second);
             }
             if (!begun) {
                 begun = true;
@@ -142,8 +184,29 @@ __global__ __launch_bounds__(256) void k_paged_append(const AppendArgs a) {
                 Target to = target[t];
                 if (p.q) to = {0, t0 + t};
                 if (to.page < 0) continue;
-                x[k].store(p.out + to.page * p.out_page + to.row * p.out_row, p.item, p.turning, p.pairs,
-                           turns + t * a.pairs);
+                if (p.turns) {
+                    const float2 *w = turns + t * a.pairs;
+                    Values u = __builtin_bit_cast(Values, x[k]), v = __builtin_bit_cast(Values, z[k]);
+                    if constexpr (INTERLEAVED) {
+#pragma unroll
+                        for (int e = 0; e < RUN; e += 2) {
+                            const float2 y = turned((float)u.v[e], (float)u.v[e + 1], w[(p.first + e) / 2]);
+                            u.v[e] = (T)y.x, u.v[e + 1] = (T)y.y;
+                            const float2 s = turned((float)v.v[e], (float)v.v[e + 1], w[(p.second + e) / 2]);
+                            v.v[e] = (T)s.x, v.v[e + 1] = (T)s.y;
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < RUN; ++e) {
+                            const float2 y = turned((float)u.v[e], (float)v.v[e], w[p.first + e]);
+                            u.v[e] = (T)y.x, v.v[e] = (T)y.y;
+                        }
+                    }
+                    x[k] = __builtin_bit_cast(Run, u), z[k] = __builtin_bit_cast(Run, v);
+                }
+                T *out = p.out + to.page * p.out_page + to.row * p.out_row;
+                *reinterpret_cast<Run *>(out + p.first) = x[k];
+                *reinterpret_cast<Run *>(out + p.second) = z[k];
             }
         }
     }
@@ -167,25 +230,17 @@ __global__ __launch_bounds__(256) void k_paged_append(const AppendArgs a) {
     }
 }
 
-template <typename T, bool INTERLEAVED> void launch_append(const AppendArgs &a, int vec, hipStream_t s) {
+template <typename T, bool INTERLEAVED> void launch_append(const AppendArgs &a, int run, hipStream_t s) {
     const dim3 grid((a.tokens + a.block_tokens - 1) / a.block_tokens), block(256);
     const size_t lds = sizeof(float2) * a.block_tokens * a.pairs;
-    switch (vec) {
-        case 8:
-            if constexpr (!INTERLEAVED && sizeof(T) == 2) {
-                hipLaunchKernelGGL((k_paged_append<T, 8, INTERLEAVED>), grid, block, lds, s, a);
-                break;
-            }
-            [[fallthrough]];
-        case 4:
-            if constexpr (!(INTERLEAVED && sizeof(T) == 4)) {
-                hipLaunchKernelGGL((k_paged_append<T, 4, INTERLEAVED>), grid, block, lds, s, a);
-                break;
-            }
-            [[fallthrough]];
-        case 2: hipLaunchKernelGGL((k_paged_append<T, 2, INTERLEAVED>), grid, block, lds, s, a); break;
-        default: hipLaunchKernelGGL((k_paged_append<T, 1, INTERLEAVED>), grid, block, lds, s, a);
-    }
+    if constexpr (sizeof(T) == 2)
+        if (run == 8) {
+            hipLaunchKernelGGL((k_paged_append<T, 8, INTERLEAVED>), grid, block, lds, s, a);
+            return;
+        }
+    if (run == 4) hipLaunchKernelGGL((k_paged_append<T, 4, INTERLEAVED>), grid, block, lds, s, a);
+    else if (run == 2) hipLaunchKernelGGL((k_paged_append<T, 2, INTERLEAVED>), grid, block, lds, s, a);
+    else if constexpr (!INTERLEAVED) hipLaunchKernelGGL((k_paged_append<T, 1, INTERLEAVED>), grid, block, lds, s, a);
 }
 
 // The stride of an axis of one entry is never used, whatever a caller's view holds there.
@@ -228,12 +283,12 @@ extern "C" int gsv_paged_append(const gsv_rotary_args *r, const void *v, int64_t
     // the widest access that both halves of a row's pairs and what follows them are aligned for
     uint64_t low = 16 | (uint64_t)(r->dim * size) | (uint64_t)((r->dim - 2 * r->pairs) * size) |
                    (uint64_t)(r->pairs * size * (r->interleaved ? 2 : 1));
-    const int bytes = (int)(low & (0 - low));
-    const int vec = r->interleaved && bytes > size ? bytes / size / 2 : bytes / size;
-    const int passed = r->interleaved && vec > 1 ? 2 * vec : vec;
-    // Tokens of a workgroup: as many as its threads hold at once, fewer where the launch would leave CUs idle; their
+    const int run = (int)((low & (0 - low)) / size);  // (2 at least where interleaved: rows and pairs are even)
+    const auto twos = [&](int runs) { return (runs + 1) / 2; };
+    const int items = (r->interleaved ? twos(2 * r->pairs / run) : r->pairs / run) + twos((r->dim - 2 * r->pairs) / run);
+    const int values = twos(r->dim / run);
+    // Tokens of a workgroup: as many as its threads take, fewer where the launch would leave CUs idle; their
     // angles within 16 KB of LDS, a lane for each.
-    const int items = r->pairs / vec + (r->dim - 2 * r->pairs) / passed, values = r->dim / passed;
     const int64_t each = (r->heads + K) * items + K * values;
     int64_t bt = kTokens * imax64(1, 256 / each);
     bt = imin64(bt, imax64(1, T / 1024));
@@ -248,13 +303,13 @@ extern "C" int gsv_paged_append(const gsv_rotary_args *r, const void *v, int64_t
                        r->tokens, r->heads, r->kv_heads, r->dim, r->pairs, r->axes, r->positions, r->frequencies,
                        r->pos_row, r->pos_axis, p->positions, p->pos_page, p->pos_row, keep, p->keep, p->keep_page,
                        keep_bytes, p->keep_bytes, lengths, starts, p->table, p->table_row, scenes, p->pages,
-                       p->page_rows, (int)rows, (int)bt, (int)each, make_fastdiv(p->page_rows),
+                       p->page_rows, (int)rows, (int)bt, (int)each, items, values, make_fastdiv(p->page_rows),
                        make_fastdiv(r->pairs ? r->pairs : 1), make_fastdiv(each), make_fastdiv(items),
                        make_fastdiv(values)};
     hipStream_t s = as_stream(stream);
     if (r->dtype == GSV_BF16)
-        r->interleaved ? launch_append<bf16, true>(a, vec, s) : launch_append<bf16, false>(a, vec, s);
+        r->interleaved ? launch_append<bf16, true>(a, run, s) : launch_append<bf16, false>(a, run, s);
     else
-        r->interleaved ? launch_append<float, true>(a, vec, s) : launch_append<float, false>(a, vec, s);
+        r->interleaved ? launch_append<float, true>(a, run, s) : launch_append<float, false>(a, run, s);
     return check_launch();
 }

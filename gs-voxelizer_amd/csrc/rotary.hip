@@ -33,15 +33,25 @@ __global__ __launch_bounds__(256) void k_rotary(const RotaryArgs a) {
     const int t0 = blockIdx.x * a.block_tokens, nt = min(a.block_tokens, a.tokens - t0);
     for (int i = threadIdx.x; i < nt * a.pairs; i += 256) {
         const int t = fastdiv(i, a.by_pairs), p = i - t * a.pairs;
-        const float2 w = turn_of(a.positions + (t0 + t) * a.pos_row, a.pos_axis, a.frequencies + p, a.pairs, a.axes);
-        turns[i] = make_float2(w.x, a.sign * w.y);
+        // the angle in binary64, brought into -pi .. pi there: a binary32 product would lose
+        // 2^-24 of an angle of some hundred radians
+        double th = 0.0;
+        for (int ax = 0; ax < a.axes; ++ax)
+            th = fma((double)a.positions[(t0 + t) * a.pos_row + ax * a.pos_axis],
+                     (double)a.frequencies[ax * a.pairs + p], th);
+        const double turn = th * 0.15915494309189533577;
+        const float r = (float)((turn - rint(turn)) * 6.283185307179586477);
+        float sn, cs;
+        sincosf(r, &sn, &cs);
+        turns[i] = make_float2(cs, a.sign * sn);
     }
     __syncthreads();
     // a row's items: its pairs, then the channels past them, which pass through
+    constexpr int W = INTERLEAVED && VEC > 1 ? 2 * VEC : VEC;
     const int all = a.heads + a.kv_heads, turning = a.pairs / VEC;
-    const int items = turning + (a.dim - 2 * a.pairs) / kPassed<VEC, INTERLEAVED>;
+    const int items = turning + (a.dim - 2 * a.pairs) / W;
     for (int i = threadIdx.x; i < nt * all * items; i += 256) {
-        const int row = fastdiv(i, a.by_items), item = i - row * items;
+        const int row = fastdiv(i, a.by_items), item = i - row * items, p = item * VEC;
         const int t = fastdiv(row, a.by_heads), h = row - t * all;
         const bool is_q = h < a.heads;
         const int64_t token = t0 + t;
@@ -49,9 +59,37 @@ __global__ __launch_bounds__(256) void k_rotary(const RotaryArgs a) {
                            : static_cast<const T *>(a.k) + token * a.k_row + (h - a.heads) * a.k_head;
         T *out = is_q ? static_cast<T *>(a.q_out) + (token * a.heads + h) * a.dim
                       : static_cast<T *>(a.k_out) + (token * a.kv_heads + h - a.heads) * a.dim;
-        TurnItem<T, VEC, INTERLEAVED> x;
-        x.load(in, item, turning, a.pairs);
-        x.store(out, item, turning, a.pairs, turns + t * a.pairs);
+        if (item >= turning) {
+            typedef Pack<T, W> P;
+            const int d = 2 * a.pairs + (item - turning) * W;
+            *reinterpret_cast<P *>(out + d) = *reinterpret_cast<const P *>(in + d);
+            continue;
+        }
+        const float2 *tp = turns + t * a.pairs + p;
+        if constexpr (INTERLEAVED && VEC == 1) {
+            const float2 z = turned((float)in[2 * p], (float)in[2 * p + 1], *tp);
+            out[2 * p] = (T)z.x, out[2 * p + 1] = (T)z.y;
+        } else if constexpr (INTERLEAVED) {
+            typedef Pack<T, 2 * VEC> P;
+            P x = *reinterpret_cast<const P *>(in + 2 * p);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float2 z = turned((float)x.v[2 * e], (float)x.v[2 * e + 1], tp[e]);
+                x.v[2 * e] = (T)z.x, x.v[2 * e + 1] = (T)z.y;
+            }
+            *reinterpret_cast<P *>(out + 2 * p) = x;
+        } else {
+            typedef Pack<T, VEC> P;
+            P x = *reinterpret_cast<const P *>(in + p);
+            P z = *reinterpret_cast<const P *>(in + a.pairs + p);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float2 y = turned((float)x.v[e], (float)z.v[e], tp[e]);
+                x.v[e] = (T)y.x, z.v[e] = (T)y.y;
+            }
+            *reinterpret_cast<P *>(out + p) = x;
+            *reinterpret_cast<P *>(out + a.pairs + p) = z;
+        }
     }
 }
 
