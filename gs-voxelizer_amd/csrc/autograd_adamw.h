@@ -83,8 +83,8 @@ py::tuple adamw_step(py::handle params, py::handle grads, py::handle exp_avgs, p
                 : c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
         return other();
     std::vector<gsv_adamw_tensor> all(n);
-    std::vector<const Tensor *> changed;
-    changed.reserve(4 * n + 1);
+    std::vector<Tensor> held;  // while other threads may run, and change the lists
+    held.reserve(5 * n + 1);
     for (Py_ssize_t i = 0; i < n; ++i) {
         const Tensor *p = tensor_in(ps[i]), *g = tensor_in(gs[i]), *m = tensor_in(ms[i]), *v = tensor_in(vs[i]), *w = nullptr;
         if (mastered && ws[i] != Py_None && !(w = tensor_in(ws[i]))) return other();
@@ -102,11 +102,11 @@ py::tuple adamw_step(py::handle params, py::handle grads, py::handle exp_avgs, p
         x.param = ptr<void>(*p), x.grad = ptr<void>(*g), x.exp_avg = ptr<float>(*m), x.exp_avg_sq = ptr<float>(*v);
         x.master = w ? ptr<float>(*w) : nullptr, x.numel = p->numel(), x.step = (int64_t)t;
         x.lr = rate, x.weight_decay = decay, x.dtype = type_code(*p), x.grad_dtype = type_code(*g);
-        for (const Tensor *c : {p, m, v})
-            changed.push_back(c);
-        if (w) changed.push_back(w);
+        for (const Tensor *t : {p, m, v, w})
+            if (t) held.push_back(*t);
+        held.push_back(*g);
     }
-    if (counter) changed.push_back(counter);
+    if (counter) held.push_back(*counter);
     gsv_adamw_args a{};
     a.tensors = all.data(), a.count = (int64_t)n;
     a.beta1 = b1, a.beta2 = b2, a.eps = eps, a.max_norm = max_norm;
@@ -127,7 +127,11 @@ py::tuple adamw_step(py::handle params, py::handle grads, py::handle exp_avgs, p
     }
     if (status == GSV_ERR_INVALID_ARGUMENT) return other();  // tensors share memory; nothing was launched
     check(status, "adamw");
-    for (const Tensor *t : changed) written(*t);
+    for (Py_ssize_t i = 0, at = 0; i < n; ++i) {
+        for (const int more = all[i].master ? 4 : 3, from = at; at < from + more; ++at) written(held[at]);
+        ++at;  // the gradient
+    }
+    if (counter) written(held.back());
     if (!norm.defined()) return py::make_tuple(true, py::none());
     return py::make_tuple(true, py::reinterpret_steal<py::object>(THPVariable_Wrap(norm)));
 }

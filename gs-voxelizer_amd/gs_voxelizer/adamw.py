@@ -42,7 +42,8 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
 
     Args:
         params: float32 or bfloat16 tensors of one device, without gaps.
-        grads: a float32 or bfloat16 gradient each; they are not changed, also not by max_norm.
+        grads: a float32 or bfloat16 gradient each, apart from what the step writes; they are not changed, also
+            not by max_norm.
         exp_avgs, exp_avg_sqs: the float32 state, laid out like the params.
         step: the number of this step, from 1, for all tensors or for each; or a (1,) int32 tensor on the
             device that counts the steps made, which the call advances.  A captured step needs the
@@ -70,7 +71,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
             if not (_is_number(x) or (what == "lr" and isinstance(x, Tensor))):
                 raise ValueError(f"{what} must be numbers, got {x!r}")
     for x in steps:
-        if not isinstance(x, int) or x < 1:
+        if not isinstance(x, int) or not 1 <= x < 2**53:
             raise ValueError(f"step must be whole numbers from 1, got {x!r}")
     return _step(params, grads, exp_avgs, exp_avg_sqs, masters, steps, counter, rates, decays, betas, eps, max_norm)
 
@@ -152,7 +153,7 @@ def _step(params, grads, exp_avgs, exp_avg_sqs, masters, steps, counter, rates, 
             _t.call("adamw", ctypes.byref(a), ws.data_ptr(), size, _t.stream(dev))
         except RuntimeError as e:
             # (what else the library refuses is checked above)
-            raise ValueError(f"{e}: tensors that the step writes share memory") if "argument" in str(e) else e
+            raise ValueError(f"{e}: a tensor that the step writes shares memory with another, or with a gradient") if "argument" in str(e) else e
     _t.written(*params, *exp_avgs, *exp_avg_sqs, *(masters or []), counter)
     return norm
 

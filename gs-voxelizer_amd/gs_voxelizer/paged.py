@@ -107,7 +107,7 @@ def append_tokens(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_t
 
     Args:
         k, v: (T, K, D) new tokens, D a multiple of 8 up to 128 (views into one projection's output are taken
-            as they are).
+            as they are, but not views of the pools).
         k_pages, v_pages: (pages, rows, K, D), rows a multiple of 16, written in place; they may be
             halves of one pool, pool[:, 0] and pool[:, 1].
         page_table: (S, most) int32.

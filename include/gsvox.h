@@ -508,7 +508,7 @@ int gsv_gated_norm_bwd(const gsv_norm *args, const void *dy, int64_t dy_row, con
  * values in the same order, aligned to their own size.  t is the tensor's step, 1 or more; with `counter` (one
  * int32 on the device, steps made so far) t = *counter + 1 for all, and the call advances it.  lr_device: NULL, or the
  * rate, one float on the device.  norm (NULL, or one float on the device) receives |all grads| where max_norm > 0.
- * Tensors that share memory are refused (GSV_ERR_INVALID_ARGUMENT).  The norm is summed in binary64 in a fixed order.
+ * Written tensors that share memory with each other or a gradient are refused (GSV_ERR_INVALID_ARGUMENT).  The norm is summed in binary64 in a fixed order.
  */
 typedef struct gsv_adamw_tensor {
     void *param;

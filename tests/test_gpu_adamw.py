@@ -313,8 +313,11 @@ def test_refusals(device):
     no("laid out like", params=[torch.zeros(5, 10, device=device).t()], grads=[torch.zeros(10, 5, device=device)],
        exp_avgs=[torch.zeros(10, 5, device=device)], exp_avg_sqs=[torch.zeros(10, 5, device=device)])
     no("needs none", masters=[torch.zeros(50, device=device), None])
-    no("share memory", exp_avgs=[s.exp_avgs[0], s.exp_avgs[0][:20]])
-    no("share memory", params=[f, f], grads=[s.grads[0]] * 2, exp_avgs=[s.exp_avgs[0], f.clone()],
+    no("shares memory", exp_avgs=[s.exp_avgs[0], s.exp_avgs[0][:20]])
+    no("shares memory", grads=[f, s.grads[1]])
+    no("shares memory", grads=[s.grads[0], s.exp_avg_sqs[0][30:]])
+    no("whole numbers", step=2**64 + 1)
+    no("shares memory", params=[f, f], grads=[s.grads[0]] * 2, exp_avgs=[s.exp_avgs[0], f.clone()],
        exp_avg_sqs=[s.exp_avg_sqs[0], f.clone()])
     no("whole numbers", step=0)
     no("whole numbers", step=1.5)

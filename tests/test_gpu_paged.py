@@ -168,6 +168,28 @@ def test_many_scenes(device, dtype, scenes):
 
 
 @TYPES
+@pytest.mark.parametrize("heads,dim", [((16, 8), 128), ((8, 8), 64), ((6, 3), 40), ((17, 1), 32), ((64, 2), 96), ((32, 32), 8)],
+                         ids=lambda x: str(x))
+@pytest.mark.parametrize("lengths", [[900, 33, 0, 2000, 1, 150] * 9, [64] * 40 + [5000], [3000] * 4],
+                         ids=["many", "long last", "few"])
+def test_heads_and_cuts(device, dtype, heads, dim, lengths):
+    """Few and many heads of one key head, that share lines of memory and that do not, in batches that are cut by
+    scenes and by equal shares."""
+    c = Case(device, dtype, lengths, *heads, dim, rows=64, cap=20.0)
+    c.check(c.run(), scenes=[0, 1, 2, 3, len(lengths) - 1])
+    alone = c.run(keep_pages=torch.ones(c.k_pages.shape[:2], dtype=torch.bool, device=device))
+    assert torch.equal(alone, c.run())  # a mask that hides nothing, the same bits
+
+
+@TYPES
+def test_no_room_and_no_scenes(device, route, dtype):
+    c = Case(device, dtype, [40, 20], 4, 2, 64)
+    assert not c.run(page_table=c.table[:, :0]).any()
+    got = c.run(q=c.q[:0], page_table=c.table[:0], lengths=c.device_lengths[:0], positions=c.positions[:0])
+    assert got.shape == (0, 4, 64)
+
+
+@TYPES
 def test_a_scene_does_not_depend_on_others_values(device, dtype):
     """Other scenes' values, of the same lengths, change no bit."""
     a, b = (Case(device, dtype, [900, 20, 0, 333], 4, 2, 64, seed=s) for s in (1, 2))

@@ -160,9 +160,11 @@ def test_a_step_s_workspace():
 
 @pytest.mark.parametrize("second", [
     dict(param=(1 << 20) + 396), dict(exp_avg=3 << 20), dict(exp_avg_sq=(4 << 20) - 396), dict(exp_avg=(1 << 20) + 4),
-    dict(param=(6 << 20), exp_avg=6 << 20), dict(dtype=1, master=(4 << 20) + 396)])
+    dict(param=(6 << 20), exp_avg=6 << 20), dict(dtype=1, master=(4 << 20) + 396), dict(grad=(1 << 20) + 396),
+    dict(grad=(4 << 20) - 396), dict(grad_dtype=1, grad=(3 << 20) - 198)])
 def test_tensors_that_share_memory_are_refused(second):
     """(Before anything is launched: these addresses are nobody's.)"""
     a, _all, st, _ = _adamw([_tensor(), _tensor(1 << 16, **second)])
     assert st == OK
+    assert _adamw([_tensor(), _tensor(1 << 16)])[2] == OK
     assert _lib.load().gsv_adamw(ctypes.byref(a), None, 0, None) == INVALID
