@@ -127,6 +127,7 @@ __device__ __forceinline__ int64_t wave_scan(int64_t x) {
 // What a workgroup takes of the scenes: `steps` from step `begin` of scene s on; s < 0: nothing.
 struct Share {
     int s, begin, steps, most;  // most: of any workgroup
+    int len;                    // rows of scene s
 };
 __device__ __forceinline__ int live_rows(const AttnArgs &a, const PageArgs &c, int s) {
     return s < a.scenes ? min(max(c.lengths[s], 0), a.k_tokens) : 0;
@@ -145,60 +146,64 @@ template <typename T> __device__ __forceinline__ int steps_of(int len) { return 
 enum Cut { kPieces, kShares };
 template <typename T, int W, Cut CUT> __device__ __forceinline__ Share share_of(const AttnArgs &a, const PageArgs &c, int n) {
     if (!c.split) {
-        const int all = __builtin_amdgcn_readfirstlane(steps_of<T>(live_rows(a, c, n)));
-        return {n, 0, all, all};
+        const int len = __builtin_amdgcn_readfirstlane(live_rows(a, c, n)), all = steps_of<T>(len);
+        return {n, 0, all, all, len};
     }
     const int lane = threadIdx.x & 63, each = (a.scenes + 63) / 64;
     const int first = lane * each, behind = min(first + each, a.scenes);
+    // the first (up to 64 scenes: the only) one's rows stay in a register: each further look at a length is a load
+    const int len = live_rows(a, c, first);
+    const auto sum = [&](auto x, const auto &of) {  // of a lane's scenes
+        if (first < behind) x += of(steps_of<T>(len));
+        for (int s = first + 1; s < behind; ++s) x += of(steps_of<T>(live_rows(a, c, s)));
+        return x;
+    };
     int holder, most, begin, steps;
     if constexpr (CUT == kPieces) {
-        const auto pieces = [&](int of) {  // of a lane's scenes
-            int x = 0;
-            for (int s = first; s < behind; ++s) x += (steps_of<T>(live_rows(a, c, s)) - 1) / of + 1;
-            return x;
-        };
-        float mine = 0.f;
-        for (int s = first; s < behind; ++s) mine += (float)steps_of<T>(live_rows(a, c, s));
         // (raised by more than what the sums of floats may have lost)
-        const float all = wave_sum(mine) * 1.00002f;
-        most = max((int)fminf(all / (float)c.shares, 1e9f) , W);
+        const float all = wave_sum(sum(0.f, [](int steps) { return (float)steps; })) * 1.00002f;
+        most = max((int)fminf(all / (float)c.shares, 1e9f), W);
         int high = max((int)fminf(all / (float)(c.shares - a.scenes), 1e9f) + 1, most);
         while (most < high) {
             const int mid = most + (high - most) / 2;
-            if (wave_sum((float)pieces(mid)) <= (float)c.shares) high = mid;  // (less than 2^12: exact)
+            const float count = wave_sum((float)sum(0, [&](int steps) { return (steps - 1) / mid + 1; }));
+            if (count <= (float)c.shares) high = mid;  // (less than 2^12: exact)
             else most = mid + 1;
         }
         most = __builtin_amdgcn_readfirstlane(most);
-        const int own = pieces(most), last = wave_scan(own);
+        const int own = sum(0, [&](int steps) { return (steps - 1) / most + 1; }), last = wave_scan(own);
         const uint64_t past = __ballot(last > n);
-        if (!past) return {-1, 0, 0, 0};
+        if (!past) return {-1, 0, 0, 0, 0};
         holder = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(past));
         begin = n - __builtin_amdgcn_readlane(last - own, holder);
         steps = most;
     } else {
-        int64_t own = 0;
-        for (int s = first; s < behind; ++s) own += steps_of<T>(live_rows(a, c, s));
+        const int64_t own = sum((int64_t)0, [](int steps) { return steps; });
         const int64_t last = wave_scan(own), all = __shfl(last, 63);
         // (a scene has less than 2^27 steps)
         most = (int)imin64(imax64((all + c.shares - 1) / c.shares, W), INT32_MAX);
         const int64_t from = (int64_t)n * most;
         const uint64_t past = __ballot(last > from);
-        if (!past) return {-1, 0, 0, 0};
+        if (!past) return {-1, 0, 0, 0, 0};
         holder = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(past));
         steps = (int)imin64(most, all - from);
-        // of the holder's scenes, each of which has less than 2^27: within 2^31 for 16 of them, else the loop ends early
-        begin = (int)imin64(from - __shfl(last - own, holder), INT32_MAX);
+        int64_t skip = from - __shfl(last - own, holder);
+        // among the holder's scenes; what is left then lies in one scene
+        int s = holder * each, rows = __builtin_amdgcn_readlane(len, holder);
+        for (int i = 1; i < each && skip >= steps_of<T>(rows); ++i) {
+            skip -= steps_of<T>(rows);
+            rows = __builtin_amdgcn_readfirstlane(live_rows(a, c, ++s));
+        }
+        return {__builtin_amdgcn_readfirstlane(s), __builtin_amdgcn_readfirstlane((int)imin64(skip, INT32_MAX / kKeys<T>)),
+                __builtin_amdgcn_readfirstlane(steps), __builtin_amdgcn_readfirstlane(most), __builtin_amdgcn_readfirstlane(rows)};
     }
-    int s = holder * each, all = 0;
-    for (int i = 0; i < each; ++i, ++s) {  // among the holder's scenes
-        all = steps_of<T>(live_rows(a, c, s));
-        const int has = CUT == kPieces ? (all - 1) / most + 1 : all;
-        if (begin < has || i + 1 == each) break;
-        begin -= has;
+    int s = holder * each, rows = __builtin_amdgcn_readlane(len, holder);
+    for (int i = 1; i < each && begin >= (steps_of<T>(rows) - 1) / most + 1; ++i) {
+        begin -= (steps_of<T>(rows) - 1) / most + 1;
+        rows = __builtin_amdgcn_readfirstlane(live_rows(a, c, ++s));
     }
-    if (CUT == kPieces) begin *= most;
-    return {__builtin_amdgcn_readfirstlane(s), __builtin_amdgcn_readfirstlane(begin),
-            __builtin_amdgcn_readfirstlane(steps), __builtin_amdgcn_readfirstlane(most)};
+    return {__builtin_amdgcn_readfirstlane(s), __builtin_amdgcn_readfirstlane(begin * most), steps, most,
+            __builtin_amdgcn_readfirstlane(rows)};
 }
 
 template <typename T, int DP, bool FAR, int CAP, Cut CUT>
@@ -247,7 +252,7 @@ __global__ __launch_bounds__((64 * kWaves<DP>)) void k_attention_paged(const Att
     constexpr int step = W * KEYS;
 
     while (true) {
-        const int s = share.s, len = __builtin_amdgcn_readfirstlane(live_rows(a, c, s));
+        const int s = share.s, len = share.len;
         const int all = steps_of<T>(len), take = min(all - share.begin, share.steps);
         const int j_begin = share.begin * KEYS, j_end = take < all - share.begin ? j_begin + take * KEYS : len;
         const bool whole = share.begin == 0 && take == all;
@@ -255,6 +260,7 @@ __global__ __launch_bounds__((64 * kWaves<DP>)) void k_attention_paged(const Att
         if (c.split && share.begin == 0 && hk == 0 && ht == 0 && threadIdx.x == 0)
             c.parts[s] = make_int2((int)number, 1 + (all - take + share.most - 1) / share.most);
         share.steps -= take, share.begin = 0, ++share.s;
+        if (CUT == kShares) share.len = __builtin_amdgcn_readfirstlane(live_rows(a, c, share.s));
 
         // the pages of 32 of this wave's steps, a lane each, and of the next 32; of the step that is
         // fetched next, each tile's page (below 0: none) and its first row in it
@@ -473,37 +479,50 @@ __global__ __launch_bounds__((64 * kJoinWaves)) void k_paged_join(const float *_
                                                                   const float2 *__restrict__ part_ms,
                                                                   const int2 *__restrict__ parts, FastDiv by_heads,
                                                                   int heads, int dim, T *__restrict__ out) {
-    __shared__ float so[kJoinWaves][128], ss[kJoinWaves];
+    constexpr int kOnce = 4;  // parts of a wave whose maxima, sums and rows are loaded together
+    __shared__ float so[kJoinWaves][128], sm[kJoinWaves], ss[kJoinWaves];
     const int row = blockIdx.x, s = fastdiv(row, by_heads), h = row - s * heads;
     const int2 own = parts[s];
     if (own.y == 1) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t first = (int64_t)own.x * heads + h;
-    const float2 *ms = part_ms + first;
-    float top = -INFINITY;
-    for (int p = lane; p < own.y; p += 64) top = fmaxf(top, ms[(int64_t)p * heads].x);
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
-    float total = 0.f, v0 = 0.f, v1 = 0.f;
     const int d0 = min(lane, dim - 1), d1 = min(lane + 64, dim - 1);
-#pragma unroll 4
-    for (int p = wave; p < own.y; p += kJoinWaves) {
-        const float2 e = ms[(int64_t)p * heads];
-        const float by = e.x == -INFINITY ? 1.f : fast_exp2(e.x - top);
-        total = fmaf(by, e.y, total);
-        const float *o = part_o + (first + (int64_t)p * heads) * dim;
-        v0 = fmaf(by, o[d0], v0);
-        v1 = fmaf(by, o[d1], v1);
+    float m = -INFINITY, total = 0.f, v0 = 0.f, v1 = 0.f;
+    for (int p = wave; p < own.y; p += kJoinWaves * kOnce) {
+        float2 e[kOnce];
+        float x0[kOnce], x1[kOnce], top = m;
+#pragma unroll
+        for (int i = 0; i < kOnce; ++i) {
+            const int64_t at = first + (int64_t)min(p + i * kJoinWaves, own.y - 1) * heads;
+            e[i] = part_ms[at], x0[i] = part_o[at * dim + d0], x1[i] = part_o[at * dim + d1];
+        }
+#pragma unroll
+        for (int i = 0; i < kOnce; ++i)
+            if (p + i * kJoinWaves < own.y) top = fmaxf(top, e[i].x);
+        const float keep = m == -INFINITY ? 1.f : fast_exp2(m - top);
+        m = top, total *= keep, v0 *= keep, v1 *= keep;
+#pragma unroll
+        for (int i = 0; i < kOnce; ++i) {
+            if (p + i * kJoinWaves >= own.y) continue;
+            // parts without keys have the maximum -inf and the sum 0; NaN sums pass
+            const float by = e[i].x == -INFINITY ? 1.f : fast_exp2(e[i].x - m);
+            total = fmaf(by, e[i].y, total), v0 = fmaf(by, x0[i], v0), v1 = fmaf(by, x1[i], v1);
+        }
     }
     so[wave][lane] = v0, so[wave][64 + lane] = v1;
-    if (lane == 0) ss[wave] = total;
+    if (lane == 0) sm[wave] = m, ss[wave] = total;
     __syncthreads();
     const int d = threadIdx.x;
     if (d >= dim) return;
+    float top = -INFINITY, v = 0.f;
     total = 0.f;
-    float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWaves; ++w) total += ss[w], v += so[w][d];
+    for (int w = 0; w < kJoinWaves; ++w) top = fmaxf(top, sm[w]);
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) {
+        const float by = sm[w] == -INFINITY ? 1.f : fast_exp2(sm[w] - top);
+        total = fmaf(by, ss[w], total), v = fmaf(by, so[w][d], v);
+    }
     out[(int64_t)row * dim + d] = (T)(total == 0.f ? 0.f : v / total);
 }
 
