@@ -9,9 +9,9 @@ voxels) its position.  A block runs
     gated_residual_norm   the norms around the block, with a gate for each scene
 
 and the loss is the L1 distance of the voxelized result from each scene's volume, so its
-gradient passes through the voxelizer, the projection and every operator.  `stream` runs the
-same blocks causally, a token of each scene at a time over a cache (cached_attention), as
-a model that generates Gaussians would.
+gradient passes through the voxelizer, the projection and every operator; AdamW updates all
+weights in one call.  `stream` runs the same blocks causally, a token of each scene at a time over a
+cache in pages (append_tokens, paged_attention), as a model that generates Gaussians would.
 
     python gs-voxelizer_amd/examples/refine_gaussians.py [steps]
 """
@@ -23,10 +23,12 @@ import torch.nn.functional as F
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
-from gs_voxelizer import attention, gated_norm, optim_to_render, rotary, voxelize  # noqa: E402
+from gs_voxelizer import (adamw, attention, gated_norm, optim_to_render, paged, rotary,  # noqa: E402
+                          voxelize)
 
 VOL, WORLD, CENTER = (32, 40, 36), (1.0, 1.0, 1.0), (0.5, 0.5, 0.5)
 PARAMETERS = 3 + 3 + 4 + 1  # centre, log scale, rotation, intensity
+PAGE = 16  # rows of a cache's page
 
 
 class Block(torch.nn.Module):
@@ -46,12 +48,10 @@ class Block(torch.nn.Module):
         f = rotary.axis_frequencies(_thirds(self.dim // 2), base=100.0)
         self.register_buffer("frequencies", f)
 
-    def heads_of(self, h, positions):
-        """q and k, turned, and v: views into one projection's output."""
+    def heads_of(self, h):
+        """q, k and v: views into one projection's output."""
         qkv = _linear(self.qkv, h).view(h.shape[0], -1, self.dim)
-        q, k = qkv[:, :self.heads], qkv[:, self.heads:self.heads + self.key_heads]
-        q, k = rotary.rotate_qk(q, k, positions, self.frequencies)
-        return q, k, qkv[:, self.heads + self.key_heads:]
+        return qkv.split((self.heads, self.key_heads, self.key_heads), 1)
 
     def finish(self, x, a, describe, scenes):
         """Both branches of the block after its attention."""
@@ -64,7 +64,8 @@ class Block(torch.nn.Module):
                                               scale=self.scale[1], gate=gates[1], **scenes)
 
     def forward(self, x, h, positions, describe, scenes, causal, keep):
-        q, k, v = self.heads_of(h, positions)
+        q, k, v = self.heads_of(h)
+        q, k = rotary.rotate_qk(q, k, positions, self.frequencies)
         a = attention.scene_attention(q, k, v, causal=causal, positions=positions,
                                       slopes=self.slopes, keep=keep, cap=30.0, **scenes)
         return self.finish(x, a, describe, scenes)
@@ -137,7 +138,7 @@ class Scenes:
 
 def train(model, scenes, steps, lr=2e-3):
     """Adam on the model's weights; returns the losses."""
-    opt = torch.optim.Adam(model.parameters(), lr=lr)
+    opt = adamw.AdamW(model.parameters(), lr=lr, weight_decay=0.0)
     losses = []
     for _ in range(steps):
         p = scenes.tokens + 0.1 * model(scenes.tokens, scenes.positions, scenes.describe,
@@ -154,19 +155,28 @@ def train(model, scenes, steps, lr=2e-3):
 def stream(model, tokens, positions, describe):
     """The model run causally, token by token: (S, N, .) tokens of S scenes of one length."""
     S, N = tokens.shape[:2]
-    lengths = torch.zeros(S, dtype=torch.int32, device=tokens.device)
-    one = dict(scene_starts=torch.arange(S + 1, dtype=torch.int32, device=tokens.device), longest=1)
-    caches = [[torch.empty(S, N, b.key_heads, b.dim, dtype=torch.bfloat16, device=tokens.device)
-               for _ in "kv"] for b in model.blocks]
+    device, most = tokens.device, -(-N // PAGE)
+    lengths = torch.zeros(S, dtype=torch.int32, device=device)
+    one = dict(scene_starts=torch.arange(S + 1, dtype=torch.int32, device=device), longest=1)
+    # a pool of pages for each block, and one of the positions; a scene gets a page when its last one is full
+    pools = [torch.empty(S * most, 2, PAGE, b.key_heads, b.dim, dtype=torch.bfloat16, device=device)
+             for b in model.blocks]
+    places = torch.empty(S * most, PAGE, 3, device=device)
+    free = torch.randperm(S * most, device=device, dtype=torch.int32)
+    table = torch.full((S, most), -1, dtype=torch.int32, device=device)
     out = []
     for t in range(N):
+        if t % PAGE == 0:
+            table[:, t // PAGE], free = free[:S], free[S:]
         x, h = model.start(tokens[:, t])
         lengths += 1
-        for block, (k_cache, v_cache) in zip(model.blocks, caches):
-            q, k_cache[:, t], v_cache[:, t] = block.heads_of(h, positions[:, t])
-            a = attention.cached_attention(q, k_cache, v_cache, lengths, cap=30.0,
-                                           positions=positions[:, t], key_positions=positions,
-                                           slopes=block.slopes)
+        for block, pool in zip(model.blocks, pools):
+            q, k, v = block.heads_of(h)
+            cache = pool[:, 0], pool[:, 1], table, lengths
+            q = paged.append_tokens(k, v, *cache, q=q, positions=positions[:, t], frequencies=block.frequencies,
+                                    position_pages=places)
+            a = paged.paged_attention(q, *cache, cap=30.0, positions=positions[:, t], position_pages=places,
+                                      slopes=block.slopes)
             x, h = block.finish(x, a, describe, one)
         out.append(model.leave(h.float()))
     return torch.stack(out, 1)
