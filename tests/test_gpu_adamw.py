@@ -509,3 +509,57 @@ def test_groups_that_are_refused(device):
     for more in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1), dict(weight_decay=-1), dict(max_norm=0)):
         with pytest.raises(ValueError):
             adamw.AdamW([a], **more)
+
+
+def test_a_captured_fit_of_gaussians(device):
+    """A fit through the voxelizer in two graphs: a replay's step is the formula's on the gradients that it left."""
+    from gs_voxelizer import graph, synthetic, voxelize
+    from helpers import small_config
+    from test_gpu_graph import _make
+    voxelize._capacity.pop(device.index or 0, None)
+    leaves, backward = _make(device, small_config(1, 3000, vol=(48, 40, 56)), seed=3)
+    rates = [1e-4, 2e-4, 1e-3, 1e-2]
+    opt = adamw.AdamW([dict(params=[p], lr=r) for p, r in zip(leaves, rates)], weight_decay=0.0, capturable=True)
+    voxelize_and_differentiate = graph.CapturedStep(backward)
+    opt.step()
+    second = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(second):
+        opt.step()
+    for i in range(4):
+        voxelize_and_differentiate.replay()
+        before = [[t.detach().double().clone() for t in (p, p.grad, opt.state[p]["exp_avg"], opt.state[p]["exp_avg_sq"])]
+                  for p in leaves]
+        second.replay()
+        torch.cuda.synchronize()
+        t = i + 2
+        for p, r, (w, g, m, v) in zip(leaves, rates, before):
+            m, v = 0.9 * m + 0.1 * g, 0.999 * v + 0.001 * g * g
+            up = r * (m / (1 - 0.9 ** t)) / ((v / (1 - 0.999 ** t)).sqrt() + 1e-8)
+            # an update is at most r / (1 - 0.9) here, and 2^-20 of that off; the weight rounds once
+            assert float((p.detach() - (w - up)).abs().max()) <= 2.0 ** -20 * 10 * r + 2.0 ** -23 * float(w.abs().max())
+    assert int(opt.state[leaves[0]]["step"]) == 5
+
+
+def test_plain_calls_take_the_native_step(device, monkeypatch):
+    assert _native.available
+    log = []
+    call = _native.adamw_step
+
+    def record(*args):
+        out = call(*args)
+        log.append(out[0])
+        return out
+
+    monkeypatch.setattr(_native, "adamw_step", record)
+    s = Step(device, [(50,), (3, 4)], ["f32", "masters"])
+    counter = torch.zeros(1, dtype=torch.int32, device=device)
+    for step in (3, [3, 4], counter):
+        for more in (dict(), dict(max_norm=1.0), dict(lr=[1e-3, 1e-2], weight_decay=(0.1, 0)), dict(lr=1)):
+            s.run(step, **more)
+    p = torch.nn.Parameter(torch.ones(5, device=device))
+    p.grad = torch.ones_like(p)
+    adamw.AdamW([p]).step()
+    adamw.AdamW([p], capturable=True, max_norm=1.0).step()
+    assert len(log) == 14 and all(log)
+    s.run(lr=torch.tensor(1e-3, device=device))
+    assert not log[-1]

@@ -758,3 +758,26 @@ def test_append_refuses(device):
                                                       scene_starts=c.starts) or k)(c.k[None])
     for t, w in zip((c.k_pages, c.v_pages, c.position_pages), before):
         assert torch.equal(t, w)
+
+
+@TYPES
+def test_plain_calls_take_the_native_functions(device, monkeypatch, dtype):
+    assert _native.available
+    log = []
+    for name in ("append_tokens", "paged_attention"):
+        def record(*args, call=getattr(_native, name)):
+            out = call(*args)
+            log.append(bool(out))
+            return out
+        monkeypatch.setattr(_native, name, record)
+    for joint in (False, True):
+        c = Tokens(device, dtype, [4, 2], [0, 3], 4, 2, 40, joint=joint)
+        keep = torch.ones(6, dtype=torch.bool, device=device)
+        kept = torch.zeros(c.k_pages.shape[:2], dtype=torch.int32, device=device)
+        c.run(), c.run(keep=keep, keep_pages=kept), c.run(q=None), c.run(interleaved=True)
+        c.run(q=None, frequencies=None), c.run(q=None, frequencies=None, positions=None, position_pages=None)
+        d = Tokens(device, dtype, [1] * 3, [5, 0, 20], 4, 2, 40, single=True)
+        d.run()
+        a = Case(device, dtype, [40, 20, 300], 4, 2, 40, joint=joint, keep=0.5)
+        a.run(), a.run(keep_pages=None), a.run(slopes=None, positions=None, position_pages=None), a.run(cap=5.0, scale=0.2)
+    assert len(log) == 22 and all(log)
