@@ -363,21 +363,20 @@ __global__ __launch_bounds__((64 * kWaves<DP>)) void k_attention_paged(const Att
                     for (int r = 0; r < 4; ++r) {
                         const float dx = x[r] - qx, dy = y[r] - qy, dz = z[r] - qz;
                         d[t][r] = __builtin_amdgcn_sqrtf(fmaf(dz, dz, fmaf(dy, dy, dx * dx)));
-                        if (!capped) w[t][r] = -far_unit * d[t][r];
                     }
                 }
 #pragma unroll
             for (int st = 0; st < DEPTH; ++st)
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) w[t] = mma16(at.rows(kt, t, st), q[st], w[t]);
-            if (capped)
+            // the distances' part last: begun with it, each of the products' sums would round at its size
 #pragma unroll
-                for (int t = 0; t < TILES; ++t)
+            for (int t = 0; t < TILES; ++t)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        w[t][r] = a.cap * tanh_of<T, CAP>(w[t][r] * in_cap);
-                        if (FAR) w[t][r] = fmaf(-far_unit, d[t][r], w[t][r]);
-                    }
+                for (int r = 0; r < 4; ++r) {
+                    if (capped) w[t][r] = a.cap * tanh_of<T, CAP>(w[t][r] * in_cap);
+                    if (FAR) w[t][r] = fmaf(-far_unit, d[t][r], w[t][r]);
+                }
             constexpr uint32_t kAll = KEYS == 32 ? ~0u : (1u << (KEYS & 31)) - 1;
             if ((live & kAll) != kAll) {
                 const uint32_t seen = live >> g4;
