@@ -14,6 +14,12 @@
 // the result, column l % 16 and rows 4 (l / 16) + r, r = 0 .. 3.  A sum does not depend on which index is called
 // which: scores come out with a lane's keys 4 (l / 16) + r (and 16 more), which are the right operand of the product
 // with the values, in that order, straight from the registers.
+//
+// 2 caches of 200,003 rows, 16 heads on 4 of 128, bfloat16, capped, bias, pages of 256 (316 MB of live rows): 64.5 us,
+// 4.9 TB/s, and 4.8 for the join; 128 of 2,000, 8 on 8 of 64 (350 MB) 74.4 us, 4.7 TB/s; 5 of 20,000, 12 on 4 of 40, float32 (66 MB)
+// 20.6 us.  Bytes bound these: each is read once (counters), vector units are at work 15 to 20 % of the time, matrix units
+// 1 to 20 %.  16 of 4,096, 8 on 2 of 64 (23 MB): 10.8 us and 3.6; there the chain from the launch to the first bytes
+// (lengths, table, keys) and a wave's two steps bound it.
 #include "gsv_attention.h"
 
 // (a product and a difference stay two roundings where they are written as two)
@@ -27,8 +33,8 @@ constexpr float kSlack = 8.f;
 constexpr int kHeads = 16;     // query heads of a workgroup
 constexpr int kPageUnit = 16;  // a page holds a multiple of so many rows: a copy never leaves one
 
-// A wave's step, and the waves of a workgroup: two workgroups fit a CU, so that one starts while another works
-// (in one workgroup a CU, 40 scenes of 4,000, 4 heads of 128, took 63 us instead of 53).
+// A wave's step, and the waves of a workgroup: two workgroups fit a CU (LDS), so that one starts while another works.
+// 40 scenes of 4,000, 4 heads of 128: 46.8 us, with twice the waves 52.3 (2 of 200,003, long pieces only: 70.0 and 68.7).
 template <typename T> constexpr int kKeys = sizeof(T) == 2 ? 32 : 16;
 template <int DP> constexpr int kWaves = DP == 128 ? 2 : 4;
 
@@ -471,7 +477,7 @@ __global__ __launch_bounds__((64 * kWaves<DP>)) void k_attention_paged(const Att
 }
 
 // One workgroup a scene and head; scenes of one part have their row already.  The waves take the parts in turn,
-// then their sums are joined, always in the same order.  Latency bounds it: NN us at 16 parts, NN at 64.
+// then their sums are joined, always in the same order.  Latency bounds it: 3.6 us at 16 parts, 4.8 at 64.
 constexpr int kJoinWaves = 8;
 template <typename T>
 __global__ __launch_bounds__((64 * kJoinWaves)) void k_paged_join(const float *__restrict__ part_o,
@@ -548,8 +554,9 @@ struct Paged {
         T *o = static_cast<T *>(out);
         const int64_t apart = ((int64_t)c.shares * (a.kv_heads / c.near) + kXcds - 1) / kXcds * kXcds;
         const dim3 grid((unsigned)(apart * c.near * c.head_tiles)), block(64 * kWaves<DP>);
-        // 16 caches of 4,096, 2 key heads of 64 (step of 16 scenes): 16.6 us in pieces, 20.7 in shares; 20 of 8,000, 4
-        // of 128 53.5 and 57.4; 90 of 2,000 68.4 and 59.6; 100 of 3,000, 8 of 64 92.4 and 83.3.
+        // Pieces and shares, us: 16 caches of 4,096, 2 key heads of 64 (256 workgroups each) 13.0 and 15.9; 20 of 100,003
+        // and less, 4 of 128 (128) 61.3 and 68.0; 40 of 4,000 46.8 and 51.5; 90 of 2,000 56.7 and 56.5, 120 of 1,500 57.3
+        // and 56.4; 50 of 3,000, 8 of 64 (64) 53.0 and 46.4.
         if (a.scenes * 2 < c.shares || !c.split)
             hipLaunchKernelGGL((k_attention_paged<T, DP, FAR, CAP, kPieces>), grid, block, 0, st, a, c, o);
         else
