@@ -107,8 +107,6 @@ def _step(params, grads, exp_avgs, exp_avg_sqs, masters, steps, counter, rates, 
     if counter is not None:
         _t.check(counter.dtype == torch.int32 and tuple(counter.shape) == (1,) and counter.device == dev,
                  f"step must be a number or a (1,) int32 tensor on {dev}")
-    elif torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("gs_voxelizer: a captured step needs its count on the device (a (1,) int32 tensor)")
     held = []  # copies that live until the kernels are enqueued
     entries = (_lib.AdamwTensor * n)()
     for i, (p, g) in enumerate(zip(params, grads)):
@@ -144,6 +142,8 @@ def _step(params, grads, exp_avgs, exp_avg_sqs, masters, steps, counter, rates, 
                    max_norm=max_norm or 0.0, counter=_t.ptr(counter))
     norm = None
     with torch.cuda.device(dev):
+        if counter is None and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("gs_voxelizer: a captured step needs its count on the device (a (1,) int32 tensor)")
         if max_norm:
             norm = torch.empty((), dtype=torch.float32, device=dev)
             a.norm = norm.data_ptr()
@@ -153,7 +153,9 @@ def _step(params, grads, exp_avgs, exp_avg_sqs, masters, steps, counter, rates, 
             _t.call("adamw", ctypes.byref(a), ws.data_ptr(), size, _t.stream(dev))
         except RuntimeError as e:
             # (what else the library refuses is checked above)
-            raise ValueError(f"{e}: a tensor that the step writes shares memory with another, or with a gradient") if "argument" in str(e) else e
+            if "argument" not in str(e):
+                raise
+            raise ValueError(f"{e}: a tensor that the step writes shares memory with another, or with a gradient")
     _t.written(*params, *exp_avgs, *exp_avg_sqs, *(masters or []), counter)
     return norm
 
@@ -167,9 +169,10 @@ class AdamW(torch.optim.Optimizer):
         masters: bfloat16 parameters get float32 masters (state ``master``), which the steps go by.
         max_norm: see `adamw_step`; over all groups, which then have one device, ``betas`` and ``eps``.  The last
             step's norm is ``self.norm``.
-        capturable: (likewise one device, ``betas`` and ``eps``) the number of steps is one counter on the device, for all parameters (those without a gradient
-            at some step, which it leaves as they are, count it too), and the step can be captured in a graph after
-            one ordinary step.  ``lr`` may be a float32 tensor of one element on the device.
+        capturable: (likewise one device, ``betas`` and ``eps``) the number of steps is one counter on the device, for
+            all parameters (those without a gradient at some step, which it leaves as they are, count it too), and
+            the step can be captured in a graph after one ordinary step.  ``lr`` may be a float32 tensor of one
+            element on the device.
 
     A step that is captured together with a voxelization would be made twice where
     `graph.CapturedStep` has to run a replay again: capture the optimiser's step in a graph of its own.
