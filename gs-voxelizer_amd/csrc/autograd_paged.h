@@ -36,6 +36,12 @@ bool are_apart(const Tensor &a, const Tensor &b) {
            (a.strides() == b.strides() && by % size == 0 && is_apart(a, 2, by / size));
 }
 
+// Whether the memory from one's first element to its last one meets the other's.
+bool meet(const Tensor &a, const Tensor &b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.data_ptr()), y = reinterpret_cast<uintptr_t>(b.data_ptr());
+    return x < y + reach_of(b) * b.element_size() && y < x + reach_of(a) * a.element_size();
+}
+
 struct PagedCache {
     Tensor k, v, table, positions, keep;
 
@@ -108,6 +114,9 @@ std::vector<Maybe> append_tokens(const Tensor &k, const Tensor &v, const Tensor 
         return {};
     for (const Tensor *t : {&k, &v, &q, &positions, &freq, &c.k, &c.v, &c.positions})
         if (wants_grad(*t)) return {};
+    for (const Tensor *t : {&k, &v, &q})
+        if (t->defined() && (meet(*t, c.k) || meet(*t, c.v))) return {};
+    if ((c.positions.defined() && meet(positions, c.positions)) || (kept.defined() && meet(kept, c.keep))) return {};
     const c10::DeviceGuard guard(dev);
     gsv_rotary_args a{};
     a.k = ptr<void>(k), a.k_row = k.stride(0), a.k_head = k.stride(1), a.kv_heads = (int)K;

@@ -59,9 +59,22 @@ def _share(a, b):
     """Whether two pools of one shape share an element: neither one behind the other nor halves of one pool."""
     a, b = sorted((a, b), key=Tensor.data_ptr)
     by, size = b.data_ptr() - a.data_ptr(), a.element_size()
-    if by >= size * (1 + sum(s * (n - 1) for s, n in zip(a.stride(), a.shape))):
+    if b.data_ptr() >= _span(a)[1]:
         return False
     return a.stride() != b.stride() or by % size != 0 or not _is_apart(a, (by // size, 2))
+
+
+def _span(t):
+    """The memory from a tensor's first element to its last one, in bytes."""
+    first = t.data_ptr()
+    return first, first + t.element_size() * (1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape)))
+
+
+def _unwritten(t, what, pages, name):
+    """Refuses tokens that lie in a pool's memory, where they may change before they are read."""
+    if t is not None and pages is not None and t.numel():
+        (a, a_end), (b, b_end) = _span(t), _span(pages)
+        _t.check(a_end <= b or b_end <= a, f"{what} must not lie in {name}")
 
 
 def _pages(k_pages, v_pages, page_table, position_pages, keep_pages, like):
@@ -102,12 +115,13 @@ def append_tokens(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_t
     Of scene s's n new tokens, the i-th becomes row ``lengths[s] - n + i``: lengths count the new
     tokens in, as `paged_attention` then takes them.  A token whose row is below 0 (a scene of
     length 0 that a fixed batch carries along), past the table or in no page is not written; all other rows
-    stay as they are.  Two tokens must not have one row (pages that scenes share are only read): which
-    one stays is not said.
+    stay as they are.  Two tokens must not have one row (pages that scenes share are only read): what it
+    then holds is not said.  As everywhere the last scene ends with the tokens: those that only fill a batch are
+    one more scene, of length 0.
 
     Args:
         k, v: (T, K, D) new tokens, D a multiple of 8 up to 128 (views into one projection's output are taken
-            as they are, but not views of the pools).
+            as they are).  No input may lie in the pools' memory.
         k_pages, v_pages: (pages, rows, K, D), rows a multiple of 16, written in place; they may be
             halves of one pool, pool[:, 0] and pool[:, 1].
         page_table: (S, most) int32.
@@ -180,7 +194,7 @@ def append_tokens(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_t
         _t.check(P >= 1 and 2 * P <= D, f"{P} channel pairs do not fit {D} channels")
         frequencies = frequencies.contiguous()
         a.frequencies, a.pairs = frequencies.data_ptr(), P
-    out = None
+    out, given_q = None, q
     if q is not None:
         _t.check(frequencies is not None, "q needs frequencies")
         _t.activations(q, "q", 3, like=k)
@@ -191,6 +205,11 @@ def append_tokens(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_t
         a.q, a.q_row, a.q_head, a.heads = q.data_ptr(), q.stride(0), q.stride(1), q.shape[1]
     _t.check(K + (0 if q is None else q.shape[1]) <= 4096, "at most 4096 heads")
     _t.check((keep is None) == (keep_pages is None), "keep and keep_pages need each other")
+    for pages, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        for t, what in ((k, "k"), (v, "v"), (given_q, "q")):
+            _unwritten(t, what, pages, name)
+    _unwritten(positions, "positions", position_pages, "position_pages")
+    _unwritten(keep, "keep", keep_pages, "keep_pages")
     if keep is not None:
         keep = _t.mask(keep, "keep", (T,), dev)
     k, v = _t.rows16(k), _t.rows16(v)

@@ -463,7 +463,7 @@ int gsv_rotary(const gsv_rotary_args *args, void *q_out, void *k_out, int32_t in
  * pools; q, turned, to q_out (heads may be 0).  dim a multiple of 8, 8 .. 128; k, v and q with pointers and
  * strides of 16 bytes.  With pages->positions the tokens' positions (axes 3) go there, with pages->keep
  * keep[t] != 0 of keep (keep_bytes 1 or 4), as 0 or 1.  starts (scenes + 1) as for gsv_attention, NULL: one token
- * a scene.  Which one stays where two tokens have the same row is not said.
+ * a scene.  What a row holds that two tokens have is not said; the inputs lie apart from the pools.
  */
 int gsv_paged_append(const gsv_rotary_args *args, const void *v, int64_t v_row, int64_t v_head,
                      const gsv_pages *pages, const int32_t *lengths, const int32_t *starts, int32_t scenes,
@@ -508,7 +508,8 @@ int gsv_gated_norm_bwd(const gsv_norm *args, const void *dy, int64_t dy_row, con
  * values in the same order, aligned to their own size.  t is the tensor's step, 1 or more; with `counter` (one
  * int32 on the device, steps made so far) t = *counter + 1 for all, and the call advances it.  lr_device: NULL, or the
  * rate, one float on the device.  norm (NULL, or one float on the device) receives |all grads| where max_norm > 0.
- * Written tensors that share memory with each other or a gradient are refused (GSV_ERR_INVALID_ARGUMENT).  The norm is summed in binary64 in a fixed order.
+ * Written tensors that share memory with each other or a gradient are refused (GSV_ERR_INVALID_ARGUMENT).  The norm is
+ * summed in binary64 in a fixed order.
  */
 typedef struct gsv_adamw_tensor {
     void *param;

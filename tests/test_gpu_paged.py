@@ -781,3 +781,29 @@ def test_plain_calls_take_the_native_functions(device, monkeypatch, dtype):
         a = Case(device, dtype, [40, 20, 300], 4, 2, 40, joint=joint, keep=0.5)
         a.run(), a.run(keep_pages=None), a.run(slopes=None, positions=None, position_pages=None), a.run(cap=5.0, scale=0.2)
     assert len(log) == 22 and all(log)
+
+
+def test_append_refuses_tokens_that_lie_in_the_pools(device, route):
+    c = Tokens(device, BF16, [4, 2], [0, 3], 4, 2, 64)
+    rows = c.k_pages.view(-1, 2, 64)
+    keeps = torch.zeros(c.k_pages.shape[:2], dtype=torch.bool, device=device)
+    before = [t.clone() for t in (c.k_pages, c.v_pages, c.position_pages, keeps)]
+    for more in (dict(k=rows[:6]), dict(v=rows[-6:]), dict(q=rows[3:9]), dict(v=c.v_pages.view(-1, 2, 64)[:6]),
+                 dict(positions=c.position_pages.view(-1, 3)[-6:]), dict(keep=keeps.view(-1)[4:10], keep_pages=keeps)):
+        _refuses(c.run, "must not lie in", ValueError, **more)
+    for t, w in zip((c.k_pages, c.v_pages, c.position_pages, keeps), before):
+        assert torch.equal(t, w)
+    # memory side by side is apart: the pools and the tokens of one allocation
+    P, n = c.k_pages.shape[0], c.k_pages[0].numel()
+    arena = torch.randn((2 * P + 1) * n, device=device).to(BF16)
+    c.k_pages, c.v_pages = arena[:2 * P * n].view(2, P, 16, 2, 64)
+    c.k = arena[2 * P * n:].view(-1, 2, 64)[:6]
+    c.check()
+
+
+def test_tokens_that_fill_a_batch_are_one_more_scene(device, route):
+    """Packed prompts of a fixed size: what is behind the last prompt is a scene of length 0, and not written."""
+    c = Tokens(device, F32, [5, 20, 7], [0, 3, 0], 4, 2, 40)
+    c.device_lengths[2] = 0
+    assert sum(1 for _ in c.targets()) == 25
+    c.check()
