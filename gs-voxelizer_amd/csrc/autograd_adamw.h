@@ -9,15 +9,18 @@
 
 namespace {
 
-// A tensor with memory of its own in one run.
-bool is_dense(const Tensor &t, const at::Device &dev) {
+// A tensor with memory of its own.
+bool is_strided(const Tensor &t, const at::Device &dev) {
     return t.defined() && t.layout() == at::kStrided && t.device() == dev &&
-           !t.key_set().has(c10::DispatchKey::Python) && t.unsafeGetTensorImpl()->has_storage() &&
-           (t.is_contiguous() || t.is_non_overlapping_and_dense());
+           !t.key_set().has(c10::DispatchKey::Python) && t.unsafeGetTensorImpl()->has_storage();
 }
-// The same shape, laid out alike.
+// In one run.
+bool is_dense(const Tensor &t, const at::Device &dev) {
+    return is_strided(t, dev) && (t.is_contiguous() || t.is_non_overlapping_and_dense());
+}
+// The shape of a dense tensor, laid out alike.
 bool is_like(const Tensor &t, const Tensor &p, const at::Device &dev) {
-    return is_dense(t, dev) && t.sizes() == p.sizes() && t.strides() == p.strides();
+    return is_strided(t, dev) && t.sizes() == p.sizes() && t.strides() == p.strides();
 }
 
 // Item i of a list or tuple of n; of anything else, or of another length, none.
