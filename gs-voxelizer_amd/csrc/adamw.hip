@@ -10,14 +10,15 @@
 // the first update: a pass of its own, whose sums one workgroup adds up, and which the
 // update then reads again, from the caches where they hold it.
 //
-// 83 million bfloat16 weights with masters, clipped (2.3 GB): 491 us, 4.7 TB/s, what a large copy reaches; 200,000 Gaussians'
-// 2.2 million values (62 MB, which the caches hold): 11.6 us; four tensors of 1,500 values: 6.5 us, the host's; the
+// 83 million bfloat16 weights with masters, clipped (2.3 GB): 479 us, 4.8 TB/s, what a large copy reaches; 200,000 Gaussians'
+// 2.2 million values (62 MB, which the caches hold): 11.2 us; four tensors of 1,500 values: 6.0 us, the host's; the
 // kernel takes 3.7.
 #include "gsv_device.h"
 
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <type_traits>
 
 namespace gsv {
 namespace {
@@ -33,11 +34,29 @@ struct Entry {
     double lr;  // lr decay is formed in binary64: 1 less it is near 1
     float decay, by_m, by_v;  // by_m = 1 / (1 - b1^t), by_v = 1 / sqrt(1 - b2^t)
 };
-constexpr int kTensors = 44;  // the arguments of a kernel end at 4 KB
-struct Table {
+// Tensors of a launch: as many as its arguments hold, which end at 4 KB; where there are few, a table of few, since the
+// host copies all of it (four tensors: 6.0 us a call, in the large table 6.8).
+constexpr int kTensors = 44, kFew = 8;
+template <int N> struct Table {
+    static constexpr int kMost = N;
     int count;
-    int first[kTensors];  // the tensors' first workgroups
-    Entry t[kTensors];
+    int first[N];  // the tensors' first workgroups
+    Entry t[N];
+    void put(int i, const gsv_adamw_tensor &x, float by_m, float by_v) {
+        t[i] = Entry{x.param, x.grad, x.exp_avg, x.exp_avg_sq, x.master, x.lr_device, x.numel, x.lr,
+                     (float)x.weight_decay, by_m, by_v};
+    }
+};
+// For the norm: the gradients alone (28 tensors 14.4 us, in the tables above 17.0; 148 of 83 million values, one launch
+// in place of four, 479 and 492).
+constexpr int kGradients = 160, kFewGradients = 32;
+template <int N> struct Gradients {
+    static constexpr int kMost = N;
+    int count;
+    int first[N];
+    const void *g[N];
+    int64_t n[N];
+    void put(int i, const gsv_adamw_tensor &x, float, float) { g[i] = x.grad, n[i] = x.numel; }
 };
 struct Rates {
     float b1, c1, b2, c2, eps;  // c = 1 - b
@@ -57,11 +76,16 @@ template <typename T> struct __align__(sizeof(T) * kVec) Four {
     T v[kVec];
 };
 
-// The tensor of a workgroup: one load over the lanes (a search one step after the other cost 2 us).
-__device__ __forceinline__ int tensor_of(const Table &t, int block) {
+// The tensor of a workgroup: loads over the lanes (a search one step after the other cost 2 us).
+template <typename Tensors> __device__ __forceinline__ int tensor_of(const Tensors &t, int block) {
     const int lane = threadIdx.x & 63;
-    const bool begun = lane < t.count && t.first[min(lane, kTensors - 1)] <= block;
-    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(begun)) - 1);
+    int begun = 0;
+#pragma unroll
+    for (int i = 0; i < Tensors::kMost; i += 64) {
+        const int first = t.first[min(i + lane, Tensors::kMost - 1)];
+        begun += __popcll(__ballot(i + lane < t.count && first <= block));
+    }
+    return __builtin_amdgcn_readfirstlane(begun - 1);
 }
 
 struct Step {
@@ -100,8 +124,8 @@ __device__ __forceinline__ float2 corrections(double beta1, double beta2, int t)
 }
 
 // STEPS: steps of a thread.  P, G: types of the param and its gradient; MASTER: a bfloat16 param's 32-bit copy.
-template <typename P, typename G, bool MASTER, int STEPS>
-__global__ __launch_bounds__(256) void k_adamw(const Table table, const Rates r) {
+template <typename P, typename G, bool MASTER, int STEPS, int N>
+__global__ __launch_bounds__(256) void k_adamw(const Table<N> table, const Rates r) {
     const int at = tensor_of(table, blockIdx.x);
     const Entry &e = table.t[at];
     const double lr = e.lr_device ? (double)*e.lr_device : e.lr;
@@ -181,12 +205,13 @@ __global__ __launch_bounds__(256) void k_adamw(const Table table, const Rates r)
 
 // Sums of squares in binary64: no overflow, and no length at which the small terms are lost.
 constexpr int kNormSteps = 8;
-template <typename G> __global__ __launch_bounds__(256) void k_adamw_squares(const Table table, double *sums, int *counter) {
+template <typename G, int N>
+__global__ __launch_bounds__(256) void k_adamw_squares(const Gradients<N> table, double *sums, int *counter) {
     if (counter && blockIdx.x == 0 && threadIdx.x == 0) *counter += 1;
     const int at = tensor_of(table, blockIdx.x);
-    const G *const g = static_cast<const G *>(table.t[at].g);
+    const G *const g = static_cast<const G *>(table.g[at]);
     constexpr int64_t kAll = 256 * kVec * kNormSteps;
-    const int64_t n = table.t[at].n, base = (int64_t)(blockIdx.x - table.first[at]) * kAll;
+    const int64_t n = table.n[at], base = (int64_t)(blockIdx.x - table.first[at]) * kAll;
     Four<G> x[kNormSteps];
     if (reinterpret_cast<uintptr_t>(g) % sizeof(Four<G>) == 0 && base + kAll <= n) {
 #pragma unroll
@@ -259,16 +284,16 @@ int adamw_check(const gsv_adamw_args *a, Sizes *out) {
 }
 
 // Tables of the tensors that `takes`, each handed to `launch` with its workgroups when it is full.
-template <typename Takes, typename Launch>
+template <typename Tensors, typename Takes, typename Launch>
 void tables(const gsv_adamw_args *a, int64_t per_block, const Takes &takes, const Launch &launch) {
-    Table t;
+    Tensors t;
     t.count = 0;
     int64_t blocks = 0;
     for (int64_t i = 0; i < a->count; ++i) {
         const gsv_adamw_tensor &x = a->tensors[i];
         if (!x.numel || !takes(x)) continue;
         const int64_t own = (x.numel + per_block - 1) / per_block;
-        if (t.count == kTensors || (t.count && blocks + own > (1 << 23))) {
+        if (t.count == Tensors::kMost || (t.count && blocks + own > (1 << 23))) {
             launch(t, blocks);
             t.count = 0, blocks = 0;
         }
@@ -278,11 +303,15 @@ void tables(const gsv_adamw_args *a, int64_t per_block, const Takes &takes, cons
             by_v = (float)(1.0 / std::sqrt(1.0 - std::pow(a->beta2, (double)x.step)));
         }
         t.first[t.count] = (int)blocks;
-        t.t[t.count++] = Entry{x.param, x.grad, x.exp_avg, x.exp_avg_sq, x.master, x.lr_device, x.numel, x.lr,
-                               (float)x.weight_decay, by_m, by_v};
+        t.put(t.count++, x, by_m, by_v);
         blocks += own;
     }
     if (t.count) launch(t, blocks);
+}
+template <typename Takes> bool at_most(const gsv_adamw_args *a, int most, const Takes &takes) {
+    for (int64_t i = 0; i < a->count; ++i)
+        if (a->tensors[i].numel && takes(a->tensors[i]) && --most < 0) return false;
+    return true;
 }
 
 template <typename P, typename G, bool MASTER>
@@ -291,21 +320,31 @@ void update_all(const gsv_adamw_args *a, const Rates &r, int steps, hipStream_t 
     const auto takes = [](const gsv_adamw_tensor &t) {
         return t.dtype == p && t.grad_dtype == g && (t.master != nullptr) == MASTER;
     };
-    tables(a, 256 * kVec * steps, takes, [&](const Table &t, int64_t blocks) {
-        const dim3 grid((unsigned)blocks), block(256);
-        if (steps == 4) hipLaunchKernelGGL((k_adamw<P, G, MASTER, 4>), grid, block, 0, st, t, r);
-        else hipLaunchKernelGGL((k_adamw<P, G, MASTER, 1>), grid, block, 0, st, t, r);
-    });
+    if (steps == 4)
+        tables<Table<kTensors>>(a, 256 * kVec * 4, takes, [&](const Table<kTensors> &t, int64_t blocks) {
+            hipLaunchKernelGGL((k_adamw<P, G, MASTER, 4, kTensors>), dim3((unsigned)blocks), dim3(256), 0, st, t, r);
+        });
+    else if (at_most(a, kFew, takes))
+        tables<Table<kFew>>(a, 256 * kVec, takes, [&](const Table<kFew> &t, int64_t blocks) {
+            hipLaunchKernelGGL((k_adamw<P, G, MASTER, 1, kFew>), dim3((unsigned)blocks), dim3(256), 0, st, t, r);
+        });
+    else
+        tables<Table<kTensors>>(a, 256 * kVec, takes, [&](const Table<kTensors> &t, int64_t blocks) {
+            hipLaunchKernelGGL((k_adamw<P, G, MASTER, 1, kTensors>), dim3((unsigned)blocks), dim3(256), 0, st, t, r);
+        });
 }
 
 template <typename G> void squares_all(const gsv_adamw_args *a, double *sums, int *counter, int64_t *at, hipStream_t st) {
     constexpr int g = sizeof(G) == 2 ? GSV_BF16 : GSV_F32;
-    tables(a, 256 * kVec * kNormSteps, [](const gsv_adamw_tensor &t) { return t.grad_dtype == g; },
-           [&](const Table &t, int64_t blocks) {
-               hipLaunchKernelGGL(k_adamw_squares<G>, dim3((unsigned)blocks), dim3(256), 0, st, t, sums + *at,
-                                  *at ? nullptr : counter);
-               *at += blocks;
-           });
+    const auto takes = [](const gsv_adamw_tensor &t) { return t.grad_dtype == g; };
+    const auto launch = [&](const auto &t, int64_t blocks) {
+        constexpr int N = std::decay_t<decltype(t)>::kMost;
+        hipLaunchKernelGGL((k_adamw_squares<G, N>), dim3((unsigned)blocks), dim3(256), 0, st, t, sums + *at,
+                           *at ? nullptr : counter);
+        *at += blocks;
+    };
+    if (at_most(a, kFewGradients, takes)) tables<Gradients<kFewGradients>>(a, 256 * kVec * kNormSteps, takes, launch);
+    else tables<Gradients<kGradients>>(a, 256 * kVec * kNormSteps, takes, launch);
 }
 
 // Whether a tensor that the step writes shares memory with another that it writes, or with a gradient.
@@ -376,7 +415,7 @@ extern "C" int gsv_adamw(const gsv_adamw_args *args, void *workspace, size_t wor
     if (need) {
         double *sums = static_cast<double *>(workspace);
         // Few sums are added up by every workgroup of the update, many by a launch of one.  28 tensors of 235,000
-        // elements: 15.6 us, with the launch 20.6.
+        // elements: 15.6 us, with the launch 20.6 (both with larger tables than now: 14.4).
         const bool few = args->max_norm > 0 && s.squares > 0 && s.squares <= 256;
         int64_t count = 0;
         if (args->max_norm > 0) {

@@ -563,3 +563,18 @@ def test_plain_calls_take_the_native_step(device, monkeypatch):
     assert len(log) == 14 and all(log)
     s.run(lr=torch.tensor(1e-3, device=device))
     assert not log[-1]
+
+
+@pytest.mark.parametrize("count", [1, 8, 9, 32, 33, 44, 45, 88, 160, 161, 321])
+@pytest.mark.parametrize("empty", [False, True], ids=["", "with empty ones"])
+def test_as_many_tensors_as_a_launch_takes(device, count, empty):
+    """Launches take so many tensors each: the last one full, or with one more to come."""
+    shapes, kinds = [(1 + (i * 613) % 1500,) for i in range(count)], ["f32"] * count
+    if empty:
+        shapes, kinds = [(0,)] + shapes[:count // 2] + [(0,)] + shapes[count // 2:], kinds + ["bf16", "f32"]
+    s = Step(device, shapes, kinds)
+    counter = torch.tensor([2], dtype=torch.int32, device=device)
+    s.check(counter, weight_decay=0.1, max_norm=0.02, count=3)
+    assert counter.tolist() == [3]
+    s = Step(device, shapes, kinds)
+    s.check(weight_decay=0.1)
