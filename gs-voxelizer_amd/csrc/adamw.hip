@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <functional>
 #include <new>
 #include <type_traits>
 
@@ -33,6 +34,7 @@ struct Entry {
     int64_t n;
     double lr;  // lr decay is formed in binary64: 1 less it is near 1
     float decay, by_m, by_v;  // by_m = 1 / (1 - b1^t), by_v = 1 / sqrt(1 - b2^t)
+    int own;                  // below 0: these; else the place of those of the tensor's own counter
 };
 // Tensors of a launch: as many as its arguments hold, which end at 4 KB; where there are few, a table of few, since the
 // host copies all of it (four tensors: 6.0 us a call, in the large table 6.8).
@@ -42,9 +44,9 @@ template <int N> struct Table {
     int count;
     int first[N];  // the tensors' first workgroups
     Entry t[N];
-    void put(int i, const gsv_adamw_tensor &x, float by_m, float by_v) {
+    void put(int i, const gsv_adamw_tensor &x, float by_m, float by_v, int own) {
         t[i] = Entry{x.param, x.grad, x.exp_avg, x.exp_avg_sq, x.master, x.lr_device, x.numel, x.lr,
-                     (float)x.weight_decay, by_m, by_v};
+                     (float)x.weight_decay, by_m, by_v, own};
     }
 };
 // For the norm: the gradients alone (28 tensors 14.4 us, in the tables above 17.0; 148 of 83 million values, one launch
@@ -56,7 +58,7 @@ template <int N> struct Gradients {
     int first[N];
     const void *g[N];
     int64_t n[N];
-    void put(int i, const gsv_adamw_tensor &x, float, float) { g[i] = x.grad, n[i] = x.numel; }
+    void put(int i, const gsv_adamw_tensor &x, float, float, int) { g[i] = x.grad, n[i] = x.numel; }
 };
 struct Rates {
     float b1, c1, b2, c2, eps;  // c = 1 - b
@@ -68,6 +70,7 @@ struct Rates {
     double max_norm, beta1, beta2;
     const int *counter;  // advanced already
     float *norm;         // for the first workgroup of a launch, or NULL
+    const float2 *own;   // by_m, by_v of the tensors' own counters
 };
 
 // Elements of a thread's step: 16 bytes of the 32-bit arrays.
@@ -141,6 +144,10 @@ __global__ __launch_bounds__(256) void k_adamw(const Table<N> table, const Rates
             const float2 by = corrections(r.beta1, r.beta2, *r.counter);
             by_m = by.x, s.by_v = by.y;
         }
+    }
+    if (e.own >= 0) {
+        const float2 by = r.own[e.own];
+        by_m = by.x, s.by_v = by.y;
     }
     s.rate = (float)(lr * (double)by_m);
     P *const p = static_cast<P *>(e.p);
@@ -251,8 +258,26 @@ __global__ __launch_bounds__(256) void k_adamw_shared(const double *sums, int co
     }
 }
 
+// Counters of their own that tensors have: each counts its step, a thread each, and the corrections of that step
+// go to the workspace for the update.  A launch before the update: one workgroup of a tensor could not
+// advance what the others still read.
+constexpr int kCounters = 256;
+struct CounterTable {
+    int count;
+    int *of[kCounters];
+};
+__global__ __launch_bounds__(kCounters) void k_adamw_counters(const CounterTable table, double b1, double b2, float2 *own) {
+    const int i = threadIdx.x;
+    if (i >= table.count) return;
+    int *const counter = table.of[i];
+    const int t = *counter + 1;
+    *counter = t;
+    own[i] = corrections(b1, b2, t);
+}
+
 struct Sizes {
     int64_t elements, squares;  // workgroups of the norm's pass
+    int64_t counters;           // tensors with a counter of their own
 };
 
 constexpr int64_t kMostElements = (int64_t)1 << 34;  // (all workgroups of a launch then fit its grid)
@@ -264,9 +289,11 @@ int adamw_check(const gsv_adamw_args *a, Sizes *out) {
     *out = Sizes{};
     for (int64_t i = 0; i < a->count; ++i) {
         const gsv_adamw_tensor &t = a->tensors[i];
-        if (t.numel < 0 || (!a->counter && t.step < 1) || (t.dtype != GSV_F32 && t.dtype != GSV_BF16) ||
+        if (t.numel < 0 || (a->counter ? t.counter != nullptr : !t.counter && t.step < 1) ||
+            reinterpret_cast<uintptr_t>(t.counter) % 4 || (t.dtype != GSV_F32 && t.dtype != GSV_BF16) ||
             (t.grad_dtype != GSV_F32 && t.grad_dtype != GSV_BF16) || (t.master && t.dtype != GSV_BF16))
             return GSV_ERR_INVALID_ARGUMENT;
+        out->counters += t.counter != nullptr;
         if (t.numel > kMostElements || out->elements > kMostElements) return GSV_ERR_SIZE_OVERFLOW;
         if (t.numel == 0) continue;
         const uintptr_t words = reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq) |
@@ -283,9 +310,36 @@ int adamw_check(const gsv_adamw_args *a, Sizes *out) {
     return GSV_OK;
 }
 
+// The tensors' own counters, each once, and which of them a tensor has (-1: none).
+struct Counters {
+    int32_t **each = nullptr;
+    int *of = nullptr;  // NULL: no tensor has one
+    int count = 0;
+    bool fits = true;
+    Counters(const gsv_adamw_args *a, const Sizes &s) {
+        if (!s.counters) return;
+        each = new (std::nothrow) int32_t *[s.counters];
+        of = new (std::nothrow) int[a->count];
+        if (!each || !of) {
+            fits = false;
+            return;
+        }
+        for (int64_t i = 0; i < a->count; ++i)
+            if (a->tensors[i].counter) each[count++] = a->tensors[i].counter;
+        std::sort(each, each + count, std::less<int32_t *>());
+        count = (int)(std::unique(each, each + count) - each);
+        for (int64_t i = 0; i < a->count; ++i) {
+            int32_t *const c = a->tensors[i].counter;
+            of[i] = c ? (int)(std::lower_bound(each, each + count, c, std::less<int32_t *>()) - each) : -1;
+        }
+    }
+    ~Counters() { delete[] each, delete[] of; }
+    Counters(const Counters &) = delete;
+};
+
 // Tables of the tensors that `takes`, each handed to `launch` with its workgroups when it is full.
 template <typename Tensors, typename Takes, typename Launch>
-void tables(const gsv_adamw_args *a, int64_t per_block, const Takes &takes, const Launch &launch) {
+void tables(const gsv_adamw_args *a, int64_t per_block, const int *counter_of, const Takes &takes, const Launch &launch) {
     Tensors t;
     t.count = 0;
     int64_t blocks = 0;
@@ -298,12 +352,12 @@ void tables(const gsv_adamw_args *a, int64_t per_block, const Takes &takes, cons
             t.count = 0, blocks = 0;
         }
         float by_m = 1.f, by_v = 1.f;
-        if (!a->counter) {
+        if (!a->counter && !x.counter) {
             by_m = (float)(1.0 / (1.0 - std::pow(a->beta1, (double)x.step)));
             by_v = (float)(1.0 / std::sqrt(1.0 - std::pow(a->beta2, (double)x.step)));
         }
         t.first[t.count] = (int)blocks;
-        t.put(t.count++, x, by_m, by_v);
+        t.put(t.count++, x, by_m, by_v, counter_of ? counter_of[i] : -1);
         blocks += own;
     }
     if (t.count) launch(t, blocks);
@@ -315,21 +369,21 @@ template <typename Takes> bool at_most(const gsv_adamw_args *a, int most, const 
 }
 
 template <typename P, typename G, bool MASTER>
-void update_all(const gsv_adamw_args *a, const Rates &r, int steps, hipStream_t st) {
+void update_all(const gsv_adamw_args *a, const Rates &r, const int *own, int steps, hipStream_t st) {
     constexpr int p = sizeof(P) == 2 ? GSV_BF16 : GSV_F32, g = sizeof(G) == 2 ? GSV_BF16 : GSV_F32;
     const auto takes = [](const gsv_adamw_tensor &t) {
         return t.dtype == p && t.grad_dtype == g && (t.master != nullptr) == MASTER;
     };
     if (steps == 4)
-        tables<Table<kTensors>>(a, 256 * kVec * 4, takes, [&](const Table<kTensors> &t, int64_t blocks) {
+        tables<Table<kTensors>>(a, 256 * kVec * 4, own, takes, [&](const Table<kTensors> &t, int64_t blocks) {
             hipLaunchKernelGGL((k_adamw<P, G, MASTER, 4, kTensors>), dim3((unsigned)blocks), dim3(256), 0, st, t, r);
         });
     else if (at_most(a, kFew, takes))
-        tables<Table<kFew>>(a, 256 * kVec, takes, [&](const Table<kFew> &t, int64_t blocks) {
+        tables<Table<kFew>>(a, 256 * kVec, own, takes, [&](const Table<kFew> &t, int64_t blocks) {
             hipLaunchKernelGGL((k_adamw<P, G, MASTER, 1, kFew>), dim3((unsigned)blocks), dim3(256), 0, st, t, r);
         });
     else
-        tables<Table<kTensors>>(a, 256 * kVec, takes, [&](const Table<kTensors> &t, int64_t blocks) {
+        tables<Table<kTensors>>(a, 256 * kVec, own, takes, [&](const Table<kTensors> &t, int64_t blocks) {
             hipLaunchKernelGGL((k_adamw<P, G, MASTER, 1, kTensors>), dim3((unsigned)blocks), dim3(256), 0, st, t, r);
         });
 }
@@ -343,8 +397,8 @@ template <typename G> void squares_all(const gsv_adamw_args *a, double *sums, in
                            *at ? nullptr : counter);
         *at += blocks;
     };
-    if (at_most(a, kFewGradients, takes)) tables<Gradients<kFewGradients>>(a, 256 * kVec * kNormSteps, takes, launch);
-    else tables<Gradients<kGradients>>(a, 256 * kVec * kNormSteps, takes, launch);
+    if (at_most(a, kFewGradients, takes)) tables<Gradients<kFewGradients>>(a, 256 * kVec * kNormSteps, nullptr, takes, launch);
+    else tables<Gradients<kGradients>>(a, 256 * kVec * kNormSteps, nullptr, takes, launch);
 }
 
 // Whether a tensor that the step writes shares memory with another that it writes, or with a gradient.
@@ -383,7 +437,17 @@ bool share_memory(const gsv_adamw_args *a) {
     return twice;
 }
 
-size_t squares_bytes(const Sizes &s) { return sizeof(double) * (size_t)s.squares; }
+// The workspace: sums of squares, the tensors' own corrections, what all share.
+struct Workspace {
+    size_t own, shared, bytes;
+};
+Workspace adamw_workspace(const gsv_adamw_args *a, const Sizes &s) {
+    Workspace w;
+    w.own = a->max_norm > 0 ? sizeof(double) * (size_t)s.squares : 0;
+    w.shared = w.own + sizeof(float2) * (size_t)s.counters;
+    w.bytes = w.shared + (a->max_norm > 0 || a->counter ? 4 * sizeof(float) : 0);
+    return w;
+}
 
 }  // namespace
 }  // namespace gsv
@@ -395,24 +459,32 @@ extern "C" int gsv_adamw_workspace_bytes(const gsv_adamw_args *args, size_t *byt
     if (!bytes) return GSV_ERR_INVALID_ARGUMENT;
     const int st = adamw_check(args, &s);
     if (st != GSV_OK) return st;
-    *bytes = args->max_norm > 0 || args->counter ? (args->max_norm > 0 ? squares_bytes(s) : 0) + 4 * sizeof(float) : 0;
+    *bytes = adamw_workspace(args, s).bytes;
     return GSV_OK;
 }
 
 extern "C" int gsv_adamw(const gsv_adamw_args *args, void *workspace, size_t workspace_bytes, void *stream) {
     Sizes s;
-    size_t need;
-    int st = adamw_check(args, &s);
+    const int st = adamw_check(args, &s);
     if (st != GSV_OK) return st;
-    if ((st = gsv_adamw_workspace_bytes(args, &need)) != GSV_OK) return st;
-    if (need > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
-    if ((need && !workspace) || reinterpret_cast<uintptr_t>(workspace) % 16 || share_memory(args))
+    const Workspace ws = adamw_workspace(args, s);
+    if (ws.bytes > workspace_bytes) return GSV_ERR_WORKSPACE_TOO_SMALL;
+    if ((ws.bytes && !workspace) || reinterpret_cast<uintptr_t>(workspace) % 16 || share_memory(args))
         return GSV_ERR_INVALID_ARGUMENT;
+    const Counters counters(args, s);
+    if (!counters.fits) return GSV_ERR_INVALID_ARGUMENT;
     hipStream_t stm = as_stream(stream);
     Rates r{(float)args->beta1, (float)(1.0 - args->beta1), (float)args->beta2, (float)(1.0 - args->beta2),
             (float)args->eps, nullptr, args->counter != nullptr, nullptr, 0, args->max_norm, args->beta1, args->beta2,
-            args->counter, args->norm};
-    if (need) {
+            args->counter, args->norm, reinterpret_cast<const float2 *>(static_cast<char *>(workspace) + ws.own)};
+    for (int first = 0; first < counters.count; first += kCounters) {
+        CounterTable t;
+        t.count = std::min(counters.count - first, kCounters);
+        std::copy_n(counters.each + first, t.count, t.of);
+        hipLaunchKernelGGL(k_adamw_counters, dim3(1), dim3(kCounters), 0, stm, t, args->beta1, args->beta2,
+                           reinterpret_cast<float2 *>(static_cast<char *>(workspace) + ws.own) + first);
+    }
+    if (args->max_norm > 0 || args->counter) {
         double *sums = static_cast<double *>(workspace);
         // Few sums are added up by every workgroup of the update, many by a launch of one.  28 tensors of 235,000
         // elements: 15.6 us, with the launch 20.6 (both with larger tables than now: 14.4).
@@ -425,7 +497,7 @@ extern "C" int gsv_adamw(const gsv_adamw_args *args, void *workspace, size_t wor
         if (few) {
             r.sums = sums, r.count = (int)count;
         } else {
-            float *shared = reinterpret_cast<float *>(static_cast<char *>(workspace) + need - 4 * sizeof(float));
+            float *shared = reinterpret_cast<float *>(static_cast<char *>(workspace) + ws.shared);
             hipLaunchKernelGGL(k_adamw_shared, dim3(1), dim3(256), 0, stm, sums, (int)count, args->max_norm,
                                args->beta1, args->beta2, args->counter, args->norm, shared);
             r.shared = shared;
@@ -433,11 +505,11 @@ extern "C" int gsv_adamw(const gsv_adamw_args *args, void *workspace, size_t wor
     }
     // Elements of a workgroup: 1,024, and 4,096 (more loads at once) where that leaves workgroups enough.
     const int steps = s.elements >= (int64_t)4096 * 2048 ? 4 : 1;
-    update_all<float, float, false>(args, r, steps, stm);
-    update_all<float, bf16, false>(args, r, steps, stm);
-    update_all<bf16, float, false>(args, r, steps, stm);
-    update_all<bf16, bf16, false>(args, r, steps, stm);
-    update_all<bf16, float, true>(args, r, steps, stm);
-    update_all<bf16, bf16, true>(args, r, steps, stm);
+    update_all<float, float, false>(args, r, counters.of, steps, stm);
+    update_all<float, bf16, false>(args, r, counters.of, steps, stm);
+    update_all<bf16, float, false>(args, r, counters.of, steps, stm);
+    update_all<bf16, bf16, false>(args, r, counters.of, steps, stm);
+    update_all<bf16, float, true>(args, r, counters.of, steps, stm);
+    update_all<bf16, bf16, true>(args, r, counters.of, steps, stm);
     return check_launch();
 }

@@ -82,21 +82,22 @@ py::tuple adamw_step(py::handle params, py::handle grads, py::handle exp_avgs, p
     if (!first || !first->is_cuda()) return other();
     const at::Device dev = first->device();
     const c10::DeviceGuard guard(dev);
-    if (counter ? !is_vector(*counter, at::kInt, dev, 1)
-                : c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
-        return other();
+    if (counter && !is_vector(*counter, at::kInt, dev, 1)) return other();
+    bool counted = true;  // all of them on the device
     std::vector<gsv_adamw_tensor> all(n);
     std::vector<Tensor> held;  // while other threads may run, and change the lists
-    held.reserve(5 * n + 1);
+    held.reserve(6 * n + 1);
     for (Py_ssize_t i = 0; i < n; ++i) {
         const Tensor *p = tensor_in(ps[i]), *g = tensor_in(gs[i]), *m = tensor_in(ms[i]), *v = tensor_in(vs[i]), *w = nullptr;
         if (mastered && ws[i] != Py_None && !(w = tensor_in(ws[i]))) return other();
+        const Tensor *c = counter || steps.one ? nullptr : tensor_in(steps.each[i]);
         double t = 0.0, rate, decay;
         if (!p || !g || !m || !v || !is_dense(*p, dev) || !token_type(*p) || !is_like(*g, *p, dev) || !token_type(*g) ||
             !is_like(*m, *p, dev) || m->scalar_type() != at::kFloat || !is_like(*v, *p, dev) ||
             v->scalar_type() != at::kFloat ||
             (w && (!is_like(*w, *p, dev) || w->scalar_type() != at::kFloat || p->scalar_type() == at::kFloat)) ||
-            (!counter && (!PyLong_CheckExact(steps.one ? step.ptr() : steps.each[i]) || !steps.get(i, &t) ||
+            (c && !is_vector(*c, at::kInt, dev, 1)) ||
+            (!counter && !c && (!PyLong_CheckExact(steps.one ? step.ptr() : steps.each[i]) || !steps.get(i, &t) ||
                           !(t >= 1 && t < 9e15))) ||
             !rates.get(i, &rate) || !(rate >= 0) || !decays.get(i, &decay) || !(decay >= 0))
             return other();
@@ -105,10 +106,13 @@ py::tuple adamw_step(py::handle params, py::handle grads, py::handle exp_avgs, p
         x.param = ptr<void>(*p), x.grad = ptr<void>(*g), x.exp_avg = ptr<float>(*m), x.exp_avg_sq = ptr<float>(*v);
         x.master = w ? ptr<float>(*w) : nullptr, x.numel = p->numel(), x.step = (int64_t)t;
         x.lr = rate, x.weight_decay = decay, x.dtype = type_code(*p), x.grad_dtype = type_code(*g);
-        for (const Tensor *t : {p, m, v, w})
+        x.counter = c ? ptr<int32_t>(*c) : nullptr;
+        counted &= counter || c;
+        held.push_back(*g);  // the others are written
+        for (const Tensor *t : {p, m, v, w, c})
             if (t) held.push_back(*t);
-        held.push_back(*g);
     }
+    if (!counted && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) return other();
     if (counter) held.push_back(*counter);
     gsv_adamw_args a{};
     a.tensors = all.data(), a.count = (int64_t)n;
@@ -131,8 +135,8 @@ py::tuple adamw_step(py::handle params, py::handle grads, py::handle exp_avgs, p
     if (status == GSV_ERR_INVALID_ARGUMENT) return other();  // tensors share memory; nothing was launched
     check(status, "adamw");
     for (Py_ssize_t i = 0, at = 0; i < n; ++i) {
-        for (const int more = all[i].master ? 4 : 3, from = at; at < from + more; ++at) written(held[at]);
-        ++at;  // the gradient
+        const Py_ssize_t last = at + 3 + (all[i].master != nullptr) + (all[i].counter != nullptr);
+        while (at++ < last) written(held[at]);
     }
     if (counter) written(held.back());
     if (!norm.defined()) return py::make_tuple(true, py::none());

@@ -40,7 +40,7 @@ Pages = _struct("Pages", (
     (_c_i64, "pos_page pos_row"), (_P, "keep"), (_c_i64, "keep_page"), (_P, "table"),
     (_c_i64, "table_row"), (_c_int, "pages page_rows table_pages keep_bytes")))
 AdamwTensor = _struct("AdamwTensor", (
-    (_P, "param grad exp_avg exp_avg_sq master lr_device"), (_c_i64, "numel step"),
+    (_P, "param grad exp_avg exp_avg_sq master lr_device counter"), (_c_i64, "numel step"),
     (ctypes.c_double, "lr weight_decay"), (_c_int, "dtype grad_dtype")))
 Adamw = _struct("Adamw", (
     (_P, "tensors"), (_c_i64, "count"), (ctypes.c_double, "beta1 beta2 eps max_norm"), (_P, "counter norm")))

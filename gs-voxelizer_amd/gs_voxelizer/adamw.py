@@ -32,7 +32,7 @@ def _is_number(x):
 
 
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
-               exp_avg_sqs: Sequence[Tensor], step: Union[int, Sequence[int], Tensor], *,
+               exp_avg_sqs: Sequence[Tensor], step: Union[int, Tensor, Sequence[Union[int, Tensor]]], *,
                lr: Union[float, Tensor, Sequence[Union[float, Tensor]]] = 1e-3,
                betas: Sequence[float] = (0.9, 0.999), eps: float = 1e-8,
                weight_decay: Union[float, Sequence[float]] = 0.0,
@@ -46,8 +46,9 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
             not by max_norm.
         exp_avgs, exp_avg_sqs: the float32 state, laid out like the params.
         step: the number of this step, from 1, for all tensors or for each; or a (1,) int32 tensor on the
-            device that counts the steps made, which the call advances.  A captured step needs the
-            latter (a number would be the same in each replay).
+            device that counts the steps made, which the call advances, for all tensors or for each (one that
+            several have advances once).  A captured step needs the latter (a number would be the same in
+            each replay).
         lr: the rate, or one for each tensor; a number, or a float32 tensor of one element on the device, which a
             captured step reads at each replay.
         weight_decay: of all tensors, or of each.
@@ -71,7 +72,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
             if not (_is_number(x) or (what == "lr" and isinstance(x, Tensor))):
                 raise ValueError(f"{what} must be numbers, got {x!r}")
     for x in steps:
-        if not isinstance(x, int) or not 1 <= x < 2**53:
+        if not isinstance(x, Tensor) and (not isinstance(x, int) or not 1 <= x < 2**53):
             raise ValueError(f"step must be whole numbers from 1, got {x!r}")
     return _step(params, grads, exp_avgs, exp_avg_sqs, masters, steps, counter, rates, decays, betas, eps, max_norm)
 
@@ -104,8 +105,9 @@ def _step(params, grads, exp_avgs, exp_avg_sqs, masters, steps, counter, rates, 
     _t.check(len(betas) == 2 and all(0 <= b < 1 for b in betas), f"betas must be two values from 0 to below 1, got {betas}")
     _t.check(eps >= 0, f"eps must not be negative, got {eps}")
     dev = params[0].device if isinstance(params[0], Tensor) else None
-    if counter is not None:
-        _t.check(counter.dtype == torch.int32 and tuple(counter.shape) == (1,) and counter.device == dev,
+    counters = [counter] if counter is not None else [x for x in steps if isinstance(x, Tensor)]
+    for c in counters:
+        _t.check(c.dtype == torch.int32 and tuple(c.shape) == (1,) and c.device == dev,
                  f"step must be a number or a (1,) int32 tensor on {dev}")
     held = []  # copies that live until the kernels are enqueued
     entries = (_lib.AdamwTensor * n)()
@@ -136,13 +138,17 @@ def _step(params, grads, exp_avgs, exp_avg_sqs, masters, steps, counter, rates, 
             _t.check(rate >= 0, f"lr must not be negative, got {rate}")
             t.lr = rate
         _t.check(decay >= 0, f"weight_decay must not be negative, got {decay}")
-        t.weight_decay, t.step = decay, 0 if counter is not None else steps[i]
+        t.weight_decay = decay
+        if counter is None and isinstance(steps[i], Tensor):
+            t.counter = steps[i].data_ptr()
+        elif counter is None:
+            t.step = steps[i]
         t.dtype, t.grad_dtype = _t.TYPES[p.dtype], _t.TYPES[g.dtype]
     a = _lib.Adamw(tensors=ctypes.addressof(entries), count=n, beta1=betas[0], beta2=betas[1], eps=eps,
                    max_norm=max_norm or 0.0, counter=_t.ptr(counter))
     norm = None
     with torch.cuda.device(dev):
-        if counter is None and torch.cuda.is_current_stream_capturing():
+        if counter is None and len(counters) < n and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("gs_voxelizer: a captured step needs its count on the device (a (1,) int32 tensor)")
         if max_norm:
             norm = torch.empty((), dtype=torch.float32, device=dev)
@@ -156,7 +162,7 @@ def _step(params, grads, exp_avgs, exp_avg_sqs, masters, steps, counter, rates, 
             if "argument" not in str(e):
                 raise
             raise ValueError(f"{e}: a tensor that the step writes shares memory with another, or with a gradient")
-    _t.written(*params, *exp_avgs, *exp_avg_sqs, *(masters or []), counter)
+    _t.written(*params, *exp_avgs, *exp_avg_sqs, *(masters or []), *counters)
     return norm
 
 
@@ -169,10 +175,12 @@ class AdamW(torch.optim.Optimizer):
         masters: bfloat16 parameters get float32 masters (state ``master``), which the steps go by.
         max_norm: see `adamw_step`; over all groups, which then have one device, ``betas`` and ``eps``.  The last
             step's norm is ``self.norm``.
-        capturable: (likewise one device, ``betas`` and ``eps``) the number of steps is one counter on the device, for
-            all parameters (those without a gradient at some step, which it leaves as they are, count it too), and
-            the step can be captured in a graph after one ordinary step.  ``lr`` may be a float32 tensor of one
-            element on the device.
+        capturable: (likewise one device, ``betas`` and ``eps``) each parameter's steps are counted on the device, and
+            the step can be captured in a graph once an ordinary step has been made with the same gradients
+            there.  ``lr`` may be a float32 tensor of one element on the device.
+
+    Each parameter counts the steps that it made itself: one without a gradient at some step is left as it is and
+    does not count it.
 
     A step that is captured together with a voxelization would be made twice where
     `graph.CapturedStep` has to run a replay again: capture the optimiser's step in a graph of its own.
@@ -190,16 +198,11 @@ class AdamW(torch.optim.Optimizer):
         self.norm: Optional[Tensor] = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
-    def _new_state(self, p, counters):
+    def _new_state(self, p):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("gs_voxelizer: the first step makes the optimiser's state: run one before the capture")
         s = self.state[p]
-        if self.capturable:
-            if p.device not in counters:
-                counters[p.device] = torch.zeros(1, dtype=torch.int32, device=p.device)
-            s["step"] = counters[p.device]
-        else:
-            s["step"] = 0
+        s["step"] = torch.zeros(1, dtype=torch.int32, device=p.device) if self.capturable else 0
         s["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
         s["exp_avg_sq"] = torch.zeros_like(s["exp_avg"])
         if self.masters and p.dtype == torch.bfloat16:
@@ -213,23 +216,19 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        counters = {p.device: s["step"] for p, s in self.state.items()} if self.capturable else {}
         calls = {}
         for group in self.param_groups:
             key = (tuple(group["betas"]), group["eps"])
             for p in group["params"]:
                 if p.grad is None:
                     continue
-                s = self.state.get(p) or self._new_state(p, counters)
+                s = self.state.get(p) or self._new_state(p)
                 calls.setdefault((p.device, *key), []).append((p, s, group["lr"], group["weight_decay"]))
         _t.check((self.max_norm is None and not self.capturable) or len(calls) <= 1,
                  "max_norm and capturable need parameters of one device, and one betas and eps in all groups")
-        for (dev, betas, eps), members in calls.items():
+        for (_, betas, eps), members in calls.items():
             ps, states = [c[0] for c in members], [c[1] for c in members]
-            if self.capturable:
-                count = counters[dev]
-            else:
-                count = [s["step"] + 1 for s in states]
+            count = [s["step"] if self.capturable else s["step"] + 1 for s in states]
             self.norm = adamw_step(
                 ps, [p.grad for p in ps], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], count,
                 lr=[c[2] for c in members], betas=betas, eps=eps, weight_decay=[c[3] for c in members],
@@ -242,7 +241,7 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """As torch's, but the state is float32 whatever the parameters' type is, and copied."""
         super().load_state_dict(state_dict)
-        saved, most = state_dict["state"], {}
+        saved = state_dict["state"]
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):
@@ -254,11 +253,8 @@ class AdamW(torch.optim.Optimizer):
                            torch.empty_like(p, dtype=torch.float32).copy_(x) if isinstance(x, Tensor) else x)
             if self.masters and p.dtype == torch.bfloat16 and "master" not in s:
                 s["master"] = p.detach().to(torch.float32)
-            most[p.device] = max(most.get(p.device, 0), s["step"])
-        if self.capturable:
-            counters = {dev: torch.tensor([n], dtype=torch.int32, device=dev) for dev, n in most.items()}
-            for p, s in self.state.items():
-                s["step"] = counters[p.device]
+            if self.capturable:
+                s["step"] = torch.tensor([s["step"]], dtype=torch.int32, device=p.device)
 
     def __getstate__(self):
         return {**super().__getstate__(), "masters": self.masters, "max_norm": self.max_norm,

@@ -506,16 +506,18 @@ int gsv_gated_norm_bwd(const gsv_norm *args, const void *dy, int64_t dy_row, con
  * with w the master where there is one (param then receives it, rounded), else the param.  param and grad are
  * GSV_F32 or GSV_BF16 (a master needs a GSV_BF16 param), the rest float32; all of numel
  * values in the same order, aligned to their own size.  t is the tensor's step, 1 or more; with `counter` (one
- * int32 on the device, steps made so far) t = *counter + 1 for all, and the call advances it.  lr_device: NULL, or the
- * rate, one float on the device.  norm (NULL, or one float on the device) receives |all grads| where max_norm > 0.
- * Written tensors that share memory with each other or a gradient are refused (GSV_ERR_INVALID_ARGUMENT).  The norm is
- * summed in binary64 in a fixed order.
+ * int32 on the device, steps made so far) t = *counter + 1 for all, and the call advances it; with a tensor's own
+ * counter likewise for that tensor (several may have one counter, which then advances once; not beside the
+ * counter for all).  lr_device: NULL, or the rate, one float on the device.  norm (NULL, or one float on the
+ * device) receives |all grads| where max_norm > 0.  Written tensors that share memory with each other or a gradient are refused
+ * (GSV_ERR_INVALID_ARGUMENT).  The norm is summed in binary64 in a fixed order.
  */
 typedef struct gsv_adamw_tensor {
     void *param;
     const void *grad;
     float *exp_avg, *exp_avg_sq, *master;
     const float *lr_device;
+    int32_t *counter;
     int64_t numel, step;
     double lr, weight_decay;
     int32_t dtype, grad_dtype;
