@@ -239,7 +239,8 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """As torch's, but the state is float32 whatever the parameters' type is, and copied."""
+        """As torch's, but the state is float32 whatever the parameters' type is, and copied.  A saved master is taken
+        where this optimiser keeps one for the parameter; where none was saved the parameter's value becomes it."""
         super().load_state_dict(state_dict)
         saved = state_dict["state"]
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
@@ -248,10 +249,13 @@ class AdamW(torch.optim.Optimizer):
             if i not in saved:
                 continue
             s = self.state[p] = {}
+            mastered = self.masters and p.dtype == torch.bfloat16
             for name, x in saved[i].items():
+                if name == "master" and not mastered:
+                    continue  # no step would keep it up to date
                 s[name] = (int(x) if name == "step" else
                            torch.empty_like(p, dtype=torch.float32).copy_(x) if isinstance(x, Tensor) else x)
-            if self.masters and p.dtype == torch.bfloat16 and "master" not in s:
+            if mastered and "master" not in s:
                 s["master"] = p.detach().to(torch.float32)
             if self.capturable:
                 s["step"] = torch.tensor([s["step"]], dtype=torch.int32, device=p.device)

@@ -53,3 +53,29 @@ def test_counters_of_tensors():
     assert _plan([1024, 1024, None], max_norm=1.0) == (OK, 3 * 8 + 2 * 8 + 16)
     assert _plan([1026])[0] == INVALID
     assert _plan([1024, None], counter=2048)[0] == INVALID
+
+
+def _with_state(dtype, masters, master=None):
+    p = torch.nn.Parameter(torch.full((3,), 5.0, dtype=dtype))
+    opt = adamw.AdamW([p], masters=masters)
+    opt.state[p] = dict(step=4, exp_avg=torch.full((3,), 0.5), exp_avg_sq=torch.full((3,), 0.25))
+    if master is not None:
+        opt.state[p]["master"] = torch.full((3,), master)
+    return opt, p
+
+
+@pytest.mark.parametrize("dtype,masters", [(torch.bfloat16, False), (torch.float32, True), (torch.float32, False)],
+                         ids=["off", "float32", "float32, off"])
+def test_masters_are_loaded_where_they_are_kept(dtype, masters):
+    """Elsewhere they would only grow old: in the state, and in what is saved from it."""
+    saved, _ = _with_state(torch.bfloat16, True, 5.0078125)
+    opt, p = _with_state(dtype, masters)
+    opt.load_state_dict(saved.state_dict())
+    assert set(opt.state[p]) == {"step", "exp_avg", "exp_avg_sq"}
+    # back on, with the weights as they are by then
+    again, q = _with_state(torch.bfloat16, True)
+    again.load_state_dict(opt.state_dict())
+    assert again.state[q]["master"].tolist() == [5.0] * 3 and again.state[q]["master"].dtype == torch.float32
+    same, q = _with_state(torch.bfloat16, True)
+    same.load_state_dict(saved.state_dict())
+    assert same.state[q]["master"].tolist() == [5.0078125] * 3

@@ -1,4 +1,4 @@
-"""Steps that are counted for each tensor on its own, on the host and on the device."""
+"""Steps that are counted for each tensor on its own, and the optimiser's state as it is made and loaded."""
 import copy
 
 import pytest
@@ -196,3 +196,30 @@ def test_looking_at_the_state_changes_nothing(device):
         ps[0].grad = torch.ones_like(ps[0])
         opt.step()
         assert int(opt.state[ps[0]]["step"]) == 1 and not opt.state[ps[1]]
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_masters_on_off_and_on_again(device, capturable):
+    """A checkpoint with masters goes on without them, and later with new ones: no step brings old weights back."""
+    def run(masters, state=None, weights=None, dtype=BF16, steps=40):
+        p = torch.nn.Parameter(torch.ones(100, dtype=dtype, device=device))
+        if weights is not None:
+            p.data.copy_(weights)
+        opt = adamw.AdamW([p], lr=1e-2, weight_decay=0.0, masters=masters, capturable=capturable)
+        if state is not None:
+            opt.load_state_dict(state)
+        for _ in range(steps):
+            p.grad = torch.ones_like(p)
+            opt.step()
+        return p.detach().clone(), copy.deepcopy(opt.state_dict())
+
+    on, on_state = run(True)
+    off, off_state = run(False, on_state, on)
+    assert "master" not in off_state["state"][0]
+    again, _ = run(True, off_state, off, steps=1)
+    # constant gradients: each step is the rate but for 1e-4 of it, and a bfloat16 of this size rounds by 2^-9 at most
+    assert (off < on - 0.3).all()
+    assert ((again.float() - (off.float() - 1e-2)).abs() <= 1e-6 + 2.0 ** -9).all()
+    wide, wide_state = run(True, on_state, on.float(), dtype=F32, steps=1)
+    assert "master" not in wide_state["state"][0]
+    assert ((wide - (on.float() - 1e-2)).abs() <= 2e-6).all()
