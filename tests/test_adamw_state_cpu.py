@@ -79,3 +79,35 @@ def test_masters_are_loaded_where_they_are_kept(dtype, masters):
     same, q = _with_state(torch.bfloat16, True)
     same.load_state_dict(saved.state_dict())
     assert same.state[q]["master"].tolist() == [5.0078125] * 3
+
+
+def test_states_that_are_refused():
+    """Another optimiser's, or another model's: nothing is loaded."""
+    def saved(make, shape=(3,), **more):
+        p = torch.nn.Parameter(torch.ones(shape))
+        p.grad = torch.ones_like(p)
+        ref = make([p], **dict(dict(lr=0.5), **more))
+        ref.step()
+        return ref.state_dict()
+
+    opt, p = _with_state(torch.float32, False)
+    for state in (saved(torch.optim.AdamW, amsgrad=True), saved(torch.optim.AdamW, maximize=True),
+                  saved(torch.optim.Adam, weight_decay=0.1), saved(torch.optim.SGD, momentum=0.9),
+                  saved(torch.optim.RMSprop), saved(torch.optim.AdamW, (1,)), saved(torch.optim.AdamW, (2, 3))):
+        with pytest.raises(ValueError):
+            opt.load_state_dict(state)
+        assert opt.state[p]["step"] == 4 and opt.param_groups[0]["lr"] == 1e-3
+    for state in (saved(torch.optim.AdamW), saved(torch.optim.AdamW, foreach=True), saved(torch.optim.Adam)):
+        opt.load_state_dict(state)
+        assert opt.state[p]["step"] == 1 and opt.param_groups[0]["lr"] == 0.5
+        assert opt.state[p]["exp_avg"].tolist() == pytest.approx([0.1] * 3)
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_state_that_was_looked_at_and_is_empty(capturable):
+    ps = [torch.nn.Parameter(torch.ones(3)) for _ in "ab"]
+    opt = adamw.AdamW(ps, capturable=capturable)
+    assert not opt.state[ps[0]]
+    again = adamw.AdamW(ps, capturable=capturable)
+    again.load_state_dict(opt.state_dict())
+    assert not again.state[ps[0]] and not again.state[ps[1]]
