@@ -241,7 +241,8 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """As torch's, but the state is float32 whatever the parameters' type is, and copied.  A saved master is taken
         where this optimiser keeps one for the parameter; where none was saved the parameter's value becomes it.
-        Raises ValueError, and loads nothing, where the state is another optimiser's or of other shapes."""
+        Raises ValueError, and loads nothing, where the state is another optimiser's or of other shapes.  A graph
+        captured before steps the state that there was: capture again."""
         saved = state_dict["state"]
         for g in state_dict["param_groups"]:
             _t.check(not (g.get("maximize") or g.get("amsgrad"))
@@ -250,9 +251,9 @@ class AdamW(torch.optim.Optimizer):
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):
-            for name in ("step", "exp_avg", "exp_avg_sq") if saved.get(i) else ():
-                _t.check(name in saved[i], f"the state of parameter {i} has no {name}")
-                _t.check(name == "step" or saved[i][name].shape == p.shape,
+            for name in ("step", "exp_avg", "exp_avg_sq", "master") if saved.get(i) else ():
+                _t.check(name in saved[i] or name == "master", f"the state of parameter {i} has no {name}")
+                _t.check(name == "step" or name not in saved[i] or saved[i][name].shape == p.shape,
                          f"{name} of parameter {i} must have shape {tuple(p.shape)}")
         super().load_state_dict(state_dict)
         for i, p in zip(ids, params):

@@ -97,6 +97,11 @@ def test_states_that_are_refused():
         with pytest.raises(ValueError):
             opt.load_state_dict(state)
         assert opt.state[p]["step"] == 4 and opt.param_groups[0]["lr"] == 1e-3
+    other, _ = _with_state(torch.bfloat16, True, 1.0)
+    state = other.state_dict()
+    state["state"][0]["master"] = torch.ones(1)
+    with pytest.raises(ValueError, match="master"):
+        opt.load_state_dict(state)
     for state in (saved(torch.optim.AdamW), saved(torch.optim.AdamW, foreach=True), saved(torch.optim.Adam)):
         opt.load_state_dict(state)
         assert opt.state[p]["step"] == 1 and opt.param_groups[0]["lr"] == 0.5
