@@ -483,10 +483,12 @@ template <typename T>
 __global__ __launch_bounds__((64 * kJoinWaves)) void k_paged_join(const float *__restrict__ part_o,
                                                                   const float2 *__restrict__ part_ms,
                                                                   const int2 *__restrict__ parts, FastDiv by_heads,
-                                                                  int heads, int dim, T *__restrict__ out) {
+                                                                  int rows, int heads, int dim, T *__restrict__ out) {
     constexpr int kOnce = 4;  // parts of a wave whose maxima, sums and rows are loaded together
     __shared__ float so[kJoinWaves][128], sm[kJoinWaves], ss[kJoinWaves];
-    const int row = blockIdx.x, s = fastdiv(row, by_heads), h = row - s * heads;
+    const int row = blockIdx.y * gridDim.x + blockIdx.x;
+    if (row >= rows) return;
+    const int s = fastdiv(row, by_heads), h = row - s * heads;
     const int2 own = parts[s];
     if (own.y == 1) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -561,9 +563,12 @@ struct Paged {
             hipLaunchKernelGGL((k_attention_paged<T, DP, FAR, CAP, kPieces>), grid, block, 0, st, a, c, o);
         else
             hipLaunchKernelGGL((k_attention_paged<T, DP, FAR, CAP, kShares>), grid, block, 0, st, a, c, o);
-        if (c.split)
-            hipLaunchKernelGGL(k_paged_join<T>, dim3((unsigned)(a.scenes * a.heads)), dim3(64 * kJoinWaves), 0, st,
-                               c.part_o, c.part_ms, c.parts, make_fastdiv(a.heads), a.heads, a.dim, o);
+        if (c.split) {
+            // (an axis of a grid holds less than 2^32 threads: 2^23 of these workgroups; rows are less than 2^24)
+            const int rows = a.scenes * a.heads, x = rows < (1 << 22) ? rows : 1 << 22;
+            hipLaunchKernelGGL(k_paged_join<T>, dim3((unsigned)x, (unsigned)((rows + x - 1) / x)), dim3(64 * kJoinWaves),
+                               0, st, c.part_o, c.part_ms, c.parts, make_fastdiv(a.heads), rows, a.heads, a.dim, o);
+        }
     }
 };
 
