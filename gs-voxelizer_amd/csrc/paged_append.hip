@@ -50,11 +50,12 @@ __device__ __forceinline__ int start_of(const AppendArgs &a, int s) {
 __device__ __forceinline__ Target target_of(const AppendArgs &a, int t, int s0) {
     int s = a.starts ? s0 : t, ahead = 1;
     if (a.starts) {
-        int step = 1;
-        while (s + step < a.scenes && start_of(a, s + step) <= t) s += step, step *= 2;
+        uint32_t step = 1;  // (scenes may be near 2^31: s + step is formed where it is one)
+        const auto takes = [&] { return step < (uint32_t)(a.scenes - s) && start_of(a, s + (int)step) <= t; };
+        while (takes()) s += (int)step, step *= 2;
         for (; step > 1;) {
             step /= 2;
-            if (s + step < a.scenes && start_of(a, s + step) <= t) s += step;
+            if (takes()) s += (int)step;
         }
         ahead = start_of(a, s + 1) - t;  // of the scene's tokens, this one and those behind it
     }
