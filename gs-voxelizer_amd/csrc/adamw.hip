@@ -280,7 +280,9 @@ struct Sizes {
     int64_t counters;           // tensors with a counter of their own
 };
 
-constexpr int64_t kMostElements = (int64_t)1 << 34;  // (all workgroups of a launch then fit its grid)
+// All workgroups of a launch then fit its grid: at most 2^22 of 4,096 elements (where there are fewer than 8.4 million,
+// 2^13 of 1,024), or 2^21 of the norm's 8,192, and one more for each tensor of a table.
+constexpr int64_t kMostElements = (int64_t)1 << 34;
 
 int adamw_check(const gsv_adamw_args *a, Sizes *out) {
     if (!a || a->count < 0 || (a->count && !a->tensors) || !(a->beta1 >= 0 && a->beta1 < 1) ||
@@ -347,7 +349,7 @@ void tables(const gsv_adamw_args *a, int64_t per_block, const int *counter_of, c
         const gsv_adamw_tensor &x = a->tensors[i];
         if (!x.numel || !takes(x)) continue;
         const int64_t own = (x.numel + per_block - 1) / per_block;
-        if (t.count == Tensors::kMost || (t.count && blocks + own > (1 << 23))) {
+        if (t.count == Tensors::kMost) {
             launch(t, blocks);
             t.count = 0, blocks = 0;
         }
