@@ -518,7 +518,8 @@ int attention_args(const gsv_attention *in, AttnArgs *a) {
     if ((g.q_tokens > 0 && !g.q) || (g.k_tokens > 0 && (!g.k || !g.v)))
         return GSV_ERR_INVALID_ARGUMENT;
     if (g.scenes > 1 && (!g.q_starts || !g.k_starts)) return GSV_ERR_INVALID_ARGUMENT;
-    if (!(g.scale > 0.f) || !(g.cap >= 0.f)) return GSV_ERR_INVALID_ARGUMENT;
+    // (an infinite cap would be infinity times tanh(0))
+    if (!(g.scale > 0.f && g.scale < INFINITY) || !(g.cap >= 0.f && g.cap < INFINITY)) return GSV_ERR_INVALID_ARGUMENT;
     if (g.slopes && ((!g.q_positions && g.q_tokens > 0) || (!g.k_positions && g.k_tokens > 0) ||
                      (g.slopes_dtype != GSV_F32 && g.slopes_dtype != GSV_BF16)))
         return GSV_ERR_INVALID_ARGUMENT;

@@ -315,7 +315,7 @@ struct AttentionCall {
             return false;
         if (!is_aligned(q) || !is_aligned(k) || !is_aligned(v)) return false;
         scale = scale_or_0 == 0 ? 1.0 / std::sqrt((double)D) : scale_or_0;
-        if (!((float)scale > 0) || !(cap >= 0)) return false;
+        if (!((float)scale > 0) || !(cap >= 0) || !std::isfinite((float)scale) || !std::isfinite((float)cap)) return false;
         return !slopes.defined() ||
                (token_type(slopes) && is_vector(slopes, slopes.scalar_type(), dev, H));
     }

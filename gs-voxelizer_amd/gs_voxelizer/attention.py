@@ -12,6 +12,7 @@ nothing; one in a key that only causality hides from some tokens can reach those
 tile.
 """
 import ctypes
+import math
 from typing import Optional
 
 import torch
@@ -42,9 +43,9 @@ def _heads(q, k, v, dims):
 def _options(a, q, scale, cap, slopes):
     D = q.shape[-1]
     a.scale = D ** -0.5 if scale is None else float(scale)
-    _t.check(a.scale > 0, f"scale must be positive, got {scale}")
+    _t.check(0 < a.scale < math.inf, f"scale must be positive and finite, got {scale}")
     a.cap = float(cap or 0.0)
-    _t.check(a.cap >= 0, f"cap must not be negative, got {cap}")
+    _t.check(0 <= a.cap < math.inf, f"cap must not be negative or infinite, got {cap}")
     if slopes is not None:
         _t.check(isinstance(slopes, Tensor) and slopes.dtype in _t.TYPES
                  and tuple(slopes.shape) == (q.shape[1],) and slopes.device == q.device,
