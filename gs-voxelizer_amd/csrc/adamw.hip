@@ -37,7 +37,7 @@ struct Entry {
     int own;                  // below 0: these; else the place of those of the tensor's own counter
 };
 // Tensors of a launch: as many as its arguments hold, which end at 4 KB; where there are few, a table of few, since the
-// host copies all of it (four tensors: 6.0 us a call, in the large table 6.8).
+// host copies all of it (four tensors: 6.03 us a call, in the large table 6.32).
 constexpr int kTensors = 44, kFew = 8;
 template <int N> struct Table {
     static constexpr int kMost = N;
@@ -49,8 +49,9 @@ template <int N> struct Table {
                      (float)x.weight_decay, by_m, by_v, own};
     }
 };
-// For the norm: the gradients alone (28 tensors 14.4 us, in the tables above 17.0; 148 of 83 million values, one launch
-// in place of four, 479 and 492).
+// For the norm: the gradients alone (148 tensors of 83 million values, one launch in place of four: 478 us, in the tables
+// above 490; 28 tensors 16.2 both ways).  4 KB would hold 200; what is not used is copied all the same: 28 tensors in a
+// table of 32 14.2 or 16.1 us (the host runs at one of two speeds, from process to process), in one of 160 14.3 or 16.4.
 constexpr int kGradients = 160, kFewGradients = 32;
 template <int N> struct Gradients {
     static constexpr int kMost = N;
@@ -260,7 +261,8 @@ __global__ __launch_bounds__(256) void k_adamw_shared(const double *sums, int co
 
 // Counters of their own that tensors have: each counts its step, a thread each, and the corrections of that step
 // go to the workspace for the update.  A launch before the update: one workgroup of a tensor could not
-// advance what the others still read.
+// advance what the others still read.  2.6 us, of 4 tensors or 148; calls of 28 tensors, not clipped, take 14.9 us so and
+// 13.6 with one counter, which k_adamw_shared counts (or the norm's pass, without a launch).
 constexpr int kCounters = 256;
 struct CounterTable {
     int count;
@@ -489,7 +491,7 @@ extern "C" int gsv_adamw(const gsv_adamw_args *args, void *workspace, size_t wor
     if (args->max_norm > 0 || args->counter) {
         double *sums = static_cast<double *>(workspace);
         // Few sums are added up by every workgroup of the update, many by a launch of one.  28 tensors of 235,000
-        // elements: 15.6 us, with the launch 20.6 (both with larger tables than now: 14.4).
+        // elements: 15.6 us, with the launch 20.6 (before the tables of few gradients).
         const bool few = args->max_norm > 0 && s.squares > 0 && s.squares <= 256;
         int64_t count = 0;
         if (args->max_norm > 0) {

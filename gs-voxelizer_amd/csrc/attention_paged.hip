@@ -18,7 +18,7 @@
 // 2 caches of 200,003 rows, 16 heads on 4 of 128, bfloat16, capped, bias, pages of 256 (316 MB of live rows): 64.5 us,
 // 4.9 TB/s, and 4.8 for the join; 128 of 2,000, 8 on 8 of 64 (350 MB) 74.4 us, 4.7 TB/s; 5 of 20,000, 12 on 4 of 40, float32 (66 MB)
 // 20.6 us.  Bytes bound these: each is read once (counters), vector units are at work 15 to 20 % of the time, matrix units
-// 1 to 20 %.  16 of 4,096, 8 on 2 of 64 (23 MB): 10.8 us and 3.6; there the chain from the launch to the first bytes
+// 1 to 20 %.  The last one's calls take 12 us (the start, the join) and their bytes at 5.3 TB/s, from 5 to 774 MB.  16 of 4,096, 8 on 2 of 64 (23 MB): 10.8 us and 3.6; there the chain from the launch to the first bytes
 // (lengths, table, keys) and a wave's two steps bound it.
 #include "gsv_attention.h"
 

@@ -211,3 +211,21 @@ def test_values_in_equal_shares(device, dtype):
         c = Case(device, dtype, lengths, 16, 8, 64, rows=48, cap=cap, bias=bias, keep=keep)
         assert 2 * len(lengths) >= _workgroups(dtype, 16, 8, 64)
         c.check(c.run(), scenes=range(0, 70, 6))
+
+
+@TYPES
+def test_a_prompt_that_continues_a_cache(device, dtype):
+    """Appended at once; its tokens attend in one call as scenes that share their pages, each with a row more."""
+    g, H, K, D, rows, old, new = _gen(device, 6), 4, 2, 64, 16, 37, 30
+    T = old + new
+    x = torch.randn(T, H + 2 * K, D, generator=g, device=device).to(dtype)
+    pool = torch.full((7, 2, rows, K, D), float("nan"), dtype=dtype, device=device)
+    cache = pool[:, 0], pool[:, 1]
+    table = _ints([[4, 0, 6, 2, 5]], device)
+    for first, last in ((0, old), (old, T)):
+        paged.append_tokens(x[first:last, H:H + K], x[first:last, H + K:], *cache, table, _ints([last], device),
+                            scene_starts=_ints([0, last - first], device))
+    lengths = torch.arange(old + 1, T + 1, dtype=torch.int32, device=device)
+    got = paged.paged_attention(x[old:, :H], *cache, table.expand(new, -1), lengths)
+    val, tol = R.attention(x[old:, :H], x[:, H:H + K], x[:, H + K:], causal=True)  # the last rows of the scene's
+    R.assert_within(got, val["out"], tol["out"], "continued")
