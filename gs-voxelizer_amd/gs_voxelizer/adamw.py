@@ -240,7 +240,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but the state is float32 whatever the parameters' type is, and copied.  A saved master is taken
-        where this optimiser keeps one for the parameter; where none was saved the parameter's value becomes it.
+        where this optimiser keeps one for the parameter; where none was saved the parameter's value becomes it (so load
+        the model's weights first).
         Raises ValueError, and loads nothing, where the state is another optimiser's or of other shapes.  A graph
         captured before steps the state that there was: capture again."""
         saved = state_dict["state"]
